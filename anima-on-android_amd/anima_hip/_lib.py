@@ -78,6 +78,15 @@ SIGNATURES = {
     "anima_hip_dit_forward_dev": (_B, [_P, _P, ct.c_int64, _P] + [_I] * 4
                                   + [_P, _P, _P, ct.c_size_t, _P]),
     "anima_hip_dit_euler_dev": (_B, [_P, _P, _P, _I, _F, _I, _I, _P, _P, ct.c_size_t, _P]),
+    "anima_hip_mx4_pack_dev": (_B, [_P, ct.c_int64, _I, _P, _P, ct.c_int64, _I, _P]),
+    "anima_hip_mx4_unpack_dev": (_B, [_P, _P, _P, ct.c_int64, _I, ct.c_int64, _I, _P]),
+    "anima_hip_linear_mx4_scratch_bytes": (ct.c_size_t, [_I] * 4),
+    "anima_hip_linear_mx4_dev": (_B, [_P, ct.c_int64, _P, _P, _P, ct.c_int64] + [_I] * 4
+                                 + [_P, ct.c_size_t, _P]),
+    "anima_hip_kv4_append_dev": (_B, [_P, _P, _I, _I64P, _I64P] + [_P] * 6 + [_I] * 5 + [_P]),
+    "anima_hip_kv4_attention_scratch_bytes": (ct.c_size_t, [_I] * 7),
+    "anima_hip_kv4_attention_dev": (_B, [_P, _I, _I64P] + [_P] * 7 + [_I64P] + [_I] * 7
+                                    + [_F, _B, _P, ct.c_size_t, _P]),
     "anima_hip_last_call_ms": (_B, [ct.POINTER(_F), ct.POINTER(_F)]),
     "anima_hip_malloc": (_P, [ct.c_size_t]),
     "anima_hip_free": (None, [_P]),

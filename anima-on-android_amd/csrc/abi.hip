@@ -1527,6 +1527,216 @@ bool anima_hip_linear_dev(const float *a, int64_t lda, const uint16_t *w, int64_
                          scratch_bytes, pick_stream(stream));
 }
 
+namespace {
+// Largest row length and row count of the 4-bit entries: their kernels hold
+// element positions of a row, and rows of a head, in 32 bits with room for a tile.
+constexpr int kMx4MaxDim = 1 << 30;
+
+bool mx4_type(const char *who, int dtype, Mx4Type &t)
+{
+    if (dtype != ANIMA_HIP_DTYPE_F32 && dtype != ANIMA_HIP_DTYPE_BF16)
+        return fail(std::string(who) + ": dtype must be ANIMA_HIP_DTYPE_F32 or "
+                                       "ANIMA_HIP_DTYPE_BF16, got " + std::to_string(dtype));
+    t = Mx4Type(dtype);
+    return true;
+}
+
+bool elem_aligned(const void *p, Mx4Type t)
+{
+    return (reinterpret_cast<uintptr_t>(p) & (t == kMx4F32 ? 3u : 1u)) == 0;
+}
+
+// The codes and scales of one operand.
+bool check_mx4(const char *who, const uint8_t *codes, const uint8_t *scales)
+{
+    if (!codes || !scales)
+        return fail(std::string(who) + ": null pointer");
+    if ((reinterpret_cast<uintptr_t>(codes) & 15u) || (reinterpret_cast<uintptr_t>(scales) & 3u))
+        return fail(std::string(who) + ": codes must be 16-byte and scales 4-byte aligned");
+    return true;
+}
+
+// Rows of K elements ld apart, packed or unpacked.
+bool check_mx4_rows(const char *who, const void *x, int64_t ld, int dtype, const uint8_t *codes,
+                    const uint8_t *scales, int64_t rows, int K, Mx4Type &t)
+{
+    const std::string w(who);
+    if (!mx4_type(who, dtype, t))
+        return false;
+    if (rows < 0 || K < 0 || K > kMx4MaxDim)
+        return fail(w + ": rows must not be negative, K between 0 and 2^30");
+    if (rows == 0 || K == 0)
+        return true;
+    if (rows > 1 && ld < K)
+        return fail(w + ": row stride shorter than a row");
+    if (!x)
+        return fail(w + ": null pointer");
+    if (!elem_aligned(x, t))
+        return fail(w + ": values must be aligned to their type");
+    return check_mx4(who, codes, scales);
+}
+
+bool check_kv4(const char *who, const Kv4Cache &c, int H_kv, int D, int S_max)
+{
+    if (D != 64 && D != 128)
+        return fail(std::string(who) + ": D must be 64 or 128, got " + std::to_string(D));
+    if (H_kv <= 0 || S_max < 0 || S_max > kMx4MaxDim)
+        return fail(std::string(who) + ": H_kv must be positive, S_max between 0 and 2^30");
+    return S_max == 0 || (check_mx4(who, c.k, c.k_scales) && check_mx4(who, c.v, c.v_scales));
+}
+}  // namespace
+
+bool anima_hip_mx4_pack_dev(const void *x, int64_t ldx, int dtype, uint8_t *codes, uint8_t *scales,
+                            int64_t rows, int K, void *stream)
+{
+    Mx4Type t;
+    if (!check_mx4_rows("mx4_pack_dev", x, ldx, dtype, codes, scales, rows, K, t))
+        return false;
+    if (!ready_for_device_call())
+        return false;
+    return launch_mx4_pack(x, ldx, t, codes, scales, rows, K, pick_stream(stream));
+}
+
+bool anima_hip_mx4_unpack_dev(const uint8_t *codes, const uint8_t *scales, void *x, int64_t ldx,
+                              int dtype, int64_t rows, int K, void *stream)
+{
+    Mx4Type t;
+    if (!check_mx4_rows("mx4_unpack_dev", x, ldx, dtype, codes, scales, rows, K, t))
+        return false;
+    if (!ready_for_device_call())
+        return false;
+    return launch_mx4_unpack(codes, scales, x, ldx, t, rows, K, pick_stream(stream));
+}
+
+size_t anima_hip_linear_mx4_scratch_bytes(int M, int N, int K, int dtype)
+{
+    if (dtype != ANIMA_HIP_DTYPE_F32 && dtype != ANIMA_HIP_DTYPE_BF16)
+        return 0;
+    if (M > kMx4MaxDim || N > kMx4MaxDim || K > kMx4MaxDim)
+        return 0;
+    return linear_mx4_scratch_bytes(M, N, K, Mx4Type(dtype));
+}
+
+bool anima_hip_linear_mx4_dev(const void *a, int64_t lda, const uint8_t *codes,
+                              const uint8_t *scales, void *c, int64_t ldc, int M, int N, int K,
+                              int dtype, void *scratch, size_t scratch_bytes, void *stream)
+{
+    Mx4Type t;
+    if (!mx4_type("linear_mx4_dev", dtype, t))
+        return false;
+    if (M < 0 || N < 0 || K < 0 || M > kMx4MaxDim || N > kMx4MaxDim || K > kMx4MaxDim)
+        return fail("linear_mx4_dev: M, N and K must be between 0 and 2^30");
+    if (M > 0 && N > 0) {
+        if (!c || (K > 0 && !a))
+            return fail("linear_mx4_dev: null pointer");
+        if (!elem_aligned(a, t) || !elem_aligned(c, t))
+            return fail("linear_mx4_dev: a and c must be aligned to their type");
+        if (M > 1 && (lda < K || ldc < N))
+            return fail("linear_mx4_dev: row stride shorter than a row");
+        if (K > 0 && !check_mx4("linear_mx4_dev", codes, scales))
+            return false;
+    }
+    if (!ready_for_device_call())
+        return false;
+    return launch_linear_mx4(a, lda, codes, scales, c, ldc, M, N, K, t, scratch, scratch_bytes,
+                             pick_stream(stream));
+}
+
+bool anima_hip_kv4_append_dev(const void *k, const void *v, int dtype, const int64_t *k_strides,
+                              const int64_t *v_strides, uint8_t *k_codes, uint8_t *k_scales,
+                              uint8_t *v_codes, uint8_t *v_scales, const int32_t *starts,
+                              const int32_t *counts, int B, int S_new, int H_kv, int D, int S_max,
+                              void *stream)
+{
+    Mx4Type t;
+    if (!mx4_type("kv4_append_dev", dtype, t) || !check_dims(B, H_kv, S_new, S_max, D))
+        return false;
+    Kv4Append p;
+    p.cache = Kv4Cache{k_codes, k_scales, v_codes, v_scales};
+    if (!check_kv4("kv4_append_dev", p.cache, H_kv, D, S_max))
+        return false;
+    if (B > 0 && S_new > 0 && S_max > 0) {
+        if (!k || !v || !starts)
+            return fail("kv4_append_dev: null pointer");
+        if (!elem_aligned(k, t) || !elem_aligned(v, t))
+            return fail("kv4_append_dev: k and v must be aligned to their type");
+    }
+    p.ks = from_array(k_strides, H_kv, S_new, D);
+    p.vs = from_array(v_strides, H_kv, S_new, D);
+    p.starts = starts;
+    p.counts = counts;
+    p.B = B;
+    p.S_new = S_new;
+    p.H_kv = H_kv;
+    p.D = D;
+    p.S_max = S_max;
+    if (!ready_for_device_call())
+        return false;
+    if (S_max == 0)
+        return true;
+    return launch_kv4_append(k, v, t, p, pick_stream(stream));
+}
+
+size_t anima_hip_kv4_attention_scratch_bytes(int B, int S_q, int H, int H_kv, int D, int S_max,
+                                             int dtype)
+{
+    if (dtype != ANIMA_HIP_DTYPE_F32 && dtype != ANIMA_HIP_DTYPE_BF16)
+        return 0;
+    return kv4_attention_scratch_bytes(B, S_q, H, H_kv, D, S_max, Mx4Type(dtype));
+}
+
+bool anima_hip_kv4_attention_dev(const void *q, int dtype, const int64_t *q_strides,
+                                 const uint8_t *k_codes, const uint8_t *k_scales,
+                                 const uint8_t *v_codes, const uint8_t *v_scales,
+                                 const int32_t *lens, const int32_t *counts, void *out,
+                                 const int64_t *o_strides, int B, int Bk, int S_q, int H, int H_kv,
+                                 int D, int S_max, float scale, bool is_causal, void *scratch,
+                                 size_t scratch_bytes, void *stream)
+{
+    Mx4Type t;
+    if (!mx4_type("kv4_attention_dev", dtype, t) || !check_dims(B, H, S_q, S_max, D))
+        return false;
+    if (!std::isfinite(scale))
+        return fail("kv4_attention_dev: scale must be finite");
+    Kv4Attention p;
+    p.cache = Kv4Cache{const_cast<uint8_t *>(k_codes), const_cast<uint8_t *>(k_scales),
+                       const_cast<uint8_t *>(v_codes), const_cast<uint8_t *>(v_scales)};
+    if (!check_kv4("kv4_attention_dev", p.cache, H_kv, D, S_max))
+        return false;
+    if (H % H_kv)
+        return fail("kv4_attention_dev: H must be a multiple of H_kv");
+    if (Bk != B && Bk != 1)
+        return fail("kv4_attention_dev: the cache must hold one sequence per batch entry, or one "
+                    "for all");
+    if (int64_t(S_q) * H > kMx4MaxDim)
+        return fail("kv4_attention_dev: S_q * H must be at most 2^30");
+    if (B > 0 && S_q > 0 && H > 0) {
+        if (!q || !out || !lens)
+            return fail("kv4_attention_dev: null pointer");
+        if (!elem_aligned(q, t) || !elem_aligned(out, t))
+            return fail("kv4_attention_dev: q and out must be aligned to their type");
+    }
+    p.q = q;
+    p.o = out;
+    p.qs = from_array(q_strides, H, S_q, D);
+    p.os = from_array(o_strides, H, S_q, D);
+    p.lens = lens;
+    p.counts = counts;
+    p.B = B;
+    p.Bk = Bk;
+    p.S_q = S_q;
+    p.H = H;
+    p.H_kv = H_kv;
+    p.D = D;
+    p.S_max = S_max;
+    p.scale = scale;
+    p.causal = is_causal;
+    p.type = t;
+    if (!ready_for_device_call())
+        return false;
+    return launch_kv4_attention(p, scratch, scratch_bytes, pick_stream(stream));
+}
+
 size_t anima_hip_attention_scratch_bytes(int B, int S_q, int Bk, int S_kv, int H, int D,
                                          int mode)
 {

@@ -459,6 +459,54 @@ bool launch_ln_modulate(const float *x, int64_t ldx, const float *mod, int64_t m
 bool launch_gate_residual(float *x, const float *y, const float *mod, int64_t M, int S, int Dm,
                           hipStream_t st);
 
+// ---- 4-bit rows (MX4: OCP microscaling, e2m1 codes, one e8m0 scale byte per
+// 32 elements; layout in mx4.h) ----
+enum Mx4Type : int { kMx4F32 = 0, kMx4BF16 = 2 };  // ANIMA_HIP_DTYPE_*
+inline int64_t mx4_groups(int K) { return (int64_t(K) + 31) / 32; }
+// Rows of x [rows][ldx] to codes [rows][16 mx4_groups(K)] and scales
+// [rows][mx4_groups(K)], and back (mx4.hip).
+bool launch_mx4_pack(const void *x, int64_t ldx, Mx4Type type, uint8_t *codes, uint8_t *scales,
+                     int64_t rows, int K, hipStream_t st);
+bool launch_mx4_unpack(const uint8_t *codes, const uint8_t *scales, void *x, int64_t ldx,
+                       Mx4Type type, int64_t rows, int K, hipStream_t st);
+// C[M,N] = A[M,K] . W[N,K]^T, W in MX4 rows, A and C both f32 or both bf16
+// (mx4_linear.hip).
+size_t linear_mx4_scratch_bytes(int M, int N, int K, Mx4Type type);
+bool launch_linear_mx4(const void *a, int64_t lda, const uint8_t *codes, const uint8_t *scales,
+                       void *c, int64_t ldc, int M, int N, int K, Mx4Type type, void *scratch,
+                       size_t scratch_bytes, hipStream_t st);
+// A 4-bit K/V cache: MX4 rows of D elements, [Bk][H_kv][S_max].
+struct Kv4Cache {
+    uint8_t *k = nullptr, *k_scales = nullptr, *v = nullptr, *v_scales = nullptr;
+};
+// Rows s < counts[b] (S_new without counts) of k and v [B, H_kv, S_new, D] into
+// cache rows starts[b] + s; rows that fall outside [0, S_max) are left out.
+struct Kv4Append {
+    Kv4Cache cache;
+    Strides ks, vs;
+    const int32_t *starts = nullptr, *counts = nullptr;  // device
+    int B = 0, S_new = 0, H_kv = 0, D = 0, S_max = 0;
+};
+bool launch_kv4_append(const void *k, const void *v, Mx4Type type, const Kv4Append &p,
+                       hipStream_t st);
+// Attention of q [B, H, S_q, D] over the first lens[b] rows of a 4-bit cache
+// (mx4_attention.hip), D 64 or 128, H a multiple of H_kv.
+struct Kv4Attention {
+    Kv4Cache cache;
+    const void *q = nullptr;
+    void *o = nullptr;
+    Strides qs, os;
+    const int32_t *lens = nullptr, *counts = nullptr;  // device
+    int B = 0, Bk = 0, S_q = 0, H = 0, H_kv = 0, D = 0, S_max = 0;
+    float scale = 1.0f;
+    bool causal = false;
+    Mx4Type type = kMx4F32;
+};
+size_t kv4_attention_scratch_bytes(int B, int S_q, int H, int H_kv, int D, int S_max,
+                                   Mx4Type type);
+bool launch_kv4_attention(const Kv4Attention &p, void *scratch, size_t scratch_bytes,
+                          hipStream_t st);
+
 // ---- Element-wise and row operators (ops.hip), device pointers ----
 // GELU (exact erf form), SiLU, LayerNorm without affine over rows of D,
 // softmax over rows of D, and C[i][j] += bias[j] for an M x N matrix.

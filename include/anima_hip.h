@@ -562,6 +562,84 @@ bool anima_hip_dit_euler_dev(anima_hip_dit *dit, float *latent, const float *sig
                              float cfg, int H, int W, const float *freqs, void *scratch,
                              size_t scratch_bytes, void *stream);
 
+/* ---- 4-bit rows (MX4) ----
+ * Linear weights and key/value caches in 4 bits, the OCP microscaling format
+ * with e2m1 elements.  No counterpart in the reference.  Every 32 consecutive
+ * elements of a row share one scale byte s, standing for 2^(s - 127) (255: the
+ * group is NaN); an element is a 4-bit code, sign in bit 3, magnitude 0, 0.5,
+ * 1, 1.5, 2, 3, 4 or 6 in bits 0 to 2.  Byte i of a row's codes holds element
+ * 2i in its low half and element 2i + 1 in its high half.  A row of K elements
+ * takes ceil(K / 32) * 16 bytes of codes, zero past K, and ceil(K / 32) scale
+ * bytes; rows follow one another without gaps.  Codes are 16-byte aligned,
+ * scales 4-byte aligned.  dtype of values and activations:
+ * ANIMA_HIP_DTYPE_F32 or ANIMA_HIP_DTYPE_BF16.  Nothing is allocated; all
+ * entries are asynchronous on `stream` and may be captured into a HIP graph.
+ * Rows and lengths of up to 2^30. */
+
+/* x [rows][ldx] (K elements of each row) to MX4 rows.  With a the largest
+ * magnitude of a group and 2^E <= a < 2^(E+1), its scale byte is E - 2 + 127,
+ * one more where a > 1.75 * 2^E, kept within 2 .. 252; elements round to the
+ * nearest magnitude, ties to the even code, and saturate at 6.  A group that
+ * holds an infinity or a NaN gets scale 255 and zero codes. */
+bool anima_hip_mx4_pack_dev(const void *x, int64_t ldx, int dtype, uint8_t *codes, uint8_t *scales,
+                            int64_t rows, int K, void *stream);
+/* The values of MX4 rows (each is exact in either type).  Also reads back the
+ * caches below, whose rows are MX4 rows of D elements. */
+bool anima_hip_mx4_unpack_dev(const uint8_t *codes, const uint8_t *scales, void *x, int64_t ldx,
+                              int dtype, int64_t rows, int K, void *stream);
+
+/* C[M,N] = A[M,K] . W[N,K]^T with W in MX4 rows (N rows of K) and A, C both of
+ * `dtype`: anima_hip_linear_dev with 4-bit weights.  The weights enter the
+ * product exactly; f32 activations do too (three bf16 terms), sums are f32 and
+ * C is rounded once.  lda, ldc: row strides in elements, any multiple of the
+ * element.  scratch: anima_hip_linear_mx4_scratch_bytes(M, N, K, dtype) bytes,
+ * 16-byte aligned (0: none needed); it holds the partial sums of a product
+ * split over K, added in a fixed order. */
+size_t anima_hip_linear_mx4_scratch_bytes(int M, int N, int K, int dtype);
+bool anima_hip_linear_mx4_dev(const void *a, int64_t lda, const uint8_t *codes,
+                              const uint8_t *scales, void *c, int64_t ldc, int M, int N, int K,
+                              int dtype, void *scratch, size_t scratch_bytes, void *stream);
+
+/* A 4-bit key/value cache is four arrays, K and V codes and scales, each of
+ * MX4 rows of D elements laid out [sequences][H_kv][S_max]; D is 64 or 128.
+ * Append: token s < counts[b] (counts == NULL: S_new) of k and v, views
+ * [B, H_kv, S_new, D] through their strides (NULL: contiguous), is packed as
+ * by anima_hip_mx4_pack_dev into cache row starts[b] + s of sequence b.
+ * starts, counts: int32 [B] on the device.  Rows that would fall outside
+ * [0, S_max) are left out; other cache rows are not touched. */
+bool anima_hip_kv4_append_dev(const void *k, const void *v, int dtype, const int64_t *k_strides,
+                              const int64_t *v_strides, uint8_t *k_codes, uint8_t *k_scales,
+                              uint8_t *v_codes, uint8_t *v_scales, const int32_t *starts,
+                              const int32_t *counts, int B, int S_new, int H_kv, int D, int S_max,
+                              void *stream);
+
+/* Attention over a 4-bit cache: out = softmax(scale * q K^T) V with q and out
+ * views [B, H, S_q, D] of `dtype` through their strides (NULL: contiguous).
+ * H is a multiple of H_kv; query head h reads K/V head h / (H / H_kv).  The
+ * cache holds Bk sequences, one per batch entry or one for all (Bk == 1).
+ * lens: int32 [Bk] on the device, the keys of each sequence (taken into
+ * [0, S_max]), the query tokens' own among them; cache rows from lens on are
+ * not used, whatever they hold.  counts: int32 [B] on the device, the query
+ * tokens of each batch entry, or NULL for S_q; rows of out from counts[b] on
+ * are not written.  is_causal: query token s of n sees the keys up to position
+ * len - n + s, its own; else every query sees all.  A query that sees no key
+ * gives zeros.  Scale bytes as the entries above write them (2 .. 252 and
+ * 255).  K and V enter the products exactly; scores, softmax and sums are f32,
+ * the probabilities enter the second product as bf16 with bf16 queries and
+ * exactly with f32 ones, and out is rounded once.  scratch:
+ * anima_hip_kv4_attention_scratch_bytes() bytes, 16-byte aligned (0: none
+ * needed), for the partial results of a cache whose keys are shared out over
+ * workgroups, joined in a fixed order. */
+size_t anima_hip_kv4_attention_scratch_bytes(int B, int S_q, int H, int H_kv, int D, int S_max,
+                                             int dtype);
+bool anima_hip_kv4_attention_dev(const void *q, int dtype, const int64_t *q_strides,
+                                 const uint8_t *k_codes, const uint8_t *k_scales,
+                                 const uint8_t *v_codes, const uint8_t *v_scales,
+                                 const int32_t *lens, const int32_t *counts, void *out,
+                                 const int64_t *o_strides, int B, int Bk, int S_q, int H, int H_kv,
+                                 int D, int S_max, float scale, bool is_causal, void *scratch,
+                                 size_t scratch_bytes, void *stream);
+
 /* Timing hook: device time of the last completed host-pointer call (the
  * anima_rt_run_* drop-ins, anima_hip_sdpa, anima_hip_attention,
  * anima_hip_cross_attention), from HIP events on the library's streams:
