@@ -9,14 +9,20 @@
 // queries enter as they are and P as one bf16 term; f32 queries and their P
 // enter as three terms each (mx4::terms2), so products are exact to f32.
 //
-// 16 query rows per wave on v_mfma_f32_16x16x32_bf16, the waves of a workgroup
-// and the workgroups of a split sharing the keys.  Bound by the one pass over
-// the cache (17/16 byte per key and dimension for K and V together), or by
-// latency where the cache is short.  Codes go from memory to registers to the
-// MFMA and nothing is staged in LDS: a lane's 16 bytes of a K row are one
-// scale group (the MFMA's k index runs over d in the order the lanes hold it),
-// and V^T fragments are pairs of V rows transposed by two byte permutes per
-// two codes.
+//   * token kernel: 16 query rows per wave on v_mfma_f32_16x16x32_bf16, the
+//     waves of a workgroup and the workgroups of a split sharing the keys.
+//     Bound by the one pass over the cache (17/16 byte per key and dimension
+//     for K and V together), or by latency where the cache is short.  Codes go
+//     from memory to registers to the MFMA and nothing is staged in LDS: a
+//     lane's 16 bytes of a K row are one scale group (the MFMA's k index runs
+//     over d in the order the lanes hold it), and V^T fragments are pairs of
+//     V rows transposed by two byte permutes per two codes.
+//   * tile kernel: many query rows.  Tiles of 64 keys are decoded once per
+//     workgroup of 128 query rows into LDS, K as rows and V transposed, while
+//     the codes of the tile after next are on their way; 32 query rows per wave
+//     on v_mfma_f32_32x32x16_bf16.  Bound by the MFMA and the softmax's VALU
+//     work together (4096 x 512 x 16 heads x 2, bf16: 58 us against 141 us by
+//     the token kernel, 24 us for the MFMAs alone).
 //
 // A masked key never reaches a row: its score is left out of the maximum and
 // the sum, and the decoded V of keys past the cache's length is finite.  Inside
@@ -403,6 +409,330 @@ __global__ __launch_bounds__(kTokWaves * 64) void kv4_token_kernel(AttnArgs a)
         a.ml[split * plane + orow] = float2{jm, jl};
 }
 
+// ------------------------------------------------------------ tile kernel
+
+constexpr int kTileWaves = 4;
+constexpr int kTileRows = 32 * kTileWaves;  // query rows of a workgroup
+constexpr int kTileKeys = 64;
+
+// 16-byte pieces of a staged K row (D / 8 of them) and V^T row (8), placed so
+// that the 16 rows a ds_read_b128 quarter touches lie in distinct banks.
+template <int D>
+__device__ __forceinline__ int k_piece(int row, int piece)
+{
+    return D == 128 ? piece ^ (row & 15) : piece ^ ((row & 7) ^ ((row >> 3) & 1));
+}
+__device__ __forceinline__ int v_piece(int row, int piece)
+{
+    return piece ^ ((row & 7) ^ ((row >> 3) & 1));
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(kTileWaves * 64, 2) void kv4_tile_kernel(AttnArgs a)
+{
+    constexpr int NT = kTerms<T>;
+    constexpr int GROUPS = D / 32;
+    constexpr int DB = D / 32;           // V^T blocks of 32 dimensions
+    constexpr int KSTEPS = D / 16;       // MFMA steps of a score
+    constexpr int KV_EL = kTileKeys * D;  // elements of a staged K or V^T tile
+    constexpr int VD = D / 16;           // dimensions of V a thread decodes, of 4 keys
+    __shared__ __attribute__((aligned(16))) u16 smem[4 * KV_EL];
+    __shared__ int nan_tile[2];
+
+    const Kv4Attention &p = a.p;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 31, half = lane >> 5;
+    const int blk = xcd_major_block();
+    const int split = blk % a.splits;
+    // Under a causal mask the last query tiles are the longest: they go first.
+    const int tile = a.tiles - 1 - (blk / a.splits) % a.tiles;
+    const int bh = (blk / a.splits) / a.tiles;
+    const int b = bh / p.H_kv, hk = bh - b * p.H_kv;
+    const Seq seq(p, b, hk);
+
+    // This lane's query row: column col of the accumulators.
+    const int row = tile * kTileRows + wave * 32 + col;
+    const int s = row / a.group, hq = hk * a.group + (row - s * a.group);
+    const bool live = row < a.rows && s < seq.nq;
+    const int limit = live ? seq.limit(p, s) : 0;
+    int most = limit, least = live ? limit : INT32_MAX;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        most = max(most, __shfl_xor(most, o));
+        least = min(least, __shfl_xor(least, o));
+    }
+    most = __builtin_amdgcn_readfirstlane(most);
+    least = __builtin_amdgcn_readfirstlane(least);
+    // Keys that any row of the workgroup sees: those of its last live row.
+    const int s_last = min((min((tile + 1) * kTileRows, a.rows) - 1) / a.group, seq.nq - 1);
+    const int wg_most = s_last >= (tile * kTileRows) / a.group ? seq.limit(p, s_last) : 0;
+    const int steps = (wg_most + kTileKeys - 1) / kTileKeys;
+    const int per = (steps + a.splits - 1) / a.splits;
+    const int first = min(split * per, steps), end = min(first + per, steps);
+
+    // Scores are kept unscaled; the sign of the scale goes into the queries.
+    const float scale2 = fabsf(a.scale2);
+    const unsigned flip = a.scale2 < 0.0f ? 0x80008000u : 0u;
+    bf16x8 qf[KSTEPS][NT];
+    {
+        const T *q = static_cast<const T *>(p.q);
+        const bool ok = live && limit > 0;
+        const T *qr = ok ? q + b * p.qs.b + hq * p.qs.h + s * p.qs.s : nullptr;
+        const bool wide = ((reinterpret_cast<uintptr_t>(q) & 15) |
+                           ((p.qs.b | p.qs.h | p.qs.s) & 7)) == 0;
+#pragma unroll
+        for (int ks = 0; ks < KSTEPS; ++ks) {
+            if (ok)
+                q_terms(qr + 16 * ks + 8 * half, wide, qf[ks]);
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+                qf[ks][j] = ok ? __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, qf[ks][j]) ^
+                                                                flip)
+                               : __builtin_bit_cast(bf16x8, u32x4{0, 0, 0, 0});
+        }
+    }
+
+    // What this thread decodes of a tile: D / 4 codes of one key's K, and V of
+    // the four keys 4 va .. 4 va + 3 in VD dimensions.
+    const int kt = tid >> 2, kpart = tid & 3;
+    const int va = tid & 15, vd = tid >> 4;
+    const int last = max(seq.len - 1, 0);
+    unsigned kc[D / 32], kscale, vc[4], vscale[4];
+    auto load = [&](int j) {
+        const int t0 = j * kTileKeys;
+        {
+            const int64_t r = seq.kv_row + min(t0 + kt, last);
+            const uint8_t *src = p.cache.k + r * (D / 2) + kpart * (D / 8);
+            if constexpr (D == 128) {
+                const u32x4 w = *reinterpret_cast<const u32x4 *>(src);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    kc[i] = w[i];
+            } else {
+                const u32x2 w = *reinterpret_cast<const u32x2 *>(src);
+                kc[0] = w[0];
+                kc[1] = w[1];
+            }
+            kscale = p.cache.k_scales[r * GROUPS + kpart * GROUPS / 4];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int64_t r = seq.kv_row + min(t0 + 4 * va + i, last);
+            const uint8_t *src = p.cache.v + r * (D / 2) + vd * (D / 32);
+            if constexpr (D == 128)
+                vc[i] = *reinterpret_cast<const unsigned *>(src);
+            else
+                vc[i] = *reinterpret_cast<const uint16_t *>(src);
+            vscale[i] = p.cache.v_scales[r * GROUPS + vd * GROUPS / 16];
+        }
+    };
+    // Quad va of keys within its row of 64: groups of 16 keys hold their quads
+    // in the order 0, 2, 1, 3, so that 16 bytes are the eight keys a lane half
+    // holds in its accumulator registers.
+    const int vq = va & 3;
+    const int vpiece = 2 * (va >> 2) + (vq & 1), vsub = vq >> 1;
+    auto store = [&](int j, int stage) {
+        unsigned ko = stage * KV_EL + kt * D + k_piece<D>(kt, kpart * (D / 32)) * 8;
+        unsigned vo = (2 + stage) * KV_EL + vd * VD * kTileKeys + v_piece(vd * VD, vpiece) * 8 +
+                      4 * vsub;
+        asm volatile("" : "+v"(ko), "+v"(vo));
+        const float ks = scale_of(kscale);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i)
+            *reinterpret_cast<bf16x8 *>(smem + (ko ^ 8 * i)) = decode8(kc[i], ks);
+        bool nan = false;
+        float vs[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const bool bad = vscale[i] == unsigned(mx4::kNanScale);
+            nan = nan || bad;
+            vs[i] = scale_of(bad ? 0u : vscale[i]);
+        }
+#pragma unroll
+        for (int c = 0; c < VD / 2; ++c) {
+            u32x2 even, odd;
+#pragma unroll
+            for (int jj = 0; jj < 2; ++jj) {
+                const unsigned x0 = decode2_at(vc[2 * jj], vs[2 * jj], c);
+                const unsigned x1 = decode2_at(vc[2 * jj + 1], vs[2 * jj + 1], c);
+                even[jj] = __builtin_amdgcn_perm(x1, x0, 0x05040100);
+                odd[jj] = __builtin_amdgcn_perm(x1, x0, 0x07060302);
+            }
+            // Rows vd * VD + 2 c and + 1: the swizzle's low bits are the row's.
+            *reinterpret_cast<u32x2 *>(smem + 2 * c * kTileKeys + (vo ^ 8 * (2 * c))) = even;
+            *reinterpret_cast<u32x2 *>(smem + (2 * c + 1) * kTileKeys + (vo ^ 8 * (2 * c + 1))) =
+                odd;
+        }
+        if (nan)
+            nan_tile[stage] = j;
+    };
+
+    f32x16 o[DB];
+#pragma unroll
+    for (int i = 0; i < DB; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+            o[i][r] = 0.0f;
+    float mx = -INFINITY, sum = 0.0f;
+
+    auto compute = [&](int j, int stage, auto masked) {
+        constexpr bool MASK = decltype(masked)::value;
+        const int t0 = j * kTileKeys;
+        // Offsets of this lane's rows with its half's first piece; the other
+        // pieces differ in bits that the row's start leaves clear.  Recomputed
+        // per tile: kept in registers for every piece they would spill.
+        unsigned ko = stage * KV_EL + col * D + k_piece<D>(col, half) * 8;
+        unsigned vo = (2 + stage) * KV_EL + col * kTileKeys + v_piece(col, half) * 8;
+        asm volatile("" : "+v"(ko), "+v"(vo));
+        f32x16 sc[2];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                sc[kb][r] = 0.0f;
+            asm volatile("" ::: "memory");
+#pragma unroll
+            for (int ks = 0; ks < KSTEPS; ++ks) {
+                const bf16x8 kf =
+                    *reinterpret_cast<const bf16x8 *>(smem + 32 * kb * D + (ko ^ 16 * ks));
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+                    sc[kb] = mfma_bf16(kf, qf[ks][t], sc[kb]);
+            }
+        }
+        // Key of register r of block kb: t0 + 32 kb + acc_row(r, half).
+        const int room = limit - t0 - 4 * half;
+        float mt = -INFINITY;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (!MASK || 32 * kb + 8 * (r >> 2) + (r & 3) < room)
+                    mt = fmaxf(mt, sc[kb][r]);
+        mt = row_pair_max(mt);
+        // The maximum moves when a row has none yet or is 2^8 behind: until
+        // then probabilities stay below 2^8 and nothing is rescaled.
+        const bool move = mx == -INFINITY ? mt > mx : (mt - mx) * scale2 > kRescaleLog2;
+        if (__builtin_amdgcn_ballot_w64(move) != 0) {
+            const float mn = move ? mt : mx;
+            const float alpha = mx == mn || mx == -INFINITY
+                                    ? 1.0f
+                                    : __builtin_amdgcn_exp2f((mx - mn) * scale2);
+            mx = mn;
+            sum *= alpha;
+#pragma unroll
+            for (int i = 0; i < DB; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    o[i][r] *= alpha;
+        }
+        const float m2 = mx * scale2;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                // bf16 queries: one fused operation, off by a rounding of the
+                // scaled maximum, far below P's own rounding.
+                const float e = NT == 1 ? __builtin_fmaf(sc[kb][r], scale2, -m2)
+                                        : (sc[kb][r] - mx) * scale2;
+                const float pr = __builtin_amdgcn_exp2f(e);
+                sc[kb][r] = !MASK || 32 * kb + 8 * (r >> 2) + (r & 3) < room ? pr : 0.0f;
+            }
+#pragma unroll
+        for (int kg = 0; kg < 4; ++kg) {
+            bf16x8 pf[NT];
+            asm volatile("" ::: "memory");
+            if constexpr (NT == 1) {
+                pf[0] = pack8(sc[kg >> 1], 8 * (kg & 1));
+                sum = row_sum8(pf[0], sum);
+            } else {
+                float pr[8];
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    pr[r] = sc[kg >> 1][8 * (kg & 1) + r];
+                    sum += pr[r];
+                }
+                p_terms(pr, pf);
+            }
+#pragma unroll
+            for (int i = 0; i < DB; ++i) {
+                const bf16x8 vf = *reinterpret_cast<const bf16x8 *>(
+                    smem + 32 * i * kTileKeys + (vo ^ 16 * kg));
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+                    o[i] = mfma_bf16(vf, pf[t], o[i]);
+            }
+        }
+        if (nan_tile[stage] == j) {
+            // NaN groups of V, decoded as zero: to the rows that see their keys.
+            for (int t = t0; t < min(t0 + kTileKeys, seq.len); ++t)
+#pragma unroll
+                for (int i = 0; i < DB; ++i)
+                    if (p.cache.v_scales[(seq.kv_row + t) * GROUPS + i] == mx4::kNanScale &&
+                        t < limit)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r)
+                            o[i][r] = NAN;
+        }
+    };
+
+    if (tid < 2)
+        nan_tile[tid] = -1;
+    __syncthreads();
+    if (first < end) {
+        load(first);
+        store(first, 0);
+        if (first + 1 < end)
+            load(first + 1);
+    }
+    __syncthreads();
+    for (int j = first; j < end; ++j) {
+        const int stage = (j - first) & 1;
+        if (j + 1 < end) {
+            store(j + 1, stage ^ 1);
+            if (j + 2 < end)
+                load(j + 2);
+        }
+        if (j * kTileKeys < most) {
+            if ((j + 1) * kTileKeys <= least)
+                compute(j, stage, std::false_type{});
+            else
+                compute(j, stage, std::true_type{});
+        }
+        __syncthreads();
+    }
+
+    // Row sums over the two halves; then O through LDS, rows of D values.
+    sum += __shfl_xor(sum, 32);
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const int64_t plane = int64_t(p.B) * p.S_q * p.H;
+    if (a.splits > 1) {
+        if (live) {
+            const int64_t at = split * plane + (int64_t(b) * p.S_q + s) * p.H + hq;
+            float *dst = a.part + at * D;
+#pragma unroll
+            for (int i = 0; i < DB; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4)
+                    *reinterpret_cast<f32x4 *>(dst + 32 * i + acc_row(r, half)) =
+                        f32x4{o[i][r] * inv, o[i][r + 1] * inv, o[i][r + 2] * inv,
+                              o[i][r + 3] * inv};
+            if (half == 0)
+                a.ml[at] = float2{mx * scale2, sum};
+        }
+        return;
+    }
+    if (!live)
+        return;
+    T *out = static_cast<T *>(p.o) + b * p.os.b + hq * p.os.h + s * p.os.s;
+#pragma unroll
+    for (int i = 0; i < DB; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+            store_o(out + 32 * i + acc_row(r, half), o[i][r] * inv);
+}
+
 // O = sum_s w_s P_s / sum_s w_s, w_s = l_s 2^(m_s - max m), over the splits
 // that saw a key.
 template <typename T>
@@ -437,6 +767,7 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(AttnArgs a)
 }
 
 struct Plan {
+    bool tile;  // the tile kernel
     int tiles, splits;
 };
 
@@ -444,12 +775,16 @@ Plan plan_of(int B, int S_q, int H, int H_kv, int S_max)
 {
     const int64_t rows = int64_t(S_q) * (H / H_kv);
     Plan pl;
-    pl.tiles = int((rows + kTokRows - 1) / kTokRows);
+    pl.tile = rows > 32;
+    const int per_tile = pl.tile ? kTileRows : kTokRows;
+    pl.tiles = int((rows + per_tile - 1) / per_tile);
     const int64_t groups = std::max<int64_t>(1, int64_t(B) * H_kv * pl.tiles);
-    // A workgroup's waves take 32 keys each at a time; splits until the grid
-    // has about four workgroups per CU or a share is one round.
-    const int64_t rounds = (int64_t(S_max) + kTokKeys * kTokWaves - 1) / (kTokKeys * kTokWaves);
-    pl.splits = int(std::max<int64_t>(1, std::min<int64_t>({1024 / groups, rounds, 64})));
+    // Splits until the grid has two (tiles) or about four workgroups per CU,
+    // or a share is two tiles of keys, or one round of a workgroup's waves.
+    const int round = pl.tile ? 2 * kTileKeys : kTokKeys * kTokWaves;
+    const int64_t rounds = (int64_t(S_max) + round - 1) / round;
+    pl.splits = int(std::max<int64_t>(
+        1, std::min<int64_t>({(pl.tile ? 512 : 1024) / groups, rounds, 64})));
     return pl;
 }
 
@@ -459,15 +794,19 @@ int64_t part_bytes(int B, int S_q, int H, int D, int splits)
 }
 
 template <typename T, int D>
-bool run_attention_kv4(AttnArgs &a, hipStream_t st)
+bool run_attention_kv4(AttnArgs &a, bool tile, hipStream_t st)
 {
     const int64_t blocks = int64_t(a.p.B) * a.p.H_kv * a.tiles * a.splits;
     const int64_t elems = int64_t(a.p.B) * a.p.S_q * a.p.H * D;
     if (blocks > INT32_MAX || (elems + 255) / 256 > INT32_MAX)
         return fail("kv4_attention_dev: too many query rows");
-    hipLaunchKernelGGL((kv4_token_kernel<T, D>), dim3(unsigned(blocks)), dim3(kTokWaves * 64), 0,
-                       st, a);
-    if (!hip_ok(hipGetLastError(), "kv4_token_kernel launch"))
+    if (tile)
+        hipLaunchKernelGGL((kv4_tile_kernel<T, D>), dim3(unsigned(blocks)), dim3(kTileWaves * 64),
+                           0, st, a);
+    else
+        hipLaunchKernelGGL((kv4_token_kernel<T, D>), dim3(unsigned(blocks)), dim3(kTokWaves * 64),
+                           0, st, a);
+    if (!hip_ok(hipGetLastError(), "kv4 attention launch"))
         return false;
     if (a.splits == 1)
         return true;
@@ -511,10 +850,10 @@ bool launch_kv4_attention(const Kv4Attention &p, void *scratch, size_t scratch_b
         a.ml = reinterpret_cast<float2 *>(a.part + int64_t(p.B) * p.S_q * p.H * pl.splits * p.D);
     }
     if (p.type == kMx4F32)
-        return p.D == 128 ? run_attention_kv4<float, 128>(a, st)
-                          : run_attention_kv4<float, 64>(a, st);
-    return p.D == 128 ? run_attention_kv4<uint16_t, 128>(a, st)
-                      : run_attention_kv4<uint16_t, 64>(a, st);
+        return p.D == 128 ? run_attention_kv4<float, 128>(a, pl.tile, st)
+                          : run_attention_kv4<float, 64>(a, pl.tile, st);
+    return p.D == 128 ? run_attention_kv4<uint16_t, 128>(a, pl.tile, st)
+                      : run_attention_kv4<uint16_t, 64>(a, pl.tile, st);
 }
 
 }  // namespace anima_hip
