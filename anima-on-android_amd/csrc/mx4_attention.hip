@@ -59,6 +59,23 @@ __device__ __forceinline__ void store_o(uint16_t *o, float v)
     *o = __builtin_bit_cast(uint16_t, b);
 }
 
+// Max over the four lanes n, n + 16, n + 32, n + 48 of a query.
+__device__ __forceinline__ float quad_max(float v)
+{
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                                    false);
+    return row_pair_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+
+// The argument of a probability's exponential.  bf16 queries: one fused
+// operation, off by a rounding of the scaled maximum, far below the rounding
+// of P; f32 queries: the maximum's own probability is exactly 1.
+template <int NT>
+__device__ __forceinline__ float exponent(float score, float mx, float scale2, float m2)
+{
+    return NT == 1 ? __builtin_fmaf(score, scale2, -m2) : (score - mx) * scale2;
+}
+
 struct AttnArgs {
     Kv4Attention p;
     float scale2;   // softmax scale * log2(e)
@@ -88,8 +105,8 @@ struct Seq {
     }
 };
 
-// A query row's eight values from d as bf16 terms.
-__device__ __forceinline__ void q_terms(const uint16_t *q, bool wide, bf16x8 (&t)[1])
+// A query row's eight values from d as bf16 terms, negated or not.
+__device__ __forceinline__ void q_terms(const uint16_t *q, bool wide, bool neg, bf16x8 (&t)[1])
 {
     u32x4 u;
     if (wide)
@@ -99,16 +116,16 @@ __device__ __forceinline__ void q_terms(const uint16_t *q, bool wide, bf16x8 (&t
         for (int i = 0; i < 4; ++i)
             u[i] = unsigned(q[2 * i]) | unsigned(q[2 * i + 1]) << 16;
     }
-    t[0] = __builtin_bit_cast(bf16x8, u);
+    t[0] = __builtin_bit_cast(bf16x8, neg ? u ^ 0x80008000u : u);
 }
 
-__device__ __forceinline__ void q_terms(const float *q, bool, bf16x8 (&t)[3])
+__device__ __forceinline__ void terms8(const float (&x)[8], bf16x8 (&t)[3])
 {
     u32x4 u[3];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         unsigned w[3];
-        terms2<3>(q[2 * i], q[2 * i + 1], w);
+        terms2<3>(x[2 * i], x[2 * i + 1], w);
 #pragma unroll
         for (int j = 0; j < 3; ++j)
             u[j][i] = w[j];
@@ -116,6 +133,15 @@ __device__ __forceinline__ void q_terms(const float *q, bool, bf16x8 (&t)[3])
 #pragma unroll
     for (int j = 0; j < 3; ++j)
         t[j] = __builtin_bit_cast(bf16x8, u[j]);
+}
+
+__device__ __forceinline__ void q_terms(const float *q, bool, bool neg, bf16x8 (&t)[3])
+{
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        x[i] = neg ? -q[i] : q[i];
+    terms8(x, t);
 }
 
 // Eight probabilities as the P operand: one rounded term or three exact ones.
@@ -130,7 +156,7 @@ __device__ __forceinline__ void p_terms(const float (&p)[8], bf16x8 (&t)[1])
 }
 __device__ __forceinline__ void p_terms(const float (&p)[8], bf16x8 (&t)[3])
 {
-    q_terms(p, true, t);
+    terms8(p, t);
 }
 
 // ----------------------------------------------------------- token kernel
@@ -141,54 +167,65 @@ constexpr int kTokWaves = 4;
 
 // A wave's loads for 32 keys.  Lane (m, g): K rows t0 + m and t0 + 16 + m,
 // dimensions g * D/4 .. ; V rows of the eight keys 4g + 0..3 and 16 + 4g +
-// 0..3, dimensions m * D/16 .. .
+// 0..3, dimensions m * D/16 .. .  Addresses are a base of the wave plus an
+// offset of the lane that stays the same from step to step.
 template <int D>
 struct TokLoads {
     static constexpr int GROUPS = D / 32;
-    static constexpr int KW = D / 32;  // words of K codes per key and lane: D/4 codes
-    unsigned kc[2][KW];
+    static constexpr int ROW = D / 2;  // bytes of a row's codes
+    unsigned kc[2][D / 32];
     unsigned ks[2];
     unsigned vc[8];
     unsigned vs[8];
 
-    template <bool TAIL>
-    __device__ __forceinline__ void load(const Kv4Cache &c, int64_t row0, int t0, int last, int m,
-                                         int g)
+    __device__ __forceinline__ void load_k(const uint8_t *codes, const uint8_t *scales, int h,
+                                           unsigned key, unsigned g)
     {
+        const uint8_t *src = codes + key * ROW + g * (D / 8);
+        if constexpr (D == 128) {
+            const u32x4 w = *reinterpret_cast<const u32x4 *>(src);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                kc[h][i] = w[i];
+        } else {
+            const u32x2 w = *reinterpret_cast<const u32x2 *>(src);
+            kc[h][0] = w[0];
+            kc[h][1] = w[1];
+        }
+        ks[h] = scales[key * GROUPS + g * GROUPS / 4];
+    }
+    __device__ __forceinline__ void load_v(const uint8_t *codes, const uint8_t *scales, int j,
+                                           unsigned key, unsigned m)
+    {
+        const uint8_t *src = codes + key * ROW + m * (D / 32);
+        if constexpr (D == 128)
+            vc[j] = *reinterpret_cast<const unsigned *>(src);
+        else
+            vc[j] = *reinterpret_cast<const uint16_t *>(src);
+        vs[j] = scales[key * GROUPS + m * GROUPS / 16];
+    }
+    // Keys row .. row + 31 of the cache; past row + over, that key again.
+    template <bool TAIL>
+    __device__ __forceinline__ void load(const Kv4Cache &c, int64_t row, unsigned over, unsigned m,
+                                         unsigned g)
+    {
+        const uint8_t *kc0 = c.k + row * ROW, *ks0 = c.k_scales + row * GROUPS;
+        const uint8_t *vc0 = c.v + row * ROW, *vs0 = c.v_scales + row * GROUPS;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const int t = TAIL ? min(t0 + 16 * h + m, last) : t0 + 16 * h + m;
-            const int64_t row = row0 + t;
-            const uint8_t *src = c.k + row * (D / 2) + g * (D / 8);
-            if constexpr (D == 128) {
-                const u32x4 w = *reinterpret_cast<const u32x4 *>(src);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    kc[h][i] = w[i];
-            } else {
-                const u32x2 w = *reinterpret_cast<const u32x2 *>(src);
-                kc[h][0] = w[0];
-                kc[h][1] = w[1];
-            }
-            ks[h] = c.k_scales[row * GROUPS + g * GROUPS / 4];
+            const unsigned key = 16 * h + m;
+            load_k(kc0, ks0, h, TAIL ? min(key, over) : key, g);
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const int key = 16 * (j >> 2) + 4 * g + (j & 3);
-            const int t = TAIL ? min(t0 + key, last) : t0 + key;
-            const int64_t row = row0 + t;
-            const uint8_t *src = c.v + row * (D / 2) + m * (D / 32);
-            if constexpr (D == 128)
-                vc[j] = *reinterpret_cast<const unsigned *>(src);
-            else
-                vc[j] = *reinterpret_cast<const uint16_t *>(src);
-            vs[j] = c.v_scales[row * GROUPS + m * GROUPS / 16];
+            const unsigned key = 16 * (j >> 2) + 4 * g + (j & 3);
+            load_v(vc0, vs0, j, TAIL ? min(key, over) : key, m);
         }
     }
 };
 
 template <typename T, int D>
-__global__ __launch_bounds__(kTokWaves * 64) void kv4_token_kernel(AttnArgs a)
+__global__ __launch_bounds__(kTokWaves * 64, 2) void kv4_token_kernel(AttnArgs a)
 {
     constexpr int NT = kTerms<T>;
     constexpr int STEPS = D / 32;  // MFMA steps of a score; V^T blocks of 16 are D / 16
@@ -206,11 +243,25 @@ __global__ __launch_bounds__(kTokWaves * 64) void kv4_token_kernel(AttnArgs a)
     const int tile = (blk / a.splits) % a.tiles;
     const int bh = (blk / a.splits) / a.tiles;
     const int b = bh / p.H_kv, hk = bh - b * p.H_kv;
-    const Seq seq(p, b, hk);
 
-    // This lane's query row (column n of the accumulators).
+    // This lane's query row (column n of the accumulators).  Rows past the last
+    // read that one and are not written; a column's values stay its own.
     const int row = tile * kTokRows + n;
-    const int s = row / a.group, hq = hk * a.group + (row - s * a.group);
+    const int rc = min(row, a.rows - 1);
+    const int s = rc / a.group, hq = hk * a.group + (rc - s * a.group);
+    // Scores are kept unscaled; the sign of the scale goes into the queries.
+    const float scale2 = fabsf(a.scale2);
+    bf16x8 qf[STEPS][NT];
+    {
+        const T *q = static_cast<const T *>(p.q);
+        const T *qr = q + b * p.qs.b + hq * p.qs.h + s * p.qs.s;
+        const bool wide = ((reinterpret_cast<uintptr_t>(q) & 15) |
+                           ((p.qs.b | p.qs.h | p.qs.s) & 7)) == 0;
+#pragma unroll
+        for (int st = 0; st < STEPS; ++st)
+            q_terms(qr + g * (D / 4) + 8 * st, wide, a.scale2 < 0.0f, qf[st]);
+    }
+    const Seq seq(p, b, hk);
     const bool live = row < a.rows && s < seq.nq;
     const int limit = live ? seq.limit(p, s) : 0;
     // Keys any row of the tile sees, and keys all of its live rows see.
@@ -227,24 +278,6 @@ __global__ __launch_bounds__(kTokWaves * 64) void kv4_token_kernel(AttnArgs a)
     const int steps = (most + kTokKeys - 1) / kTokKeys;
     const int per = (steps + a.splits - 1) / a.splits;
     const int first = split * per, end = min(first + per, steps);
-
-    bf16x8 qf[STEPS][NT];
-    {
-        const T *q = static_cast<const T *>(p.q);
-        const bool ok = live && limit > 0;
-        const T *qr = ok ? q + b * p.qs.b + hq * p.qs.h + s * p.qs.s : nullptr;
-        const bool wide = ((reinterpret_cast<uintptr_t>(q) & 15) |
-                           ((p.qs.b | p.qs.h | p.qs.s) & 7)) == 0;
-#pragma unroll
-        for (int st = 0; st < STEPS; ++st) {
-            if (ok)
-                q_terms(qr + g * (D / 4) + 8 * st, wide, qf[st]);
-            else
-#pragma unroll
-                for (int j = 0; j < NT; ++j)
-                    qf[st][j] = __builtin_bit_cast(bf16x8, u32x4{0, 0, 0, 0});
-        }
-    }
 
     f32x4 o[VB];
 #pragma unroll
@@ -269,28 +302,40 @@ __global__ __launch_bounds__(kTokWaves * 64) void kv4_token_kernel(AttnArgs a)
             }
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-                sc[4 * h + r] = acc[r] * a.scale2;
+                sc[4 * h + r] = acc[r];
         }
+        const int room = limit - t0 - 4 * g;  // keys 16 h + r below it are seen
         float mt = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (!MASK || t0 + 16 * (i >> 2) + 4 * g + (i & 3) < limit)
+        for (int i = 0; i < 8; ++i)
+            if (!MASK || 16 * (i >> 2) + (i & 3) < room)
                 mt = fmaxf(mt, sc[i]);
+        mt = quad_max(mt);
+        // The maximum moves when a row has none yet or is 2^8 behind: until
+        // then probabilities stay below 2^8 and nothing is rescaled.
+        const bool move = mx == -INFINITY ? mt > mx : (mt - mx) * scale2 > kRescaleLog2;
+        if (__builtin_amdgcn_ballot_w64(move) != 0) {
+            const float mn = move ? mt : mx;
+            const float alpha = mx == mn || mx == -INFINITY
+                                    ? 1.0f
+                                    : __builtin_amdgcn_exp2f((mx - mn) * scale2);
+            mx = mn;
+            sum *= alpha;
+#pragma unroll
+            for (int i = 0; i < VB; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    o[i][r] *= alpha;
         }
-        mt = fmaxf(mt, __shfl_xor(mt, 16));
-        mt = fmaxf(mt, __shfl_xor(mt, 32));
-        const float mn = fmaxf(mx, mt);
-        // No key seen yet (or all scores -inf): nothing to rescale.
-        const float alpha = mx == mn ? 1.0f : __builtin_amdgcn_exp2f(mx - mn);
-        mx = mn;
-        float pr[8], ps = 0.0f;
+        const float m2 = mx * scale2;
+        float pr[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const bool seen = !MASK || t0 + 16 * (i >> 2) + 4 * g + (i & 3) < limit;
-            pr[i] = seen ? __builtin_amdgcn_exp2f(sc[i] - mn) : 0.0f;
-            ps += pr[i];
+            pr[i] = __builtin_amdgcn_exp2f(exponent<NT>(sc[i], mx, scale2, m2));
+            if (MASK && 16 * (i >> 2) + (i & 3) >= room)
+                pr[i] = 0.0f;
+            sum += pr[i];
         }
-        sum = sum * alpha + ps;
         bf16x8 pf[NT];
         p_terms(pr, pf);
         float vsc[8];
@@ -304,11 +349,6 @@ __global__ __launch_bounds__(kTokWaves * 64) void kv4_token_kernel(AttnArgs a)
             }
             vsc[j] = scale_of(byte);
         }
-#pragma unroll
-        for (int i = 0; i < VB; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                o[i][r] *= alpha;
         // V^T blocks 2c and 2c + 1: dimensions m * VB + 2c and + 2c + 1 of keys j.
 #pragma unroll
         for (int c = 0; c < VB / 2; ++c) {
@@ -348,17 +388,31 @@ __global__ __launch_bounds__(kTokWaves * 64) void kv4_token_kernel(AttnArgs a)
         }
     };
 
-    const int last = max(seq.len - 1, 0);
-    for (int i = first + wave; i < end; i += kTokWaves) {
+    auto load = [&](TokLoads<D> &ld, int i) {
         const int t0 = i * kTokKeys;
-        TokLoads<D> ld;
-        if (t0 + kTokKeys <= least) {
-            ld.template load<false>(p.cache, seq.kv_row, t0, last, n, g);
-            step(ld, t0, std::false_type{});
-        } else {
-            ld.template load<true>(p.cache, seq.kv_row, t0, last, n, g);
-            step(ld, t0, std::true_type{});
-        }
+        const int64_t at = seq.kv_row + t0;
+        if (t0 + kTokKeys <= seq.len)
+            ld.template load<false>(p.cache, at, 0, n, g);
+        else
+            ld.template load<true>(p.cache, at, unsigned(seq.len - 1 - t0), n, g);
+    };
+    // The next step's codes are on their way while this one's are used.  Steps
+    // that every row sees whole come first.
+    TokLoads<D> cur, next;
+    int i = first + wave;
+    if (i < end)
+        load(cur, i);
+    for (; i < end && (i + 1) * kTokKeys <= least; i += kTokWaves) {
+        if (i + kTokWaves < end)
+            load(next, i + kTokWaves);
+        step(cur, i * kTokKeys, std::false_type{});
+        cur = next;
+    }
+    for (; i < end; i += kTokWaves) {
+        if (i + kTokWaves < end)
+            load(next, i + kTokWaves);
+        step(cur, i * kTokKeys, std::true_type{});
+        cur = next;
     }
 
     // Join the waves.  Lane (n, g) holds O^T rows d = (4 g + r) * VB + i of query n.
@@ -370,7 +424,7 @@ __global__ __launch_bounds__(kTokWaves * 64) void kv4_token_kernel(AttnArgs a)
         for (int i = 0; i < VB; ++i)
             so[wave][n][(4 * g + r) * VB + i] = o[i][r];
     if (g == 0) {
-        sm[wave][n] = mx;
+        sm[wave][n] = mx * scale2;
         sl[wave][n] = sum;
     }
     __syncthreads();
@@ -451,9 +505,11 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void kv4_tile_kernel(AttnArgs a
     const int b = bh / p.H_kv, hk = bh - b * p.H_kv;
     const Seq seq(p, b, hk);
 
-    // This lane's query row: column col of the accumulators.
+    // This lane's query row: column col of the accumulators.  Rows past the
+    // last read that one and are not written.
     const int row = tile * kTileRows + wave * 32 + col;
-    const int s = row / a.group, hq = hk * a.group + (row - s * a.group);
+    const int rc = min(row, a.rows - 1);
+    const int s = rc / a.group, hq = hk * a.group + (rc - s * a.group);
     const bool live = row < a.rows && s < seq.nq;
     const int limit = live ? seq.limit(p, s) : 0;
     int most = limit, least = live ? limit : INT32_MAX;
@@ -473,24 +529,15 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void kv4_tile_kernel(AttnArgs a
 
     // Scores are kept unscaled; the sign of the scale goes into the queries.
     const float scale2 = fabsf(a.scale2);
-    const unsigned flip = a.scale2 < 0.0f ? 0x80008000u : 0u;
     bf16x8 qf[KSTEPS][NT];
     {
         const T *q = static_cast<const T *>(p.q);
-        const bool ok = live && limit > 0;
-        const T *qr = ok ? q + b * p.qs.b + hq * p.qs.h + s * p.qs.s : nullptr;
+        const T *qr = q + b * p.qs.b + hq * p.qs.h + s * p.qs.s;
         const bool wide = ((reinterpret_cast<uintptr_t>(q) & 15) |
                            ((p.qs.b | p.qs.h | p.qs.s) & 7)) == 0;
 #pragma unroll
-        for (int ks = 0; ks < KSTEPS; ++ks) {
-            if (ok)
-                q_terms(qr + 16 * ks + 8 * half, wide, qf[ks]);
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
-                qf[ks][j] = ok ? __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, qf[ks][j]) ^
-                                                                flip)
-                               : __builtin_bit_cast(bf16x8, u32x4{0, 0, 0, 0});
-        }
+        for (int ks = 0; ks < KSTEPS; ++ks)
+            q_terms(qr + 16 * ks + 8 * half, wide, a.scale2 < 0.0f, qf[ks]);
     }
 
     // What this thread decodes of a tile: D / 4 codes of one key's K, and V of
@@ -632,11 +679,8 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void kv4_tile_kernel(AttnArgs a
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                // bf16 queries: one fused operation, off by a rounding of the
-                // scaled maximum, far below P's own rounding.
-                const float e = NT == 1 ? __builtin_fmaf(sc[kb][r], scale2, -m2)
-                                        : (sc[kb][r] - mx) * scale2;
-                const float pr = __builtin_amdgcn_exp2f(e);
+                const float pr =
+                    __builtin_amdgcn_exp2f(exponent<NT>(sc[kb][r], mx, scale2, m2));
                 sc[kb][r] = !MASK || 32 * kb + 8 * (r >> 2) + (r & 3) < room ? pr : 0.0f;
             }
 #pragma unroll
@@ -734,36 +778,60 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void kv4_tile_kernel(AttnArgs a
 }
 
 // O = sum_s w_s P_s / sum_s w_s, w_s = l_s 2^(m_s - max m), over the splits
-// that saw a key.
-template <typename T>
+// that saw a key (at most 64).  One wave per row: lane s weighs split s, then
+// the lanes take D / 64 dimensions each, the splits in order.
+constexpr int kMaxSplits = 64;
+
+template <typename T, int D>
 __global__ __launch_bounds__(256) void kv4_join_kernel(AttnArgs a)
 {
+    constexpr int E = D / 64;
     const Kv4Attention &p = a.p;
     const int64_t plane = int64_t(p.B) * p.S_q * p.H;
-    const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
-    const int64_t row = i / p.D;
+    const int lane = threadIdx.x & 63;
+    const int64_t row =
+        int64_t(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
     if (row >= plane)
-        return;
-    const int d = int(i - row * p.D);
+        return;  // whole wave
     const int h = int(row % p.H);
     const int64_t bs = row / p.H;
     const int b = int(bs / p.S_q), s = int(bs % p.S_q);
     if (p.counts && s >= p.counts[b])
         return;
-    float m = -INFINITY;
-    for (int k = 0; k < a.splits; ++k)
-        m = fmaxf(m, a.ml[k * plane + row].x);
-    float l = 0.0f, v = 0.0f;
-    for (int k = 0; k < a.splits; ++k) {
-        const float2 ml = a.ml[k * plane + row];
-        if (ml.y == 0.0f)
-            continue;
-        const float w = (ml.x == m ? 1.0f : __builtin_amdgcn_exp2f(ml.x - m)) * ml.y;
-        l += w;
-        v += w * a.part[(k * plane + row) * p.D + d];
+    const float2 ml = lane < a.splits ? a.ml[lane * plane + row] : float2{-INFINITY, 0.0f};
+    float m = ml.y == 0.0f ? -INFINITY : ml.x;
+#pragma unroll
+    for (int o = 32; o; o >>= 1)
+        m = fmaxf(m, __shfl_xor(m, o));
+    // A split of which no key was seen weighs nothing, whatever its maximum.
+    float w = ml.y == 0.0f ? 0.0f
+                           : (ml.x == m ? 1.0f : __builtin_amdgcn_exp2f(ml.x - m)) * ml.y;
+    float l = w;
+#pragma unroll
+    for (int o = 32; o; o >>= 1)
+        l += __shfl_xor(l, o);
+    const float *src = a.part + row * D + lane * E;
+    float v[E] = {};
+    for (int k0 = 0; k0 < a.splits; k0 += 8) {
+        float x[8][E];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                x[k][e] = src[min(k0 + k, a.splits - 1) * plane * D + e];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float wk = __shfl(w, k0 + k);
+            if (k0 + k < a.splits && wk != 0.0f)
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    v[e] += wk * x[k][e];
+        }
     }
-    store_o(static_cast<T *>(p.o) + b * p.os.b + h * p.os.h + s * p.os.s + d,
-            l == 0.0f ? 0.0f : v / l);
+    T *out = static_cast<T *>(p.o) + b * p.os.b + h * p.os.h + s * p.os.s + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        store_o(out + e, l == 0.0f ? 0.0f : v[e] / l);
 }
 
 struct Plan {
@@ -780,11 +848,11 @@ Plan plan_of(int B, int S_q, int H, int H_kv, int S_max)
     pl.tiles = int((rows + per_tile - 1) / per_tile);
     const int64_t groups = std::max<int64_t>(1, int64_t(B) * H_kv * pl.tiles);
     // Splits until the grid has two (tiles) or about four workgroups per CU,
-    // or a share is two tiles of keys, or one round of a workgroup's waves.
-    const int round = pl.tile ? 2 * kTileKeys : kTokKeys * kTokWaves;
+    // or a share is two tiles of keys, or four rounds of a workgroup's waves.
+    const int round = pl.tile ? 2 * kTileKeys : 4 * kTokKeys * kTokWaves;
     const int64_t rounds = (int64_t(S_max) + round - 1) / round;
     pl.splits = int(std::max<int64_t>(
-        1, std::min<int64_t>({(pl.tile ? 512 : 1024) / groups, rounds, 64})));
+        1, std::min<int64_t>({(pl.tile ? 512 : 1024) / groups, rounds, kMaxSplits})));
     return pl;
 }
 
@@ -797,8 +865,8 @@ template <typename T, int D>
 bool run_attention_kv4(AttnArgs &a, bool tile, hipStream_t st)
 {
     const int64_t blocks = int64_t(a.p.B) * a.p.H_kv * a.tiles * a.splits;
-    const int64_t elems = int64_t(a.p.B) * a.p.S_q * a.p.H * D;
-    if (blocks > INT32_MAX || (elems + 255) / 256 > INT32_MAX)
+    const int64_t rows = int64_t(a.p.B) * a.p.S_q * a.p.H;
+    if (blocks > INT32_MAX || rows > INT32_MAX)
         return fail("kv4_attention_dev: too many query rows");
     if (tile)
         hipLaunchKernelGGL((kv4_tile_kernel<T, D>), dim3(unsigned(blocks)), dim3(kTileWaves * 64),
@@ -810,7 +878,7 @@ bool run_attention_kv4(AttnArgs &a, bool tile, hipStream_t st)
         return false;
     if (a.splits == 1)
         return true;
-    hipLaunchKernelGGL(kv4_join_kernel<T>, dim3(unsigned((elems + 255) / 256)), dim3(256), 0, st,
+    hipLaunchKernelGGL((kv4_join_kernel<T, D>), dim3(unsigned((rows + 3) / 4)), dim3(256), 0, st,
                        a);
     return hip_ok(hipGetLastError(), "kv4_join_kernel launch");
 }
