@@ -85,8 +85,9 @@ __device__ __forceinline__ int scale_byte(unsigned top)
 
 // x as `N` bf16 terms whose sum is x exactly (three terms: 3 x 8 bits): each
 // term is the leading eight bits of what is left, by truncation.  An infinity
-// is its own first term, with no NaN behind it.  Terms are packed in pairs.
-template <int N>
+// is its own first term, with no NaN behind it (INF: there may be one).  Terms
+// are packed in pairs.
+template <int N, bool INF = true>
 __device__ __forceinline__ void terms2(float x0, float x1, unsigned (&t)[N])
 {
 #pragma unroll
@@ -96,8 +97,8 @@ __device__ __forceinline__ void terms2(float x0, float x1, unsigned (&t)[N])
         if (i + 1 < N) {
             const float h0 = __uint_as_float(u0 & 0xFFFF0000u);
             const float h1 = __uint_as_float(u1 & 0xFFFF0000u);
-            x0 = x0 == h0 ? 0.0f : x0 - h0;
-            x1 = x1 == h1 ? 0.0f : x1 - h1;
+            x0 = INF && x0 == h0 ? 0.0f : x0 - h0;
+            x1 = INF && x1 == h1 ? 0.0f : x1 - h1;
         }
     }
 }

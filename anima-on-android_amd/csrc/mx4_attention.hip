@@ -119,13 +119,14 @@ __device__ __forceinline__ void q_terms(const uint16_t *q, bool wide, bool neg, 
     t[0] = __builtin_bit_cast(bf16x8, neg ? u ^ 0x80008000u : u);
 }
 
+template <bool INF = true>
 __device__ __forceinline__ void terms8(const float (&x)[8], bf16x8 (&t)[3])
 {
     u32x4 u[3];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         unsigned w[3];
-        terms2<3>(x[2 * i], x[2 * i + 1], w);
+        terms2<3, INF>(x[2 * i], x[2 * i + 1], w);
 #pragma unroll
         for (int j = 0; j < 3; ++j)
             u[j][i] = w[j];
@@ -156,7 +157,7 @@ __device__ __forceinline__ void p_terms(const float (&p)[8], bf16x8 (&t)[1])
 }
 __device__ __forceinline__ void p_terms(const float (&p)[8], bf16x8 (&t)[3])
 {
-    terms8(p, t);
+    terms8<false>(p, t);  // at most 2^8
 }
 
 // ----------------------------------------------------------- token kernel
@@ -238,10 +239,12 @@ __global__ __launch_bounds__(kTokWaves * 64, 2) void kv4_token_kernel(AttnArgs a
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 15, g = lane >> 4;
-    const int blk = xcd_major_block();
+    // Neighbouring workgroups go to different XCDs, and the shares of a long
+    // sequence with them.
+    const int blk = blockIdx.x;
     const int split = blk % a.splits;
-    const int tile = (blk / a.splits) % a.tiles;
-    const int bh = (blk / a.splits) / a.tiles;
+    const int bh = (blk / a.splits) % (p.B * p.H_kv);
+    const int tile = (blk / a.splits) / (p.B * p.H_kv);
     const int b = bh / p.H_kv, hk = bh - b * p.H_kv;
 
     // This lane's query row (column n of the accumulators).  Rows past the last
@@ -747,39 +750,77 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void kv4_tile_kernel(AttnArgs a
         __syncthreads();
     }
 
-    // Row sums over the two halves; then O through LDS, rows of D values.
+    // Row sums over the two halves; then O^T through the stages' LDS (every
+    // wave has left them), so that rows go out whole: f32 rows of D / 4 pieces
+    // of 16 bytes, placed by their row's low bits against bank conflicts.
     sum += __shfl_xor(sum, 32);
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const int64_t plane = int64_t(p.B) * p.S_q * p.H;
-    if (a.splits > 1) {
-        if (live) {
-            const int64_t at = split * plane + (int64_t(b) * p.S_q + s) * p.H + hq;
-            float *dst = a.part + at * D;
-#pragma unroll
-            for (int i = 0; i < DB; ++i)
-#pragma unroll
-                for (int r = 0; r < 16; r += 4)
-                    *reinterpret_cast<f32x4 *>(dst + 32 * i + acc_row(r, half)) =
-                        f32x4{o[i][r] * inv, o[i][r + 1] * inv, o[i][r + 2] * inv,
-                              o[i][r + 3] * inv};
-            if (half == 0)
-                a.ml[at] = float2{mx * scale2, sum};
-        }
-        return;
-    }
-    if (!live)
-        return;
-    T *out = static_cast<T *>(p.o) + b * p.os.b + hq * p.os.h + s * p.os.s;
+    float *so = reinterpret_cast<float *>(smem) + wave * 32 * D;
+    constexpr int PIECES = D / 4;
 #pragma unroll
     for (int i = 0; i < DB; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-            store_o(out + 32 * i + acc_row(r, half), o[i][r] * inv);
+        for (int r = 0; r < 16; r += 4)
+            *reinterpret_cast<f32x4 *>(so + col * D +
+                                       ((8 * i + acc_row(r, half) / 4) ^ (col & 15)) * 4) =
+                f32x4{o[i][r] * inv, o[i][r + 1] * inv, o[i][r + 2] * inv, o[i][r + 3] * inv};
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const bool parts = a.splits > 1;
+    const int64_t plane = int64_t(p.B) * p.S_q * p.H;
+    const int64_t prow = split * plane + (int64_t(b) * p.S_q + s) * p.H + hq;
+    if (parts && live && half == 0)
+        a.ml[prow] = float2{mx * scale2, sum};
+    // Where this lane's row starts (elements), for the lanes that write it.
+    const int64_t at = !live   ? -1
+                       : parts ? prow * D
+                               : b * p.os.b + hq * p.os.h + s * p.os.s;
+    const bool wide_o = ((reinterpret_cast<uintptr_t>(p.o) & 15) |
+                         ((p.os.b | p.os.h | p.os.s) & 7)) == 0;
+    if (parts || NT == 3) {
+        float *dst = parts ? a.part : static_cast<float *>(p.o);
+#pragma unroll
+        for (int i = 0; i < PIECES / 2; ++i) {
+            const int f = i * 64 + lane, r = f / PIECES, piece = f % PIECES;
+            const int64_t off = __shfl(at, r);
+            const f32x4 v = *reinterpret_cast<const f32x4 *>(so + r * D + (piece ^ (r & 15)) * 4);
+            if (off < 0)
+                continue;
+            if (parts || wide_o)
+                *reinterpret_cast<f32x4 *>(dst + off + 4 * piece) = v;
+            else
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    dst[off + 4 * piece + e] = v[e];
+        }
+    } else {
+        u16 *dst = static_cast<u16 *>(p.o);
+#pragma unroll
+        for (int i = 0; i < PIECES / 4; ++i) {
+            const int f = i * 64 + lane, r = f / (PIECES / 2), piece = f % (PIECES / 2) * 2;
+            const int64_t off = __shfl(at, r);
+            const float *src = so + r * D;
+            const f32x4 v0 = *reinterpret_cast<const f32x4 *>(src + (piece ^ (r & 15)) * 4);
+            const f32x4 v1 = *reinterpret_cast<const f32x4 *>(src + ((piece + 1) ^ (r & 15)) * 4);
+            if (off < 0)
+                continue;
+            const float v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+            if (wide_o) {
+                bf16x8 t[1];
+                p_terms(v, t);
+                *reinterpret_cast<bf16x8 *>(dst + off + 4 * piece) = t[0];
+            } else
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    store_o(dst + off + 4 * piece + e, v[e]);
+        }
+    }
 }
 
 // O = sum_s w_s P_s / sum_s w_s, w_s = l_s 2^(m_s - max m), over the splits
-// that saw a key (at most 64).  One wave per row: lane s weighs split s, then
-// the lanes take D / 64 dimensions each, the splits in order.
+// that saw a key (at most 64).  One workgroup per row: in each wave lane s
+// weighs split s; wave w adds the splits w, w + 4, .., its loads all in flight,
+// D / 64 dimensions per lane, and the waves' sums are added in their order.
 constexpr int kMaxSplits = 64;
 
 template <typename T, int D>
@@ -788,11 +829,10 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(AttnArgs a)
     constexpr int E = D / 64;
     const Kv4Attention &p = a.p;
     const int64_t plane = int64_t(p.B) * p.S_q * p.H;
+    __shared__ float part[4][D];
     const int lane = threadIdx.x & 63;
-    const int64_t row =
-        int64_t(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
-    if (row >= plane)
-        return;  // whole wave
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t row = blockIdx.x;
     const int h = int(row % p.H);
     const int64_t bs = row / p.H;
     const int b = int(bs / p.S_q), s = int(bs % p.S_q);
@@ -811,27 +851,32 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(AttnArgs a)
     for (int o = 32; o; o >>= 1)
         l += __shfl_xor(l, o);
     const float *src = a.part + row * D + lane * E;
-    float v[E] = {};
-    for (int k0 = 0; k0 < a.splits; k0 += 8) {
-        float x[8][E];
+    float x[kMaxSplits / 4][E], v[E] = {};
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
+    for (int k = 0; k < kMaxSplits / 4; ++k)
+        if (wave + 4 * k < a.splits)
 #pragma unroll
             for (int e = 0; e < E; ++e)
-                x[k][e] = src[min(k0 + k, a.splits - 1) * plane * D + e];
+                x[k][e] = src[(wave + 4 * k) * plane * D + e];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const float wk = __shfl(w, k0 + k);
-            if (k0 + k < a.splits && wk != 0.0f)
+    for (int k = 0; k < kMaxSplits / 4; ++k)
+        if (wave + 4 * k < a.splits) {
+            const float wk = __shfl(w, wave + 4 * k);
+            if (wk != 0.0f)
 #pragma unroll
                 for (int e = 0; e < E; ++e)
                     v[e] += wk * x[k][e];
         }
-    }
-    T *out = static_cast<T *>(p.o) + b * p.os.b + h * p.os.h + s * p.os.s + lane * E;
 #pragma unroll
     for (int e = 0; e < E; ++e)
-        store_o(out + e, l == 0.0f ? 0.0f : v[e] / l);
+        part[wave][lane * E + e] = v[e];
+    __syncthreads();
+    const int d = threadIdx.x;
+    if (d < D) {
+        const float o = part[0][d] + part[1][d] + part[2][d] + part[3][d];
+        store_o(static_cast<T *>(p.o) + b * p.os.b + h * p.os.h + s * p.os.s + d,
+                l == 0.0f ? 0.0f : o / l);
+    }
 }
 
 struct Plan {
@@ -847,12 +892,12 @@ Plan plan_of(int B, int S_q, int H, int H_kv, int S_max)
     const int per_tile = pl.tile ? kTileRows : kTokRows;
     pl.tiles = int((rows + per_tile - 1) / per_tile);
     const int64_t groups = std::max<int64_t>(1, int64_t(B) * H_kv * pl.tiles);
-    // Splits until the grid has two (tiles) or about four workgroups per CU,
+    // Splits until the grid has two workgroups per CU,
     // or a share is two tiles of keys, or four rounds of a workgroup's waves.
     const int round = pl.tile ? 2 * kTileKeys : 4 * kTokKeys * kTokWaves;
     const int64_t rounds = (int64_t(S_max) + round - 1) / round;
     pl.splits = int(std::max<int64_t>(
-        1, std::min<int64_t>({(pl.tile ? 512 : 1024) / groups, rounds, kMaxSplits})));
+        1, std::min<int64_t>({512 / groups, rounds, kMaxSplits})));
     return pl;
 }
 
@@ -878,7 +923,7 @@ bool run_attention_kv4(AttnArgs &a, bool tile, hipStream_t st)
         return false;
     if (a.splits == 1)
         return true;
-    hipLaunchKernelGGL((kv4_join_kernel<T, D>), dim3(unsigned((rows + 3) / 4)), dim3(256), 0, st,
+    hipLaunchKernelGGL((kv4_join_kernel<T, D>), dim3(unsigned(rows)), dim3(256), 0, st,
                        a);
     return hip_ok(hipGetLastError(), "kv4_join_kernel launch");
 }
