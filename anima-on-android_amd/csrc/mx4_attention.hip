@@ -494,7 +494,7 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void kv4_tile_kernel(AttnArgs a
     constexpr int KV_EL = kTileKeys * D;  // elements of a staged K or V^T tile
     constexpr int VD = D / 16;           // dimensions of V a thread decodes, of 4 keys
     __shared__ __attribute__((aligned(16))) u16 smem[4 * KV_EL];
-    __shared__ int nan_tile[2];
+    __shared__ int any_nan;  // of the workgroup's V
 
     const Kv4Attention &p = a.p;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -547,13 +547,16 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void kv4_tile_kernel(AttnArgs a
     // the four keys 4 va .. 4 va + 3 in VD dimensions.
     const int kt = tid >> 2, kpart = tid & 3;
     const int va = tid & 15, vd = tid >> 4;
-    const int last = max(seq.len - 1, 0);
     unsigned kc[D / 32], kscale, vc[4], vscale[4];
     auto load = [&](int j) {
-        const int t0 = j * kTileKeys;
+        // Keys past the cache's length read its last one again.
+        const unsigned over = unsigned(min(seq.len - 1 - j * kTileKeys, kTileKeys - 1));
+        const int64_t row = seq.kv_row + int64_t(j) * kTileKeys;
+        const uint8_t *kc0 = p.cache.k + row * (D / 2), *ks0 = p.cache.k_scales + row * GROUPS;
+        const uint8_t *vc0 = p.cache.v + row * (D / 2), *vs0 = p.cache.v_scales + row * GROUPS;
         {
-            const int64_t r = seq.kv_row + min(t0 + kt, last);
-            const uint8_t *src = p.cache.k + r * (D / 2) + kpart * (D / 8);
+            const unsigned key = min(unsigned(kt), over);
+            const uint8_t *src = kc0 + (key * (D / 2) + kpart * (D / 8));
             if constexpr (D == 128) {
                 const u32x4 w = *reinterpret_cast<const u32x4 *>(src);
 #pragma unroll
@@ -564,17 +567,17 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void kv4_tile_kernel(AttnArgs a
                 kc[0] = w[0];
                 kc[1] = w[1];
             }
-            kscale = p.cache.k_scales[r * GROUPS + kpart * GROUPS / 4];
+            kscale = ks0[key * GROUPS + kpart * GROUPS / 4];
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int64_t r = seq.kv_row + min(t0 + 4 * va + i, last);
-            const uint8_t *src = p.cache.v + r * (D / 2) + vd * (D / 32);
+            const unsigned key = min(unsigned(4 * va + i), over);
+            const uint8_t *src = vc0 + (key * (D / 2) + vd * (D / 32));
             if constexpr (D == 128)
                 vc[i] = *reinterpret_cast<const unsigned *>(src);
             else
                 vc[i] = *reinterpret_cast<const uint16_t *>(src);
-            vscale[i] = p.cache.v_scales[r * GROUPS + vd * GROUPS / 16];
+            vscale[i] = vs0[key * GROUPS + vd * GROUPS / 16];
         }
     };
     // Quad va of keys within its row of 64: groups of 16 keys hold their quads
@@ -582,7 +585,7 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void kv4_tile_kernel(AttnArgs a
     // holds in its accumulator registers.
     const int vq = va & 3;
     const int vpiece = 2 * (va >> 2) + (vq & 1), vsub = vq >> 1;
-    auto store = [&](int j, int stage) {
+    auto store = [&](int stage) {
         unsigned ko = stage * KV_EL + kt * D + k_piece<D>(kt, kpart * (D / 32)) * 8;
         unsigned vo = (2 + stage) * KV_EL + vd * VD * kTileKeys + v_piece(vd * VD, vpiece) * 8 +
                       4 * vsub;
@@ -615,7 +618,7 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void kv4_tile_kernel(AttnArgs a
                 odd;
         }
         if (nan)
-            nan_tile[stage] = j;
+            any_nan = 1;
     };
 
     f32x16 o[DB];
@@ -626,16 +629,15 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void kv4_tile_kernel(AttnArgs a
             o[i][r] = 0.0f;
     float mx = -INFINITY, sum = 0.0f;
 
-    auto compute = [&](int j, int stage, auto masked) {
-        constexpr bool MASK = decltype(masked)::value;
-        const int t0 = j * kTileKeys;
-        // Offsets of this lane's rows with its half's first piece; the other
-        // pieces differ in bits that the row's start leaves clear.  Recomputed
-        // per tile: kept in registers for every piece they would spill.
-        unsigned ko = stage * KV_EL + col * D + k_piece<D>(col, half) * 8;
-        unsigned vo = (2 + stage) * KV_EL + col * kTileKeys + v_piece(col, half) * 8;
-        asm volatile("" : "+v"(ko), "+v"(vo));
-        f32x16 sc[2];
+    // Offsets of this lane's K rows and V^T rows, with its half's first piece,
+    // in stage 0; other pieces differ in bits that a row's start leaves clear.
+    // Recomputed per tile: kept in registers for every piece they would spill.
+    const unsigned ko0 = col * D + k_piece<D>(col, half) * 8;
+    const unsigned vo0 = 2 * KV_EL + col * kTileKeys + v_piece(col, half) * 8;
+    f32x16 sc[2];  // key t0 + 32 kb + acc_row(r, half) in sc[kb][r]
+    auto scores = [&](int stage) {
+        unsigned ko = ko0 + stage * KV_EL;
+        asm volatile("" : "+v"(ko));
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
 #pragma unroll
@@ -651,15 +653,28 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void kv4_tile_kernel(AttnArgs a
                     sc[kb] = mfma_bf16(kf, qf[ks][t], sc[kb]);
             }
         }
-        // Key of register r of block kb: t0 + 32 kb + acc_row(r, half).
+    };
+    auto softmax_pv = [&](int j, int stage) {
+        const int t0 = j * kTileKeys;
+        const bool masked = t0 + kTileKeys > least;  // uniform over the wave
         const int room = limit - t0 - 4 * half;
+        unsigned vo = vo0 + stage * KV_EL;
+        asm volatile("" : "+v"(vo));
+        if (masked)
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    float x = 32 * kb + 8 * (r >> 2) + (r & 3) < room ? sc[kb][r] : -INFINITY;
+                    asm volatile("" : "+v"(x));  // stays behind the branch
+                    sc[kb][r] = x;
+                }
         float mt = -INFINITY;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
             for (int r = 0; r < 16; ++r)
-                if (!MASK || 32 * kb + 8 * (r >> 2) + (r & 3) < room)
-                    mt = fmaxf(mt, sc[kb][r]);
+                mt = fmaxf(mt, sc[kb][r]);
         mt = row_pair_max(mt);
         // The maximum moves when a row has none yet or is 2^8 behind: until
         // then probabilities stay below 2^8 and nothing is rescaled.
@@ -678,77 +693,83 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void kv4_tile_kernel(AttnArgs a
                     o[i][r] *= alpha;
         }
         const float m2 = mx * scale2;
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const float pr =
-                    __builtin_amdgcn_exp2f(exponent<NT>(sc[kb][r], mx, scale2, m2));
-                sc[kb][r] = !MASK || 32 * kb + 8 * (r >> 2) + (r & 3) < room ? pr : 0.0f;
-            }
+        // Sixteen keys at a time: the MFMAs of one group run under the
+        // exponentials of the next.
 #pragma unroll
         for (int kg = 0; kg < 4; ++kg) {
-            bf16x8 pf[NT];
             asm volatile("" ::: "memory");
-            if constexpr (NT == 1) {
-                pf[0] = pack8(sc[kg >> 1], 8 * (kg & 1));
-                sum = row_sum8(pf[0], sum);
-            } else {
-                float pr[8];
+            bf16x8 vf[DB];
+#pragma unroll
+            for (int i = 0; i < DB; ++i)
+                vf[i] = *reinterpret_cast<const bf16x8 *>(smem + 32 * i * kTileKeys +
+                                                          (vo ^ 16 * kg));
+            float pr[8];
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+                pr[r] = __builtin_amdgcn_exp2f(
+                    exponent<NT>(sc[kg >> 1][8 * (kg & 1) + r], mx, scale2, m2));
+            // Not left to exp2(-inf): a row's maximum may be -inf, or the scale 0.
+            if (masked)
 #pragma unroll
                 for (int r = 0; r < 8; ++r) {
-                    pr[r] = sc[kg >> 1][8 * (kg & 1) + r];
-                    sum += pr[r];
+                    float x = 16 * kg + 8 * (r >> 2) + (r & 3) < room ? pr[r] : 0.0f;
+                    asm volatile("" : "+v"(x));
+                    pr[r] = x;
                 }
-                p_terms(pr, pf);
-            }
+            bf16x8 pf[NT];
+            p_terms(pr, pf);
+            if constexpr (NT == 1)
+                sum = row_sum8(pf[0], sum);
+            else
 #pragma unroll
-            for (int i = 0; i < DB; ++i) {
-                const bf16x8 vf = *reinterpret_cast<const bf16x8 *>(
-                    smem + 32 * i * kTileKeys + (vo ^ 16 * kg));
+                for (int r = 0; r < 8; ++r)
+                    sum += pr[r];
+#pragma unroll
+            for (int i = 0; i < DB; ++i)
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
-                    o[i] = mfma_bf16(vf, pf[t], o[i]);
-            }
-        }
-        if (nan_tile[stage] == j) {
-            // NaN groups of V, decoded as zero: to the rows that see their keys.
-            for (int t = t0; t < min(t0 + kTileKeys, seq.len); ++t)
-#pragma unroll
-                for (int i = 0; i < DB; ++i)
-                    if (p.cache.v_scales[(seq.kv_row + t) * GROUPS + i] == mx4::kNanScale &&
-                        t < limit)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r)
-                            o[i][r] = NAN;
+                    o[i] = mfma_bf16(vf[i], pf[t], o[i]);
         }
     };
 
-    if (tid < 2)
-        nan_tile[tid] = -1;
+    if (tid == 0)
+        any_nan = 0;
     __syncthreads();
     if (first < end) {
         load(first);
-        store(first, 0);
+        store(0);
         if (first + 1 < end)
             load(first + 1);
     }
     __syncthreads();
     for (int j = first; j < end; ++j) {
         const int stage = (j - first) & 1;
+        // The next tile is decoded under the scores' MFMAs.
+        const bool seen = j * kTileKeys < most;
+        if (seen)
+            scores(stage);
         if (j + 1 < end) {
-            store(j + 1, stage ^ 1);
+            store(stage ^ 1);
             if (j + 2 < end)
                 load(j + 2);
         }
-        if (j * kTileKeys < most) {
-            if ((j + 1) * kTileKeys <= least)
-                compute(j, stage, std::false_type{});
-            else
-                compute(j, stage, std::true_type{});
+        if (seen) {
+            __builtin_amdgcn_s_setprio(1);
+            softmax_pv(j, stage);
+            __builtin_amdgcn_s_setprio(0);
         }
         __syncthreads();
     }
+
+    // NaN groups of V, decoded as zero: to the rows that see their keys.
+    if (any_nan)
+        for (int t = first * kTileKeys; t < min(end * kTileKeys, seq.len); ++t)
+#pragma unroll
+            for (int i = 0; i < DB; ++i)
+                if (p.cache.v_scales[(seq.kv_row + t) * GROUPS + i] == mx4::kNanScale && t < limit)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        o[i][r] = NAN;
 
     // Row sums over the two halves; then O^T through the stages' LDS (every
     // wave has left them), so that rows go out whole: f32 rows of D / 4 pieces
