@@ -359,6 +359,207 @@ __global__ __launch_bounds__(WM *WN * 64) void linear_tile_kernel(LinArgs p)
     }
 }
 
+// ----------------------------------------------------------- wide tiles
+
+constexpr int kWideK = 128;   // K elements per chunk: 256-byte rows of A, 64 bytes of codes
+constexpr int kWideN = 256;   // weight rows of a tile
+
+// bf16 activations, K a multiple of 128, 16-byte aligned rows.  Tiles of
+// 64 MB x 256: 8 waves as 2 (M) x 4 (N), each 32 MB rows and 64 columns, C^T
+// on 32x32x16 MFMAs (W the first operand), so that a lane's four consecutive
+// accumulators are four columns of one row.
+// A's rows and W's codes reach LDS by DMA, two stages of 128 elements of K; 16-byte
+// pieces are placed by piece ^ (row & 15) (A) and piece ^ (row / 4 & 3) (codes).
+// A lane takes 64 contiguous codes of a weight row from there, two scale groups,
+// and decodes them as the MFMA's k index wants them, k = 64 half + 8 step + j,
+// the order A is read in: the decoded weights never pass through LDS, whose reads
+// would take as long as the MFMAs with them (256 x 256 tiles with both operands
+// decoded to LDS: 200 us at 4608 x 8192 x 2048, this kernel 124 us).  Codes read
+// by each wave from memory instead, 16 bytes of 64 rows per instruction, kept
+// the address unit as busy as the MFMAs (146 us).
+// Bound by the MFMA at the clock that power allows: 1.25 PFLOP/s at that
+// size, where a library product of bf16 operands of 8192 x 8192 x 8192 runs 1.4.
+template <int MB>
+__global__ __launch_bounds__(512, 2) void linear_wide_kernel(LinArgs p)
+{
+    constexpr int BM = 64 * MB;
+    constexpr int STAGE = BM * kWideK;
+    constexpr int WINDOWS = 2 * MB;  // 1 KiB DMA windows (4 rows) per wave and chunk
+    constexpr int NB = 2;
+    constexpr int CODES = kWideN * 64;  // bytes of a stage's codes
+    __shared__ __attribute__((aligned(16))) u16 smem[2 * STAGE + CODES];  // two stages of codes
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave & 1, wn = wave >> 1;
+    const int col = lane & 31, half = lane >> 5;
+    const int blk = xcd_major_block();
+    // Four M tiles by all N tiles at a time, M inside: the 32 CUs of an XCD work
+    // on about 4 x 8 tiles.
+    const int band = blk / (4 * p.tiles_n), in_band = blk - band * 4 * p.tiles_n;
+    const int bm = min(4, p.tiles_m - 4 * band);
+    const int tn = in_band / bm, tm = 4 * band + in_band - tn * bm;
+    const int row0 = tm * BM, col0 = tn * kWideN;
+    const int chunks = p.K / kWideK;
+
+    unsigned off[WINDOWS];
+#pragma unroll
+    for (int i = 0; i < WINDOWS; ++i) {
+        const int r = (wave * WINDOWS + i) * 4 + (lane >> 4);
+        const int rr = min(row0 + r, p.M - 1) - row0;  // rows past M: not stored
+        off[i] = unsigned(int64_t(rr) * p.lda * 2 + 16 * ((lane & 15) ^ (r & 15)));
+    }
+    const char *a0 = reinterpret_cast<const char *>(static_cast<const u16 *>(p.a) +
+                                                    int64_t(row0) * p.lda);
+    // Codes: 16 windows of 16 rows x 64 bytes, two per wave, 16-byte pieces
+    // placed by piece ^ (row / 4 & 3).
+    unsigned woff[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int r = (wave * 2 + i) * 16 + (lane >> 2);
+        const int rr = min(col0 + r, p.N - 1) - col0;
+        woff[i] = unsigned(rr * (p.K / 2) + 16 * ((lane & 3) ^ (r >> 2 & 3)));
+    }
+    const char *w0 = reinterpret_cast<const char *>(p.codes + int64_t(col0) * (p.K / 2));
+    u16 *const smem_w = smem + 2 * STAGE;
+    auto dma = [&](int c, int stage) {
+        const char *src = a0 + int64_t(c) * (kWideK * 2);
+#pragma unroll
+        for (int i = 0; i < WINDOWS; ++i)
+            dma16s(src, off[i], smem + stage * STAGE + (wave * WINDOWS + i) * 512);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            dma16s(w0 + c * (kWideK / 2), woff[i],
+                   smem_w + stage * (CODES / 2) + (wave * 2 + i) * 512);
+    };
+
+    // The scales of this wave's 64 rows, one row per lane.
+    const uint8_t *ws = p.scales + int64_t(min(col0 + wn * 64 + lane, p.N - 1)) * p.groups;
+    unsigned sc[NB], sc_next = 0;
+    u32x4 codes[NB][2];
+    auto load = [&](int c) { sc_next = *reinterpret_cast<const unsigned *>(ws + c * 4); };
+    // Rows wn * 64 + 32 j + col: 64 codes of this half, and their two scales.
+    auto fetch = [&](int stage) {
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            const int r = wn * 64 + 32 * j + col;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                codes[j][h] = *reinterpret_cast<const u32x4 *>(
+                    smem_w + stage * (CODES / 2) + r * 32 + ((2 * half + h) ^ (r >> 2 & 3)) * 8);
+            sc[j] = unsigned(__shfl(int(sc_next), 32 * j + col)) >> (16 * half) & 0xFFFFu;
+        }
+    };
+
+    f32x16 acc[MB][NB];
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                acc[i][j][r] = 0.0f;
+
+    // Fragments of a step are read, and its weights decoded, while the MFMAs of
+    // the step before run; a chunk's first ones under the last step of the chunk
+    // before it, behind the barrier that ends that chunk.
+    bf16x8 af[2][MB], wf[2][NB];
+    unsigned ao = 0;
+    auto read = [&](int st, bf16x8 (&f)[MB]) {
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+            f[i] = *reinterpret_cast<const bf16x8 *>(smem + 32 * i * kWideK + (ao ^ 8 * st));
+    };
+    auto decode = [&](int st, bf16x8 (&f)[NB]) {
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+            f[j] = decode8(codes[j][st >> 2][st & 3],
+                           scale_of(st < 4 ? sc[j] & 255u : sc[j] >> 8));
+    };
+    // Chunk c is staged and its codes are here; the one after next may come.
+    auto enter = [&](int c) {
+        wait_vmcnt<0>();
+        ring_barrier();
+        fetch(c & 1);
+        if (c + 1 < chunks) {
+            load(c + 1);
+            dma(c + 1, (c + 1) & 1);
+        }
+        // Piece 8 half + step of rows wm * 32 MB + 32 i + col.
+        ao = (c & 1) * STAGE + (wm * 32 * MB + col) * kWideK + ((8 * half) ^ (col & 15)) * 8;
+        asm volatile("" : "+v"(ao));
+    };
+    load(0);
+    dma(0, 0);
+    enter(0);
+    read(0, af[0]);
+    decode(0, wf[0]);
+    for (int c = 0; c < chunks; ++c) {
+#pragma unroll
+        for (int st = 0; st < 8; ++st) {
+            if (st < 7)
+                read(st + 1, af[(st + 1) & 1]);
+            else if (c + 1 < chunks) {
+                enter(c + 1);
+                read(0, af[0]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < MB; ++i)
+#pragma unroll
+                for (int j = 0; j < NB; ++j)
+                    acc[i][j] = mfma_bf16(wf[st & 1][j], af[st & 1][i], acc[i][j]);
+            decode((st + 1) & 7, wf[(st + 1) & 1]);
+        }
+    }
+
+    // Lane (col, half): row col of its blocks, columns acc_row(r, half).  Through
+    // LDS, so that rows go out in 128-byte runs.
+    __syncthreads();
+    constexpr int PITCH = 72;  // bf16 elements of a staged row: 64 and 16 bytes against conflicts
+    static_assert(8 * 32 * PITCH <= 2 * STAGE, "the staged rows fit");
+    u16 *so = smem + wave * 32 * PITCH;
+    const int n0 = col0 + wn * 64;
+    const bool wide = (reinterpret_cast<uintptr_t>(p.c) & 15) == 0 && p.ldc % 8 == 0 &&
+                      n0 + 64 <= p.N;
+#pragma unroll
+    for (int i = 0; i < MB; ++i) {
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                u32x2 v;
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    v[e] = __builtin_bit_cast(
+                        unsigned, __builtin_convertvector(f32x2{acc[i][j][r + 2 * e],
+                                                                acc[i][j][r + 2 * e + 1]},
+                                                          bf16x2));
+                *reinterpret_cast<u32x2 *>(so + col * PITCH + 32 * j + acc_row(r, half)) = v;
+            }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int r = 8 * q + (lane >> 3), piece = lane & 7;
+            const int m = row0 + (wm * MB + i) * 32 + r;
+            const u32x4 v = *reinterpret_cast<const u32x4 *>(so + r * PITCH + 8 * piece);
+            if (m >= p.M)
+                continue;
+            u16 *dst = static_cast<u16 *>(p.c) + int64_t(m) * p.ldc + n0 + 8 * piece;
+            if (wide)
+                __builtin_nontemporal_store(v, reinterpret_cast<u32x4 *>(dst));
+            else
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (n0 + 8 * piece + e < p.N)
+                        dst[e] = u16(v[e >> 1] >> (16 * (e & 1)));
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
 // C = the planes' sum, in split order.
 template <typename T>
 __global__ __launch_bounds__(256) void linear_sum_kernel(const float *part, T *c, int64_t ldc,
@@ -380,14 +581,17 @@ __global__ __launch_bounds__(256) void linear_sum_kernel(const float *part, T *c
 struct TileShape {
     int bm, bn;
 };
-constexpr TileShape kShapes[] = {{32, 128}, {64, 128}, {128, 128}, {256, 256}};
+// The last three are the wide kernel's.
+constexpr TileShape kShapes[] = {{32, 128},  {64, 128},  {128, 128},
+                                 {128, 256}, {192, 256}, {256, 256}};
 
 struct Plan {
     int shape;  // -1: few rows
     int tiles_m = 0, tiles_n = 0, splits = 1, per_split = 0, chunks = 0;
 };
 
-Plan plan_of(int M, int N, int K, Mx4Type type)
+// What a plan may assume of the pointers and strides (scratch sizes assume the best).
+Plan plan_of(int M, int N, int K, Mx4Type type, bool wide = true)
 {
     Plan pl;
     if (M <= kFewRows) {
@@ -396,14 +600,26 @@ Plan plan_of(int M, int N, int K, Mx4Type type)
     }
     pl.chunks = (K + kTileK - 1) / kTileK;
     pl.shape = M <= 32 ? 0 : M <= 64 ? 1 : 2;
-    if (type == kMx4BF16 && int64_t((M + 255) / 256) * ((N + 255) / 256) >= 192)
-        pl.shape = 3;
+    // The wide tiles where they fill the GPU, of the height whose rounds over the
+    // CUs take least.
+    if (type == kMx4BF16 && K > 0 && K % kWideK == 0 && wide) {
+        int64_t best = INT64_MAX;
+        for (int sh = 3; sh < 6; ++sh) {
+            const TileShape &t = kShapes[sh];
+            const int64_t tiles = int64_t((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn);
+            const int64_t cost = (tiles + 255) / 256 * (t.bm + 32);
+            if (tiles >= 192 && cost < best) {
+                best = cost;
+                pl.shape = sh;
+            }
+        }
+    }
     const TileShape &s = kShapes[pl.shape];
     pl.tiles_m = (M + s.bm - 1) / s.bm;
     pl.tiles_n = (N + s.bn - 1) / s.bn;
     const int64_t tiles = int64_t(pl.tiles_m) * pl.tiles_n;
     int splits = int(std::min<int64_t>(256 / std::max<int64_t>(tiles, 1), pl.chunks / 4));
-    splits = std::max(1, std::min(splits, 16));
+    splits = pl.shape >= 3 ? 1 : std::max(1, std::min(splits, 16));
     pl.per_split = (pl.chunks + splits - 1) / splits;
     pl.splits = pl.per_split ? (pl.chunks + pl.per_split - 1) / pl.per_split : 1;
     return pl;
@@ -446,10 +662,14 @@ bool run_tiles(LinArgs &p, const Plan &pl, hipStream_t st)
         hipLaunchKernelGGL((linear_tile_kernel<T, 128, 128, 2, 2, VEC>), grid, dim3(256), 0, st,
                            p);
         break;
+    case 3:
+        hipLaunchKernelGGL((linear_wide_kernel<2>), grid, dim3(512), 0, st, p);
+        break;
+    case 4:
+        hipLaunchKernelGGL((linear_wide_kernel<3>), grid, dim3(512), 0, st, p);
+        break;
     default:
-        if constexpr (kTerms<T> == 1)
-            hipLaunchKernelGGL((linear_tile_kernel<T, 256, 256, 2, 4, VEC>), grid, dim3(512), 0,
-                               st, p);
+        hipLaunchKernelGGL((linear_wide_kernel<4>), grid, dim3(512), 0, st, p);
         break;
     }
     if (!hip_ok(hipGetLastError(), "linear_tile_kernel launch"))
@@ -464,10 +684,9 @@ bool run_tiles(LinArgs &p, const Plan &pl, hipStream_t st)
 }
 
 template <typename T>
-bool run_linear(LinArgs &p, const Plan &pl, hipStream_t st)
+bool run_linear(LinArgs &p, const Plan &pl, bool rows16, hipStream_t st)
 {
-    const int e = 16 / int(sizeof(T));
-    const bool vec = aligned(p.a, 16) && p.lda % e == 0 && p.K % 8 == 0;
+    const bool vec = rows16 && p.K % 8 == 0;
     if (pl.shape < 0)
         return vec ? run_few<T, true>(p, st) : run_few<T, false>(p, st);
     return vec ? run_tiles<T, true>(p, pl, st) : run_tiles<T, false>(p, pl, st);
@@ -489,7 +708,9 @@ bool launch_linear_mx4(const void *a, int64_t lda, const uint8_t *codes, const u
 {
     if (M <= 0 || N <= 0)
         return true;
-    Plan pl = plan_of(M, N, K, type);
+    const bool rows16 = aligned(a, 16) && lda % (type == kMx4F32 ? 4 : 8) == 0;
+    // Row offsets within a wide tile are 32-bit byte counts.
+    Plan pl = plan_of(M, N, K, type, rows16 && lda <= (1 << 22));
     LinArgs p{};
     p.a = a;
     p.codes = codes;
@@ -512,7 +733,8 @@ bool launch_linear_mx4(const void *a, int64_t lda, const uint8_t *codes, const u
             return fail("linear_mx4_dev: scratch must be 16-byte aligned");
         p.part = static_cast<float *>(scratch);
     }
-    return type == kMx4F32 ? run_linear<float>(p, pl, st) : run_linear<uint16_t>(p, pl, st);
+    return type == kMx4F32 ? run_linear<float>(p, pl, rows16, st)
+                           : run_linear<uint16_t>(p, pl, rows16, st);
 }
 
 }  // namespace anima_hip
