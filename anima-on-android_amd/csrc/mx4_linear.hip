@@ -6,17 +6,22 @@
 // bf16 terms whose sum is the f32 value (terms2), three MFMAs per product.
 // Sums are f32, and C is rounded once, to its own type.
 //
-// Two kernels:
+// Three kernels:
 //   * few rows (M <= 16), bound by the one pass over the codes (17/32 byte per
 //     weight) or, below about 8 MiB of codes, by latency: a workgroup takes 16
 //     weight rows, its waves share K in blocks of 128, and the weights go from
 //     memory to registers to the MFMA without touching LDS;
-//   * tiles (M > 16), bound by the MFMA at large M: A (as terms) and the decoded
-//     weights staged in LDS, two stages, split over K across workgroups where
-//     the tiles alone would leave CUs idle.
+//   * staged tiles (K a multiple of 128, 16-byte aligned rows of A), from 32 x 64 at
+//     small M to 192 x 256 (bf16) and 256 x 256 (f32): bound by latency and the stream
+//     into LDS at the small end, by the MFMA at the large;
+//   * plain tiles for every other K and alignment: A (as terms) and the decoded
+//     weights staged in LDS, two stages.
+// The last two split K across workgroups where the tiles alone would leave CUs idle.
 #include "mx4.h"
 
 #include <algorithm>
+#include <cmath>
+#include <iterator>
 
 namespace anima_hip {
 namespace {
@@ -359,96 +364,136 @@ __global__ __launch_bounds__(WM *WN * 64) void linear_tile_kernel(LinArgs p)
     }
 }
 
-// ----------------------------------------------------------- wide tiles
+// --------------------------------------------------------- staged tiles
 
-constexpr int kWideK = 128;   // K elements per chunk: 256-byte rows of A, 64 bytes of codes
-constexpr int kWideN = 256;   // weight rows of a tile
-
-// bf16 activations, K a multiple of 128, 16-byte aligned rows.  Tiles of
-// 64 MB x 256: 8 waves as 2 (M) x 4 (N), each 32 MB rows and 64 columns, C^T
-// on 32x32x16 MFMAs (W the first operand), so that a lane's four consecutive
+// K a multiple of 128 and 16-byte aligned rows of A.  Tiles of 32 MB WM rows of
+// A by 32 NB WN rows of W; waves as WM x WN x KS, each 32 MB x 32 NB of C on the
+// K steps of its share (KS > 1: the shares are added through LDS at the end).
+// C^T on 32x32x16 MFMAs, W the first operand, so that a lane's four consecutive
 // accumulators are four columns of one row.
-// A's rows and W's codes reach LDS by DMA, two stages of 128 elements of K; 16-byte
-// pieces are placed by piece ^ (row & 15) (A) and piece ^ (row / 4 & 3) (codes).
-// A lane takes 64 contiguous codes of a weight row from there, two scale groups,
-// and decodes them as the MFMA's k index wants them, k = 64 half + 8 step + j,
-// the order A is read in: the decoded weights never pass through LDS, whose reads
-// would take as long as the MFMAs with them (256 x 256 tiles with both operands
-// decoded to LDS: 200 us at 4608 x 8192 x 2048, this kernel 124 us).  Codes read
-// by each wave from memory instead, 16 bytes of 64 rows per instruction, kept
-// the address unit as busy as the MFMAs (146 us).
-// Bound by the MFMA at the clock that power allows: 1.25 PFLOP/s at that
-// size, where a library product of bf16 operands of 8192 x 8192 x 8192 runs 1.4.
-template <int MB>
-__global__ __launch_bounds__(512, 2) void linear_wide_kernel(LinArgs p)
+//
+// A's rows, W's codes and scales reach LDS by DMA through S stages.  A stage is 256
+// bytes of each row of A, 128 bf16 or 64 f32 elements, and the codes of as many;
+// 16-byte pieces are placed by piece ^ (row & 15) (A), ^ (row / 4 & 3) or
+// ^ (row / 8 & 1) (codes of 64 and of 32 bytes) against bank conflicts.
+// A lane takes the contiguous codes of its half of the chunk and decodes them in
+// registers, as the MFMA's k index wants them: k = KC / 2 half + 8 step + j, the
+// order A is read in.  f32 A is split into its three terms there too, once for
+// NB products.  With the decoded weights in LDS its reads take as long as the
+// MFMAs (256 x 256 tiles at 4608 x 8192 x 2048, bf16: 200 us, this kernel 124),
+// and codes read by each wave from memory, 16 bytes of 64 rows per
+// instruction, keep the address unit as busy as the MFMAs (146 us).
+// Fragments of a step are read, and its weights decoded, while the MFMAs of the
+// step before run; a chunk's first ones under the last step of the chunk before,
+// behind the barrier that ends it.
+template <typename T, int MB, int NB, int WM, int WN, int KS, int S>
+struct Staged {
+    static constexpr int NT = kTerms<T>;
+    static constexpr int WAVES = WM * WN * KS, THREADS = WAVES * 64;
+    static constexpr int BM = 32 * MB * WM, BN = 32 * NB * WN;
+    static constexpr int KC = 256 / int(sizeof(T));  // K elements of a chunk
+    static constexpr int STEPS = KC / 16, SHARE = STEPS / KS;
+    // LDS in u16: A rows of 128, codes rows of KC / 4, scales one dword a row.
+    static constexpr int A_EL = BM * 128, C_EL = BN * (KC / 4), STAGE = A_EL + C_EL + BN * 2;
+    // 1 KiB windows (scales: 256 bytes) per chunk, and per wave; a wave without
+    // one copies the last again, so that all count the same.
+    static constexpr int A_WIN = BM / 4, C_WIN = C_EL / 512, S_WIN = (BN + 63) / 64;
+    static constexpr int A_OPS = (A_WIN + WAVES - 1) / WAVES;
+    static constexpr int C_OPS = (C_WIN + WAVES - 1) / WAVES;
+    static constexpr int S_OPS = (S_WIN + WAVES - 1) / WAVES;
+    static constexpr int OPS = A_OPS + C_OPS + S_OPS;
+    // The epilogue's rows of one 32-row block per wave, and the shares' sums.
+    static constexpr int PITCH = 32 * NB + 16 / int(sizeof(T));
+    static constexpr int OUT_EL = WAVES / KS * 32 * PITCH * int(sizeof(T)) / 2;
+    static constexpr int RED_EL = (KS - 1) * (WAVES / KS) * MB * NB * 2048;
+    static constexpr int LDS =
+        S * STAGE > RED_EL ? (S * STAGE > OUT_EL ? S * STAGE : OUT_EL)
+                           : (RED_EL > OUT_EL ? RED_EL : OUT_EL);
+    static_assert(BN % 64 == 0 && STEPS % KS == 0 && LDS <= 81920, "160 KiB of LDS");
+    static_assert((S - 2) * OPS < 16, "counted by vmcnt");
+};
+
+// One dword per lane from base + voff to the 256-byte LDS window at `lds`, as
+// flash_tile::dma16s copies 16 bytes.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void dma4s(const void *base, unsigned voff, u16 *lds)
 {
-    constexpr int BM = 64 * MB;
-    constexpr int STAGE = BM * kWideK;
-    constexpr int WINDOWS = 2 * MB;  // 1 KiB DMA windows (4 rows) per wave and chunk
-    constexpr int NB = 2;
-    constexpr int CODES = kWideN * 64;  // bytes of a stage's codes
-    __shared__ __attribute__((aligned(16))) u16 smem[2 * STAGE + CODES];  // two stages of codes
+    const unsigned m0 = static_cast<unsigned>(
+        reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void *)lds));
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2"
+                 :
+                 : "s"(m0), "v"(voff), "s"(base)
+                 : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+template <typename T, int MB, int NB, int WM, int WN, int KS, int S>
+__global__ __launch_bounds__(WM *WN *KS * 64) void linear_staged_kernel(LinArgs p)
+{
+    using G = Staged<T, MB, NB, WM, WN, KS, S>;
+    constexpr int NT = G::NT;
+    __shared__ __attribute__((aligned(16))) u16 smem[G::LDS];
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wm = wave & 1, wn = wave >> 1;
+    const int wm = wave % WM, wn = wave / WM % WN, share = wave / (WM * WN);
     const int col = lane & 31, half = lane >> 5;
+    const int tiles = p.tiles_m * p.tiles_n;
     const int blk = xcd_major_block();
+    const int split = blk / tiles, t = blk - split * tiles;
     // Four M tiles by all N tiles at a time, M inside: the 32 CUs of an XCD work
     // on about 4 x 8 tiles.
-    const int band = blk / (4 * p.tiles_n), in_band = blk - band * 4 * p.tiles_n;
+    const int band = t / (4 * p.tiles_n), in_band = t - band * 4 * p.tiles_n;
     const int bm = min(4, p.tiles_m - 4 * band);
     const int tn = in_band / bm, tm = 4 * band + in_band - tn * bm;
-    const int row0 = tm * BM, col0 = tn * kWideN;
-    const int chunks = p.K / kWideK;
+    const int row0 = tm * G::BM, col0 = tn * G::BN;
+    const int c0 = split * p.per_split, c1 = min(c0 + p.per_split, p.K / G::KC);
 
-    unsigned off[WINDOWS];
+    // This lane's part of each copy, in bytes from the tile's first row; rows past
+    // M or N read the last one again (their results are not stored).
+    unsigned aoff[G::A_OPS], coff[G::C_OPS], soff[G::S_OPS];
+    int adst[G::A_OPS], cdst[G::C_OPS], sdst[G::S_OPS];
+    constexpr int CROWS = 2048 / G::KC;  // rows of a codes window
+    constexpr int CP = G::KC / 32;       // 16-byte pieces of a row's codes
 #pragma unroll
-    for (int i = 0; i < WINDOWS; ++i) {
-        const int r = (wave * WINDOWS + i) * 4 + (lane >> 4);
-        const int rr = min(row0 + r, p.M - 1) - row0;  // rows past M: not stored
-        off[i] = unsigned(int64_t(rr) * p.lda * 2 + 16 * ((lane & 15) ^ (r & 15)));
+    for (int i = 0; i < G::A_OPS; ++i) {
+        const int w = min(i * G::WAVES + wave, G::A_WIN - 1);
+        const int r = w * 4 + (lane >> 4);
+        aoff[i] = unsigned(int64_t(min(row0 + r, p.M - 1) - row0) * p.lda * int(sizeof(T)) +
+                           16 * ((lane & 15) ^ (r & 15)));
+        adst[i] = w * 512;
     }
-    const char *a0 = reinterpret_cast<const char *>(static_cast<const u16 *>(p.a) +
+#pragma unroll
+    for (int i = 0; i < G::C_OPS; ++i) {
+        const int w = min(i * G::WAVES + wave, G::C_WIN - 1);
+        const int r = w * CROWS + lane / CP;
+        const int piece = lane % CP ^ (CP == 4 ? r >> 2 & 3 : r >> 3 & 1);
+        coff[i] = unsigned((min(col0 + r, p.N - 1) - col0) * (p.K / 2) + 16 * piece);
+        cdst[i] = G::A_EL + w * 512;
+    }
+#pragma unroll
+    for (int i = 0; i < G::S_OPS; ++i) {
+        const int w = min(i * G::WAVES + wave, G::S_WIN - 1);
+        soff[i] = unsigned((min(col0 + w * 64 + lane, p.N - 1) - col0) * p.groups);
+        sdst[i] = G::A_EL + G::C_EL + w * 128;
+    }
+    const char *a0 = reinterpret_cast<const char *>(static_cast<const T *>(p.a) +
                                                     int64_t(row0) * p.lda);
-    // Codes: 16 windows of 16 rows x 64 bytes, two per wave, 16-byte pieces
-    // placed by piece ^ (row / 4 & 3).
-    unsigned woff[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int r = (wave * 2 + i) * 16 + (lane >> 2);
-        const int rr = min(col0 + r, p.N - 1) - col0;
-        woff[i] = unsigned(rr * (p.K / 2) + 16 * ((lane & 3) ^ (r >> 2 & 3)));
-    }
-    const char *w0 = reinterpret_cast<const char *>(p.codes + int64_t(col0) * (p.K / 2));
-    u16 *const smem_w = smem + 2 * STAGE;
+    const char *w0 = reinterpret_cast<const char *>(p.codes) + int64_t(col0) * (p.K / 2);
+    const char *s0 = reinterpret_cast<const char *>(p.scales) + int64_t(col0) * p.groups;
     auto dma = [&](int c, int stage) {
-        const char *src = a0 + int64_t(c) * (kWideK * 2);
+        u16 *dst = smem + stage * G::STAGE;
 #pragma unroll
-        for (int i = 0; i < WINDOWS; ++i)
-            dma16s(src, off[i], smem + stage * STAGE + (wave * WINDOWS + i) * 512);
+        for (int i = 0; i < G::A_OPS; ++i)
+            dma16s(a0 + int64_t(c) * 256, aoff[i], dst + adst[i]);
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-            dma16s(w0 + c * (kWideK / 2), woff[i],
-                   smem_w + stage * (CODES / 2) + (wave * 2 + i) * 512);
-    };
-
-    // The scales of this wave's 64 rows, one row per lane.
-    const uint8_t *ws = p.scales + int64_t(min(col0 + wn * 64 + lane, p.N - 1)) * p.groups;
-    unsigned sc[NB], sc_next = 0;
-    u32x4 codes[NB][2];
-    auto load = [&](int c) { sc_next = *reinterpret_cast<const unsigned *>(ws + c * 4); };
-    // Rows wn * 64 + 32 j + col: 64 codes of this half, and their two scales.
-    auto fetch = [&](int stage) {
+        for (int i = 0; i < G::C_OPS; ++i)
+            dma16s(w0 + int64_t(c) * (G::KC / 2), coff[i], dst + cdst[i]);
+        // Four scales a row: of this chunk, or of the pair of chunks it is in.
 #pragma unroll
-        for (int j = 0; j < NB; ++j) {
-            const int r = wn * 64 + 32 * j + col;
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-                codes[j][h] = *reinterpret_cast<const u32x4 *>(
-                    smem_w + stage * (CODES / 2) + r * 32 + ((2 * half + h) ^ (r >> 2 & 3)) * 8);
-            sc[j] = unsigned(__shfl(int(sc_next), 32 * j + col)) >> (16 * half) & 0xFFFFu;
-        }
+        for (int i = 0; i < G::S_OPS; ++i)
+            dma4s(s0 + (c * (G::KC / 32) & ~3), soff[i], dst + sdst[i]);
     };
 
     f32x16 acc[MB][NB];
@@ -460,107 +505,249 @@ __global__ __launch_bounds__(512, 2) void linear_wide_kernel(LinArgs p)
             for (int r = 0; r < 16; ++r)
                 acc[i][j][r] = 0.0f;
 
-    // Fragments of a step are read, and its weights decoded, while the MFMAs of
-    // the step before run; a chunk's first ones under the last step of the chunk
-    // before it, behind the barrier that ends that chunk.
-    bf16x8 af[2][MB], wf[2][NB];
+    constexpr int W = G::KC / 16;  // words of a lane's codes, 64 or 32 of them
+    unsigned codes[NB][W], sc[NB];
     unsigned ao = 0;
-    auto read = [&](int st, bf16x8 (&f)[MB]) {
+    typedef u32x4 Raw[NT == 3 ? 2 : 1];  // eight elements of A as they are stored
+    Raw raw[2][MB];
+    bf16x8 wf[2][NB];
+    auto read = [&](int st, Raw(&f)[MB]) {
 #pragma unroll
         for (int i = 0; i < MB; ++i)
-            f[i] = *reinterpret_cast<const bf16x8 *>(smem + 32 * i * kWideK + (ao ^ 8 * st));
+#pragma unroll
+            for (int h = 0; h < (NT == 3 ? 2 : 1); ++h)
+                f[i][h] = *reinterpret_cast<const u32x4 *>(
+                    smem + 32 * i * 128 + (ao ^ (NT == 3 ? 16 * st + 8 * h : 8 * st)));
     };
     auto decode = [&](int st, bf16x8 (&f)[NB]) {
 #pragma unroll
         for (int j = 0; j < NB; ++j)
-            f[j] = decode8(codes[j][st >> 2][st & 3],
-                           scale_of(st < 4 ? sc[j] & 255u : sc[j] >> 8));
+            f[j] = decode8(codes[j][st], scale_of(sc[j] >> (st >> 2) * 8 & 255u));
     };
-    // Chunk c is staged and its codes are here; the one after next may come.
     auto enter = [&](int c) {
-        wait_vmcnt<0>();
-        ring_barrier();
-        fetch(c & 1);
-        if (c + 1 < chunks) {
-            load(c + 1);
-            dma(c + 1, (c + 1) & 1);
-        }
-        // Piece 8 half + step of rows wm * 32 MB + 32 i + col.
-        ao = (c & 1) * STAGE + (wm * 32 * MB + col) * kWideK + ((8 * half) ^ (col & 15)) * 8;
+        // Chunk c has landed when at most the S - 2 behind it are on their way.
+        if (c + S - 2 < c1)
+            wait_vmcnt<(S - 2) * G::OPS>();
+        else
+            wait_vmcnt<0>();
+        ring_barrier();  // for every wave; and all have left the stage before it
+        if (c + S - 1 < c1)
+            dma(c + S - 1, (c + S - 1 - c0) % S);
+        const unsigned base = (c - c0) % S * G::STAGE;
+        // Rows (wm MB + i) 32 + col, this half of the chunk.
+        ao = base + (wm * 32 * MB + col) * 128 + ((8 * half) ^ (col & 15)) * 8;
         asm volatile("" : "+v"(ao));
-    };
-    load(0);
-    dma(0, 0);
-    enter(0);
-    read(0, af[0]);
-    decode(0, wf[0]);
-    for (int c = 0; c < chunks; ++c) {
 #pragma unroll
-        for (int st = 0; st < 8; ++st) {
-            if (st < 7)
-                read(st + 1, af[(st + 1) & 1]);
-            else if (c + 1 < chunks) {
+        for (int j = 0; j < NB; ++j) {
+            const int r = (wn * NB + j) * 32 + col;
+            const u16 *row = smem + base + G::A_EL + r * (G::KC / 4);
+#pragma unroll
+            for (int h = 0; h < W / 4; ++h) {
+                const int piece = CP == 4 ? (2 * half + h) ^ (r >> 2 & 3) : half ^ (r >> 3 & 1);
+                const u32x4 v = *reinterpret_cast<const u32x4 *>(row + 8 * piece);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    codes[j][4 * h + e] = v[e];
+            }
+            const unsigned s4 = *reinterpret_cast<const unsigned *>(smem + base + G::A_EL +
+                                                                    G::C_EL + r * 2);
+            sc[j] = s4 >> (CP == 4 ? 16 * half : 16 * (c & 1) + 8 * half);
+        }
+    };
+    auto multiply = [&](const Raw(&f)[MB], const bf16x8 (&w)[NB]) {
+#pragma unroll
+        for (int i = 0; i < MB; ++i) {
+            bf16x8 term[NT];
+            if constexpr (NT == 3) {
+                const f32x4 x[2] = {__builtin_bit_cast(f32x4, f[i][0]),
+                                    __builtin_bit_cast(f32x4, f[i][1])};
+                u32x4 u[3];
+                split_terms8(x, u);
+#pragma unroll
+                for (int q = 0; q < 3; ++q)
+                    term[q] = __builtin_bit_cast(bf16x8, u[q]);
+            } else
+                term[0] = __builtin_bit_cast(bf16x8, f[i][0]);
+#pragma unroll
+            for (int q = 0; q < NT; ++q)
+#pragma unroll
+                for (int j = 0; j < NB; ++j)
+                    acc[i][j] = mfma_bf16(w[j], term[q], acc[i][j]);
+        }
+    };
+
+    // This wave's steps of a chunk: share * SHARE .. .  The step within the
+    // share is a constant where codes and scales are picked from registers.
+    auto step_of = [&](int i) { return KS == 1 ? i : share * G::SHARE + i; };
+    auto pick = [&](int i, bf16x8 (&f)[NB]) {
+        if constexpr (KS == 1)
+            decode(i, f);
+        else
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+                if (share == k)
+                    decode(k * G::SHARE + i, f);
+    };
+    static_assert(S >= 2, "a stage to fill while one is used");
+    if (c0 < c1) {
+#pragma unroll
+        for (int i = 0; i < S - 1; ++i)
+            if (c0 + i < c1)
+                dma(c0 + i, i);
+        enter(c0);
+        read(step_of(0), raw[0]);
+        pick(0, wf[0]);
+    }
+    for (int c = c0; c < c1; ++c) {
+#pragma unroll
+        for (int st = 0; st < G::SHARE; ++st) {
+            constexpr int LAST = G::SHARE - 1;
+            const int now = G::SHARE == 1 ? 0 : st & 1, next = G::SHARE == 1 ? 1 : now ^ 1;
+            if (st < LAST)
+                read(step_of(st + 1), raw[next]);
+            else if (c + 1 < c1) {
                 enter(c + 1);
-                read(0, af[0]);
+                read(step_of(0), raw[next]);
             }
             __builtin_amdgcn_sched_barrier(0);
+            multiply(raw[now], wf[now]);
+            pick(st < LAST ? st + 1 : 0, wf[next]);
+            if (G::SHARE % 2 == 1 && st == LAST) {
+#pragma unroll
+                for (int i = 0; i < MB; ++i)
+#pragma unroll
+                    for (int h = 0; h < (NT == 3 ? 2 : 1); ++h)
+                        raw[0][i][h] = raw[next][i][h];
+#pragma unroll
+                for (int j = 0; j < NB; ++j)
+                    wf[0][j] = wf[next][j];
+            }
+        }
+    }
+
+    __syncthreads();
+    if constexpr (KS > 1) {
+        // The shares' sums, in their order.
+        f32x4 *red = reinterpret_cast<f32x4 *>(smem);
+        constexpr int BLOCKS = WM * WN * MB * NB;
+        const int w0i = wave % (WM * WN);
+        if (share > 0)
 #pragma unroll
             for (int i = 0; i < MB; ++i)
 #pragma unroll
                 for (int j = 0; j < NB; ++j)
-                    acc[i][j] = mfma_bf16(wf[st & 1][j], af[st & 1][i], acc[i][j]);
-            decode((st + 1) & 7, wf[(st + 1) & 1]);
-        }
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        red[(((share - 1) * BLOCKS + (w0i * MB + i) * NB + j) * 4 + q) * 64 + lane] =
+                            f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
+                                  acc[i][j][4 * q + 3]};
+        __syncthreads();
+        if (share == 0)
+#pragma unroll
+            for (int k = 0; k < KS - 1; ++k)
+#pragma unroll
+                for (int i = 0; i < MB; ++i)
+#pragma unroll
+                    for (int j = 0; j < NB; ++j)
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const f32x4 v =
+                                red[((k * BLOCKS + (w0i * MB + i) * NB + j) * 4 + q) * 64 + lane];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                acc[i][j][4 * q + e] += v[e];
+                        }
+        __syncthreads();
+        if (share > 0)
+            return;
     }
 
-    // Lane (col, half): row col of its blocks, columns acc_row(r, half).  Through
-    // LDS, so that rows go out in 128-byte runs.
-    __syncthreads();
-    constexpr int PITCH = 72;  // bf16 elements of a staged row: 64 and 16 bytes against conflicts
-    static_assert(8 * 32 * PITCH <= 2 * STAGE, "the staged rows fit");
-    u16 *so = smem + wave * 32 * PITCH;
-    const int n0 = col0 + wn * 64;
-    const bool wide = (reinterpret_cast<uintptr_t>(p.c) & 15) == 0 && p.ldc % 8 == 0 &&
-                      n0 + 64 <= p.N;
+    // Lane (col, half): row col of its blocks, columns acc_row(r, half).
+    const int n0 = col0 + wn * 32 * NB;
+    if (p.part) {
+        float *plane = p.part + int64_t(split) * p.M * p.N;
+        const bool wide = p.N % 4 == 0;
+#pragma unroll
+        for (int i = 0; i < MB; ++i) {
+            const int m = row0 + (wm * MB + i) * 32 + col;
+            if (m >= p.M)
+                continue;
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4) {
+                    const int nn = n0 + 32 * j + acc_row(r, half);
+                    float *dst = plane + int64_t(m) * p.N + nn;
+                    if (wide && nn < p.N)
+                        *reinterpret_cast<f32x4 *>(dst) = f32x4{acc[i][j][r], acc[i][j][r + 1],
+                                                                acc[i][j][r + 2], acc[i][j][r + 3]};
+                    else
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (nn + e < p.N)
+                                dst[e] = acc[i][j][r + e];
+                }
+        }
+        return;
+    }
+    // Through LDS, so that rows go out in runs of 32 NB columns.
+    T *so = reinterpret_cast<T *>(smem) + (wave % (WM * WN)) * 32 * G::PITCH;
+    constexpr int E = 16 / int(sizeof(T));  // elements of a 16-byte piece
+    constexpr int PIECES = 32 * NB / E;
+    const bool wide = (reinterpret_cast<uintptr_t>(p.c) & 15) == 0 && p.ldc % E == 0 &&
+                      n0 + 32 * NB <= p.N;
 #pragma unroll
     for (int i = 0; i < MB; ++i) {
 #pragma unroll
         for (int j = 0; j < NB; ++j)
 #pragma unroll
             for (int r = 0; r < 16; r += 4) {
-                u32x2 v;
+                T *dst = so + col * G::PITCH + 32 * j + acc_row(r, half);
+                if constexpr (NT == 3)
+                    *reinterpret_cast<f32x4 *>(dst) = f32x4{acc[i][j][r], acc[i][j][r + 1],
+                                                            acc[i][j][r + 2], acc[i][j][r + 3]};
+                else {
+                    u32x2 v;
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
-                    v[e] = __builtin_bit_cast(
-                        unsigned, __builtin_convertvector(f32x2{acc[i][j][r + 2 * e],
-                                                                acc[i][j][r + 2 * e + 1]},
-                                                          bf16x2));
-                *reinterpret_cast<u32x2 *>(so + col * PITCH + 32 * j + acc_row(r, half)) = v;
+                    for (int e = 0; e < 2; ++e)
+                        v[e] = __builtin_bit_cast(
+                            unsigned, __builtin_convertvector(f32x2{acc[i][j][r + 2 * e],
+                                                                    acc[i][j][r + 2 * e + 1]},
+                                                              bf16x2));
+                    *reinterpret_cast<u32x2 *>(dst) = v;
+                }
             }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int r = 8 * q + (lane >> 3), piece = lane & 7;
+        for (int q = 0; q < PIECES / 2; ++q) {
+            const int f = q * 64 + lane, r = f / PIECES, piece = f % PIECES;
             const int m = row0 + (wm * MB + i) * 32 + r;
-            const u32x4 v = *reinterpret_cast<const u32x4 *>(so + r * PITCH + 8 * piece);
+            const u32x4 v = *reinterpret_cast<const u32x4 *>(so + r * G::PITCH + E * piece);
             if (m >= p.M)
                 continue;
-            u16 *dst = static_cast<u16 *>(p.c) + int64_t(m) * p.ldc + n0 + 8 * piece;
+            const int nn = n0 + E * piece;
+            T *dst = static_cast<T *>(p.c) + int64_t(m) * p.ldc + nn;
             if (wide)
                 __builtin_nontemporal_store(v, reinterpret_cast<u32x4 *>(dst));
             else
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (n0 + 8 * piece + e < p.N)
-                        dst[e] = u16(v[e >> 1] >> (16 * (e & 1)));
+                for (int e = 0; e < E; ++e)
+                    if (nn + e < p.N) {
+                        if constexpr (NT == 3)
+                            dst[e] = __uint_as_float(v[e]);
+                        else
+                            dst[e] = u16(v[e >> 1] >> (16 * (e & 1)));
+                    }
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
     }
 }
 
-// C = the planes' sum, in split order.
+// C = the planes' sum, in split order (at most 16 of them), all loads in flight.
+constexpr int kMaxSplits = 16;
+
 template <typename T>
 __global__ __launch_bounds__(256) void linear_sum_kernel(const float *part, T *c, int64_t ldc,
                                                          int M, int N, int splits)
@@ -569,59 +756,123 @@ __global__ __launch_bounds__(256) void linear_sum_kernel(const float *part, T *c
     const int64_t plane = int64_t(M) * N;
     if (i >= plane)
         return;
-    float sum = part[i];
-    for (int s = 1; s < splits; ++s)
-        sum += part[s * plane + i];
+    float x[kMaxSplits];
+#pragma unroll
+    for (int s = 0; s < kMaxSplits; ++s)
+        if (s < splits)
+            x[s] = part[s * plane + i];
+    float sum = x[0];
+#pragma unroll
+    for (int s = 1; s < kMaxSplits; ++s)
+        if (s < splits)
+            sum += x[s];
     const int64_t m = i / N;
     store_c(c + m * ldc + (i - m * N), sum);
 }
 
 // ----------------------------------------------------------------- plans
 
+// Shapes of the staged kernel: MB, NB, WM, WN, KS, S.
+#define STAGED_BF16(X) \
+    X(0, 3, 2, 2, 4, 1, 2) X(1, 2, 2, 2, 4, 1, 2) X(2, 2, 2, 2, 2, 2, 2) X(3, 1, 2, 2, 2, 2, 3) \
+    X(4, 1, 1, 2, 2, 2, 4) X(5, 1, 1, 1, 2, 4, 4)
+#define STAGED_F32(X) \
+    X(0, 2, 4, 4, 2, 1, 2) X(1, 1, 4, 4, 2, 1, 3) X(2, 1, 4, 2, 1, 4, 3) X(3, 1, 2, 1, 1, 4, 4)
+
 struct TileShape {
     int bm, bn;
+    // Microseconds of a workgroup per chunk of K (256 bytes of a row of A) where half
+    // the CUs have one, and where all have (large tiles: at a lower clock; small
+    // ones: several workgroups on a CU, per workgroup).
+    double half_us, full_us;
 };
-// The last three are the wide kernel's.
-constexpr TileShape kShapes[] = {{32, 128},  {64, 128},  {128, 128},
-                                 {128, 256}, {192, 256}, {256, 256}};
+// Measured at M from 24 to 4096, N x K of 2048 x 2048, 2048 x 8192, 8192 x 2048,
+// 6144 x 256 and 256 x 2048; the model below is within 15 % of most of them.
+constexpr TileShape kBf16Shapes[] = {{192, 256, 2.0, 2.45}, {128, 256, 1.24, 1.7},
+                                     {128, 128, 0.93, 1.15}, {64, 128, 0.66, 0.62},
+                                     {64, 64, 0.47, 0.58},   {32, 64, 0.37, 0.36}};
+constexpr TileShape kF32Shapes[] = {{256, 256, 4.2, 5.4}, {128, 256, 2.33, 2.75},
+                                    {64, 128, 1.0, 1.02}, {32, 64, 0.52, 0.33}};
+constexpr TileShape kTileShapes[] = {{32, 128, 0, 0}, {64, 128, 0, 0}, {128, 128, 0, 0}};
+#define SHAPE_CHECK(table, i, mb, nb, wm, wn) \
+    static_assert(table[i].bm == 32 * mb * wm && table[i].bn == 32 * nb * wn, "shape table");
+#define CHECK_BF16(i, mb, nb, wm, wn, ks, s) SHAPE_CHECK(kBf16Shapes, i, mb, nb, wm, wn)
+#define CHECK_F32(i, mb, nb, wm, wn, ks, s) SHAPE_CHECK(kF32Shapes, i, mb, nb, wm, wn)
+STAGED_BF16(CHECK_BF16)
+STAGED_F32(CHECK_F32)
 
+enum Kernel { kFew, kTiles, kStaged };
 struct Plan {
-    int shape;  // -1: few rows
+    Kernel kernel = kFew;
+    int shape = 0;
     int tiles_m = 0, tiles_n = 0, splits = 1, per_split = 0, chunks = 0;
 };
 
-// What a plan may assume of the pointers and strides (scratch sizes assume the best).
-Plan plan_of(int M, int N, int K, Mx4Type type, bool wide = true)
+// The tile grid of a shape with K shared out over up to `splits` workgroups.
+void set_grid(Plan &pl, const TileShape &t, int M, int N, int splits)
 {
-    Plan pl;
-    if (M <= kFewRows) {
-        pl.shape = -1;
-        return pl;
-    }
-    pl.chunks = (K + kTileK - 1) / kTileK;
-    pl.shape = M <= 32 ? 0 : M <= 64 ? 1 : 2;
-    // The wide tiles where they fill the GPU, of the height whose rounds over the
-    // CUs take least.
-    if (type == kMx4BF16 && K > 0 && K % kWideK == 0 && wide) {
-        int64_t best = INT64_MAX;
-        for (int sh = 3; sh < 6; ++sh) {
-            const TileShape &t = kShapes[sh];
-            const int64_t tiles = int64_t((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn);
-            const int64_t cost = (tiles + 255) / 256 * (t.bm + 32);
-            if (tiles >= 192 && cost < best) {
-                best = cost;
-                pl.shape = sh;
-            }
-        }
-    }
-    const TileShape &s = kShapes[pl.shape];
-    pl.tiles_m = (M + s.bm - 1) / s.bm;
-    pl.tiles_n = (N + s.bn - 1) / s.bn;
-    const int64_t tiles = int64_t(pl.tiles_m) * pl.tiles_n;
-    int splits = int(std::min<int64_t>(256 / std::max<int64_t>(tiles, 1), pl.chunks / 4));
-    splits = pl.shape >= 3 ? 1 : std::max(1, std::min(splits, 16));
+    pl.tiles_m = (M + t.bm - 1) / t.bm;
+    pl.tiles_n = (N + t.bn - 1) / t.bn;
     pl.per_split = (pl.chunks + splits - 1) / splits;
     pl.splits = pl.per_split ? (pl.chunks + pl.per_split - 1) / pl.per_split : 1;
+}
+
+// Predicted time of a staged grid: 4 us of latency and epilogue, the chunks of the
+// fullest CU, and the sum of the planes.
+double staged_us(const Plan &pl, const TileShape &t, int M, int N)
+{
+    const double wgs = double(pl.tiles_m) * pl.tiles_n * pl.splits;
+    const double rounds = std::ceil(wgs / 256);
+    const double load = std::min(1.0, std::max(0.0, wgs / 128 - 1));
+    const double alone = t.half_us + (t.full_us > t.half_us ? (t.full_us - t.half_us) * load : 0);
+    double us = 4.2 + pl.per_split * (rounds > 1 ? std::max(alone, rounds * t.full_us) : alone);
+    if (pl.splits > 1)
+        us += 2.3 + double(pl.splits) * M * N * 4 / 1.8e6;
+    return us;
+}
+
+// `staged`: the pointers and strides suit the staged kernel.
+Plan plan_of(int M, int N, int K, Mx4Type type, bool staged)
+{
+    const bool f32 = type == kMx4F32;
+    Plan pl;
+    // Few rows, unless their terms take long to stage in every workgroup: 16 rows of
+    // 8192 bf16 take 12.5 us against 9.8 (N = 2048), 8 rows of 8192 f32 18 against
+    // 15, 16 of 2048 13 against 8.8; 4 rows of 8192 f32 12 against 15, 16 of 2048
+    // bf16 5.5 against 7.4.
+    const int64_t terms = int64_t(M) * (f32 ? 3 : 1);
+    if (M <= kFewRows &&
+        (!staged || K % 128 || terms * K <= 24576 || (terms <= 24 && terms * K <= 100000)))
+        return pl;
+    if (staged && K > 0 && K % 128 == 0) {
+        pl.kernel = kStaged;
+        pl.chunks = K / (f32 ? 64 : 128);
+        Plan best = pl;
+        double best_us = 1e300;
+        const int n = f32 ? int(std::size(kF32Shapes)) : int(std::size(kBf16Shapes));
+        for (pl.shape = 0; pl.shape < n; ++pl.shape)
+            for (int splits = 1; splits <= 8; splits *= 2) {
+                const TileShape &t = f32 ? kF32Shapes[pl.shape] : kBf16Shapes[pl.shape];
+                if (splits > 1 && (splits > pl.chunks || double(M) * N * splits > 256.0 * 32768 * 2))
+                    break;
+                set_grid(pl, t, M, N, splits);
+                const double us = staged_us(pl, t, M, N);
+                if (us < best_us) {
+                    best_us = us;
+                    best = pl;
+                }
+            }
+        return best;
+    }
+    pl.kernel = kTiles;
+    pl.shape = M <= 32 ? 0 : M <= 64 ? 1 : 2;
+    pl.chunks = (K + kTileK - 1) / kTileK;
+    const TileShape &t = kTileShapes[pl.shape];
+    set_grid(pl, t, M, N, 1);
+    const int64_t tiles = int64_t(pl.tiles_m) * pl.tiles_n;
+    const int64_t splits = std::min<int64_t>({256 / tiles, pl.chunks / 4, kMaxSplits});
+    if (splits > 1)
+        set_grid(pl, t, M, N, int(splits));
     return pl;
 }
 
@@ -645,51 +896,63 @@ bool run_few(LinArgs &p, hipStream_t st)
 }
 
 template <typename T, bool VEC>
-bool run_tiles(LinArgs &p, const Plan &pl, hipStream_t st)
+bool run_tiles(const LinArgs &p, int shape, dim3 grid, hipStream_t st)
 {
-    const int64_t blocks = int64_t(pl.tiles_m) * pl.tiles_n * pl.splits;
-    if (blocks > INT32_MAX)
-        return fail("linear_mx4_dev: too many tiles");
-    const dim3 grid(static_cast<unsigned>(blocks));
-    switch (pl.shape) {
+    switch (shape) {
     case 0:
         hipLaunchKernelGGL((linear_tile_kernel<T, 32, 128, 1, 4, VEC>), grid, dim3(256), 0, st, p);
         break;
     case 1:
         hipLaunchKernelGGL((linear_tile_kernel<T, 64, 128, 2, 2, VEC>), grid, dim3(256), 0, st, p);
         break;
-    case 2:
+    default:
         hipLaunchKernelGGL((linear_tile_kernel<T, 128, 128, 2, 2, VEC>), grid, dim3(256), 0, st,
                            p);
         break;
-    case 3:
-        hipLaunchKernelGGL((linear_wide_kernel<2>), grid, dim3(512), 0, st, p);
-        break;
-    case 4:
-        hipLaunchKernelGGL((linear_wide_kernel<3>), grid, dim3(512), 0, st, p);
-        break;
-    default:
-        hipLaunchKernelGGL((linear_wide_kernel<4>), grid, dim3(512), 0, st, p);
-        break;
     }
-    if (!hip_ok(hipGetLastError(), "linear_tile_kernel launch"))
-        return false;
-    if (pl.splits > 1) {
-        const int64_t n = int64_t(p.M) * p.N;
-        hipLaunchKernelGGL(linear_sum_kernel<T>, dim3(unsigned((n + 255) / 256)), dim3(256), 0, st,
-                           p.part, static_cast<T *>(p.c), p.ldc, p.M, p.N, pl.splits);
-        return hip_ok(hipGetLastError(), "linear_sum_kernel launch");
+    return hip_ok(hipGetLastError(), "linear_tile_kernel launch");
+}
+
+#define STAGED_CASE(i, mb, nb, wm, wn, ks, s)                                                    \
+    case i:                                                                                       \
+        hipLaunchKernelGGL((linear_staged_kernel<T, mb, nb, wm, wn, ks, s>), grid,               \
+                           dim3(wm * wn * ks * 64), 0, st, p);                                   \
+        break;
+
+template <typename T>
+bool run_staged(const LinArgs &p, int shape, dim3 grid, hipStream_t st)
+{
+    if constexpr (kTerms<T> == 1) {
+        switch (shape) {
+            STAGED_BF16(STAGED_CASE)
+        }
+    } else {
+        switch (shape) {
+            STAGED_F32(STAGED_CASE)
+        }
     }
-    return true;
+    return hip_ok(hipGetLastError(), "linear_staged_kernel launch");
 }
 
 template <typename T>
 bool run_linear(LinArgs &p, const Plan &pl, bool rows16, hipStream_t st)
 {
     const bool vec = rows16 && p.K % 8 == 0;
-    if (pl.shape < 0)
+    if (pl.kernel == kFew)
         return vec ? run_few<T, true>(p, st) : run_few<T, false>(p, st);
-    return vec ? run_tiles<T, true>(p, pl, st) : run_tiles<T, false>(p, pl, st);
+    const int64_t blocks = int64_t(pl.tiles_m) * pl.tiles_n * pl.splits;
+    if (blocks > INT32_MAX)
+        return fail("linear_mx4_dev: too many tiles");
+    const dim3 grid(static_cast<unsigned>(blocks));
+    const bool ok = pl.kernel == kStaged ? run_staged<T>(p, pl.shape, grid, st)
+                    : vec                ? run_tiles<T, true>(p, pl.shape, grid, st)
+                                         : run_tiles<T, false>(p, pl.shape, grid, st);
+    if (!ok || pl.splits == 1)
+        return ok;
+    const int64_t n = int64_t(p.M) * p.N;
+    hipLaunchKernelGGL(linear_sum_kernel<T>, dim3(unsigned((n + 255) / 256)), dim3(256), 0, st,
+                       p.part, static_cast<T *>(p.c), p.ldc, p.M, p.N, pl.splits);
+    return hip_ok(hipGetLastError(), "linear_sum_kernel launch");
 }
 
 }  // namespace
@@ -698,8 +961,10 @@ size_t linear_mx4_scratch_bytes(int M, int N, int K, Mx4Type type)
 {
     if (M <= 0 || N <= 0 || K <= 0)
         return 0;
-    const Plan pl = plan_of(M, N, K, type);
-    return pl.splits > 1 ? size_t(pl.splits) * size_t(M) * size_t(N) * 4 : 0;
+    // For any pointers and strides.
+    const int splits = std::max(plan_of(M, N, K, type, true).splits,
+                                plan_of(M, N, K, type, false).splits);
+    return splits > 1 ? size_t(splits) * size_t(M) * size_t(N) * 4 : 0;
 }
 
 bool launch_linear_mx4(const void *a, int64_t lda, const uint8_t *codes, const uint8_t *scales,
@@ -709,8 +974,8 @@ bool launch_linear_mx4(const void *a, int64_t lda, const uint8_t *codes, const u
     if (M <= 0 || N <= 0)
         return true;
     const bool rows16 = aligned(a, 16) && lda % (type == kMx4F32 ? 4 : 8) == 0;
-    // Row offsets within a wide tile are 32-bit byte counts.
-    Plan pl = plan_of(M, N, K, type, rows16 && lda <= (1 << 22));
+    // Row offsets within a staged tile are 32-bit byte counts (of up to 256 rows).
+    const Plan pl = plan_of(M, N, K, type, rows16 && lda <= (1 << 21) && K <= (1 << 22));
     LinArgs p{};
     p.a = a;
     p.codes = codes;
@@ -726,13 +991,15 @@ bool launch_linear_mx4(const void *a, int64_t lda, const uint8_t *codes, const u
     p.tiles_n = pl.tiles_n;
     p.chunks = pl.chunks;
     p.per_split = pl.per_split;
-    if (pl.splits > 1) {
-        if (scratch_bytes < linear_mx4_scratch_bytes(M, N, K, type) || !scratch)
+    const size_t need = linear_mx4_scratch_bytes(M, N, K, type);
+    if (need > 0) {
+        if (scratch_bytes < need || !scratch)
             return fail("linear_mx4_dev: scratch smaller than anima_hip_linear_mx4_scratch_bytes");
         if (!aligned(scratch, 16))
             return fail("linear_mx4_dev: scratch must be 16-byte aligned");
-        p.part = static_cast<float *>(scratch);
     }
+    if (pl.splits > 1)
+        p.part = static_cast<float *>(scratch);
     return type == kMx4F32 ? run_linear<float>(p, pl, rows16, st)
                            : run_linear<uint16_t>(p, pl, rows16, st);
 }
