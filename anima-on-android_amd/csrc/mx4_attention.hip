@@ -839,87 +839,133 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void kv4_tile_kernel(AttnArgs a
 }
 
 // O = sum_s w_s P_s / sum_s w_s, w_s = l_s 2^(m_s - max m), over the splits
-// that saw a key (at most 64).  One workgroup per row: in each wave lane s
-// weighs split s; wave w adds the splits w, w + 4, .., its loads all in flight,
+// that saw a key (at most 64).  PER waves per row: in each, lane s weighs split s;
+// wave w adds the splits w, w + PER, .., at most 16, its loads all in flight,
 // D / 64 dimensions per lane, and the waves' sums are added in their order.
 constexpr int kMaxSplits = 64;
 
-template <typename T, int D>
+template <typename T, int D, int PER>
 __global__ __launch_bounds__(256) void kv4_join_kernel(AttnArgs a)
 {
     constexpr int E = D / 64;
     const Kv4Attention &p = a.p;
     const int64_t plane = int64_t(p.B) * p.S_q * p.H;
-    __shared__ float part[4][D];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t row = blockIdx.x;
-    const int h = int(row % p.H);
-    const int64_t bs = row / p.H;
-    const int b = int(bs / p.S_q), s = int(bs % p.S_q);
+    const unsigned row = blockIdx.x * unsigned(4 / PER) + unsigned(PER == 4 ? 0 : wave);
+    const int first = PER == 4 ? wave : 0;
+    if (row >= unsigned(plane))
+        return;  // whole wave; with PER == 4 no workgroup
+    const unsigned bs = row / unsigned(p.H), b = bs / unsigned(p.S_q);
+    const int h = int(row - bs * unsigned(p.H)), s = int(bs - b * unsigned(p.S_q));
     if (p.counts && s >= p.counts[b])
-        return;
+        return;  // likewise
+    const float *src = a.part + int64_t(row) * D + lane * E;
+    float x[kMaxSplits / 4][E], v[E] = {};
+#pragma unroll
+    for (int k = 0; k < kMaxSplits / 4; ++k)
+        if (first + PER * k < a.splits)
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                x[k][e] = src[(first + PER * k) * plane * D + e];
     const float2 ml = lane < a.splits ? a.ml[lane * plane + row] : float2{-INFINITY, 0.0f};
     float m = ml.y == 0.0f ? -INFINITY : ml.x;
 #pragma unroll
     for (int o = 32; o; o >>= 1)
         m = fmaxf(m, __shfl_xor(m, o));
     // A split of which no key was seen weighs nothing, whatever its maximum.
-    float w = ml.y == 0.0f ? 0.0f
-                           : (ml.x == m ? 1.0f : __builtin_amdgcn_exp2f(ml.x - m)) * ml.y;
+    const float w = ml.y == 0.0f
+                        ? 0.0f
+                        : (ml.x == m ? 1.0f : __builtin_amdgcn_exp2f(ml.x - m)) * ml.y;
     float l = w;
 #pragma unroll
     for (int o = 32; o; o >>= 1)
         l += __shfl_xor(l, o);
-    const float *src = a.part + row * D + lane * E;
-    float x[kMaxSplits / 4][E], v[E] = {};
 #pragma unroll
     for (int k = 0; k < kMaxSplits / 4; ++k)
-        if (wave + 4 * k < a.splits)
-#pragma unroll
-            for (int e = 0; e < E; ++e)
-                x[k][e] = src[(wave + 4 * k) * plane * D + e];
-#pragma unroll
-    for (int k = 0; k < kMaxSplits / 4; ++k)
-        if (wave + 4 * k < a.splits) {
-            const float wk = __shfl(w, wave + 4 * k);
+        if (first + PER * k < a.splits) {
+            const float wk = __shfl(w, first + PER * k);
             if (wk != 0.0f)
 #pragma unroll
                 for (int e = 0; e < E; ++e)
                     v[e] += wk * x[k][e];
         }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    T *out = static_cast<T *>(p.o) + b * p.os.b + h * p.os.h + s * p.os.s;
+    if constexpr (PER == 1) {
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-        part[wave][lane * E + e] = v[e];
-    __syncthreads();
-    const int d = threadIdx.x;
-    if (d < D) {
-        const float o = part[0][d] + part[1][d] + part[2][d] + part[3][d];
-        store_o(static_cast<T *>(p.o) + b * p.os.b + h * p.os.h + s * p.os.s + d,
-                l == 0.0f ? 0.0f : o / l);
+        for (int e = 0; e < E; ++e)
+            store_o(out + lane * E + e, v[e] * inv);
+    } else {
+        __shared__ float part[4][D];
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            part[wave][lane * E + e] = v[e];
+        __syncthreads();
+        const int d = threadIdx.x;
+        if (d < D)
+            store_o(out + d, (part[0][d] + part[1][d] + part[2][d] + part[3][d]) * inv);
     }
 }
 
 struct Plan {
-    bool tile;  // the tile kernel
-    int tiles, splits;
+    bool tile = false;  // the tile kernel
+    int tiles = 0, splits = 1;
 };
 
-Plan plan_of(int B, int S_q, int H, int H_kv, int S_max)
+// Microseconds of a workgroup per 128 keys (token kernel, 16 query rows) and per 64 keys
+// (tile kernel, 128 rows), alone on a CU and as its share of a CU that has two;
+// bf16 and f32 queries, D of 64 and 128.  Measured at one query to 2048 over 200 to
+// 20000 keys.
+struct Rate {
+    double token1, token2, tile1, tile2;
+};
+constexpr Rate kRates[2][2] = {{{0.65, 0.46, 1.45, 0.9}, {0.78, 0.62, 1.75, 1.45}},
+                               {{0.8, 0.59, 2.15, 1.85}, {1.05, 0.85, 4.8, 3.0}}};
+
+// The kernel and the split that the model expects to take least: about 6 us of
+// latency, the keys of the longest share or of a full CU, and with splits the partial
+// results written and joined.  The token kernel, which meets at no barrier, is ahead to
+// some hundred query rows of a K/V head and in f32 further: 2048 rows of 512 keys,
+// 4 K/V heads, take 10.8 us by it and 18.7 by the tile kernel (bf16); 4096 x 512 keys,
+// 32 heads, 50 us by the tile kernel against 141 by the first token kernel.
+Plan plan_of(int B, int S_q, int H, int H_kv, int D, int S_max, Mx4Type type, bool causal)
 {
+    const Rate &rate = kRates[type == kMx4F32][D == 128];
     const int64_t rows = int64_t(S_q) * (H / H_kv);
-    Plan pl;
-    pl.tile = rows > 32;
-    const int per_tile = pl.tile ? kTileRows : kTokRows;
-    pl.tiles = int((rows + per_tile - 1) / per_tile);
-    const int64_t groups = std::max<int64_t>(1, int64_t(B) * H_kv * pl.tiles);
-    // Splits until the grid has two workgroups per CU,
-    // or a share is two tiles of keys, or four rounds of a workgroup's waves.
-    const int round = pl.tile ? 2 * kTileKeys : 4 * kTokKeys * kTokWaves;
-    const int64_t rounds = (int64_t(S_max) + round - 1) / round;
-    pl.splits = int(std::max<int64_t>(
-        1, std::min<int64_t>({512 / groups, rounds, kMaxSplits})));
-    return pl;
+    // Under a causal mask the query tiles see S_max - S_q .. S_max keys.
+    const double part = causal && S_q > 1 && S_max > 0
+                            ? 1.0 - 0.5 * std::min(S_q, S_max) / S_max : 1.0;
+    Plan best;
+    double best_us = 1e300;
+    for (int tile = 0; tile < 2; ++tile) {
+        Plan pl;
+        pl.tile = tile != 0;
+        const int per_tile = pl.tile ? kTileRows : kTokRows;
+        pl.tiles = int((rows + per_tile - 1) / per_tile);
+        const double groups = double(B) * H_kv * pl.tiles;
+        const int keys = pl.tile ? kTileKeys : kTokKeys * kTokWaves;
+        const int64_t rounds = (int64_t(S_max) + keys - 1) / keys;
+        for (pl.splits = 1; pl.splits <= kMaxSplits; pl.splits *= 2) {
+            const double bytes = double(B) * S_q * H * pl.splits * D * 4;
+            if (pl.splits > 1 && (pl.splits > rounds || bytes > 512e6))
+                break;
+            const double share = std::ceil(double(rounds) / pl.splits);
+            const double load = groups * pl.splits / 256;  // workgroups per CU
+            // The longest share, or the work of a full CU.
+            const double alone = pl.tile ? rate.tile1 : rate.token1;
+            const double full = pl.tile ? rate.tile2 : rate.token2;
+            double us = 6 + std::max(share * alone, share * part * load * full) +
+                        3 * std::max(0.0, load / 2 - 1);
+            if (pl.splits > 1)
+                us += 3 + bytes / 4e6 + bytes / 6e6;
+            if (us < best_us) {
+                best_us = us;
+                best = pl;
+            }
+        }
+    }
+    return best;
 }
 
 int64_t part_bytes(int B, int S_q, int H, int D, int splits)
@@ -944,19 +990,26 @@ bool run_attention_kv4(AttnArgs &a, bool tile, hipStream_t st)
         return false;
     if (a.splits == 1)
         return true;
-    hipLaunchKernelGGL((kv4_join_kernel<T, D>), dim3(unsigned(rows)), dim3(256), 0, st,
-                       a);
+    // A workgroup per row where rows are few: 16 rows of 16 splits 10.9 us in all
+    // against 11.4, 32000 rows of 2 splits 76 against 45.
+    if (a.splits > kMaxSplits / 4 || rows <= 1024)
+        hipLaunchKernelGGL((kv4_join_kernel<T, D, 4>), dim3(unsigned(rows)), dim3(256), 0, st, a);
+    else
+        hipLaunchKernelGGL((kv4_join_kernel<T, D, 1>), dim3(unsigned((rows + 3) / 4)), dim3(256),
+                           0, st, a);
     return hip_ok(hipGetLastError(), "kv4_join_kernel launch");
 }
 
 }  // namespace
 
-size_t kv4_attention_scratch_bytes(int B, int S_q, int H, int H_kv, int D, int S_max, Mx4Type)
+size_t kv4_attention_scratch_bytes(int B, int S_q, int H, int H_kv, int D, int S_max, Mx4Type type)
 {
     if (B <= 0 || S_q <= 0 || H <= 0 || H_kv <= 0 || D <= 0 || S_max <= 0 || H % H_kv)
         return 0;
-    const Plan pl = plan_of(B, S_q, H, H_kv, S_max);
-    return pl.splits > 1 ? size_t(part_bytes(B, S_q, H, D, pl.splits)) : 0;
+    // With a causal mask or without.
+    const int splits = std::max(plan_of(B, S_q, H, H_kv, D, S_max, type, true).splits,
+                                plan_of(B, S_q, H, H_kv, D, S_max, type, false).splits);
+    return splits > 1 ? size_t(part_bytes(B, S_q, H, D, splits)) : 0;
 }
 
 bool launch_kv4_attention(const Kv4Attention &p, void *scratch, size_t scratch_bytes,
@@ -964,7 +1017,7 @@ bool launch_kv4_attention(const Kv4Attention &p, void *scratch, size_t scratch_b
 {
     if (p.B <= 0 || p.S_q <= 0 || p.H <= 0)
         return true;
-    const Plan pl = plan_of(p.B, p.S_q, p.H, p.H_kv, p.S_max);
+    const Plan pl = plan_of(p.B, p.S_q, p.H, p.H_kv, p.D, p.S_max, p.type, p.causal);
     AttnArgs a{};
     a.p = p;
     a.scale2 = p.scale * kLog2e;
@@ -972,14 +1025,15 @@ bool launch_kv4_attention(const Kv4Attention &p, void *scratch, size_t scratch_b
     a.rows = p.S_q * a.group;
     a.tiles = pl.tiles;
     a.splits = pl.splits;
-    if (pl.splits > 1) {
-        if (!scratch ||
-            scratch_bytes < kv4_attention_scratch_bytes(p.B, p.S_q, p.H, p.H_kv, p.D, p.S_max,
-                                                        p.type))
+    const size_t need = kv4_attention_scratch_bytes(p.B, p.S_q, p.H, p.H_kv, p.D, p.S_max, p.type);
+    if (need > 0) {
+        if (!scratch || scratch_bytes < need)
             return fail(
                 "kv4_attention_dev: scratch smaller than anima_hip_kv4_attention_scratch_bytes");
         if (!aligned(scratch, 16))
             return fail("kv4_attention_dev: scratch must be 16-byte aligned");
+    }
+    if (pl.splits > 1) {
         a.part = static_cast<float *>(scratch);
         a.ml = reinterpret_cast<float2 *>(a.part + int64_t(p.B) * p.S_q * p.H * pl.splits * p.D);
     }
