@@ -30,6 +30,7 @@
 // its key: such groups are decoded as zero and their NaN is added to the rows
 // that do see them.
 #include "mx4.h"
+#include "mx4_plan.h"
 
 #include <algorithm>
 #include <cmath>
@@ -48,6 +49,7 @@ using mx4::mfma16;
 using mx4::scale_of;
 using mx4::terms2;
 using mx4::u32x2;
+using namespace mx4_plan;
 
 template <typename T>
 constexpr int kTerms = sizeof(T) == 4 ? 3 : 1;
@@ -162,9 +164,6 @@ __device__ __forceinline__ void p_terms(const float (&p)[8], bf16x8 (&t)[3])
 
 // ----------------------------------------------------------- token kernel
 
-constexpr int kTokRows = 16;   // query rows of a workgroup
-constexpr int kTokKeys = 32;   // keys a wave takes at a time
-constexpr int kTokWaves = 4;
 
 // A wave's loads for 32 keys.  Lane (m, g): K rows t0 + m and t0 + 16 + m,
 // dimensions g * D/4 .. ; V rows of the eight keys 4g + 0..3 and 16 + 4g +
@@ -468,9 +467,6 @@ __global__ __launch_bounds__(kTokWaves * 64, 2) void kv4_token_kernel(AttnArgs a
 
 // ------------------------------------------------------------ tile kernel
 
-constexpr int kTileWaves = 4;
-constexpr int kTileRows = 32 * kTileWaves;  // query rows of a workgroup
-constexpr int kTileKeys = 64;
 
 // 16-byte pieces of a staged K row (D / 8 of them) and V^T row (8), placed so
 // that the 16 rows a ds_read_b128 quarter touches lie in distinct banks.
@@ -842,8 +838,6 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void kv4_tile_kernel(AttnArgs a
 // that saw a key (at most 64).  PER waves per row: in each, lane s weighs split s;
 // wave w adds the splits w, w + PER, .., at most 16, its loads all in flight,
 // D / 64 dimensions per lane, and the waves' sums are added in their order.
-constexpr int kMaxSplits = 64;
-
 template <typename T, int D, int PER>
 __global__ __launch_bounds__(256) void kv4_join_kernel(AttnArgs a)
 {
@@ -861,9 +855,9 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(AttnArgs a)
     if (p.counts && s >= p.counts[b])
         return;  // likewise
     const float *src = a.part + int64_t(row) * D + lane * E;
-    float x[kMaxSplits / 4][E], v[E] = {};
+    float x[kAttnMaxSplits / 4][E], v[E] = {};
 #pragma unroll
-    for (int k = 0; k < kMaxSplits / 4; ++k)
+    for (int k = 0; k < kAttnMaxSplits / 4; ++k)
         if (first + PER * k < a.splits)
 #pragma unroll
             for (int e = 0; e < E; ++e)
@@ -882,7 +876,7 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(AttnArgs a)
     for (int o = 32; o; o >>= 1)
         l += __shfl_xor(l, o);
 #pragma unroll
-    for (int k = 0; k < kMaxSplits / 4; ++k)
+    for (int k = 0; k < kAttnMaxSplits / 4; ++k)
         if (first + PER * k < a.splits) {
             const float wk = __shfl(w, first + PER * k);
             if (wk != 0.0f)
@@ -906,66 +900,6 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(AttnArgs a)
         if (d < D)
             store_o(out + d, (part[0][d] + part[1][d] + part[2][d] + part[3][d]) * inv);
     }
-}
-
-struct Plan {
-    bool tile = false;  // the tile kernel
-    int tiles = 0, splits = 1;
-};
-
-// Microseconds of a workgroup per 128 keys (token kernel, 16 query rows) and per 64 keys
-// (tile kernel, 128 rows), alone on a CU and as its share of a CU that has two;
-// bf16 and f32 queries, D of 64 and 128.  Measured at one query to 2048 over 200 to
-// 20000 keys.
-struct Rate {
-    double token1, token2, tile1, tile2;
-};
-constexpr Rate kRates[2][2] = {{{0.65, 0.46, 1.45, 0.9}, {0.78, 0.62, 1.75, 1.45}},
-                               {{0.8, 0.59, 2.15, 1.85}, {1.05, 0.85, 4.8, 3.0}}};
-
-// The kernel and the split that the model expects to take least: about 6 us of
-// latency, the keys of the longest share or of a full CU, and with splits the partial
-// results written and joined.  The token kernel, which meets at no barrier, is ahead to
-// some hundred query rows of a K/V head and in f32 further: 2048 rows of 512 keys,
-// 4 K/V heads, take 10.8 us by it and 18.7 by the tile kernel (bf16); 4096 x 512 keys,
-// 32 heads, 50 us by the tile kernel against 141 by the first token kernel.
-Plan plan_of(int B, int S_q, int H, int H_kv, int D, int S_max, Mx4Type type, bool causal)
-{
-    const Rate &rate = kRates[type == kMx4F32][D == 128];
-    const int64_t rows = int64_t(S_q) * (H / H_kv);
-    // Under a causal mask the query tiles see S_max - S_q .. S_max keys.
-    const double part = causal && S_q > 1 && S_max > 0
-                            ? 1.0 - 0.5 * std::min(S_q, S_max) / S_max : 1.0;
-    Plan best;
-    double best_us = 1e300;
-    for (int tile = 0; tile < 2; ++tile) {
-        Plan pl;
-        pl.tile = tile != 0;
-        const int per_tile = pl.tile ? kTileRows : kTokRows;
-        pl.tiles = int((rows + per_tile - 1) / per_tile);
-        const double groups = double(B) * H_kv * pl.tiles;
-        const int keys = pl.tile ? kTileKeys : kTokKeys * kTokWaves;
-        const int64_t rounds = (int64_t(S_max) + keys - 1) / keys;
-        for (pl.splits = 1; pl.splits <= kMaxSplits; pl.splits *= 2) {
-            const double bytes = double(B) * S_q * H * pl.splits * D * 4;
-            if (pl.splits > 1 && (pl.splits > rounds || bytes > 512e6))
-                break;
-            const double share = std::ceil(double(rounds) / pl.splits);
-            const double load = groups * pl.splits / 256;  // workgroups per CU
-            // The longest share, or the work of a full CU.
-            const double alone = pl.tile ? rate.tile1 : rate.token1;
-            const double full = pl.tile ? rate.tile2 : rate.token2;
-            double us = 6 + std::max(share * alone, share * part * load * full) +
-                        3 * std::max(0.0, load / 2 - 1);
-            if (pl.splits > 1)
-                us += 3 + bytes / 4e6 + bytes / 6e6;
-            if (us < best_us) {
-                best_us = us;
-                best = pl;
-            }
-        }
-    }
-    return best;
 }
 
 int64_t part_bytes(int B, int S_q, int H, int D, int splits)
@@ -992,7 +926,7 @@ bool run_attention_kv4(AttnArgs &a, bool tile, hipStream_t st)
         return true;
     // A workgroup per row where rows are few: 16 rows of 16 splits 10.9 us in all
     // against 11.4, 32000 rows of 2 splits 76 against 45.
-    if (a.splits > kMaxSplits / 4 || rows <= 1024)
+    if (a.splits > kAttnMaxSplits / 4 || rows <= 1024)
         hipLaunchKernelGGL((kv4_join_kernel<T, D, 4>), dim3(unsigned(rows)), dim3(256), 0, st, a);
     else
         hipLaunchKernelGGL((kv4_join_kernel<T, D, 1>), dim3(unsigned((rows + 3) / 4)), dim3(256),
@@ -1007,8 +941,8 @@ size_t kv4_attention_scratch_bytes(int B, int S_q, int H, int H_kv, int D, int S
     if (B <= 0 || S_q <= 0 || H <= 0 || H_kv <= 0 || D <= 0 || S_max <= 0 || H % H_kv)
         return 0;
     // With a causal mask or without.
-    const int splits = std::max(plan_of(B, S_q, H, H_kv, D, S_max, type, true).splits,
-                                plan_of(B, S_q, H, H_kv, D, S_max, type, false).splits);
+    const int splits = std::max(attn_plan(B, S_q, H, H_kv, D, S_max, type == kMx4F32, true).splits,
+                                attn_plan(B, S_q, H, H_kv, D, S_max, type == kMx4F32, false).splits);
     return splits > 1 ? size_t(part_bytes(B, S_q, H, D, splits)) : 0;
 }
 
@@ -1017,7 +951,8 @@ bool launch_kv4_attention(const Kv4Attention &p, void *scratch, size_t scratch_b
 {
     if (p.B <= 0 || p.S_q <= 0 || p.H <= 0)
         return true;
-    const Plan pl = plan_of(p.B, p.S_q, p.H, p.H_kv, p.D, p.S_max, p.type, p.causal);
+    const AttnPlan pl = attn_plan(p.B, p.S_q, p.H, p.H_kv, p.D, p.S_max, p.type == kMx4F32,
+                                  p.causal);
     AttnArgs a{};
     a.p = p;
     a.scale2 = p.scale * kLog2e;

@@ -18,10 +18,9 @@
 //     weights staged in LDS, two stages.
 // The last two split K across workgroups where the tiles alone would leave CUs idle.
 #include "mx4.h"
+#include "mx4_plan.h"
 
 #include <algorithm>
-#include <cmath>
-#include <iterator>
 
 namespace anima_hip {
 namespace {
@@ -32,6 +31,7 @@ using mx4::mfma16;
 using mx4::scale_of;
 using mx4::terms2;
 using mx4::u32x2;
+using namespace mx4_plan;
 
 // bf16 terms of an activation: f32 takes three, bf16 is its own.
 template <typename T>
@@ -109,7 +109,6 @@ struct LinArgs {
 
 // ------------------------------------------------------------- few rows
 
-constexpr int kFewRows = 16;             // batch rows of a workgroup
 constexpr int kFewLds = 32768;           // staged bf16 elements (64 KiB)
 constexpr int kFewBlock = 128;           // K elements a wave takes at a time
 constexpr int kFewPad = 8;               // elements between staged rows (16 bytes)
@@ -197,7 +196,6 @@ __global__ __launch_bounds__(WAVES * 64) void linear_few_kernel(LinArgs p)
 
 // ---------------------------------------------------------------- tiles
 
-constexpr int kTileK = 64;  // K elements per chunk: 128-byte rows of bf16
 
 // 16-byte pieces of a staged 128-byte row, so that the 16 rows of a
 // ds_read_b128 quarter touch distinct banks.
@@ -745,9 +743,7 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void linear_staged_kernel(LinArgs 
     }
 }
 
-// C = the planes' sum, in split order (at most 16 of them), all loads in flight.
-constexpr int kMaxSplits = 16;
-
+// C = the planes' sum, in split order (at most kLinMaxSplits), all loads in flight.
 template <typename T>
 __global__ __launch_bounds__(256) void linear_sum_kernel(const float *part, T *c, int64_t ldc,
                                                          int M, int N, int splits)
@@ -756,21 +752,63 @@ __global__ __launch_bounds__(256) void linear_sum_kernel(const float *part, T *c
     const int64_t plane = int64_t(M) * N;
     if (i >= plane)
         return;
-    float x[kMaxSplits];
+    float x[kLinMaxSplits];
 #pragma unroll
-    for (int s = 0; s < kMaxSplits; ++s)
+    for (int s = 0; s < kLinMaxSplits; ++s)
         if (s < splits)
             x[s] = part[s * plane + i];
     float sum = x[0];
 #pragma unroll
-    for (int s = 1; s < kMaxSplits; ++s)
+    for (int s = 1; s < kLinMaxSplits; ++s)
         if (s < splits)
             sum += x[s];
     const int64_t m = i / N;
     store_c(c + m * ldc + (i - m * N), sum);
 }
 
-// ----------------------------------------------------------------- plans
+// Copies with K padded to a multiple of 128: A with zeros, the weights with zero
+// codes of a finite scale.  A thread writes 16 bytes of a row of A, or one group of
+// a weight row; the first `a_blocks` workgroups take A.
+template <typename T>
+__global__ __launch_bounds__(256) void linear_pad_kernel(LinArgs p, T *a, uint8_t *codes,
+                                                         uint8_t *scales, int padded,
+                                                         unsigned a_blocks)
+{
+    constexpr int E = 16 / int(sizeof(T));
+    if (blockIdx.x < a_blocks) {
+        const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
+        const int pieces = padded / E;
+        const int64_t m = i / pieces;
+        if (m >= p.M)
+            return;
+        const int k0 = int(i - m * pieces) * E;
+        const T *row = static_cast<const T *>(p.a) + m * p.lda;
+        T v[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            v[e] = k0 + e < p.K ? row[k0 + e] : T(0);
+        u32x4 w;
+        __builtin_memcpy(&w, v, 16);
+        *reinterpret_cast<u32x4 *>(a + m * padded + k0) = w;
+        return;
+    }
+    const int64_t i = int64_t(blockIdx.x - a_blocks) * 256 + threadIdx.x;
+    const int groups = padded / 32;
+    const int64_t n = i / groups;
+    if (n >= p.N)
+        return;
+    const int g = int(i - n * groups);
+    u32x4 c = {0, 0, 0, 0};
+    unsigned s = 127;
+    if (g < p.groups) {
+        c = *reinterpret_cast<const u32x4 *>(p.codes + (n * p.groups + g) * 16);
+        s = p.scales[n * p.groups + g];
+    }
+    *reinterpret_cast<u32x4 *>(codes + i * 16) = c;
+    scales[i] = uint8_t(s);
+}
+
+// -------------------------------------------------------------- launches
 
 // Shapes of the staged kernel: MB, NB, WM, WN, KS, S.
 #define STAGED_BF16(X) \
@@ -779,21 +817,6 @@ __global__ __launch_bounds__(256) void linear_sum_kernel(const float *part, T *c
 #define STAGED_F32(X) \
     X(0, 2, 4, 4, 2, 1, 2) X(1, 1, 4, 4, 2, 1, 3) X(2, 1, 4, 2, 1, 4, 3) X(3, 1, 2, 1, 1, 4, 4)
 
-struct TileShape {
-    int bm, bn;
-    // Microseconds of a workgroup per chunk of K (256 bytes of a row of A) where half
-    // the CUs have one, and where all have (large tiles: at a lower clock; small
-    // ones: several workgroups on a CU, per workgroup).
-    double half_us, full_us;
-};
-// Measured at M from 24 to 4096, N x K of 2048 x 2048, 2048 x 8192, 8192 x 2048,
-// 6144 x 256 and 256 x 2048; the model below is within 15 % of most of them.
-constexpr TileShape kBf16Shapes[] = {{192, 256, 2.0, 2.45}, {128, 256, 1.24, 1.7},
-                                     {128, 128, 0.93, 1.15}, {64, 128, 0.66, 0.62},
-                                     {64, 64, 0.47, 0.58},   {32, 64, 0.37, 0.36}};
-constexpr TileShape kF32Shapes[] = {{256, 256, 4.2, 5.4}, {128, 256, 2.33, 2.75},
-                                    {64, 128, 1.0, 1.02}, {32, 64, 0.52, 0.33}};
-constexpr TileShape kTileShapes[] = {{32, 128, 0, 0}, {64, 128, 0, 0}, {128, 128, 0, 0}};
 #define SHAPE_CHECK(table, i, mb, nb, wm, wn) \
     static_assert(table[i].bm == 32 * mb * wm && table[i].bn == 32 * nb * wn, "shape table");
 #define CHECK_BF16(i, mb, nb, wm, wn, ks, s) SHAPE_CHECK(kBf16Shapes, i, mb, nb, wm, wn)
@@ -801,80 +824,6 @@ constexpr TileShape kTileShapes[] = {{32, 128, 0, 0}, {64, 128, 0, 0}, {128, 128
 STAGED_BF16(CHECK_BF16)
 STAGED_F32(CHECK_F32)
 
-enum Kernel { kFew, kTiles, kStaged };
-struct Plan {
-    Kernel kernel = kFew;
-    int shape = 0;
-    int tiles_m = 0, tiles_n = 0, splits = 1, per_split = 0, chunks = 0;
-};
-
-// The tile grid of a shape with K shared out over up to `splits` workgroups.
-void set_grid(Plan &pl, const TileShape &t, int M, int N, int splits)
-{
-    pl.tiles_m = (M + t.bm - 1) / t.bm;
-    pl.tiles_n = (N + t.bn - 1) / t.bn;
-    pl.per_split = (pl.chunks + splits - 1) / splits;
-    pl.splits = pl.per_split ? (pl.chunks + pl.per_split - 1) / pl.per_split : 1;
-}
-
-// Predicted time of a staged grid: 4 us of latency and epilogue, the chunks of the
-// fullest CU, and the sum of the planes.
-double staged_us(const Plan &pl, const TileShape &t, int M, int N)
-{
-    const double wgs = double(pl.tiles_m) * pl.tiles_n * pl.splits;
-    const double rounds = std::ceil(wgs / 256);
-    const double load = std::min(1.0, std::max(0.0, wgs / 128 - 1));
-    const double alone = t.half_us + (t.full_us > t.half_us ? (t.full_us - t.half_us) * load : 0);
-    double us = 4.2 + pl.per_split * (rounds > 1 ? std::max(alone, rounds * t.full_us) : alone);
-    if (pl.splits > 1)
-        us += 2.3 + double(pl.splits) * M * N * 4 / 1.8e6;
-    return us;
-}
-
-// `staged`: the pointers and strides suit the staged kernel.
-Plan plan_of(int M, int N, int K, Mx4Type type, bool staged)
-{
-    const bool f32 = type == kMx4F32;
-    Plan pl;
-    // Few rows, unless their terms take long to stage in every workgroup: 16 rows of
-    // 8192 bf16 take 12.5 us against 9.8 (N = 2048), 8 rows of 8192 f32 18 against
-    // 15, 16 of 2048 13 against 8.8; 4 rows of 8192 f32 12 against 15, 16 of 2048
-    // bf16 5.5 against 7.4.
-    const int64_t terms = int64_t(M) * (f32 ? 3 : 1);
-    if (M <= kFewRows &&
-        (!staged || K % 128 || terms * K <= 24576 || (terms <= 24 && terms * K <= 100000)))
-        return pl;
-    if (staged && K > 0 && K % 128 == 0) {
-        pl.kernel = kStaged;
-        pl.chunks = K / (f32 ? 64 : 128);
-        Plan best = pl;
-        double best_us = 1e300;
-        const int n = f32 ? int(std::size(kF32Shapes)) : int(std::size(kBf16Shapes));
-        for (pl.shape = 0; pl.shape < n; ++pl.shape)
-            for (int splits = 1; splits <= 8; splits *= 2) {
-                const TileShape &t = f32 ? kF32Shapes[pl.shape] : kBf16Shapes[pl.shape];
-                if (splits > 1 && (splits > pl.chunks || double(M) * N * splits > 256.0 * 32768 * 2))
-                    break;
-                set_grid(pl, t, M, N, splits);
-                const double us = staged_us(pl, t, M, N);
-                if (us < best_us) {
-                    best_us = us;
-                    best = pl;
-                }
-            }
-        return best;
-    }
-    pl.kernel = kTiles;
-    pl.shape = M <= 32 ? 0 : M <= 64 ? 1 : 2;
-    pl.chunks = (K + kTileK - 1) / kTileK;
-    const TileShape &t = kTileShapes[pl.shape];
-    set_grid(pl, t, M, N, 1);
-    const int64_t tiles = int64_t(pl.tiles_m) * pl.tiles_n;
-    const int64_t splits = std::min<int64_t>({256 / tiles, pl.chunks / 4, kMaxSplits});
-    if (splits > 1)
-        set_grid(pl, t, M, N, int(splits));
-    return pl;
-}
 
 template <typename T, bool VEC>
 bool run_few(LinArgs &p, hipStream_t st)
@@ -935,7 +884,20 @@ bool run_staged(const LinArgs &p, int shape, dim3 grid, hipStream_t st)
 }
 
 template <typename T>
-bool run_linear(LinArgs &p, const Plan &pl, bool rows16, hipStream_t st)
+bool run_pad(const LinArgs &p, void *a, uint8_t *codes, uint8_t *scales, hipStream_t st)
+{
+    const int padded = lin_padded(p.K);
+    const int64_t a_blocks = (int64_t(p.M) * (padded * int(sizeof(T)) / 16) + 255) / 256;
+    const int64_t w_blocks = (int64_t(p.N) * (padded / 32) + 255) / 256;
+    if (a_blocks + w_blocks > INT32_MAX)
+        return fail("linear_mx4_dev: too many rows");
+    hipLaunchKernelGGL(linear_pad_kernel<T>, dim3(unsigned(a_blocks + w_blocks)), dim3(256), 0, st,
+                       p, static_cast<T *>(a), codes, scales, padded, unsigned(a_blocks));
+    return hip_ok(hipGetLastError(), "linear_pad_kernel launch");
+}
+
+template <typename T>
+bool run_linear(LinArgs &p, const LinPlan &pl, bool rows16, hipStream_t st)
 {
     const bool vec = rows16 && p.K % 8 == 0;
     if (pl.kernel == kFew)
@@ -962,9 +924,9 @@ size_t linear_mx4_scratch_bytes(int M, int N, int K, Mx4Type type)
     if (M <= 0 || N <= 0 || K <= 0)
         return 0;
     // For any pointers and strides.
-    const int splits = std::max(plan_of(M, N, K, type, true).splits,
-                                plan_of(M, N, K, type, false).splits);
-    return splits > 1 ? size_t(splits) * size_t(M) * size_t(N) * 4 : 0;
+    const bool f32 = type == kMx4F32;
+    return size_t(std::max(lin_scratch(lin_plan(M, N, K, f32, true), M, N, K, f32).bytes,
+                           lin_scratch(lin_plan(M, N, K, f32, false), M, N, K, f32).bytes));
 }
 
 bool launch_linear_mx4(const void *a, int64_t lda, const uint8_t *codes, const uint8_t *scales,
@@ -973,9 +935,18 @@ bool launch_linear_mx4(const void *a, int64_t lda, const uint8_t *codes, const u
 {
     if (M <= 0 || N <= 0)
         return true;
-    const bool rows16 = aligned(a, 16) && lda % (type == kMx4F32 ? 4 : 8) == 0;
-    // Row offsets within a staged tile are 32-bit byte counts (of up to 256 rows).
-    const Plan pl = plan_of(M, N, K, type, rows16 && lda <= (1 << 21) && K <= (1 << 22));
+    const bool f32 = type == kMx4F32;
+    const bool rows16 = aligned(a, 16) && lda % (f32 ? 4 : 8) == 0;
+    const LinPlan pl = lin_plan(M, N, K, f32, rows16 && lda <= kStagedMaxK / 2);
+    const size_t need = linear_mx4_scratch_bytes(M, N, K, type);
+    if (need > 0) {
+        if (scratch_bytes < need || !scratch)
+            return fail("linear_mx4_dev: scratch smaller than anima_hip_linear_mx4_scratch_bytes");
+        if (!aligned(scratch, 16))
+            return fail("linear_mx4_dev: scratch must be 16-byte aligned");
+    }
+    const LinScratch parts = lin_scratch(pl, M, N, K, f32);
+    char *const mem = static_cast<char *>(scratch);
     LinArgs p{};
     p.a = a;
     p.codes = codes;
@@ -991,17 +962,22 @@ bool launch_linear_mx4(const void *a, int64_t lda, const uint8_t *codes, const u
     p.tiles_n = pl.tiles_n;
     p.chunks = pl.chunks;
     p.per_split = pl.per_split;
-    const size_t need = linear_mx4_scratch_bytes(M, N, K, type);
-    if (need > 0) {
-        if (scratch_bytes < need || !scratch)
-            return fail("linear_mx4_dev: scratch smaller than anima_hip_linear_mx4_scratch_bytes");
-        if (!aligned(scratch, 16))
-            return fail("linear_mx4_dev: scratch must be 16-byte aligned");
-    }
     if (pl.splits > 1)
-        p.part = static_cast<float *>(scratch);
-    return type == kMx4F32 ? run_linear<float>(p, pl, rows16, st)
-                           : run_linear<uint16_t>(p, pl, rows16, st);
+        p.part = reinterpret_cast<float *>(mem + parts.planes);
+    if (pl.pad) {
+        void *const pa = mem + parts.a;
+        uint8_t *const pc = reinterpret_cast<uint8_t *>(mem + parts.codes);
+        uint8_t *const ps = reinterpret_cast<uint8_t *>(mem + parts.scales);
+        if (!(f32 ? run_pad<float>(p, pa, pc, ps, st) : run_pad<uint16_t>(p, pa, pc, ps, st)))
+            return false;
+        p.a = pa;
+        p.codes = pc;
+        p.scales = ps;
+        p.K = lin_padded(K);
+        p.lda = p.K;
+        p.groups = p.K / 32;
+    }
+    return f32 ? run_linear<float>(p, pl, rows16, st) : run_linear<uint16_t>(p, pl, rows16, st);
 }
 
 }  // namespace anima_hip

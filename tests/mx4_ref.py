@@ -87,3 +87,32 @@ def attention(q, k, v, lens, counts, causal, scale):
                 out[b, s, h] = w @ v[bk, hk, :m]
                 mag[b, s, h] = w @ np.abs(v[bk, hk, :m])
     return out, mag
+
+
+def attention_rows(q, k, v, lens, counts, causal, scale):
+    """attention() with all queries of a head at once, for many of them."""
+    B, S, H, D = q.shape
+    Bk, H_kv = k.shape[:2]
+    out, mag = np.zeros(q.shape), np.zeros(q.shape)
+    for b in range(B):
+        bk = 0 if Bk == 1 else b
+        n = min(max(lens[bk], 0), k.shape[2])
+        nq = S if counts is None else min(max(counts[b], 0), S)
+        if n == 0 or nq == 0:
+            continue
+        limit = np.clip(n - nq + np.arange(nq) + 1, 0, n) if causal else np.full(nq, n)
+        seen = np.arange(n) < limit[:, None]
+        for h in range(H):
+            hk = h // (H // H_kv)
+            kk, vv = k[bk, hk, :n], v[bk, hk, :n]
+            w = np.where(seen, q[b, :nq, h] @ kk.T * scale, -np.inf)
+            top = np.where(limit[:, None] > 0, w.max(-1, keepdims=True), 0.0)
+            w = np.where(seen, np.exp(w - top), 0.0)
+            w /= np.maximum(w.sum(-1, keepdims=True), 1e-300)
+            bad = np.isnan(vv)
+            vv = np.where(bad, 0.0, vv)
+            # A NaN value reaches the rows that see its key, whatever their weight for it.
+            nan = (seen.astype(float) @ bad.astype(float)) > 0
+            out[b, :nq, h] = np.where(nan, np.nan, w @ vv)
+            mag[b, :nq, h] = w @ np.abs(vv)
+    return out, mag
