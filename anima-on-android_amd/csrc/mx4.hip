@@ -48,37 +48,6 @@ __device__ __forceinline__ void load8(const uint16_t *row, int k0, int K, bool v
         x[i] = k0 + i < K ? __uint_as_float(unsigned(row[k0 + i]) << 16) : 0.0f;
 }
 
-__device__ __forceinline__ void store8(float *row, int k0, int K, bool vec, const float (&x)[8])
-{
-    if (vec && k0 + 8 <= K) {
-        *reinterpret_cast<f32x4 *>(row + k0) = f32x4{x[0], x[1], x[2], x[3]};
-        *reinterpret_cast<f32x4 *>(row + k0 + 4) = f32x4{x[4], x[5], x[6], x[7]};
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (k0 + i < K)
-            row[k0 + i] = x[i];
-}
-
-// MX4 values are bf16 numbers: their upper halves are the values themselves.
-__device__ __forceinline__ void store8(uint16_t *row, int k0, int K, bool vec, const float (&x)[8])
-{
-    unsigned u[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        u[i] = __float_as_uint(x[i]) >> 16;
-    if (vec && k0 + 8 <= K) {
-        *reinterpret_cast<u32x4 *>(row + k0) = u32x4{u[0] | u[1] << 16, u[2] | u[3] << 16,
-                                                     u[4] | u[5] << 16, u[6] | u[7] << 16};
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (k0 + i < K)
-            row[k0 + i] = uint16_t(u[i]);
-}
-
 // One group over four neighbouring lanes, eight elements each.  Groups with an
 // infinity or a NaN have zero codes, so that packing is a function of the
 // values alone.
@@ -113,25 +82,62 @@ __global__ __launch_bounds__(256) void mx4_pack_kernel(const T *x, int64_t ldx, 
     pack_group(v, codes + int64_t(gi) * 16, scales + gi, piece);
 }
 
+// Values of a row from k0: as many as 16 bytes hold.
+template <typename T, int E>
+__device__ __forceinline__ void store16(T *row, int k0, int K, bool vec, const float (&x)[E])
+{
+    T v[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+        if constexpr (sizeof(T) == 4)
+            v[i] = x[i];
+        else  // MX4 values are bf16 numbers: their upper halves are the values themselves
+            v[i] = uint16_t(__float_as_uint(x[i]) >> 16);
+    if (vec && k0 + E <= K) {
+        u32x4 w;
+        __builtin_memcpy(&w, v, 16);
+        *reinterpret_cast<u32x4 *>(row + k0) = w;
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+        if (k0 + i < K)
+            row[k0 + i] = v[i];
+}
+
 template <typename T>
 __global__ __launch_bounds__(256) void mx4_unpack_kernel(const uint8_t *codes,
                                                          const uint8_t *scales, T *x, int64_t ldx,
                                                          unsigned groups, unsigned total, int K,
                                                          bool vec)
 {
-    const unsigned gi = blockIdx.x * 64u + (threadIdx.x >> 2);
+    constexpr int E = 16 / int(sizeof(T)), LANES = kGroup / E;  // lanes of a group
+    const unsigned gi = blockIdx.x * (256u / LANES) + threadIdx.x / LANES;
     if (gi >= total)
         return;
-    const int piece = threadIdx.x & 3;
+    const int piece = threadIdx.x % LANES;
     const unsigned row = gi / groups;
-    const unsigned w = reinterpret_cast<const unsigned *>(codes + int64_t(gi) * 16)[piece];
     const float s = scale_of(scales[gi]);
-    const f32x2 p0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 0);
-    const f32x2 p1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 1);
-    const f32x2 p2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 2);
-    const f32x2 p3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 3);
-    const float v[8] = {p0[0], p0[1], p1[0], p1[1], p2[0], p2[1], p3[0], p3[1]};
-    store8(x + int64_t(row) * ldx, int(gi - row * groups) * kGroup + 8 * piece, K, vec, v);
+    const uint8_t *src = codes + int64_t(gi) * 16 + piece * (E / 2);
+    float v[E];
+    if constexpr (E == 8) {
+        const unsigned w = *reinterpret_cast<const unsigned *>(src);
+        const f32x2 p[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 0),
+                            __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 1),
+                            __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 2),
+                            __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 3)};
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            v[i] = p[i >> 1][i & 1];
+    } else {
+        const unsigned w = *reinterpret_cast<const uint16_t *>(src);
+        const f32x2 p[2] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 0),
+                            __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 1)};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            v[i] = p[i >> 1][i & 1];
+    }
+    store16(x + int64_t(row) * ldx, int(gi - row * groups) * kGroup + E * piece, K, vec, v);
 }
 
 template <typename T>
@@ -211,7 +217,8 @@ bool launch_mx4_unpack(const uint8_t *codes, const uint8_t *scales, void *x, int
         return false;
     if (total == 0)
         return true;
-    const dim3 grid((total + 63) / 64), block(256);
+    const unsigned per = type == kMx4F32 ? 32 : 64;  // groups of a workgroup
+    const dim3 grid((total + per - 1) / per), block(256);
     const bool vec = wide(x, ldx, type);
     if (type == kMx4F32)
         hipLaunchKernelGGL(mx4_unpack_kernel<float>, grid, block, 0, st, codes, scales,
