@@ -20,9 +20,14 @@
 //   * tile kernel: many query rows.  Tiles of 64 keys are decoded once per
 //     workgroup of 128 query rows into LDS, K as rows and V transposed, while
 //     the codes of the tile after next are on their way; 32 query rows per wave
-//     on v_mfma_f32_32x32x16_bf16.  Bound by the MFMA and the softmax's VALU
-//     work together (4096 x 512 x 16 heads x 2, bf16: 58 us against 141 us by
-//     the token kernel, 24 us for the MFMAs alone).
+//     on v_mfma_f32_32x32x16_bf16, two workgroups on a CU.  Bound by the
+//     softmax's VALU work and the MFMAs, which overlap only between the two
+//     waves of a SIMD: bf16 303 us (0.91 PFLOP/s) at 4096 x 4096 x 16 heads x 2,
+//     50 us at 4096 x 512 (24 us for its MFMAs alone, 141 us by the first
+//     token kernel).  Workgroups of 256 rows over 128 keys, one on a CU, take
+//     2 to 6 % less at whole multiples of 256 rows and more elsewhere; the
+//     scores of the next tile computed between the exponentials of this one take
+//     18 % more, the registers for both tiles' scores being short.
 //
 // A masked key never reaches a row: its score is left out of the maximum and
 // the sum, and the decoded V of keys past the cache's length is finite.  Inside
