@@ -68,8 +68,9 @@ def pack(x):
         xd, codes, scales = bufs.upload("x", x), bufs.get("codes", nc), bufs.get("scales", ns)
         _lib.check(_lib.load().anima_hip_mx4_pack_dev(xd.ptr, K, dtype, codes.ptr, scales.ptr, rows,
                                                       K, None), "anima_hip_mx4_pack_dev")
-        return (codes.download((rows, nc // max(rows, 1)), np.uint8),
-                scales.download((rows, ns // max(rows, 1)), np.uint8))
+        groups = -(-K // 32)
+        return (codes.download((rows, groups * 16), np.uint8),
+                scales.download((rows, groups), np.uint8))
     finally:
         bufs.close()
 

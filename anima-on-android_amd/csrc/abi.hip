@@ -1576,13 +1576,15 @@ bool check_mx4_rows(const char *who, const void *x, int64_t ld, int dtype, const
     return check_mx4(who, codes, scales);
 }
 
-bool check_kv4(const char *who, const Kv4Cache &c, int H_kv, int D, int S_max)
+// Sizes of a cache, and where a call has work, its arrays.
+bool check_kv4(const char *who, const Kv4Cache &c, int H_kv, int D, int S_max, bool work)
 {
     if (D != 64 && D != 128)
         return fail(std::string(who) + ": D must be 64 or 128, got " + std::to_string(D));
     if (H_kv <= 0 || S_max < 0 || S_max > kMx4MaxDim)
         return fail(std::string(who) + ": H_kv must be positive, S_max between 0 and 2^30");
-    return S_max == 0 || (check_mx4(who, c.k, c.k_scales) && check_mx4(who, c.v, c.v_scales));
+    return !work || S_max == 0 ||
+           (check_mx4(who, c.k, c.k_scales) && check_mx4(who, c.v, c.v_scales));
 }
 }  // namespace
 
@@ -1653,9 +1655,10 @@ bool anima_hip_kv4_append_dev(const void *k, const void *v, int dtype, const int
         return false;
     Kv4Append p;
     p.cache = Kv4Cache{k_codes, k_scales, v_codes, v_scales};
-    if (!check_kv4("kv4_append_dev", p.cache, H_kv, D, S_max))
+    const bool work = B > 0 && S_new > 0;
+    if (!check_kv4("kv4_append_dev", p.cache, H_kv, D, S_max, work))
         return false;
-    if (B > 0 && S_new > 0 && S_max > 0) {
+    if (work && S_max > 0) {
         if (!k || !v || !starts)
             return fail("kv4_append_dev: null pointer");
         if (!elem_aligned(k, t) || !elem_aligned(v, t))
@@ -1701,7 +1704,8 @@ bool anima_hip_kv4_attention_dev(const void *q, int dtype, const int64_t *q_stri
     Kv4Attention p;
     p.cache = Kv4Cache{const_cast<uint8_t *>(k_codes), const_cast<uint8_t *>(k_scales),
                        const_cast<uint8_t *>(v_codes), const_cast<uint8_t *>(v_scales)};
-    if (!check_kv4("kv4_attention_dev", p.cache, H_kv, D, S_max))
+    const bool work = B > 0 && S_q > 0 && H > 0;
+    if (!check_kv4("kv4_attention_dev", p.cache, H_kv, D, S_max, work))
         return false;
     if (H % H_kv)
         return fail("kv4_attention_dev: H must be a multiple of H_kv");
@@ -1710,7 +1714,7 @@ bool anima_hip_kv4_attention_dev(const void *q, int dtype, const int64_t *q_stri
                     "for all");
     if (int64_t(S_q) * H > kMx4MaxDim)
         return fail("kv4_attention_dev: S_q * H must be at most 2^30");
-    if (B > 0 && S_q > 0 && H > 0) {
+    if (work) {
         if (!q || !out || !lens)
             return fail("kv4_attention_dev: null pointer");
         if (!elem_aligned(q, t) || !elem_aligned(out, t))

@@ -574,7 +574,8 @@ bool anima_hip_dit_euler_dev(anima_hip_dit *dit, float *latent, const float *sig
  * scales 4-byte aligned.  dtype of values and activations:
  * ANIMA_HIP_DTYPE_F32 or ANIMA_HIP_DTYPE_BF16.  Nothing is allocated; all
  * entries are asynchronous on `stream` and may be captured into a HIP graph.
- * Rows and lengths of up to 2^30. */
+ * Rows and lengths of up to 2^30.  Calls that overlap in time need scratch of
+ * their own. */
 
 /* x [rows][ldx] (K elements of each row) to MX4 rows.  With a the largest
  * magnitude of a group and 2^E <= a < 2^(E+1), its scale byte is E - 2 + 127,
@@ -583,18 +584,21 @@ bool anima_hip_dit_euler_dev(anima_hip_dit *dit, float *latent, const float *sig
  * holds an infinity or a NaN gets scale 255 and zero codes. */
 bool anima_hip_mx4_pack_dev(const void *x, int64_t ldx, int dtype, uint8_t *codes, uint8_t *scales,
                             int64_t rows, int K, void *stream);
-/* The values of MX4 rows (each is exact in either type).  Also reads back the
- * caches below, whose rows are MX4 rows of D elements. */
+/* The values of MX4 rows, each exact in either type (but magnitudes of 2^128 and
+ * more, which only scale bytes 253 and 254 reach: infinite).  Also reads back
+ * the caches below, whose rows are MX4 rows of D elements. */
 bool anima_hip_mx4_unpack_dev(const uint8_t *codes, const uint8_t *scales, void *x, int64_t ldx,
                               int dtype, int64_t rows, int K, void *stream);
 
 /* C[M,N] = A[M,K] . W[N,K]^T with W in MX4 rows (N rows of K) and A, C both of
  * `dtype`: anima_hip_linear_dev with 4-bit weights.  The weights enter the
- * product exactly; f32 activations do too (three bf16 terms), sums are f32 and
- * C is rounded once.  lda, ldc: row strides in elements, any multiple of the
- * element.  scratch: anima_hip_linear_mx4_scratch_bytes(M, N, K, dtype) bytes,
- * 16-byte aligned (0: none needed); it holds the partial sums of a product
- * split over K, added in a fixed order. */
+ * product exactly, whatever their scale bytes (an element of 2^128 or more, see
+ * above, gives an infinity or NaN); f32 activations do too (three bf16 terms),
+ * sums are f32 and C is rounded once.  lda, ldc: row strides in elements.
+ * scratch: anima_hip_linear_mx4_scratch_bytes(M, N, K, dtype) bytes, 16-byte
+ * aligned (0: none needed); it holds the partial sums of a product split over
+ * K, added in a fixed order, or for a large product whose K is no multiple of
+ * 128 the operands padded to one, laid out anew by each call. */
 size_t anima_hip_linear_mx4_scratch_bytes(int M, int N, int K, int dtype);
 bool anima_hip_linear_mx4_dev(const void *a, int64_t lda, const uint8_t *codes,
                               const uint8_t *scales, void *c, int64_t ldc, int M, int N, int K,
