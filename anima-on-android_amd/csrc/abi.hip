@@ -1699,8 +1699,8 @@ bool anima_hip_kv4_attention_dev(const void *q, int dtype, const int64_t *q_stri
     Mx4Type t;
     if (!mx4_type("kv4_attention_dev", dtype, t) || !check_dims(B, H, S_q, S_max, D))
         return false;
-    if (!std::isfinite(scale))
-        return fail("kv4_attention_dev: scale must be finite");
+    if (!std::isfinite(scale * 2.0f))  // times log2(e) too
+        return fail("kv4_attention_dev: scale must be finite, its magnitude below 2^127");
     Kv4Attention p;
     p.cache = Kv4Cache{const_cast<uint8_t *>(k_codes), const_cast<uint8_t *>(k_scales),
                        const_cast<uint8_t *>(v_codes), const_cast<uint8_t *>(v_scales)};

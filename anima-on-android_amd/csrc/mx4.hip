@@ -169,6 +169,8 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(const T *k, const T *v,
                (is_v ? p.cache.v_scales : p.cache.k_scales) + dst, piece);
 }
 
+constexpr int64_t kMx4MaxGroups = (int64_t(1) << 29) - 64;
+
 // Pieces of eight elements can move as 16-byte accesses: base, and every
 // stride in elements.
 bool wide(const void *p, int64_t ld, Mx4Type t)
@@ -176,10 +178,10 @@ bool wide(const void *p, int64_t ld, Mx4Type t)
     return flash_tile::aligned(p, 16) && ld % (t == kMx4F32 ? 4 : 8) == 0;
 }
 
-// Groups of a call as a 32-bit count: 2^31 groups are 2^36 elements.
+// Groups of a call, up to eight threads each, in one launch of at most 2^32 threads.
 bool group_count(const char *who, int64_t rows, int64_t groups, unsigned &total)
 {
-    if (groups > 0 && rows > INT32_MAX / groups)
+    if (groups > 0 && rows > kMx4MaxGroups / groups)
         return fail(std::string(who) + ": too many elements");
     total = unsigned(rows * groups);
     return true;
@@ -234,7 +236,7 @@ bool launch_kv4_append(const void *k, const void *v, Mx4Type type, const Kv4Appe
 {
     unsigned total = 0;
     const int64_t rows = int64_t(p.B) * p.S_new;
-    if (p.H_kv > 0 && rows > INT32_MAX / p.H_kv)
+    if (p.H_kv > 0 && rows > kMx4MaxGroups / p.H_kv)
         return fail("kv4_append_dev: too many elements");
     if (!group_count("kv4_append_dev", rows * p.H_kv, mx4_groups(p.D), total))
         return false;

@@ -75,12 +75,22 @@ __device__ __forceinline__ float quad_max(float v)
 }
 
 // The argument of a probability's exponential.  bf16 queries: one fused
-// operation, off by a rounding of the scaled maximum, far below the rounding
-// of P; f32 queries: the maximum's own probability is exactly 1.
+// operation, off by a rounding of the scaled maximum for all keys of a row
+// alike (from 2^24 on, where that passes 1, see far_row); f32 queries: the
+// maximum's own probability is exactly 1.
 template <int NT>
 __device__ __forceinline__ float exponent(float score, float mx, float scale2, float m2)
 {
     return NT == 1 ? __builtin_fmaf(score, scale2, -m2) : (score - mx) * scale2;
+}
+
+// bf16 queries: a row whose scaled maximum m2 has no fraction left.  Its scores
+// take their distance from the maximum first.
+constexpr float kFarLog2 = 0x1p24f;
+template <int NT>
+__device__ __forceinline__ bool far_row(float mx, float m2)
+{
+    return NT == 1 && mx != -INFINITY && fabsf(m2) > kFarLog2;
 }
 
 struct AttnArgs {
@@ -168,7 +178,6 @@ __device__ __forceinline__ void p_terms(const float (&p)[8], bf16x8 (&t)[3])
 }
 
 // ----------------------------------------------------------- token kernel
-
 
 // A wave's loads for 32 keys.  Lane (m, g): K rows t0 + m and t0 + 16 + m,
 // dimensions g * D/4 .. ; V rows of the eight keys 4g + 0..3 and 16 + 4g +
@@ -334,7 +343,16 @@ __global__ __launch_bounds__(kTokWaves * 64, 2) void kv4_token_kernel(AttnArgs a
                 for (int r = 0; r < 4; ++r)
                     o[i][r] *= alpha;
         }
-        const float m2 = mx * scale2;
+        float m2 = mx * scale2;
+        if (NT == 1 && __builtin_amdgcn_ballot_w64(far_row<NT>(mx, m2)) != 0) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                float x = sc[i] - mx;
+                asm volatile("" : "+v"(x));  // stays behind the branch
+                sc[i] = x;
+            }
+            m2 = 0.0f;
+        }
         float pr[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -471,7 +489,6 @@ __global__ __launch_bounds__(kTokWaves * 64, 2) void kv4_token_kernel(AttnArgs a
 }
 
 // ------------------------------------------------------------ tile kernel
-
 
 // 16-byte pieces of a staged K row (D / 8 of them) and V^T row (8), placed so
 // that the 16 rows a ds_read_b128 quarter touches lie in distinct banks.
@@ -693,7 +710,18 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void kv4_tile_kernel(AttnArgs a
                 for (int r = 0; r < 16; ++r)
                     o[i][r] *= alpha;
         }
-        const float m2 = mx * scale2;
+        float m2 = mx * scale2;
+        if (NT == 1 && __builtin_amdgcn_ballot_w64(far_row<NT>(mx, m2)) != 0) {
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    float x = sc[kb][r] - mx;
+                    asm volatile("" : "+v"(x));
+                    sc[kb][r] = x;
+                }
+            m2 = 0.0f;
+        }
         // Sixteen keys at a time: the MFMAs of one group run under the
         // exponentials of the next.
 #pragma unroll
@@ -917,8 +945,8 @@ bool run_attention_kv4(AttnArgs &a, bool tile, hipStream_t st)
 {
     const int64_t blocks = int64_t(a.p.B) * a.p.H_kv * a.tiles * a.splits;
     const int64_t rows = int64_t(a.p.B) * a.p.S_q * a.p.H;
-    if (blocks > INT32_MAX || rows > INT32_MAX)
-        return fail("kv4_attention_dev: too many query rows");
+    if (!launch_fits(blocks, 256) || !launch_fits(a.splits > 1 ? rows : 0, 256))
+        return fail("kv4_attention_dev: too many query rows for one launch");
     if (tile)
         hipLaunchKernelGGL((kv4_tile_kernel<T, D>), dim3(unsigned(blocks)), dim3(kTileWaves * 64),
                            0, st, a);

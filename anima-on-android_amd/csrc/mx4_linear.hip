@@ -196,7 +196,6 @@ __global__ __launch_bounds__(WAVES * 64) void linear_few_kernel(LinArgs p)
 
 // ---------------------------------------------------------------- tiles
 
-
 // 16-byte pieces of a staged 128-byte row, so that the 16 rows of a
 // ds_read_b128 quarter touch distinct banks.
 __device__ __forceinline__ int swizzle(int row, int piece)
@@ -824,7 +823,6 @@ __global__ __launch_bounds__(256) void linear_pad_kernel(LinArgs p, T *a, uint8_
 STAGED_BF16(CHECK_BF16)
 STAGED_F32(CHECK_F32)
 
-
 template <typename T, bool VEC>
 bool run_few(LinArgs &p, hipStream_t st)
 {
@@ -835,9 +833,12 @@ bool run_few(LinArgs &p, hipStream_t st)
     const int chunk_blocks = std::min(room, blocks);
     p.chunk = chunk_blocks * kFewBlock;
     const dim3 grid((p.N + 15) / 16);
-    if (chunk_blocks >= 12)
+    const int waves = chunk_blocks >= 12 ? 16 : chunk_blocks >= 6 ? 8 : 4;
+    if (!launch_fits(grid.x, waves * 64))
+        return fail("linear_mx4_dev: too many weight rows for one launch");
+    if (waves == 16)
         hipLaunchKernelGGL((linear_few_kernel<T, 16, VEC>), grid, dim3(1024), 0, st, p);
-    else if (chunk_blocks >= 6)
+    else if (waves == 8)
         hipLaunchKernelGGL((linear_few_kernel<T, 8, VEC>), grid, dim3(512), 0, st, p);
     else
         hipLaunchKernelGGL((linear_few_kernel<T, 4, VEC>), grid, dim3(256), 0, st, p);
@@ -889,8 +890,8 @@ bool run_pad(const LinArgs &p, void *a, uint8_t *codes, uint8_t *scales, hipStre
     const int padded = lin_padded(p.K);
     const int64_t a_blocks = (int64_t(p.M) * (padded * int(sizeof(T)) / 16) + 255) / 256;
     const int64_t w_blocks = (int64_t(p.N) * (padded / 32) + 255) / 256;
-    if (a_blocks + w_blocks > INT32_MAX)
-        return fail("linear_mx4_dev: too many rows");
+    if (!launch_fits(a_blocks + w_blocks, 256))
+        return fail("linear_mx4_dev: operands too large for one launch");
     hipLaunchKernelGGL(linear_pad_kernel<T>, dim3(unsigned(a_blocks + w_blocks)), dim3(256), 0, st,
                        p, static_cast<T *>(a), codes, scales, padded, unsigned(a_blocks));
     return hip_ok(hipGetLastError(), "linear_pad_kernel launch");
@@ -903,8 +904,8 @@ bool run_linear(LinArgs &p, const LinPlan &pl, bool rows16, hipStream_t st)
     if (pl.kernel == kFew)
         return vec ? run_few<T, true>(p, st) : run_few<T, false>(p, st);
     const int64_t blocks = int64_t(pl.tiles_m) * pl.tiles_n * pl.splits;
-    if (blocks > INT32_MAX)
-        return fail("linear_mx4_dev: too many tiles");
+    if (!launch_fits(blocks, pl.kernel == kStaged ? 512 : 256))
+        return fail("linear_mx4_dev: too many tiles for one launch");
     const dim3 grid(static_cast<unsigned>(blocks));
     const bool ok = pl.kernel == kStaged ? run_staged<T>(p, pl.shape, grid, st)
                     : vec                ? run_tiles<T, true>(p, pl.shape, grid, st)

@@ -10,6 +10,9 @@
 namespace anima_hip {
 namespace mx4_plan {
 
+// The runtime counts the threads of a launch in 32 bits.
+inline bool launch_fits(int64_t blocks, int threads) { return blocks <= UINT32_MAX / threads; }
+
 // ------------------------------------------------- linear (mx4_linear.hip)
 
 constexpr int kFewRows = 16;  // most rows of A of the few-rows kernel

@@ -574,7 +574,8 @@ bool anima_hip_dit_euler_dev(anima_hip_dit *dit, float *latent, const float *sig
  * scales 4-byte aligned.  dtype of values and activations:
  * ANIMA_HIP_DTYPE_F32 or ANIMA_HIP_DTYPE_BF16.  Nothing is allocated; all
  * entries are asynchronous on `stream` and may be captured into a HIP graph.
- * Rows and lengths of up to 2^30.  Calls that overlap in time need scratch of
+ * Rows and lengths of up to 2^30; a call that would take more than 2^32 threads
+ * (from 2^34 values on) is refused.  Calls that overlap in time need scratch of
  * their own. */
 
 /* x [rows][ldx] (K elements of each row) to MX4 rows.  With a the largest

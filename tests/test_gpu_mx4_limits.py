@@ -154,3 +154,49 @@ def test_empty_calls():
                                            out.addr, None, 1, 1, 2, 2, 2, 64, 0, ct.c_float(1.0),
                                            True, None, 0, None)
     assert (out.get((1, 2, 2, 64)) == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [ref.F32, ref.BF16])
+@pytest.mark.parametrize("S_q", [2, 300])
+@pytest.mark.parametrize("power", [20, 31, 45, 90])
+def test_far_scores(power, S_q, dtype):
+    """Scores of up to 6 * 2^power, some steps of 2^power / 2 apart, exact in f32: each row is the
+    mean of the values of the keys of its largest score, which one in seven keys has."""
+    B, H, D, S, scale = 1, 2, 128, 333, 0.1
+    rng = np.random.default_rng(power)
+    k, v = np.zeros((B, S, H, D)), rng.standard_normal((B, S, H, D))
+    steps = np.array([0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0])
+    k[..., 0] = steps[np.arange(S) % 7][None, :, None]
+    q = np.zeros((B, S_q, H, D))
+    q[..., 0] = 2.0 ** power * np.where(np.arange(S_q) % 2, -1, 1)[None, :, None]
+    cache = kv4.Cache(B, H, S, D)
+    kv4.append(cache, ref.typed(k, dtype)[0], ref.typed(v, dtype)[0], dtype, [0])
+    got = kv4.attend(cache, ref.typed(q, dtype)[0], dtype, [S], causal=False, scale=scale)
+    _, vc = cache.values()
+    for s in range(2):
+        top = np.arange(S) % 7 == (0 if s else 6)
+        val = vc[:, :, top]                                   # [B, H, keys, D]
+        want, mag = val.mean(2)[:, None], np.abs(val).mean(2)[:, None]
+        rows = got[:, s::2]
+        # Probabilities of 2^r (the top) and 0, one rounding each; f32 sums; out once.
+        bound = (2 * ref.HALF[dtype] + (S + 64) * kv4.U) * mag + ref.HALF[dtype] * np.abs(want)
+        assert (np.abs(rows - want) <= bound).all(), (power, s)
+
+
+def test_too_large_for_one_launch():
+    """Refused on the host, before any launch."""
+    from devmem import DevBuf
+    lib = _lib.load()
+    mem = DevBuf(4096)
+    at = mem.addr
+    for call in (
+            lambda: lib.anima_hip_mx4_pack_dev(at, 32, 0, at, at, 1 << 29, 32, None),
+            lambda: lib.anima_hip_mx4_unpack_dev(at, at, at, 32, 0, 1 << 29, 32, None),
+            lambda: lib.anima_hip_kv4_append_dev(at, at, 0, None, None, at, at, at, at, at, None,
+                                                 1 << 20, 1 << 8, 4, 64, 1 << 20, None),
+            lambda: lib.anima_hip_linear_mx4_dev(at, 128, at, at, at, 1 << 30, 1, 1 << 30, 128, 2,
+                                                 at, 4096, None),
+            lambda: lib.anima_hip_kv4_attention_dev(at, 2, None, at, at, at, at, at, None, at, None,
+                                                    1 << 23, 1, 1, 32, 32, 64, 512, ct.c_float(1.0),
+                                                    True, at, 4096, None)):
+        assert not call() and ("too many" in _lib.last_error() or "launch" in _lib.last_error())
