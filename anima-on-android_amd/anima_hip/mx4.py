@@ -40,6 +40,7 @@ class _Buffers:
         b = self._bufs.get(role)
         if b is None or b.nbytes < nbytes:
             if b is not None:
+                del self._bufs[role]  # first: the allocation below may fail
                 b.close()
             b = self._bufs[role] = DeviceArray(max(int(nbytes), 16))
         return b
