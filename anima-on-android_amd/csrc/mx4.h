@@ -97,8 +97,9 @@ __device__ __forceinline__ void terms2(float x0, float x1, unsigned (&t)[N])
         if (i + 1 < N) {
             const float h0 = __uint_as_float(u0 & 0xFFFF0000u);
             const float h1 = __uint_as_float(u1 & 0xFFFF0000u);
-            x0 = INF && x0 == h0 ? 0.0f : x0 - h0;
-            x1 = INF && x1 == h1 ? 0.0f : x1 - h1;
+            // What is left of an infinity is none.
+            x0 = INF && i == 0 && x0 == h0 ? 0.0f : x0 - h0;
+            x1 = INF && i == 0 && x1 == h1 ? 0.0f : x1 - h1;
         }
     }
 }

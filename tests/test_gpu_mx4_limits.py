@@ -200,3 +200,30 @@ def test_too_large_for_one_launch():
                                                     1 << 23, 1, 1, 32, 32, 64, 512, ct.c_float(1.0),
                                                     True, at, 4096, None)):
         assert not call() and ("too many" in _lib.last_error() or "launch" in _lib.last_error())
+
+
+@pytest.mark.parametrize("K", [128, 100])
+@pytest.mark.parametrize("M", [3, 40, 200])
+def test_linear_nan_patterns(M, K):
+    """f32 NaN of every kind (quiet, signalling, payload in the low half alone) make their row NaN;
+    infinities of both signs give infinities of the weight's sign."""
+    N = 64
+    rng = np.random.default_rng(M)
+    a = rng.standard_normal((M, K)).astype(np.float32)
+    bits = a.view(np.uint32)
+    bits[0, 5], bits[M // 2, K - 1], bits[M - 1, 40] = 0x7F800001, 0xFF800002, 0x7FC00000
+    bits[1, 7], bits[M - 2 if M > 3 else 1, 8] = 0x7F800000, 0xFF800000
+    w = rng.choice([-1.0, 1.0], (N, K)) * rng.choice([0.5, 1.0, 3.0, 6.0], (N, K))
+    codes, scales = ref.pack(w)
+    wv = ref.unpack(codes, scales, K)
+    assert (wv != 0).all()
+    got = mx4.linear(a, codes, scales, K, N, ref.F32)
+    with np.errstate(invalid="ignore"):
+        want = np.stack([[np.sum(a[m].astype(float) * wv[n]) for n in range(N)] for m in range(M)])
+    np.testing.assert_array_equal(np.isnan(got), np.isnan(want))
+    far = np.isinf(want)
+    np.testing.assert_array_equal(got[far], want[far])
+    ok = np.isfinite(want)
+    mag = np.abs(np.where(np.isfinite(a), a, 0).astype(float)) @ np.abs(wv).T
+    bound = (K + 32) * kv4.U * mag + kv4.U * np.abs(want)
+    assert (np.abs(got[ok] - want[ok]) <= bound[ok]).all()
