@@ -195,7 +195,7 @@ struct TokLoads {
     __device__ __forceinline__ void load_k(const uint8_t *codes, const uint8_t *scales, int h,
                                            unsigned key, unsigned g)
     {
-        const uint8_t *src = codes + key * ROW + g * (D / 8);
+        const uint8_t *src = codes + (key * ROW + g * (D / 8));
         if constexpr (D == 128) {
             const u32x4 w = *reinterpret_cast<const u32x4 *>(src);
 #pragma unroll
@@ -206,12 +206,12 @@ struct TokLoads {
             kc[h][0] = w[0];
             kc[h][1] = w[1];
         }
-        ks[h] = scales[key * GROUPS + g * GROUPS / 4];
+        ks[h] = *(scales + (key * GROUPS + g * GROUPS / 4));
     }
     __device__ __forceinline__ void load_v(const uint8_t *codes, const uint8_t *scales, int j,
                                            unsigned key, unsigned m)
     {
-        const uint8_t *src = codes + key * ROW + m * (D / 32);
+        const uint8_t *src = codes + (key * ROW + m * (D / 32));
         if constexpr (D == 128)
             vc[j] = *reinterpret_cast<const unsigned *>(src);
         else
