@@ -206,7 +206,7 @@ struct TokLoads {
             kc[h][0] = w[0];
             kc[h][1] = w[1];
         }
-        ks[h] = *(scales + (key * GROUPS + g * GROUPS / 4));
+        ks[h] = scales[key * GROUPS + g * GROUPS / 4];
     }
     __device__ __forceinline__ void load_v(const uint8_t *codes, const uint8_t *scales, int j,
                                            unsigned key, unsigned m)

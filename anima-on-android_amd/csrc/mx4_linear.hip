@@ -10,7 +10,8 @@
 //   * few rows (M <= 16), bound by the one pass over the codes (17/32 byte per
 //     weight) or, below about 8 MiB of codes, by latency: a workgroup takes 16
 //     weight rows, its waves share K in blocks of 128, and the weights go from
-//     memory to registers to the MFMA without touching LDS;
+//     memory to registers to the MFMA without touching LDS; or, of many weight
+//     rows, each wave takes 16 through all of K;
 //   * staged tiles (K a multiple of 128, 16-byte aligned rows of A), from 32 x 64 at
 //     small M to 192 x 256 (bf16) and 256 x 256 (f32): bound by latency and the stream
 //     into LDS at the small end, by the MFMA at the large;
@@ -191,6 +192,111 @@ __global__ __launch_bounds__(WAVES * 64) void linear_few_kernel(LinArgs p)
         for (int r = 0; r < 4; ++r)
             if (row0 + 4 * g + r < p.N)
                 store_c(c + r, sum[r]);
+    }
+}
+
+// ------------------------------------------ few rows, many weight rows
+
+// The rows of A stay in LDS, and each wave takes 16 weight rows at a time through all
+// of K, four blocks (256 bytes of each row) ahead across the ends of the rows:
+// no barrier after the first, and no sums between waves.  From 2048 strips of 16
+// weight rows on, a workgroup for every CU, if A's terms fit half a CU's LDS.
+// bf16, this kernel against the one above: 11.0 and 15.0 us at N x K = 32768 x
+// 2048, 10.5 and 7.6 at 16384 x 2048, 6.3 and 14.3 at 65536 x 500, 19.0 and 27.5
+// at 65536 x 2048, 146 and 143 at 131072 x 8192, M = 1; 35 (4.1 TB/s) and 54 at
+// 131072 x 2048, M = 8, 38 and 82 at M = 16; f32 162 and 173 at 131072 x 8192, M =
+// 1.  Blocks loaded one by one leave each row of the memory
+// too soon (163), eight at a time take 3 to 5 % more or less.
+constexpr int kWideWaves = 8, kWideBlocks = 4;
+constexpr int kWideStrips = 256 * kWideWaves;
+constexpr int kWideLds = 40960;  // staged bf16 elements (80 KiB)
+
+template <typename T, bool VEC>
+__global__ __launch_bounds__(kWideWaves * 64) void linear_wide_kernel(LinArgs p)
+{
+    constexpr int NT = kTerms<T>;
+    __shared__ __attribute__((aligned(16))) uint16_t smem[kWideLds];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 15, g = lane >> 4;
+    const int ld = p.chunk + kFewPad;
+    const int pieces = p.chunk / 8;
+    const int blocks = p.chunk / kFewBlock;
+    const int strips = (p.N + 15) / 16, step = int(gridDim.x) * kWideWaves;
+    int strip = int(blockIdx.x) * kWideWaves + wave;  // of the products
+    int lstrip = strip, lblk = 0;                     // of the next load
+
+    struct Batch {
+        u32x4 codes[kWideBlocks];
+        unsigned scale[kWideBlocks];
+    } cur, next;
+    const int batches = (blocks + kWideBlocks - 1) / kWideBlocks;
+    auto load = [&](Batch &b) {
+        const int64_t row = int64_t(min(lstrip * 16 + n, p.N - 1)) * p.groups;
+#pragma unroll
+        for (int i = 0; i < kWideBlocks; ++i) {
+            const int kg = (lblk * kWideBlocks + i) * 4 + g;
+            b.codes[i] = u32x4{0, 0, 0, 0};
+            b.scale[i] = 127;
+            if (kg < p.groups) {
+                b.codes[i] = *reinterpret_cast<const u32x4 *>(p.codes + (row + kg) * 16);
+                b.scale[i] = p.scales[row + kg];
+            }
+        }
+        if (++lblk == batches) {
+            lblk = 0;
+            lstrip += step;
+        }
+    };
+    if (strip < strips)
+        load(cur);
+    for (int i = tid; i < pieces * p.M; i += kWideWaves * 64) {
+        const int m = i / pieces, k8 = (i - m * pieces) * 8;
+        u32x4 t[NT];
+        load_terms8<VEC>(static_cast<const T *>(p.a) + m * p.lda, k8, p.K, t);
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+            *reinterpret_cast<u32x4 *>(smem + (j * p.M + m) * ld + k8) = t[j];
+    }
+    __syncthreads();
+
+    const uint16_t *x = smem + min(n, p.M - 1) * ld + 32 * g;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int t = 0; strip < strips;) {
+        if (lstrip < strips)
+            load(next);
+#pragma unroll
+        for (int i = 0; i < kWideBlocks; ++i) {
+            const int blk = t * kWideBlocks + i;
+            if (blk >= blocks)
+                break;
+            const float s = scale_of(cur.scale[i]);
+#pragma unroll
+            for (int st = 0; st < 4; ++st) {
+                const bf16x8 wf = decode8(cur.codes[i][st], s);
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+                    acc = mfma16(wf,
+                                 *reinterpret_cast<const bf16x8 *>(x + j * p.M * ld +
+                                                                   blk * kFewBlock + 8 * st),
+                                 acc);
+            }
+        }
+        cur = next;
+        if (++t < batches)
+            continue;
+        // Lane (n, g) holds weight rows 4g .. 4g+3 of batch row n.
+        const int c0 = strip * 16 + 4 * g;
+        if (n < p.M) {
+            T *c = static_cast<T *>(p.c) + n * p.ldc + c0;
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (c0 + r < p.N)
+                    store_c(c + r, acc[r]);
+        }
+        acc = f32x4{0.f, 0.f, 0.f, 0.f};
+        t = 0;
+        strip += step;
     }
 }
 
@@ -826,13 +932,21 @@ STAGED_F32(CHECK_F32)
 template <typename T, bool VEC>
 bool run_few(LinArgs &p, hipStream_t st)
 {
+    const int blocks = std::max(1, (p.K + kFewBlock - 1) / kFewBlock);
+    const int strips = (p.N + 15) / 16;
+    if (strips >= kWideStrips &&
+        kTerms<T> * p.M * (int64_t(blocks) * kFewBlock + kFewPad) <= kWideLds) {
+        p.chunk = blocks * kFewBlock;
+        const dim3 grid(std::min(512, (strips + kWideWaves - 1) / kWideWaves));
+        hipLaunchKernelGGL((linear_wide_kernel<T, VEC>), grid, dim3(kWideWaves * 64), 0, st, p);
+        return hip_ok(hipGetLastError(), "linear_wide_kernel launch");
+    }
     // Elements of K staged at once, in whole blocks, and as many waves as have
     // a block of it each.
-    const int blocks = std::max(1, (p.K + kFewBlock - 1) / kFewBlock);
     const int room = (kFewLds / (kTerms<T> * p.M) - kFewPad) / kFewBlock;
     const int chunk_blocks = std::min(room, blocks);
     p.chunk = chunk_blocks * kFewBlock;
-    const dim3 grid((p.N + 15) / 16);
+    const dim3 grid(strips);
     const int waves = chunk_blocks >= 12 ? 16 : chunk_blocks >= 6 ? 8 : 4;
     if (!launch_fits(grid.x, waves * 64))
         return fail("linear_mx4_dev: too many weight rows for one launch");

@@ -194,7 +194,7 @@ def test_too_large_for_one_launch():
             lambda: lib.anima_hip_mx4_unpack_dev(at, at, at, 32, 0, 1 << 29, 32, None),
             lambda: lib.anima_hip_kv4_append_dev(at, at, 0, None, None, at, at, at, at, at, None,
                                                  1 << 20, 1 << 8, 4, 64, 1 << 20, None),
-            lambda: lib.anima_hip_linear_mx4_dev(at, 128, at, at, at, 1 << 30, 1, 1 << 30, 128, 2,
+            lambda: lib.anima_hip_linear_mx4_dev(at, 4096, at, at, at, 1 << 30, 16, 1 << 30, 4096, 2,
                                                  at, 4096, None),
             lambda: lib.anima_hip_kv4_attention_dev(at, 2, None, at, at, at, at, at, None, at, None,
                                                     1 << 23, 1, 1, 32, 32, 64, 512, ct.c_float(1.0),
@@ -227,3 +227,25 @@ def test_linear_nan_patterns(M, K):
     mag = np.abs(np.where(np.isfinite(a), a, 0).astype(float)) @ np.abs(wv).T
     bound = (K + 32) * kv4.U * mag + kv4.U * np.abs(want)
     assert (np.abs(got[ok] - want[ok]) <= bound[ok]).all()
+
+
+@pytest.mark.parametrize("dtype", [ref.F32, ref.BF16])
+@pytest.mark.parametrize("M,N,K", [(1, 32753, 2048), (3, 70001, 500), (16, 33333, 96), (5, 65537, 1000),
+                                   (1, 40000, 1), (16, 32768, 768), (4, 50007, 2560)])
+def test_linear_many_weight_rows(M, N, K, dtype):
+    """N of 2048 strips of 16 and more: 97 distinct weight rows over and over (97 shares no factor
+    with a strip), one of them with a NaN group, which is its column's alone."""
+    rng = np.random.default_rng(N)
+    raw, a = ref.typed(rng.standard_normal((M, K)), dtype)
+    codes, scales = ref.pack(rng.standard_normal((97, K)) * 0.05)
+    scales[13, -1] = 255
+    rows = np.arange(N) % 97
+    for shift, ld in ((0, K), (1, K + 3)):
+        got = mx4.linear(raw, codes[rows], scales[rows], K, N, dtype, lda=ld, shift=shift)
+        wv = ref.unpack(codes, scales, K)
+        want, mag = a @ wv.T, np.abs(a) @ np.abs(wv).T
+        assert np.isnan(got[:, rows == 13]).all()
+        ok = rows != 13
+        err = np.abs(got - want[:, rows])[:, ok]
+        bound = (K + 32) * kv4.U * mag + ref.HALF[dtype] * np.abs(want)
+        assert (err <= bound[:, rows][:, ok]).all()
