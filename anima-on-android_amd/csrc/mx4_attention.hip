@@ -12,7 +12,9 @@
 //   * token kernel: 16 query rows per wave on v_mfma_f32_16x16x32_bf16, the
 //     waves of a workgroup and the workgroups of a split sharing the keys.
 //     Bound by the one pass over the cache (17/16 byte per key and dimension
-//     for K and V together), or by latency where the cache is short.  Codes go
+//     for K and V together: 91 MB in 22 us, 4.2 TB/s, for a query each of 16
+//     sequences of up to 16384 keys), by latency where the cache is short (200
+//     keys 8 us), and by its VALU work where the rows are many.  Codes go
 //     from memory to registers to the MFMA and nothing is staged in LDS: a
 //     lane's 16 bytes of a K row are one scale group (the MFMA's k index runs
 //     over d in the order the lanes hold it), and V^T fragments are pairs of

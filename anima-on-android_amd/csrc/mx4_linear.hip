@@ -8,7 +8,7 @@
 //
 // Three kernels:
 //   * few rows (M <= 16), bound by the one pass over the codes (17/32 byte per
-//     weight) or, below about 8 MiB of codes, by latency: a workgroup takes 16
+//     weight) or, below about 8 MiB of codes, by latency (2048 x 2048 4.0 us): a workgroup takes 16
 //     weight rows, its waves share K in blocks of 128, and the weights go from
 //     memory to registers to the MFMA without touching LDS; or, of many weight
 //     rows, each wave takes 16 through all of K;
