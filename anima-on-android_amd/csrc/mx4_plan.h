@@ -161,17 +161,20 @@ struct AttnPlan {
 
 // Microseconds of a workgroup per 128 keys (token kernel, 16 query rows) and per 64 keys
 // (tile kernel, 128 rows), alone on a CU and as its share of a CU that has two;
-// bf16 and f32 queries, D of 64 and 128.  Measured at one query to 2048 over 200 to
-// 20000 keys.
+// bf16 and f32 queries, D of 64 and 128.  These and the constants of the model are
+// fitted to the times of 1400 calls, 1 to 64 sequences of unequal lengths of 100
+// to 30000 keys, 1 to 1000 queries, 1 to 32 K/V heads.
 struct Rate {
     double token1, token2, tile1, tile2;
 };
-constexpr Rate kRates[2][2] = {{{0.65, 0.46, 1.45, 0.9}, {0.78, 0.62, 1.75, 1.45}},
-                               {{0.8, 0.59, 2.15, 1.85}, {1.05, 0.85, 4.8, 3.0}}};
+constexpr Rate kRates[2][2] = {{{0.71, 0.47, 1.59, 0.99}, {0.92, 0.59, 1.81, 1.1}},
+                               {{0.7, 0.5, 2.04, 1.4}, {1.03, 0.97, 5.08, 3.29}}};
 
-// The kernel and the split that the model expects to take least: about 6 us of
-// latency, the keys of the longest share or of a full CU, and with splits the partial
-// results written and joined.  The token kernel, which meets at no barrier, is ahead to
+// The kernel and the split that the model expects to take least: latency, the keys
+// of the longest share or of a full CU (half a workgroup's more on the fullest),
+// and with splits the partial results written and joined.  On 500 calls beside those
+// of the fit the choice is 0.8 % behind the fastest of all kernels and splits on
+// average, 11 % in the worst twentieth.  The token kernel, which meets at no barrier, is ahead to
 // some hundred query rows of a K/V head and in f32 further: 2048 rows of 512 keys,
 // 4 K/V heads, take 10.8 us by it and 18.7 by the tile kernel (bf16); 4096 x 512 keys,
 // 32 heads, 50 us by the tile kernel against 141 by the first token kernel.
@@ -202,10 +205,11 @@ inline AttnPlan attn_plan(int B, int S_q, int H, int H_kv, int D, int S_max, boo
             // The longest share, or the work of a full CU.
             const double alone = pl.tile ? rate.tile1 : rate.token1;
             const double full = pl.tile ? rate.tile2 : rate.token2;
-            double us = 6 + std::max(share * alone, share * part * load * full) +
-                        3 * std::max(0.0, load / 2 - 1);
+            const double work = part * load + 0.5 * std::min(load, 1.0);
+            double us = 6.6 + std::max(share * alone, share * work * full) +
+                        2.4 * std::max(0.0, load / 2 - 1);
             if (pl.splits > 1)
-                us += 3 + bytes / 4e6 + bytes / 6e6;
+                us += 3.1 + bytes / 2e6;
             if (us < best_us) {
                 best_us = us;
                 best = pl;
