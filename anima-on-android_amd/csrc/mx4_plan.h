@@ -95,13 +95,14 @@ inline LinPlan staged_plan(int M, int N, int K, bool f32)
 inline LinPlan lin_plan(int M, int N, int K, bool f32, bool staged)
 {
     LinPlan pl;
-    // Few rows, unless their terms take long to stage in every workgroup: 16 rows of
-    // 8192 bf16 take 12.5 us against 9.8 (N = 2048), 8 rows of 8192 f32 18 against
-    // 15, 16 of 2048 13 against 8.8; 4 rows of 8192 f32 12 against 15, 16 of 2048
-    // bf16 5.5 against 7.4.
-    const int64_t terms = int64_t(M) * (f32 ? 3 : 1);
-    if (M <= kFewRows &&
-        (!staged || K % 128 || terms * K <= 24576 || (terms <= 24 && terms * K <= 100000)))
+    // Few rows, unless their terms take long to stage in every workgroup.  bf16, N =
+    // 2048: 16 rows of 8192 take 12.5 us against 9.8 on staged tiles, 16 of 2048 5.5
+    // against 7.4.  f32: 4 rows of 11008 13.6 against 18.2 (N = 2048), 8 of 8192 27.7
+    // against 28.7 (8192) but of 11008 32.2 against 28.8 (6144), 12 of 2048 10.8 against
+    // 12.5 (6144) but of 4096 13.1 against 10.9 (2048), 16 of 1024 7.7 against 8.1 (512) but
+    // of 1408 9.8 against 8.6 (2048).
+    const int64_t limit = !f32 || (M > 8 && M <= 12) ? 100000 : M <= 8 ? 200000 : 50000;
+    if (M <= kFewRows && (!staged || K % 128 || int64_t(M) * (f32 ? 3 : 1) * K <= limit))
         return pl;
     if (K > 0 && K % 128 == 0 && K <= kStagedMaxK && staged)
         return staged_plan(M, N, K, f32);
