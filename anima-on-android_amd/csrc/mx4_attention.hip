@@ -9,8 +9,11 @@
 // queries enter as they are and P as one bf16 term; f32 queries and their P
 // enter as three terms each (mx4::terms2), so products are exact to f32.
 //
-//   * token kernel: 16 query rows per wave on v_mfma_f32_16x16x32_bf16, the
-//     waves of a workgroup and the workgroups of a split sharing the keys.
+//   * token kernel: 16 or 32 query rows per wave on v_mfma_f32_16x16x32_bf16, the
+//     waves of a workgroup and the workgroups of a split sharing the keys.  32 rows
+//     read and decode a key once where 16 do so twice: 16 sequences of up to 8192
+//     keys, 8 queries, 32 heads on 8 of 128, bf16, 44.8 -> 35.5 us; in f32 at D = 128
+//     they take more registers than there are (56 -> 87).
 //     Bound by the one pass over the cache (17/16 byte per key and dimension
 //     for K and V together: 91 MB in 22 us, 4.2 TB/s, for a query each of 16
 //     sequences of up to 16384 keys), by latency where the cache is short (200
@@ -240,15 +243,15 @@ struct TokLoads {
     }
 };
 
-template <typename T, int D>
+template <typename T, int D, int RB>
 __global__ __launch_bounds__(kTokWaves * 64, 2) void kv4_token_kernel(AttnArgs a)
 {
     constexpr int NT = kTerms<T>;
     constexpr int STEPS = D / 32;  // MFMA steps of a score; V^T blocks of 16 are D / 16
     constexpr int VB = D / 16;
-    constexpr int OPITCH = D + 4;
-    __shared__ __attribute__((aligned(16))) float so[kTokWaves][kTokRows][OPITCH];
-    __shared__ float sm[kTokWaves][kTokRows], sl[kTokWaves][kTokRows];
+    constexpr int OPITCH = D + 4, ROWS = RB * kTokRows;
+    __shared__ __attribute__((aligned(16))) float so[kTokWaves][ROWS][OPITCH];
+    __shared__ float sm[kTokWaves][ROWS], sl[kTokWaves][ROWS];
 
     const Kv4Attention &p = a.p;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -262,28 +265,31 @@ __global__ __launch_bounds__(kTokWaves * 64, 2) void kv4_token_kernel(AttnArgs a
     const int tile = (blk / a.splits) / (p.B * p.H_kv);
     const int b = bh / p.H_kv, hk = bh - b * p.H_kv;
 
-    // This lane's query row (column n of the accumulators).  Rows past the last
+    // This lane's query rows (column n of the accumulators).  Rows past the last
     // read that one and are not written; a column's values stay its own.
-    const int row = tile * kTokRows + n;
-    const int rc = min(row, a.rows - 1);
-    const int s = rc / a.group, hq = hk * a.group + (rc - s * a.group);
+    const Seq seq(p, b, hk);
     // Scores are kept unscaled; the sign of the scale goes into the queries.
     const float scale2 = fabsf(a.scale2);
-    bf16x8 qf[STEPS][NT];
-    {
+    bf16x8 qf[RB][STEPS][NT];
+    int limit[RB], most = 0, least = INT32_MAX;
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+        const int row = tile * ROWS + kTokRows * rb + n;
+        const int rc = min(row, a.rows - 1);
+        const int s = rc / a.group, hq = hk * a.group + (rc - s * a.group);
         const T *q = static_cast<const T *>(p.q);
         const T *qr = q + b * p.qs.b + hq * p.qs.h + s * p.qs.s;
         const bool wide = ((reinterpret_cast<uintptr_t>(q) & 15) |
                            ((p.qs.b | p.qs.h | p.qs.s) & 7)) == 0;
 #pragma unroll
         for (int st = 0; st < STEPS; ++st)
-            q_terms(qr + g * (D / 4) + 8 * st, wide, a.scale2 < 0.0f, qf[st]);
+            q_terms(qr + g * (D / 4) + 8 * st, wide, a.scale2 < 0.0f, qf[rb][st]);
+        const bool live = row < a.rows && s < seq.nq;
+        limit[rb] = live ? seq.limit(p, s) : 0;
+        most = max(most, limit[rb]);
+        least = min(least, live ? limit[rb] : INT32_MAX);
     }
-    const Seq seq(p, b, hk);
-    const bool live = row < a.rows && s < seq.nq;
-    const int limit = live ? seq.limit(p, s) : 0;
     // Keys any row of the tile sees, and keys all of its live rows see.
-    int most = limit, least = live ? limit : INT32_MAX;
 #pragma unroll
     for (int o = 8; o; o >>= 1) {
         most = max(most, __shfl_xor(most, o));
@@ -297,74 +303,90 @@ __global__ __launch_bounds__(kTokWaves * 64, 2) void kv4_token_kernel(AttnArgs a
     const int per = (steps + a.splits - 1) / a.splits;
     const int first = split * per, end = min(first + per, steps);
 
-    f32x4 o[VB];
+    f32x4 o[RB][VB];
+    float mx[RB], sum[RB];
 #pragma unroll
-    for (int i = 0; i < VB; ++i)
-        o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float mx = -INFINITY, sum = 0.0f;
+    for (int rb = 0; rb < RB; ++rb) {
+#pragma unroll
+        for (int i = 0; i < VB; ++i)
+            o[rb][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        mx[rb] = -INFINITY;
+        sum[rb] = 0.0f;
+    }
 
     auto step = [&](const TokLoads<D> &ld, int t0, auto masked) {
         constexpr bool MASK = decltype(masked)::value;
-        // Scores: key 16 h + 4 g + r of query n in sc[4 h + r].
-        float sc[8];
+        // Scores: key 16 h + 4 g + r of query n in sc[rb][4 h + r].
+        float sc[RB][8];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+            f32x4 acc[RB];
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb)
+                acc[rb] = f32x4{0.f, 0.f, 0.f, 0.f};
             const float ksc = scale_of(ld.ks[h]);
 #pragma unroll
             for (int st = 0; st < STEPS; ++st) {
                 const bf16x8 kf = decode8(ld.kc[h][st], ksc);
 #pragma unroll
-                for (int j = 0; j < NT; ++j)
-                    acc = mfma16(kf, qf[st][j], acc);
+                for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+                        acc[rb] = mfma16(kf, qf[rb][st][j], acc[rb]);
             }
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                sc[4 * h + r] = acc[r];
-        }
-        const int room = limit - t0 - 4 * g;  // keys 16 h + r below it are seen
-        float mt = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (!MASK || 16 * (i >> 2) + (i & 3) < room)
-                mt = fmaxf(mt, sc[i]);
-        mt = quad_max(mt);
-        // The maximum moves when a row has none yet or is 2^8 behind: until
-        // then probabilities stay below 2^8 and nothing is rescaled.
-        const bool move = mx == -INFINITY ? mt > mx : (mt - mx) * scale2 > kRescaleLog2;
-        if (__builtin_amdgcn_ballot_w64(move) != 0) {
-            const float mn = move ? mt : mx;
-            const float alpha = mx == mn || mx == -INFINITY
-                                    ? 1.0f
-                                    : __builtin_amdgcn_exp2f((mx - mn) * scale2);
-            mx = mn;
-            sum *= alpha;
-#pragma unroll
-            for (int i = 0; i < VB; ++i)
+            for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    o[i][r] *= alpha;
+                    sc[rb][4 * h + r] = acc[rb][r];
         }
-        float m2 = mx * scale2;
-        if (NT == 1 && __builtin_amdgcn_ballot_w64(far_row<NT>(mx, m2)) != 0) {
+        bf16x8 pf[RB][NT];
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+            const int room = limit[rb] - t0 - 4 * g;  // keys 16 h + r below it are seen
+            float mt = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (!MASK || 16 * (i >> 2) + (i & 3) < room)
+                    mt = fmaxf(mt, sc[rb][i]);
+            mt = quad_max(mt);
+            // The maximum moves when a row has none yet or is 2^8 behind: until
+            // then probabilities stay below 2^8 and nothing is rescaled.
+            const bool move =
+                mx[rb] == -INFINITY ? mt > mx[rb] : (mt - mx[rb]) * scale2 > kRescaleLog2;
+            if (__builtin_amdgcn_ballot_w64(move) != 0) {
+                const float mn = move ? mt : mx[rb];
+                const float alpha = mx[rb] == mn || mx[rb] == -INFINITY
+                                        ? 1.0f
+                                        : __builtin_amdgcn_exp2f((mx[rb] - mn) * scale2);
+                mx[rb] = mn;
+                sum[rb] *= alpha;
+#pragma unroll
+                for (int i = 0; i < VB; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        o[rb][i][r] *= alpha;
+            }
+            float m2 = mx[rb] * scale2;
+            if (NT == 1 && __builtin_amdgcn_ballot_w64(far_row<NT>(mx[rb], m2)) != 0) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    float x = sc[rb][i] - mx[rb];
+                    asm volatile("" : "+v"(x));  // stays behind the branch
+                    sc[rb][i] = x;
+                }
+                m2 = 0.0f;
+            }
+            float pr[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                float x = sc[i] - mx;
-                asm volatile("" : "+v"(x));  // stays behind the branch
-                sc[i] = x;
+                pr[i] = __builtin_amdgcn_exp2f(exponent<NT>(sc[rb][i], mx[rb], scale2, m2));
+                if (MASK && 16 * (i >> 2) + (i & 3) >= room)
+                    pr[i] = 0.0f;
+                sum[rb] += pr[i];
             }
-            m2 = 0.0f;
+            p_terms(pr, pf[rb]);
         }
-        float pr[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            pr[i] = __builtin_amdgcn_exp2f(exponent<NT>(sc[i], mx, scale2, m2));
-            if (MASK && 16 * (i >> 2) + (i & 3) >= room)
-                pr[i] = 0.0f;
-            sum += pr[i];
-        }
-        bf16x8 pf[NT];
-        p_terms(pr, pf);
         float vsc[8];
         unsigned nan = 0;
 #pragma unroll
@@ -388,10 +410,14 @@ __global__ __launch_bounds__(kTokWaves * 64, 2) void kv4_token_kernel(AttnArgs a
                 odd[jj] = __builtin_amdgcn_perm(x1, x0, 0x07060302);
             }
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                o[2 * c] = mfma16(__builtin_bit_cast(bf16x8, even), pf[j], o[2 * c]);
-                o[2 * c + 1] = mfma16(__builtin_bit_cast(bf16x8, odd), pf[j], o[2 * c + 1]);
-            }
+            for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    o[rb][2 * c] =
+                        mfma16(__builtin_bit_cast(bf16x8, even), pf[rb][j], o[rb][2 * c]);
+                    o[rb][2 * c + 1] =
+                        mfma16(__builtin_bit_cast(bf16x8, odd), pf[rb][j], o[rb][2 * c + 1]);
+                }
         }
         if (MASK && __builtin_amdgcn_ballot_w64(nan != 0) != 0) {
             // NaN groups of V: to the rows that see their keys.  Lane (m, g')
@@ -402,15 +428,18 @@ __global__ __launch_bounds__(kTokWaves * 64, 2) void kv4_token_kernel(AttnArgs a
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const unsigned bits = unsigned(__shfl(int(nan), 16 * gg + 4 * g + r));
-                    bool hit = false;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        hit = hit || ((bits >> j & 1u) &&
-                                      t0 + 16 * (j >> 2) + 4 * gg + (j & 3) < limit);
-                    if (hit)
+                    for (int rb = 0; rb < RB; ++rb) {
+                        bool hit = false;
 #pragma unroll
-                        for (int i = 0; i < VB; ++i)
-                            o[i][r] = NAN;
+                        for (int j = 0; j < 8; ++j)
+                            hit = hit || ((bits >> j & 1u) &&
+                                          t0 + 16 * (j >> 2) + 4 * gg + (j & 3) < limit[rb]);
+                        if (hit)
+#pragma unroll
+                            for (int i = 0; i < VB; ++i)
+                                o[rb][i][r] = NAN;
+                    }
                 }
         }
     };
@@ -443,21 +472,25 @@ __global__ __launch_bounds__(kTokWaves * 64, 2) void kv4_token_kernel(AttnArgs a
     }
 
     // Join the waves.  Lane (n, g) holds O^T rows d = (4 g + r) * VB + i of query n.
-    sum += __shfl_xor(sum, 16);
-    sum += __shfl_xor(sum, 32);
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+    for (int rb = 0; rb < RB; ++rb) {
+        const int nr = kTokRows * rb + n;
+        sum[rb] += __shfl_xor(sum[rb], 16);
+        sum[rb] += __shfl_xor(sum[rb], 32);
 #pragma unroll
-        for (int i = 0; i < VB; ++i)
-            so[wave][n][(4 * g + r) * VB + i] = o[i][r];
-    if (g == 0) {
-        sm[wave][n] = mx * scale2;
-        sl[wave][n] = sum;
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int i = 0; i < VB; ++i)
+                so[wave][nr][(4 * g + r) * VB + i] = o[rb][i][r];
+        if (g == 0) {
+            sm[wave][nr] = mx[rb] * scale2;
+            sl[wave][nr] = sum[rb];
+        }
     }
     __syncthreads();
-    constexpr int LANES = kTokWaves * 64 / kTokRows;  // threads of a row
+    constexpr int LANES = kTokWaves * 64 / ROWS;  // threads of a row
     const int jr = tid / LANES, jc = tid % LANES;
-    const int jrow = tile * kTokRows + jr;
+    const int jrow = tile * ROWS + jr;
     const int js = jrow / a.group, jh = hk * a.group + (jrow - js * a.group);
     if (jrow >= a.rows || js >= seq.nq)
         return;
@@ -943,18 +976,19 @@ int64_t part_bytes(int B, int S_q, int H, int D, int splits)
 }
 
 template <typename T, int D>
-bool run_attention_kv4(AttnArgs &a, bool tile, hipStream_t st)
+bool run_attention_kv4(AttnArgs &a, const AttnPlan &pl, hipStream_t st)
 {
     const int64_t blocks = int64_t(a.p.B) * a.p.H_kv * a.tiles * a.splits;
     const int64_t rows = int64_t(a.p.B) * a.p.S_q * a.p.H;
     if (!launch_fits(blocks, 256) || !launch_fits(a.splits > 1 ? rows : 0, 256))
         return fail("kv4_attention_dev: too many query rows for one launch");
-    if (tile)
-        hipLaunchKernelGGL((kv4_tile_kernel<T, D>), dim3(unsigned(blocks)), dim3(kTileWaves * 64),
-                           0, st, a);
-    else
-        hipLaunchKernelGGL((kv4_token_kernel<T, D>), dim3(unsigned(blocks)), dim3(kTokWaves * 64),
-                           0, st, a);
+    const dim3 grid{unsigned(blocks)};
+    if (pl.tile)
+        hipLaunchKernelGGL((kv4_tile_kernel<T, D>), grid, dim3(kTileWaves * 64), 0, st, a);
+    else if (pl.row_blocks == 1)
+        hipLaunchKernelGGL((kv4_token_kernel<T, D, 1>), grid, dim3(kTokWaves * 64), 0, st, a);
+    else if constexpr (two_row_blocks(kTerms<T> == 3, D))
+        hipLaunchKernelGGL((kv4_token_kernel<T, D, 2>), grid, dim3(kTokWaves * 64), 0, st, a);
     if (!hip_ok(hipGetLastError(), "kv4 attention launch"))
         return false;
     if (a.splits == 1)
@@ -1008,10 +1042,10 @@ bool launch_kv4_attention(const Kv4Attention &p, void *scratch, size_t scratch_b
         a.ml = reinterpret_cast<float2 *>(a.part + int64_t(p.B) * p.S_q * p.H * pl.splits * p.D);
     }
     if (p.type == kMx4F32)
-        return p.D == 128 ? run_attention_kv4<float, 128>(a, pl.tile, st)
-                          : run_attention_kv4<float, 64>(a, pl.tile, st);
-    return p.D == 128 ? run_attention_kv4<uint16_t, 128>(a, pl.tile, st)
-                      : run_attention_kv4<uint16_t, 64>(a, pl.tile, st);
+        return p.D == 128 ? run_attention_kv4<float, 128>(a, pl, st)
+                          : run_attention_kv4<float, 64>(a, pl, st);
+    return p.D == 128 ? run_attention_kv4<uint16_t, 128>(a, pl, st)
+                      : run_attention_kv4<uint16_t, 64>(a, pl, st);
 }
 
 }  // namespace anima_hip

@@ -147,7 +147,7 @@ inline LinScratch lin_scratch(const LinPlan &pl, int M, int N, int K, bool f32)
 
 // -------------------------------------------- attention (mx4_attention.hip)
 
-constexpr int kTokRows = 16;   // query rows of a workgroup
+constexpr int kTokRows = 16;   // query rows of a block; a workgroup has one or two
 constexpr int kTokKeys = 32;   // keys a wave takes at a time
 constexpr int kTokWaves = 4;
 constexpr int kTileWaves = 4;
@@ -155,30 +155,37 @@ constexpr int kTileRows = 32 * kTileWaves;  // query rows of a workgroup
 constexpr int kTileKeys = 64;
 constexpr int kAttnMaxSplits = 64;
 
+// Two blocks of rows fit the token kernel's registers.
+constexpr bool two_row_blocks(bool f32, int D) { return !f32 || D == 64; }
+
 struct AttnPlan {
     bool tile = false;  // the tile kernel
+    int row_blocks = 1;  // of the token kernel
     int tiles = 0, splits = 1;
 };
 
-// Microseconds of a workgroup per 128 keys (token kernel, 16 query rows) and per 64 keys
-// (tile kernel, 128 rows), alone on a CU and as its share of a CU that has two;
+// Microseconds of a workgroup per 128 keys (token kernel, 16 and 32 query rows) and per 64
+// keys (tile kernel, 128 rows), alone on a CU and as its share of a CU that has two;
 // bf16 and f32 queries, D of 64 and 128.  These and the constants of the model are
-// fitted to the times of 1400 calls, 1 to 64 sequences of unequal lengths of 100
+// fitted to the times of 1900 calls, 1 to 64 sequences of unequal lengths of 100
 // to 30000 keys, 1 to 1000 queries, 1 to 32 K/V heads.
 struct Rate {
-    double token1, token2, tile1, tile2;
+    double alone[3], full[3];
 };
-constexpr Rate kRates[2][2] = {{{0.71, 0.47, 1.59, 0.99}, {0.92, 0.59, 1.81, 1.1}},
-                               {{0.7, 0.5, 2.04, 1.4}, {1.03, 0.97, 5.08, 3.29}}};
+constexpr Rate kRates[2][2] = {{{{0.64, 1.79, 1.51}, {0.52, 0.82, 0.98}},
+                                {{0.92, 1.43, 1.72}, {0.58, 0.98, 0.98}}},
+                               {{{0.8, 2.14, 1.79}, {0.67, 1.13, 1.81}},
+                                {{1.03, 0, 6.63}, {0.96, 0, 3.73}}}};
 
 // The kernel and the split that the model expects to take least: latency, the keys
-// of the longest share or of a full CU (half a workgroup's more on the fullest),
-// and with splits the partial results written and joined.  On 500 calls beside those
-// of the fit the choice is 0.8 % behind the fastest of all kernels and splits on
-// average, 11 % in the worst twentieth.  The token kernel, which meets at no barrier, is ahead to
-// some hundred query rows of a K/V head and in f32 further: 2048 rows of 512 keys,
-// 4 K/V heads, take 10.8 us by it and 18.7 by the tile kernel (bf16); 4096 x 512 keys,
-// 32 heads, 50 us by the tile kernel against 141 by the first token kernel.
+// of the longest share or of a full CU (half a workgroup's more on the fullest, and
+// part of the last round's empty places), and with splits the partial results
+// written and joined.  On those calls it is 0.8 % behind the fastest of all kernels
+// and splits on average, 11 % in the worst twentieth.  The token kernel, which meets
+// at no barrier, is ahead to some hundred query rows of a K/V head and in f32
+// further: 2048 rows of 512 keys, 4 K/V heads, take 10.8 us by it and 18.7 by the
+// tile kernel (bf16); 4096 x 512 keys, 32 heads, 50 us by the tile kernel against 141
+// by the first token kernel.
 inline AttnPlan attn_plan(int B, int S_q, int H, int H_kv, int D, int S_max, bool f32,
                           bool causal)
 {
@@ -189,10 +196,13 @@ inline AttnPlan attn_plan(int B, int S_q, int H, int H_kv, int D, int S_max, boo
                             ? 1.0 - 0.5 * std::min(S_q, S_max) / S_max : 1.0;
     AttnPlan best;
     double best_us = 1e300;
-    for (int tile = 0; tile < 2; ++tile) {
+    for (int kind = 0; kind < 3; ++kind) {
         AttnPlan pl;
-        pl.tile = tile != 0;
-        const int per_tile = pl.tile ? kTileRows : kTokRows;
+        pl.tile = kind == 2;
+        pl.row_blocks = kind == 1 ? 2 : 1;
+        if (kind == 1 && (rows <= kTokRows || !two_row_blocks(f32, D)))
+            continue;
+        const int per_tile = pl.tile ? kTileRows : pl.row_blocks * kTokRows;
         pl.tiles = int((rows + per_tile - 1) / per_tile);
         const double groups = double(B) * H_kv * pl.tiles;
         const int keys = pl.tile ? kTileKeys : kTokKeys * kTokWaves;
@@ -204,13 +214,12 @@ inline AttnPlan attn_plan(int B, int S_q, int H, int H_kv, int D, int S_max, boo
             const double share = std::ceil(double(rounds) / pl.splits);
             const double load = groups * pl.splits / 256;  // workgroups per CU
             // The longest share, or the work of a full CU.
-            const double alone = pl.tile ? rate.tile1 : rate.token1;
-            const double full = pl.tile ? rate.tile2 : rate.token2;
-            const double work = part * load + 0.5 * std::min(load, 1.0);
-            double us = 6.6 + std::max(share * alone, share * work * full) +
-                        2.4 * std::max(0.0, load / 2 - 1);
+            const double rest = load > 1 ? 0.3 * (std::ceil(load) - load) : 0.0;
+            const double work = part * (load + rest) + 0.5 * std::min(load, 1.0);
+            double us = 6.6 + std::max(share * rate.alone[kind], share * work * rate.full[kind]) +
+                        5.4 * std::max(0.0, load / 2 - 1);
             if (pl.splits > 1)
-                us += 3.1 + bytes / 2e6;
+                us += 3.2 + bytes / 1.8e6;
             if (us < best_us) {
                 best_us = us;
                 best = pl;
