@@ -476,9 +476,11 @@ __global__ __launch_bounds__(WM *WN * 64) void linear_tile_kernel(LinArgs p)
 // accumulators are four columns of one row.
 //
 // A's rows, W's codes and scales reach LDS by DMA through S stages.  A stage is 256
-// bytes of each row of A, 128 bf16 or 64 f32 elements, and the codes of as many;
-// 16-byte pieces are placed by piece ^ (row & 15) (A), ^ (row / 4 & 3) or
-// ^ (row / 8 & 1) (codes of 64 and of 32 bytes) against bank conflicts.
+// bytes of each row of A, 128 bf16 or 64 f32 elements, and the codes of as many, or
+// twice that (CM = 2: the smaller tiles, whose barrier and addresses take as long as
+// their products; 333 x 2048 x 1024 f32 16.1 -> 13.8 us, 160 x 4096 x 4096 bf16 20.5 ->
+// 17.5); 16-byte pieces are placed by piece ^ (row & 15) (A) and by code_swizzle
+// against bank conflicts.
 // A lane takes the contiguous codes of its half of the chunk and decodes them in
 // registers, as the MFMA's k index wants them: k = KC / 2 half + 8 step + j, the
 // order A is read in.  f32 A is split into its three terms there too, once for
@@ -489,18 +491,21 @@ __global__ __launch_bounds__(WM *WN * 64) void linear_tile_kernel(LinArgs p)
 // Fragments of a step are read, and its weights decoded, while the MFMAs of the
 // step before run; a chunk's first ones under the last step of the chunk before,
 // behind the barrier that ends it.
-template <typename T, int MB, int NB, int WM, int WN, int KS, int S>
+template <typename T, int MB, int NB, int WM, int WN, int KS, int S, int CM>
 struct Staged {
     static constexpr int NT = kTerms<T>;
     static constexpr int WAVES = WM * WN * KS, THREADS = WAVES * 64;
     static constexpr int BM = 32 * MB * WM, BN = 32 * NB * WN;
-    static constexpr int KC = 256 / int(sizeof(T));  // K elements of a chunk
+    static constexpr int KC = CM * 256 / int(sizeof(T));  // K elements of a chunk
     static constexpr int STEPS = KC / 16, SHARE = STEPS / KS;
-    // LDS in u16: A rows of 128, codes rows of KC / 4, scales one dword a row.
-    static constexpr int A_EL = BM * 128, C_EL = BN * (KC / 4), STAGE = A_EL + C_EL + BN * 2;
+    static constexpr int CP = KC / 32;        // 16-byte pieces of a row's codes, and its scales
+    static constexpr int SD = CP > 4 ? 2 : 1;  // dwords of a row's scales
+    // LDS in u16: A rows of 128 CM, codes rows of KC / 4, scales SD planes of a dword a row.
+    static constexpr int A_ROW = 128 * CM;
+    static constexpr int A_EL = BM * A_ROW, C_EL = BN * (KC / 4), STAGE = (A_EL + C_EL + BN * 2 * SD + A_ROW - 1) / A_ROW * A_ROW;
     // 1 KiB windows (scales: 256 bytes) per chunk, and per wave; a wave without
     // one copies the last again, so that all count the same.
-    static constexpr int A_WIN = BM / 4, C_WIN = C_EL / 512, S_WIN = (BN + 63) / 64;
+    static constexpr int A_WIN = BM * CM / 4, C_WIN = C_EL / 512, S_WIN = SD * BN / 64;
     static constexpr int A_OPS = (A_WIN + WAVES - 1) / WAVES;
     static constexpr int C_OPS = (C_WIN + WAVES - 1) / WAVES;
     static constexpr int S_OPS = (S_WIN + WAVES - 1) / WAVES;
@@ -531,11 +536,11 @@ __device__ __forceinline__ void dma4s(const void *base, unsigned voff, u16 *lds)
 }
 #pragma clang diagnostic pop
 
-template <typename T, int MB, int NB, int WM, int WN, int KS, int S>
+template <typename T, int MB, int NB, int WM, int WN, int KS, int S, int CM>
 __global__ __launch_bounds__(WM *WN *KS * 64) void linear_staged_kernel(LinArgs p)
 {
-    using G = Staged<T, MB, NB, WM, WN, KS, S>;
-    constexpr int NT = G::NT;
+    using G = Staged<T, MB, NB, WM, WN, KS, S, CM>;
+    constexpr int NT = G::NT, CP = G::CP;
     __shared__ __attribute__((aligned(16))) u16 smem[G::LDS];
 
     const int tid = threadIdx.x, lane = tid & 63;
@@ -557,28 +562,29 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void linear_staged_kernel(LinArgs 
     // M or N read the last one again (their results are not stored).
     unsigned aoff[G::A_OPS], coff[G::C_OPS], soff[G::S_OPS];
     int adst[G::A_OPS], cdst[G::C_OPS], sdst[G::S_OPS];
-    constexpr int CROWS = 2048 / G::KC;  // rows of a codes window
-    constexpr int CP = G::KC / 32;       // 16-byte pieces of a row's codes
+    constexpr int AROWS = 4 / CM, CROWS = 2048 / G::KC;  // rows of a window
+    auto code_swizzle = [](int r) { return CP == 8 ? r & 7 : CP == 4 ? r >> 2 & 3 : r >> 3 & 1; };
 #pragma unroll
     for (int i = 0; i < G::A_OPS; ++i) {
         const int w = min(i * G::WAVES + wave, G::A_WIN - 1);
-        const int r = w * 4 + (lane >> 4);
+        const int r = w * AROWS + lane / (16 * CM);
         aoff[i] = unsigned(int64_t(min(row0 + r, p.M - 1) - row0) * p.lda * int(sizeof(T)) +
-                           16 * ((lane & 15) ^ (r & 15)));
+                           16 * (lane % (16 * CM) ^ (r & 15)));
         adst[i] = w * 512;
     }
 #pragma unroll
     for (int i = 0; i < G::C_OPS; ++i) {
         const int w = min(i * G::WAVES + wave, G::C_WIN - 1);
         const int r = w * CROWS + lane / CP;
-        const int piece = lane % CP ^ (CP == 4 ? r >> 2 & 3 : r >> 3 & 1);
+        const int piece = lane % CP ^ code_swizzle(r);
         coff[i] = unsigned((min(col0 + r, p.N - 1) - col0) * (p.K / 2) + 16 * piece);
         cdst[i] = G::A_EL + w * 512;
     }
 #pragma unroll
     for (int i = 0; i < G::S_OPS; ++i) {
         const int w = min(i * G::WAVES + wave, G::S_WIN - 1);
-        soff[i] = unsigned((min(col0 + w * 64 + lane, p.N - 1) - col0) * p.groups);
+        const int r = w % (G::BN / 64) * 64 + lane;
+        soff[i] = unsigned((min(col0 + r, p.N - 1) - col0) * p.groups + w / (G::BN / 64) * 4);
         sdst[i] = G::A_EL + G::C_EL + w * 128;
     }
     const char *a0 = reinterpret_cast<const char *>(static_cast<const T *>(p.a) +
@@ -589,7 +595,7 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void linear_staged_kernel(LinArgs 
         u16 *dst = smem + stage * G::STAGE;
 #pragma unroll
         for (int i = 0; i < G::A_OPS; ++i)
-            dma16s(a0 + int64_t(c) * 256, aoff[i], dst + adst[i]);
+            dma16s(a0 + int64_t(c) * (256 * CM), aoff[i], dst + adst[i]);
 #pragma unroll
         for (int i = 0; i < G::C_OPS; ++i)
             dma16s(w0 + int64_t(c) * (G::KC / 2), coff[i], dst + cdst[i]);
@@ -620,7 +626,7 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void linear_staged_kernel(LinArgs 
 #pragma unroll
             for (int h = 0; h < (NT == 3 ? 2 : 1); ++h)
                 f[i][h] = *reinterpret_cast<const u32x4 *>(
-                    smem + 32 * i * 128 + (ao ^ (NT == 3 ? 16 * st + 8 * h : 8 * st)));
+                    smem + 32 * i * G::A_ROW + (ao ^ (NT == 3 ? 16 * st + 8 * h : 8 * st)));
     };
     auto decode = [&](int st, bf16x8 (&f)[NB]) {
 #pragma unroll
@@ -638,7 +644,7 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void linear_staged_kernel(LinArgs 
             dma(c + S - 1, (c + S - 1 - c0) % S);
         const unsigned base = (c - c0) % S * G::STAGE;
         // Rows (wm MB + i) 32 + col, this half of the chunk.
-        ao = base + (wm * 32 * MB + col) * 128 + ((8 * half) ^ (col & 15)) * 8;
+        ao = base + (wm * 32 * MB + col) * G::A_ROW + ((8 * CM * half) ^ (col & 15)) * 8;
         asm volatile("" : "+v"(ao));
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
@@ -646,15 +652,15 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void linear_staged_kernel(LinArgs 
             const u16 *row = smem + base + G::A_EL + r * (G::KC / 4);
 #pragma unroll
             for (int h = 0; h < W / 4; ++h) {
-                const int piece = CP == 4 ? (2 * half + h) ^ (r >> 2 & 3) : half ^ (r >> 3 & 1);
+                const int piece = (CP / 2 * half + h) ^ code_swizzle(r);
                 const u32x4 v = *reinterpret_cast<const u32x4 *>(row + 8 * piece);
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     codes[j][4 * h + e] = v[e];
             }
-            const unsigned s4 = *reinterpret_cast<const unsigned *>(smem + base + G::A_EL +
-                                                                    G::C_EL + r * 2);
-            sc[j] = s4 >> (CP == 4 ? 16 * half : 16 * (c & 1) + 8 * half);
+            const unsigned s4 = *reinterpret_cast<const unsigned *>(
+                smem + base + G::A_EL + G::C_EL + (CP == 8 ? half * G::BN * 2 : 0) + r * 2);
+            sc[j] = s4 >> (CP == 8 ? 0 : CP == 4 ? 16 * half : 16 * (c & 1) + 8 * half);
         }
     };
     auto multiply = [&](const Raw(&f)[MB], const bf16x8 (&w)[NB]) {
@@ -915,19 +921,25 @@ __global__ __launch_bounds__(256) void linear_pad_kernel(LinArgs p, T *a, uint8_
 
 // -------------------------------------------------------------- launches
 
-// Shapes of the staged kernel: MB, NB, WM, WN, KS, S.
-#define STAGED_BF16(X) \
-    X(0, 3, 2, 2, 4, 1, 2) X(1, 2, 2, 2, 4, 1, 2) X(2, 2, 2, 2, 2, 2, 2) X(3, 1, 2, 2, 2, 2, 3) \
-    X(4, 1, 1, 2, 2, 2, 4) X(5, 1, 1, 1, 2, 4, 4)
-#define STAGED_F32(X) \
-    X(0, 2, 4, 4, 2, 1, 2) X(1, 1, 4, 4, 2, 1, 3) X(2, 1, 4, 2, 1, 4, 3) X(3, 1, 2, 1, 1, 4, 4)
+// Shapes of the staged kernel, MB, NB, WM, WN, KS, S, and of the same with two chunks
+// at once.
+#define STAGED_BF16(X, cm) \
+    X(cm, 0, 3, 2, 2, 4, 1, 2) X(cm, 1, 2, 2, 2, 4, 1, 2) X(cm, 2, 2, 2, 2, 2, 2, 2) \
+    X(cm, 3, 1, 2, 2, 2, 2, 3) X(cm, 4, 1, 1, 2, 2, 2, 4) X(cm, 5, 1, 1, 1, 2, 4, 4)
+#define PAIRED_BF16(X, cm) \
+    X(cm, 3, 1, 2, 2, 2, 2, 2) X(cm, 4, 1, 1, 2, 2, 2, 2) X(cm, 5, 1, 1, 1, 2, 4, 3)
+#define STAGED_F32(X, cm) X(cm, 0, 2, 4, 4, 2, 1, 2) X(cm, 1, 1, 4, 4, 2, 1, 3)
+#define PAIRED_F32(X, cm) X(cm, 2, 1, 4, 2, 1, 4, 2) X(cm, 3, 1, 2, 1, 1, 4, 3)
 
-#define SHAPE_CHECK(table, i, mb, nb, wm, wn) \
-    static_assert(table[i].bm == 32 * mb * wm && table[i].bn == 32 * nb * wn, "shape table");
-#define CHECK_BF16(i, mb, nb, wm, wn, ks, s) SHAPE_CHECK(kBf16Shapes, i, mb, nb, wm, wn)
-#define CHECK_F32(i, mb, nb, wm, wn, ks, s) SHAPE_CHECK(kF32Shapes, i, mb, nb, wm, wn)
-STAGED_BF16(CHECK_BF16)
-STAGED_F32(CHECK_F32)
+#define SHAPE_CHECK(table, i, mb, nb, wm, wn, cm) \
+    static_assert(table[i].bm == 32 * mb * wm && table[i].bn == 32 * nb * wn && \
+                  (cm == 1 || table[i].pairs), "shape table");
+#define CHECK_BF16(cm, i, mb, nb, wm, wn, ks, s) SHAPE_CHECK(kBf16Shapes, i, mb, nb, wm, wn, cm)
+#define CHECK_F32(cm, i, mb, nb, wm, wn, ks, s) SHAPE_CHECK(kF32Shapes, i, mb, nb, wm, wn, cm)
+STAGED_BF16(CHECK_BF16, 1)
+PAIRED_BF16(CHECK_BF16, 2)
+STAGED_F32(CHECK_F32, 1)
+PAIRED_F32(CHECK_F32, 2)
 
 template <typename T, bool VEC>
 bool run_few(LinArgs &p, hipStream_t st)
@@ -977,22 +989,29 @@ bool run_tiles(const LinArgs &p, int shape, dim3 grid, hipStream_t st)
     return hip_ok(hipGetLastError(), "linear_tile_kernel launch");
 }
 
-#define STAGED_CASE(i, mb, nb, wm, wn, ks, s)                                                    \
-    case i:                                                                                       \
-        hipLaunchKernelGGL((linear_staged_kernel<T, mb, nb, wm, wn, ks, s>), grid,               \
+constexpr int kPairs = 16;  // beside a shape's number: two chunks at once
+#define STAGED_CASE(cm, i, mb, nb, wm, wn, ks, s)                                                \
+    case i + (cm == 2 ? kPairs : 0):                                                             \
+        hipLaunchKernelGGL((linear_staged_kernel<T, mb, nb, wm, wn, ks, s, cm>), grid,           \
                            dim3(wm * wn * ks * 64), 0, st, p);                                   \
         break;
 
 template <typename T>
-bool run_staged(const LinArgs &p, int shape, dim3 grid, hipStream_t st)
+bool run_staged(LinArgs p, const LinPlan &pl, dim3 grid, hipStream_t st)
 {
+    if (pl.pairs)
+        p.per_split /= 2;
+    // f32 chunks come in pairs, K being a multiple of 128.
+    const int shape = pl.shape + (pl.pairs ? kPairs : 0);
     if constexpr (kTerms<T> == 1) {
         switch (shape) {
-            STAGED_BF16(STAGED_CASE)
+            STAGED_BF16(STAGED_CASE, 1)
+            PAIRED_BF16(STAGED_CASE, 2)
         }
     } else {
         switch (shape) {
-            STAGED_F32(STAGED_CASE)
+            STAGED_F32(STAGED_CASE, 1)
+            PAIRED_F32(STAGED_CASE, 2)
         }
     }
     return hip_ok(hipGetLastError(), "linear_staged_kernel launch");
@@ -1021,7 +1040,7 @@ bool run_linear(LinArgs &p, const LinPlan &pl, bool rows16, hipStream_t st)
     if (!launch_fits(blocks, pl.kernel == kStaged ? 512 : 256))
         return fail("linear_mx4_dev: too many tiles for one launch");
     const dim3 grid(static_cast<unsigned>(blocks));
-    const bool ok = pl.kernel == kStaged ? run_staged<T>(p, pl.shape, grid, st)
+    const bool ok = pl.kernel == kStaged ? run_staged<T>(p, pl, grid, st)
                     : vec                ? run_tiles<T, true>(p, pl.shape, grid, st)
                                          : run_tiles<T, false>(p, pl.shape, grid, st);
     if (!ok || pl.splits == 1)

@@ -26,19 +26,21 @@ struct TileShape {
     // the CUs have one, and where all have (large tiles: at a lower clock; small
     // ones: several workgroups on a CU, per workgroup).
     double half_us, full_us;
+    bool pairs = false;  // two chunks at once where K has an even number of them
 };
 // Measured at M from 24 to 4096, N x K of 2048 x 2048, 2048 x 8192, 8192 x 2048,
 // 6144 x 256 and 256 x 2048; the model below is within 15 % of most of them.
-constexpr TileShape kBf16Shapes[] = {{192, 256, 2.0, 2.45}, {128, 256, 1.24, 1.7},
-                                     {128, 128, 0.93, 1.15}, {64, 128, 0.66, 0.62},
-                                     {64, 64, 0.47, 0.58},   {32, 64, 0.37, 0.36}};
-constexpr TileShape kF32Shapes[] = {{256, 256, 4.2, 5.4}, {128, 256, 2.33, 2.75},
-                                    {64, 128, 1.0, 1.02}, {32, 64, 0.52, 0.33}};
+constexpr TileShape kBf16Shapes[] = {{192, 256, 2.0, 2.45},       {128, 256, 1.24, 1.7},
+                                     {128, 128, 0.93, 1.15},      {64, 128, 0.61, 0.58, true},
+                                     {64, 64, 0.4, 0.5, true},    {32, 64, 0.32, 0.31, true}};
+constexpr TileShape kF32Shapes[] = {{256, 256, 4.2, 5.0}, {128, 256, 2.33, 2.5},
+                                    {64, 128, 0.9, 0.92, true}, {32, 64, 0.44, 0.29, true}};
 constexpr TileShape kTileShapes[] = {{32, 128, 0, 0}, {64, 128, 0, 0}, {128, 128, 0, 0}};
 enum LinKernel { kFew, kTiles, kStaged };
 struct LinPlan {
     LinKernel kernel = kFew;
     bool pad = false;  // staged, on copies of the operands with K padded to 128
+    bool pairs = false;  // staged, two chunks at once
     int shape = 0;
     int tiles_m = 0, tiles_n = 0, splits = 1, per_split = 0, chunks = 0;
 };
@@ -49,6 +51,9 @@ inline void set_grid(LinPlan &pl, const TileShape &t, int M, int N, int splits)
     pl.tiles_m = (M + t.bm - 1) / t.bm;
     pl.tiles_n = (N + t.bn - 1) / t.bn;
     pl.per_split = (pl.chunks + splits - 1) / splits;
+    pl.pairs = t.pairs && pl.chunks % 2 == 0;
+    if (pl.pairs)
+        pl.per_split += pl.per_split & 1;
     pl.splits = pl.per_split ? (pl.chunks + pl.per_split - 1) / pl.per_split : 1;
 }
 

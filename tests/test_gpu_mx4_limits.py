@@ -249,3 +249,11 @@ def test_linear_many_weight_rows(M, N, K, dtype):
         err = np.abs(got - want[:, rows])[:, ok]
         bound = (K + 32) * kv4.U * mag + ref.HALF[dtype] * np.abs(want)
         assert (err <= bound[:, rows][:, ok]).all()
+
+
+@pytest.mark.parametrize("dtype", [ref.F32, ref.BF16])
+@pytest.mark.parametrize("M,N,K", [(700, 2047, 384), (333, 2001, 640), (130, 1001, 128),
+                                   (24, 300, 1408), (60, 257, 11008), (90, 515, 896), (260, 600, 1152)])
+def test_linear_odd_and_even_chunks(M, N, K, dtype):
+    """K of odd and even numbers of 128 elements, whole and in splits of either."""
+    mx4.check_linear(M, N, K, dtype, M + K)
