@@ -101,13 +101,12 @@ inline LinPlan staged_plan(int M, int N, int K, bool f32)
 inline LinPlan lin_plan(int M, int N, int K, bool f32, bool staged)
 {
     LinPlan pl;
-    // Few rows, unless their terms take long to stage in every workgroup.  bf16, N =
-    // 2048: 16 rows of 8192 take 12.5 us against 9.8 on staged tiles, 16 of 2048 5.5
-    // against 7.4.  f32: 4 rows of 11008 13.6 against 18.2 (N = 2048), 8 of 8192 27.7
-    // against 28.7 (8192) but of 11008 32.2 against 28.8 (6144), 12 of 2048 10.8 against
-    // 12.5 (6144) but of 4096 13.1 against 10.9 (2048), 16 of 1024 7.7 against 8.1 (512) but
-    // of 1408 9.8 against 8.6 (2048).
-    const int64_t limit = !f32 || (M > 8 && M <= 12) ? 100000 : M <= 8 ? 200000 : 50000;
+    // Few rows, unless their terms take long to stage in every workgroup.  Time by the
+    // few-rows kernel over that by staged tiles, by the staged terms of a workgroup
+    // (rows x terms x K): bf16 0.7 at 22000, 0.95 at 88000, 1.3 at 131000; f32 at 3 to 8
+    // rows 0.6 to 0.8 at 49000, 0.9 at 132000, 1.1 at 197000, at 12 rows 0.8 at 51000,
+    // 1.0 at 74000, 1.2 at 147000, at 16 rows 0.7 at 25000, 1.1 at 49000, 2 at 264000.
+    const int64_t limit = !f32 ? 90000 : M <= 8 ? 150000 : M <= 12 ? 100000 : 40000;
     if (M <= kFewRows && (!staged || K % 128 || int64_t(M) * (f32 ? 3 : 1) * K <= limit))
         return pl;
     if (K > 0 && K % 128 == 0 && K <= kStagedMaxK && staged)
