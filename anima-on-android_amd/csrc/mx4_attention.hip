@@ -93,10 +93,15 @@ __device__ __forceinline__ float exponent(float score, float mx, float scale2, f
 // take their distance from the maximum first.
 constexpr float kFarLog2 = 0x1p24f;
 template <int NT>
-__device__ __forceinline__ bool far_row(float mx, float m2)
+__device__ __forceinline__ bool far_row(float m2)
 {
-    return NT == 1 && mx != -INFINITY && fabsf(m2) > kFarLog2;
+    return NT == 1 && fabsf(m2) > kFarLog2;
 }
+
+// What scores are taken against.  A row whose scores are all -inf so far (products past
+// the range of f32) has no distance from its maximum, which would be NaN: against
+// zero each of them weighs nothing, and a NaN score stays one.
+__device__ __forceinline__ float max_or_zero(float mx) { return mx == -INFINITY ? 0.0f : mx; }
 
 struct AttnArgs {
     Kv4Attention p;
@@ -367,11 +372,12 @@ __global__ __launch_bounds__(kTokWaves * 64, 2) void kv4_token_kernel(AttnArgs a
                     for (int r = 0; r < 4; ++r)
                         o[rb][i][r] *= alpha;
             }
-            float m2 = mx[rb] * scale2;
-            if (NT == 1 && __builtin_amdgcn_ballot_w64(far_row<NT>(mx[rb], m2)) != 0) {
+            const float mref = max_or_zero(mx[rb]);
+            float m2 = mref * scale2;
+            if (NT == 1 && __builtin_amdgcn_ballot_w64(far_row<NT>(m2)) != 0) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    float x = sc[rb][i] - mx[rb];
+                    float x = sc[rb][i] - mref;
                     asm volatile("" : "+v"(x));  // stays behind the branch
                     sc[rb][i] = x;
                 }
@@ -380,7 +386,7 @@ __global__ __launch_bounds__(kTokWaves * 64, 2) void kv4_token_kernel(AttnArgs a
             float pr[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                pr[i] = __builtin_amdgcn_exp2f(exponent<NT>(sc[rb][i], mx[rb], scale2, m2));
+                pr[i] = __builtin_amdgcn_exp2f(exponent<NT>(sc[rb][i], mref, scale2, m2));
                 if (MASK && 16 * (i >> 2) + (i & 3) >= room)
                     pr[i] = 0.0f;
                 sum[rb] += pr[i];
@@ -745,13 +751,14 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void kv4_tile_kernel(AttnArgs a
                 for (int r = 0; r < 16; ++r)
                     o[i][r] *= alpha;
         }
-        float m2 = mx * scale2;
-        if (NT == 1 && __builtin_amdgcn_ballot_w64(far_row<NT>(mx, m2)) != 0) {
+        const float mref = max_or_zero(mx);
+        float m2 = mref * scale2;
+        if (NT == 1 && __builtin_amdgcn_ballot_w64(far_row<NT>(m2)) != 0) {
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    float x = sc[kb][r] - mx;
+                    float x = sc[kb][r] - mref;
                     asm volatile("" : "+v"(x));
                     sc[kb][r] = x;
                 }
@@ -771,8 +778,8 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void kv4_tile_kernel(AttnArgs a
 #pragma unroll
             for (int r = 0; r < 8; ++r)
                 pr[r] = __builtin_amdgcn_exp2f(
-                    exponent<NT>(sc[kg >> 1][8 * (kg & 1) + r], mx, scale2, m2));
-            // Not left to exp2(-inf): a row's maximum may be -inf, or the scale 0.
+                    exponent<NT>(sc[kg >> 1][8 * (kg & 1) + r], mref, scale2, m2));
+            // Not left to exp2(-inf): the scale may be 0.
             if (masked)
 #pragma unroll
                 for (int r = 0; r < 8; ++r) {

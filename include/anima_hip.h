@@ -629,8 +629,11 @@ bool anima_hip_kv4_append_dev(const void *k, const void *v, int dtype, const int
  * are not written.  is_causal: query token s of n sees the keys up to position
  * len - n + s, its own; else every query sees all.  A query that sees no key
  * gives zeros.  Scale bytes as the entries above write them (2 .. 252 and
- * 255).  K and V enter the products exactly; scores, softmax and sums are f32,
- * the probabilities enter the second product as bf16 with bf16 queries and
+ * 255).  K and V enter the products exactly; scores, softmax and sums are f32.
+ * q K^T is held before the scale is applied: where it passes f32's range, a
+ * score that the scale makes -inf weighs nothing, and a query with no other gives
+ * zeros; +inf, or an infinity times a scale of 0, gives NaN.  The
+ * probabilities enter the second product as bf16 with bf16 queries and
  * exactly with f32 ones, and out is rounded once.  scratch:
  * anima_hip_kv4_attention_scratch_bytes() bytes, 16-byte aligned (0: none
  * needed), for the partial results of a cache whose keys are shared out over

@@ -1,0 +1,70 @@
+"""Attention over a 4-bit cache where scores are infinite: each kernel, with its keys in one workgroup
+and shared out over several, so that every place that joins partial results is met."""
+import numpy as np
+import pytest
+
+import mx4_ref as ref
+import test_gpu_kv4 as kv4
+from anima_hip import rt
+
+pytestmark = pytest.mark.gpu
+
+F, B = ref.F32, ref.BF16
+U = kv4.U
+
+# (dtype, B, S_q, H, H_kv, D, S, kernel, row blocks, splits), one cached sequence for all entries.
+SHAPES = [(t, 1, 3, 16, 4, D, 300, "token", 1, 1) for t in (F, B) for D in (64, 128)]
+SHAPES += [(t, 1, 3, 16, 4, D, 3000, "token", 1, 16) for t in (F, B) for D in (64, 128)]
+SHAPES += [(F, 72, 5, 32, 8, 64, 300, "token", 2, 1), (B, 72, 5, 32, 8, 128, 300, "token", 2, 1),
+           (F, 40, 5, 8, 2, 64, 3000, "token", 2, 8), (B, 40, 5, 8, 2, 64, 3000, "token", 2, 8),
+           (B, 40, 5, 8, 2, 128, 3000, "token", 2, 4),
+           (F, 1, 300, 64, 64, 64, 140, "tile", 1, 1), (F, 1, 500, 64, 64, 128, 70, "tile", 1, 1),
+           (B, 1, 300, 64, 64, 64, 300, "tile", 1, 1), (B, 1, 300, 64, 64, 128, 300, "tile", 1, 1),
+           (F, 1, 500, 8, 1, 64, 9000, "tile", 1, 16), (B, 1, 250, 16, 1, 64, 5000, "tile", 1, 8),
+           (B, 1, 250, 16, 1, 128, 5000, "tile", 1, 8)]
+EACH = pytest.mark.parametrize("dtype,Bn,S_q,H,H_kv,D,S,kernel,blocks,splits", SHAPES)
+
+
+def some(x):
+    """The first, a middle and the last batch entry."""
+    return x[sorted({0, len(x) // 2, len(x) - 1})]
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _init():
+    rt.init()
+
+
+@EACH
+@pytest.mark.parametrize("scale", [0.1, -0.3])
+def test_infinite_scores_weigh_nothing(dtype, Bn, S_q, H, H_kv, D, S, kernel, blocks, splits, scale):
+    """Scores of -2^140, -inf in f32, on the first 32, 64, 128 or half of the keys, on every second
+    one, and on all: the attention over the others, and zeros where there is no other.
+
+    The bound is test_gpu_kv4.py's on the keys that are left, whose dimension 0 is zero."""
+    print(f"{kernel} {blocks} {splits} D={D} dtype={dtype} scale={scale}", flush=True)
+    rng = np.random.default_rng(S + D)
+    base, v = (np.float32(rng.standard_normal((1, H_kv, S, D))).astype(float) for _ in range(2))
+    base[..., 0] = 0
+    q = rng.standard_normal((Bn, S_q, H, D))
+    q[..., 0] = -2.0 ** 70 * np.sign(scale)
+    raw, q = ref.typed(q, dtype)
+    key = np.arange(S)
+    for out in (key < 32, key < 64, key < 128, key < S // 2, key % 2 == 0, key >= 0):
+        k = base.copy()
+        k[..., out, 0] = 2.0 ** 70
+        cache = kv4.Cache.of(k, v)
+        got = kv4.attend(cache, raw, dtype, [S], None, False, scale)
+        if out.all():
+            assert (got == 0).all()
+            continue
+        kc, vc = cache.values()
+        kc, vc, qq = kc[:, :, ~out], vc[:, :, ~out], q.copy()
+        qq[..., 0] = 0
+        got, qq = some(got), some(qq)
+        want, mag = ref.attention_rows(qq, kc, vc, [kc.shape[2]], None, False, scale)
+        d = (3 * D + 6) * U * abs(scale) * np.abs(qq).sum(-1, keepdims=True) * np.abs(kc).max()
+        r = 2.0 ** -8 if dtype == B else 0.0
+        bound = ((4 * d + (S + 64) * U + r) * mag + ref.HALF[dtype] * np.abs(want)
+                 + S * 2.0 ** -126 * np.abs(vc).max())
+        assert (np.abs(got - want) <= bound).all(), out.sum()
