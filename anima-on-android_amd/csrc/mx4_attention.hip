@@ -103,6 +103,14 @@ __device__ __forceinline__ bool far_row(float m2)
 // zero each of them weighs nothing, and a NaN score stays one.
 __device__ __forceinline__ float max_or_zero(float mx) { return mx == -INFINITY ? 0.0f : mx; }
 
+// A partial result times its weight.  A NaN value reaches the row however little its
+// key weighs beside the others, wherever it lies; a sum that passed the range of f32 among
+// keys that weigh nothing does not.
+__device__ __forceinline__ float weighed(float w, float x)
+{
+    return w != 0.0f || x != x ? w * x : 0.0f;
+}
+
 struct AttnArgs {
     Kv4Attention p;
     float scale2;   // softmax scale * log2(e)
@@ -517,8 +525,7 @@ __global__ __launch_bounds__(kTokWaves * 64, 2) void kv4_token_kernel(AttnArgs a
         float v = 0.0f;
 #pragma unroll
         for (int i = 0; i < kTokWaves; ++i)
-            if (w[i] != 0.0f)
-                v += w[i] * so[i][jr][d];
+            v += weighed(w[i], so[i][jr][d]);
         v *= inv;
         if (a.splits > 1)
             a.part[(split * plane + orow) * D + d] = v;
@@ -954,10 +961,9 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(AttnArgs a)
     for (int k = 0; k < kAttnMaxSplits / 4; ++k)
         if (first + PER * k < a.splits) {
             const float wk = __shfl(w, first + PER * k);
-            if (wk != 0.0f)
 #pragma unroll
-                for (int e = 0; e < E; ++e)
-                    v[e] += wk * x[k][e];
+            for (int e = 0; e < E; ++e)
+                v[e] += weighed(wk, x[k][e]);
         }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     T *out = static_cast<T *>(p.o) + b * p.os.b + h * p.os.h + s * p.os.s;

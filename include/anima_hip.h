@@ -632,9 +632,10 @@ bool anima_hip_kv4_append_dev(const void *k, const void *v, int dtype, const int
  * 255).  K and V enter the products exactly; scores, softmax and sums are f32.
  * q K^T is held before the scale is applied: where it passes f32's range, a
  * score that the scale makes -inf weighs nothing, and a query with no other gives
- * zeros; +inf, or an infinity times a scale of 0, gives NaN.  The
- * probabilities enter the second product as bf16 with bf16 queries and
- * exactly with f32 ones, and out is rounded once.  scratch:
+ * zeros; +inf, or an infinity times a scale of 0, gives NaN.  A NaN group of V
+ * makes its dimensions NaN for every query that sees its key, however little the
+ * key weighs.  The probabilities enter the second product as bf16 with bf16
+ * queries and exactly with f32 ones, and out is rounded once.  scratch:
  * anima_hip_kv4_attention_scratch_bytes() bytes, 16-byte aligned (0: none
  * needed), for the partial results of a cache whose keys are shared out over
  * workgroups, joined in a fixed order. */

@@ -1,5 +1,6 @@
-"""Attention over a 4-bit cache where scores are infinite: each kernel, with its keys in one workgroup
-and shared out over several, so that every place that joins partial results is met."""
+"""Attention over a 4-bit cache where scores are infinite, and where a value is NaN behind a weight of
+zero: each kernel, with its keys in one workgroup and shared out over several, so that every place
+that joins partial results is met."""
 import numpy as np
 import pytest
 
@@ -68,3 +69,36 @@ def test_infinite_scores_weigh_nothing(dtype, Bn, S_q, H, H_kv, D, S, kernel, bl
         bound = ((4 * d + (S + 64) * U + r) * mag + ref.HALF[dtype] * np.abs(want)
                  + S * 2.0 ** -126 * np.abs(vc).max())
         assert (np.abs(got - want) <= bound).all(), out.sum()
+
+
+@EACH
+@pytest.mark.parametrize("far", [300.0, np.inf])
+def test_nan_value_behind_a_weight_of_zero(dtype, Bn, S_q, H, H_kv, D, S, kernel, blocks, splits, far):
+    """One key has a score `far` above all others, whose weights are zero in f32 beside it (far
+    scores of -inf: -2^140).  A NaN group of V among the others reaches its 32 dimensions wherever
+    its key lies; the rest of the row is the far key's value, bit for bit."""
+    print(f"{kernel} {blocks} {splits} D={D} dtype={dtype} far={far}", flush=True)
+    rng = np.random.default_rng(S)
+    top, size = S // 2, 2.0 ** 70 if far == np.inf else 16.0
+    k, v = np.zeros((1, H_kv, S, D)), rng.standard_normal((1, H_kv, S, D))
+    k[..., 0] = size
+    k[:, :, top, 0] = 0
+    q = np.zeros((Bn, S_q, H, D))
+    q[..., 0] = -size if far == np.inf else -far
+    raw, q = ref.typed(q, dtype)
+    cache = kv4.Cache.of(k, v)
+    codes, scales = cache.raw()[1]
+    value = np.repeat(cache.values()[1][0, :, top], H // H_kv, 0)
+    at = sorted(n for n in {0, 5, 31, 33, 64, 100, S // 3, top - 1, top + 1, S - 33, S - 2, S - 1}
+                if n < S)
+    for nan in at:
+        bad = scales.copy()
+        bad[0, nan % H_kv, nan, 1] = 255
+        cache.bufs[3].put(bad, 0)
+        got = kv4.attend(cache, raw, dtype, [S], None, False, 1 / 16)
+        want = np.broadcast_to(value, got.shape).copy()
+        group = H // H_kv
+        want[:, :, nan % H_kv * group:(nan % H_kv + 1) * group, 32:64] = np.nan
+        np.testing.assert_array_equal(np.isnan(got), np.isnan(want), err_msg=str(nan))
+        ok = ~np.isnan(want)
+        np.testing.assert_array_equal(got[ok], want[ok])
