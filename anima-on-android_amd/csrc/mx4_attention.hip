@@ -79,16 +79,6 @@ __device__ __forceinline__ float quad_max(float v)
     return row_pair_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
 }
 
-// The argument of a probability's exponential.  bf16 queries: one fused
-// operation, off by a rounding of the scaled maximum for all keys of a row
-// alike (from 2^24 on, where that passes 1, see far_row); f32 queries: the
-// maximum's own probability is exactly 1.
-template <int NT>
-__device__ __forceinline__ float exponent(float score, float mx, float scale2, float m2)
-{
-    return NT == 1 ? __builtin_fmaf(score, scale2, -m2) : (score - mx) * scale2;
-}
-
 // bf16 queries: a row whose scaled maximum m2 has no fraction left.  Its scores
 // take their distance from the maximum first.
 constexpr float kFarLog2 = 0x1p24f;
@@ -102,6 +92,33 @@ __device__ __forceinline__ bool far_row(float m2)
 // the range of f32) has no distance from its maximum, which would be NaN: against
 // zero each of them weighs nothing, and a NaN score stays one.
 __device__ __forceinline__ float max_or_zero(float mx) { return mx == -INFINITY ? 0.0f : mx; }
+
+// The argument of a probability's exponential.  f32 queries and far rows (whose scores
+// are distances by then, with m2 = 0): (score - mx) * scale2.  Other rows of bf16 queries: one
+// fused operation, which takes the scaled maximum as it was rounded; base_shift is what that
+// adds to all arguments against the same maximum.
+template <int NT>
+__device__ __forceinline__ float exponent(float score, float mx, float scale2, float m2)
+{
+    return NT == 1 ? __builtin_fmaf(score, scale2, -m2) : (score - mx) * scale2;
+}
+template <int NT>
+__device__ __forceinline__ float base_shift(float mx, float scale2)
+{
+    const float m2 = mx * scale2;
+    return NT == 3 || mx == -INFINITY || far_row<NT>(m2) ? 0.0f
+                                                          : __builtin_fmaf(mx, scale2, -m2);
+}
+
+// What takes probabilities and their sums from the maximum `from` to `to`, both raw scores:
+// waves, splits and the steps of one wave meet at their distance, which stays exact where
+// their scaled values have lost it, and at the shifts their exponents hold (up to 0.5).
+template <int NT>
+__device__ __forceinline__ float rebase(float from, float to, float scale2)
+{
+    return __builtin_amdgcn_exp2f((from - to) * scale2 +
+                                  (base_shift<NT>(to, scale2) - base_shift<NT>(from, scale2)));
+}
 
 // A partial result times its weight.  A NaN value reaches the row however little its
 // key weighs beside the others, wherever it lies; a sum that passed the range of f32 among
@@ -119,7 +136,7 @@ struct AttnArgs {
     int tiles;      // query tiles of a K/V head
     int splits;
     float *part;    // [splits][B * S_q * H][D] O of each split, normalised
-    float2 *ml;     // [splits][B * S_q * H] (max in log2 units, sum); sum 0: no key seen
+    float2 *ml;     // [splits][B * S_q * H] (max of the raw scores, sum); sum 0: no weight
 };
 
 // The sequence a workgroup works on.
@@ -371,7 +388,7 @@ __global__ __launch_bounds__(kTokWaves * 64, 2) void kv4_token_kernel(AttnArgs a
                 const float mn = move ? mt : mx[rb];
                 const float alpha = mx[rb] == mn || mx[rb] == -INFINITY
                                         ? 1.0f
-                                        : __builtin_amdgcn_exp2f((mx[rb] - mn) * scale2);
+                                        : rebase<NT>(mx[rb], mn, scale2);
                 mx[rb] = mn;
                 sum[rb] *= alpha;
 #pragma unroll
@@ -382,14 +399,16 @@ __global__ __launch_bounds__(kTokWaves * 64, 2) void kv4_token_kernel(AttnArgs a
             }
             const float mref = max_or_zero(mx[rb]);
             float m2 = mref * scale2;
-            if (NT == 1 && __builtin_amdgcn_ballot_w64(far_row<NT>(m2)) != 0) {
+            const bool far = far_row<NT>(m2);
+            if (NT == 1 && __builtin_amdgcn_ballot_w64(far) != 0) {
+                const float back = far ? mref : 0.0f;  // the wave's other rows stay as they are
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    float x = sc[rb][i] - mref;
+                    float x = sc[rb][i] - back;
                     asm volatile("" : "+v"(x));  // stays behind the branch
                     sc[rb][i] = x;
                 }
-                m2 = 0.0f;
+                m2 = far ? 0.0f : m2;
             }
             float pr[8];
 #pragma unroll
@@ -497,7 +516,7 @@ __global__ __launch_bounds__(kTokWaves * 64, 2) void kv4_token_kernel(AttnArgs a
             for (int i = 0; i < VB; ++i)
                 so[wave][nr][(4 * g + r) * VB + i] = o[rb][i][r];
         if (g == 0) {
-            sm[wave][nr] = mx[rb] * scale2;
+            sm[wave][nr] = mx[rb];
             sl[wave][nr] = sum[rb];
         }
     }
@@ -514,7 +533,7 @@ __global__ __launch_bounds__(kTokWaves * 64, 2) void kv4_token_kernel(AttnArgs a
         jm = fmaxf(jm, sm[i][jr]);
 #pragma unroll
     for (int i = 0; i < kTokWaves; ++i) {
-        w[i] = sl[i][jr] == 0.0f ? 0.0f : sm[i][jr] == jm ? 1.0f : __builtin_amdgcn_exp2f(sm[i][jr] - jm);
+        w[i] = sl[i][jr] == 0.0f ? 0.0f : sm[i][jr] == jm ? 1.0f : rebase<NT>(sm[i][jr], jm, scale2);
         jl += w[i] * sl[i][jr];
     }
     const float inv = jl == 0.0f ? 0.0f : 1.0f / jl;
@@ -747,9 +766,8 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void kv4_tile_kernel(AttnArgs a
         const bool move = mx == -INFINITY ? mt > mx : (mt - mx) * scale2 > kRescaleLog2;
         if (__builtin_amdgcn_ballot_w64(move) != 0) {
             const float mn = move ? mt : mx;
-            const float alpha = mx == mn || mx == -INFINITY
-                                    ? 1.0f
-                                    : __builtin_amdgcn_exp2f((mx - mn) * scale2);
+            const float alpha =
+                mx == mn || mx == -INFINITY ? 1.0f : rebase<NT>(mx, mn, scale2);
             mx = mn;
             sum *= alpha;
 #pragma unroll
@@ -760,16 +778,18 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void kv4_tile_kernel(AttnArgs a
         }
         const float mref = max_or_zero(mx);
         float m2 = mref * scale2;
-        if (NT == 1 && __builtin_amdgcn_ballot_w64(far_row<NT>(m2)) != 0) {
+        const bool far = far_row<NT>(m2);
+        if (NT == 1 && __builtin_amdgcn_ballot_w64(far) != 0) {
+            const float back = far ? mref : 0.0f;  // the wave's other rows stay as they are
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    float x = sc[kb][r] - mref;
+                    float x = sc[kb][r] - back;
                     asm volatile("" : "+v"(x));
                     sc[kb][r] = x;
                 }
-            m2 = 0.0f;
+            m2 = far ? 0.0f : m2;
         }
         // Sixteen keys at a time: the MFMAs of one group run under the
         // exponentials of the next.
@@ -869,7 +889,7 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void kv4_tile_kernel(AttnArgs a
     const int64_t plane = int64_t(p.B) * p.S_q * p.H;
     const int64_t prow = split * plane + (int64_t(b) * p.S_q + s) * p.H + hq;
     if (parts && live && half == 0)
-        a.ml[prow] = float2{mx * scale2, sum};
+        a.ml[prow] = float2{mx, sum};
     // Where this lane's row starts (elements), for the lanes that write it.
     const int64_t at = !live   ? -1
                        : parts ? prow * D
@@ -916,8 +936,8 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void kv4_tile_kernel(AttnArgs a
     }
 }
 
-// O = sum_s w_s P_s / sum_s w_s, w_s = l_s 2^(m_s - max m), over the splits
-// that saw a key (at most 64).  PER waves per row: in each, lane s weighs split s;
+// O = sum_s w_s P_s / sum_s w_s, w_s = l_s rebase(m_s, max m), over the splits (at most
+// 64); one of which no key was seen has l_s = 0.  PER waves per row: in each, lane s weighs split s;
 // wave w adds the splits w, w + PER, .., at most 16, its loads all in flight,
 // D / 64 dimensions per lane, and the waves' sums are added in their order.
 template <typename T, int D, int PER>
@@ -950,9 +970,10 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(AttnArgs a)
     for (int o = 32; o; o >>= 1)
         m = fmaxf(m, __shfl_xor(m, o));
     // A split of which no key was seen weighs nothing, whatever its maximum.
-    const float w = ml.y == 0.0f
-                        ? 0.0f
-                        : (ml.x == m ? 1.0f : __builtin_amdgcn_exp2f(ml.x - m)) * ml.y;
+    const float w =
+        ml.y == 0.0f
+            ? 0.0f
+            : (ml.x == m ? 1.0f : rebase<kTerms<T>>(ml.x, m, fabsf(a.scale2))) * ml.y;
     float l = w;
 #pragma unroll
     for (int o = 32; o; o >>= 1)

@@ -1,6 +1,6 @@
-"""Attention over a 4-bit cache where scores are infinite, and where a value is NaN behind a weight of
-zero: each kernel, with its keys in one workgroup and shared out over several, so that every place
-that joins partial results is met."""
+"""Attention over a 4-bit cache where scores are infinite, or large and close to each other, and where
+a value is NaN behind a weight of zero: each kernel, with its keys in one workgroup and shared out
+over several, so that every place that joins partial results is met."""
 import numpy as np
 import pytest
 
@@ -102,3 +102,79 @@ def test_nan_value_behind_a_weight_of_zero(dtype, Bn, S_q, H, H_kv, D, S, kernel
         np.testing.assert_array_equal(np.isnan(got), np.isnan(want), err_msg=str(nan))
         ok = ~np.isnan(want)
         np.testing.assert_array_equal(got[ok], want[ok])
+
+
+# Scores that are exact in f32, their distances a few steps of f32 apart: a weight is off by the
+# rounding of its exponent's two products, each at most 64 in log2 units, and of the exponential.
+WEIGHT = 4 * 64 * U
+LOG2E = 1.4426950408889634
+
+
+def check_exact_scores(cache, q, raw, dtype, scale):
+    k, v = cache.values()
+    S = k.shape[2]
+    got = some(kv4.attend(cache, raw, dtype, [S], None, False, scale))
+    want, mag = ref.attention_rows(some(q), k, v, [S], None, False, scale)
+    r = 2.0 ** -8 if dtype == B else 0.0
+    bound = ((2 * WEIGHT + (S + 64) * U + r) * mag + ref.HALF[dtype] * np.abs(want)
+             + S * 2.0 ** -126)
+    err = np.abs(got - want)
+    assert (err <= bound).all(), (err / bound).max()
+
+
+@EACH
+@pytest.mark.parametrize("power", [10, 21, 24, 27, 40])
+def test_large_scores_keep_their_distances(dtype, Bn, S_q, H, H_kv, D, S, kernel, blocks, splits,
+                                           power):
+    """Scores of q0 + 0 to 6 steps, q0 between 2^power and 2^(power + 1) and a step f32's there (at
+    least 1): one number of steps to a run of 32 keys, of which waves take their turns, and less
+    of them in every third part of the keys, which splits share out.  At a scale of 2 / step a
+    step is 2.9 in log2 units.  V is 1 where the score is high and -1 or 1 where it is low,
+    so that a weight's error is the result's."""
+    print(f"{kernel} {blocks} {splits} D={D} dtype={dtype} 2^{power}", flush=True)
+    step = max(1.0, 2.0 ** (power - 23))
+    rng = np.random.default_rng(power)
+    runs = np.array([0, 1.0, 2, 3, 4, 6])[rng.integers(0, 6, S // 32 + 1)]
+    k, v = np.zeros((1, H_kv, S, D)), np.ones((1, H_kv, S, D))
+    k[..., 0] = 1
+    for h in range(H_kv):
+        steps = np.roll(runs, h)[np.arange(S) // 32]
+        part = np.arange(S) * 16 // S
+        k[0, h, :, 32] = np.where((part + h) % 3 == 0, np.minimum(steps, 2), steps)
+        v[0, h, :, ::2] = np.where(k[0, h, :, 32] >= 3, 1, -1)[:, None]
+        v[0, h, :, 1::2] = np.where(np.arange(S) // 32 % 2, 1, -1)[:, None]
+    cache = kv4.Cache.of(k, v)
+    for c0 in (1.0, 1.375, 1.625, -1.125):
+        q = np.zeros((Bn, S_q, H, D))
+        q[..., 0] = c0 * 2.0 ** power * (1 + np.arange(S_q)[None, :, None] % 4 / 64)
+        q[..., 32] = step
+        raw, q = ref.typed(q, dtype)
+        for scale in (2 / step, 1 / step, 0.25 / step):
+            check_exact_scores(cache, q, raw, dtype, scale)
+
+
+@EACH
+@pytest.mark.parametrize("high", [1, 30])
+def test_rising_scores_keep_their_distances(dtype, Bn, S_q, H, H_kv, D, S, kernel, blocks, splits,
+                                            high):
+    """Scores of about 2^25 of which the last key's is some 10 higher in log2 units, where a running
+    maximum moves (in the last case past 2^24 of them); every second row's scores rise by 2^(24 +
+    high) in the half behind.  Keys before weigh what they should beside those behind, whatever
+    the rows beside them do."""
+    print(f"{kernel} {blocks} {splits} D={D} dtype={dtype} high={high}", flush=True)
+    k, v = np.zeros((1, H_kv, S, D)), np.ones((1, H_kv, S, D))
+    key = np.arange(S)
+    k[..., 0] = 1
+    k[..., 32] = np.where(key == S - 1, 6, 0)
+    k[..., 33] = np.where(key >= S // 2, 1, 0)
+    v[..., ::2] = np.where(key >= S // 2, 1, -1)[None, None, :, None]
+    v[..., 1::2] = np.where(key == S - 1, 1, -1)[None, None, :, None]
+    cache = kv4.Cache.of(k, v)
+    for c0, rise, scale in ((1.0, 4, 0.275), (1.5, 8, 0.1375), (-1.25, 8, 0.1375), (1.75, 8, 0.15),
+                            (1.109375, 4, 0.26), (1.25, 4, (2 ** 24 - 4) / (LOG2E * 1.25 * 2 ** 25))):
+        q = np.zeros((Bn, S_q, H, D))
+        q[..., 0] = c0 * 2.0 ** 25
+        q[:, ::2, :, 32] = rise
+        q[:, 1::2, :, 33] = 2.0 ** (24 + high)
+        raw, q = ref.typed(q, dtype)
+        check_exact_scores(cache, q, raw, dtype, scale)
