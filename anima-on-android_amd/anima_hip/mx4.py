@@ -159,7 +159,8 @@ class MX4Linear:
 
 class KV4Cache:
     """Keys and values of `batch` sequences of up to `max_tokens` tokens, `heads` K/V heads of
-    `head_dim` (64 or 128), on the GPU in 4 bits.  ``lens`` holds each sequence's tokens."""
+    `head_dim` (64 or 128), on the GPU in 4 bits.  ``lens`` holds each sequence's tokens; set to
+    fewer, it takes sequences back to their first ones."""
 
     def __init__(self, batch, heads, head_dim, max_tokens):
         if min(batch, heads, max_tokens) < 1:
@@ -172,6 +173,15 @@ class KV4Cache:
         self._bufs = _Buffers()
         self._cache = [self._bufs.get(n, b) for n, b in (("kc", nc), ("ks", ns), ("vc", nc),
                                                          ("vs", ns))]
+
+    def _held(self):
+        """lens as the library reads it: int32, one of each sequence."""
+        n = np.asarray(self.lens)
+        if n.shape != (self.batch,) or n.dtype.kind not in "iu" or (n < 0).any() or \
+                (n > self.max_tokens).any():
+            raise ValueError(f"lens must be {self.batch} whole numbers between 0 and max_tokens = "
+                             f"{self.max_tokens}")
+        return n.astype(np.int32)
 
     def _counts(self, counts, S):
         c = np.full(self.batch, S, np.int32) if counts is None else np.asarray(counts, np.int32)
@@ -187,17 +197,17 @@ class KV4Cache:
         if k.shape != want or v.shape != want or dtype != dv:
             raise ValueError(f"append: k {k.shape}, v {v.shape} for a cache of {want}")
         S = k.shape[1]
-        c = self._counts(counts, S)
-        if (self.lens.astype(np.int64) + c > self.max_tokens).any():
+        c, lens = self._counts(counts, S), self._held()
+        if (lens.astype(np.int64) + c > self.max_tokens).any():
             raise ValueError(f"append: more than max_tokens = {self.max_tokens} tokens")
         kd, vd = self._bufs.upload("k", k), self._bufs.upload("v", v)
-        at, cd = self._bufs.upload("starts", self.lens), self._bufs.upload("counts", c)
+        at, cd = self._bufs.upload("starts", lens), self._bufs.upload("counts", c)
         st = _lib.strides((S * self.heads * self.head_dim, self.head_dim,
                            self.heads * self.head_dim))
         _lib.check(self._lib.anima_hip_kv4_append_dev(
             kd.ptr, vd.ptr, dtype, st, st, *(b.ptr for b in self._cache), at.ptr, cd.ptr, self.batch,
             S, self.heads, self.head_dim, self.max_tokens, None), "anima_hip_kv4_append_dev")
-        self.lens = self.lens + c
+        self.lens = lens + c
 
     def attend(self, q, counts=None, is_causal=True, scale=None):
         """softmax(scale q K^T) V of q [B, S, H, head_dim], H a multiple of the cache's heads and B
@@ -214,7 +224,7 @@ class KV4Cache:
             if c.shape != (B,):
                 raise ValueError(f"counts must be {B} numbers")
         scale = 1.0 / math.sqrt(D) if scale is None else scale
-        qd, ld = self._bufs.upload("q", q), self._bufs.upload("lens", self.lens)
+        qd, ld = self._bufs.upload("q", q), self._bufs.upload("lens", self._held())
         cd = None if c is None else self._bufs.upload("qcounts", c)
         od = self._bufs.upload("o", np.zeros_like(q)) if c is not None else \
             self._bufs.get("o", q.nbytes)
