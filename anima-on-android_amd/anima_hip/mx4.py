@@ -165,6 +165,10 @@ class KV4Cache:
     def __init__(self, batch, heads, head_dim, max_tokens):
         if min(batch, heads, max_tokens) < 1:
             raise ValueError("batch, heads and max_tokens must be positive")
+        if head_dim not in (64, 128):
+            raise ValueError(f"head_dim must be 64 or 128, got {head_dim}")
+        if max_tokens > 1 << 30:
+            raise ValueError(f"max_tokens must be at most 2^30, got {max_tokens}")
         self._lib = _lib.load()
         self.batch, self.heads = int(batch), int(heads)
         self.head_dim, self.max_tokens = int(head_dim), int(max_tokens)

@@ -101,3 +101,12 @@ def test_lens_out_of_place_are_refused(lib, lens):
         with pytest.raises(ValueError, match="lens"):
             call()
     assert not lib.seen
+
+
+@pytest.mark.parametrize("args,word", [((1, 2, 80, 8), "head_dim"), ((1, 2, 256, 8), "head_dim"),
+                                       ((1, 2, 0, 8), "head_dim"), ((0, 2, 64, 8), "positive"),
+                                       ((1, 2, 64, 2 ** 30 + 1), "2\\^30")])
+def test_caches_that_no_call_would_take(lib, args, word):
+    """Refused when they are made, before memory is taken for them."""
+    with pytest.raises(ValueError, match=word):
+        mx4.KV4Cache(*args)
