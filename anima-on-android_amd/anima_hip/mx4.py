@@ -4,12 +4,15 @@ MX4 rows are the OCP microscaling format with e2m1 elements and one scale byte
 per 32 of them (include/anima_hip.h): 4.25 bits per value.  `MX4Linear` keeps a
 layer's weights so and multiplies float32 or bf16 activations by them; `KV4Cache`
 keeps keys and values so and attends over them.  Arrays are float32, or uint16
-holding bf16 bit patterns; results have the type of the activations.
+holding bf16 bit patterns; results have the type of the activations.  An object may be
+called from several threads; its calls take turns.
 """
 from __future__ import annotations
 
 import ctypes as ct
+import functools
 import math
+import threading
 
 import numpy as np
 
@@ -31,10 +34,11 @@ def _sizes(rows, K):
 
 
 class _Buffers:
-    """Grow-only device buffers by role."""
+    """Grow-only device buffers by role, one call's at a time (`lock`)."""
 
     def __init__(self):
         self._bufs = {}
+        self.lock = threading.RLock()
 
     def get(self, role, nbytes):
         b = self._bufs.get(role)
@@ -54,6 +58,16 @@ class _Buffers:
         for b in self._bufs.values():
             b.close()
         self._bufs = {}
+
+
+def _one_at_a_time(method):
+    """The foreign calls release the interpreter's lock: without the object's own another thread
+    could refill or close a device array that a call is about to read."""
+    @functools.wraps(method)
+    def call(self, *args, **kwargs):
+        with self._bufs.lock:
+            return method(self, *args, **kwargs)
+    return call
 
 
 def pack(x):
@@ -130,6 +144,7 @@ class MX4Linear:
                    "anima_hip_mx4_pack_dev")
         _lib.check(self._lib.anima_hip_synchronize(), "anima_hip_synchronize")
 
+    @_one_at_a_time
     def __call__(self, x):
         """x [..., K] -> [..., N], float32 or bf16 bits like x."""
         x, dtype = _typed(x)
@@ -148,7 +163,8 @@ class MX4Linear:
 
     def close(self):
         if getattr(self, "_bufs", None) is not None:
-            self._bufs.close()
+            with self._bufs.lock:
+                self._bufs.close()
 
     def __del__(self):
         try:
@@ -193,6 +209,7 @@ class KV4Cache:
             raise ValueError(f"counts must be {self.batch} numbers between 0 and {S}")
         return np.ascontiguousarray(c)
 
+    @_one_at_a_time
     def append(self, k, v, counts=None):
         """Tokens k, v [batch, S, heads, head_dim] behind each sequence's last; counts: how many
         of the S each sequence takes (all, when None)."""
@@ -213,6 +230,7 @@ class KV4Cache:
             S, self.heads, self.head_dim, self.max_tokens, None), "anima_hip_kv4_append_dev")
         self.lens = lens + c
 
+    @_one_at_a_time
     def attend(self, q, counts=None, is_causal=True, scale=None):
         """softmax(scale q K^T) V of q [B, S, H, head_dim], H a multiple of the cache's heads and B
         the cache's batch, or any with a cache of one sequence.  Causal: the S queries (counts[b]
@@ -242,6 +260,7 @@ class KV4Cache:
             bool(is_causal), scratch.ptr, n, None), "anima_hip_kv4_attention_dev")
         return od.download(q.shape, q.dtype)
 
+    @_one_at_a_time
     def values(self):
         """(keys, values) as float32 [batch, heads, max_tokens, head_dim]; tokens past lens hold
         whatever the memory does."""
@@ -258,7 +277,8 @@ class KV4Cache:
 
     def close(self):
         if getattr(self, "_bufs", None) is not None:
-            self._bufs.close()
+            with self._bufs.lock:
+                self._bufs.close()
 
     def __del__(self):
         try:

@@ -1,6 +1,8 @@
 """MX4Linear and KV4Cache without a GPU: what they hand to the library, over device arrays held in host
 memory and a library that notes its calls."""
 import ctypes as ct
+import threading
+import time
 
 import numpy as np
 import pytest
@@ -110,3 +112,62 @@ def test_caches_that_no_call_would_take(lib, args, word):
     """Refused when they are made, before memory is taken for them."""
     with pytest.raises(ValueError, match=word):
         mx4.KV4Cache(*args)
+
+
+def in_threads(n, work):
+    """work(i) in n threads at once; what each returned, or raised."""
+    got, gate = [None] * n, threading.Barrier(n)
+
+    def run(i):
+        gate.wait()
+        try:
+            got[i] = work(i)
+        except Exception as e:
+            got[i] = e
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(n)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    return got
+
+
+def test_linear_from_several_threads(lib, monkeypatch):
+    """A layer's device arrays are one call's at a time: each thread gets its own result, and no
+    array is closed while a call holds it.  The library copies x to the output, slowly."""
+    def slow_copy(x, ldx, codes, scales, out, *args):
+        assert x and out
+        time.sleep(0.02)
+        ct.memmove(out, x, args[1] * ldx * 4)
+        return True
+
+    lib.anima_hip_linear_mx4_scratch_bytes = lambda *args: 0
+    lib.anima_hip_linear_mx4_dev = slow_copy
+    lin = mx4.MX4Linear(np.zeros((32, 32), np.float32))
+    xs = [np.full((i + 1, 32), i, np.float32) for i in range(6)]
+    for x, got in zip(xs, in_threads(len(xs), lambda i: lin(xs[i]))):
+        np.testing.assert_array_equal(got, x)
+
+
+def test_cache_from_several_threads(lib, monkeypatch):
+    """Appends from several threads each get places of their own; an attention sees the lens that
+    go with it."""
+    def slow(note):
+        def call(*args):
+            time.sleep(0.01)
+            return note(*args)
+        return call
+
+    lib.anima_hip_kv4_append_dev = slow(lib.anima_hip_kv4_append_dev)
+    cache = mx4.KV4Cache(2, 1, 64, 50)
+    x = np.zeros((2, 3, 1, 64), np.float32)
+
+    def work(i):
+        cache.append(x, x)
+        cache.attend(x)
+
+    assert in_threads(5, work) == [None] * 5
+    assert cache.lens.tolist() == [15, 15]
+    starts = [n for what, n in lib.seen if what == "append"]
+    assert sorted(starts) == [[3 * i, 3 * i] for i in range(5)]
