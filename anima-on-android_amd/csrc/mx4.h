@@ -83,8 +83,9 @@ __device__ __forceinline__ int scale_byte(unsigned top)
     return min(max(e, kMinScale), kMaxScale);
 }
 
-// x as `N` bf16 terms whose sum is x exactly (three terms: 3 x 8 bits): each
-// term is the leading eight bits of what is left, by truncation.  An infinity
+// x as `N` bf16 terms whose sum is x exactly (three terms: 3 x 8 bits; below 2^-110,
+// where the last of them lie under bf16's smallest number 2^-133, x cut off to a
+// multiple of it): each term is the leading eight bits of what is left, by truncation.  An infinity
 // is its own first term, with no NaN behind it (INF: there may be one).  Terms
 // are packed in pairs.
 template <int N, bool INF = true>

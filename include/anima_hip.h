@@ -594,8 +594,9 @@ bool anima_hip_mx4_unpack_dev(const uint8_t *codes, const uint8_t *scales, void 
 /* C[M,N] = A[M,K] . W[N,K]^T with W in MX4 rows (N rows of K) and A, C both of
  * `dtype`: anima_hip_linear_dev with 4-bit weights.  The weights enter the
  * product exactly, whatever their scale bytes (an element of 2^128 or more, see
- * above, gives an infinity or NaN); f32 activations do too (three bf16 terms),
- * sums are f32 and C is rounded once.  lda, ldc: row strides in elements.
+ * above, gives an infinity or NaN); f32 activations do too (three bf16 terms;
+ * magnitudes below 2^-110 are cut off to a multiple of 2^-133), sums are f32 and
+ * C is rounded once.  lda, ldc: row strides in elements.
  * scratch: anima_hip_linear_mx4_scratch_bytes(M, N, K, dtype) bytes, 16-byte
  * aligned (0: none needed); it holds the partial sums of a product split over
  * K, added in a fixed order, or for a large product whose K is no multiple of
@@ -635,10 +636,11 @@ bool anima_hip_kv4_append_dev(const void *k, const void *v, int dtype, const int
  * zeros; +inf, or an infinity times a scale of 0, gives NaN.  A NaN group of V
  * makes its dimensions NaN for every query that sees its key, however little the
  * key weighs.  The probabilities enter the second product as bf16 with bf16
- * queries and exactly with f32 ones, and out is rounded once.  scratch:
- * anima_hip_kv4_attention_scratch_bytes() bytes, 16-byte aligned (0: none
- * needed), for the partial results of a cache whose keys are shared out over
- * workgroups, joined in a fixed order. */
+ * queries and exactly with f32 ones (these and their queries as three bf16
+ * terms, with the cut-off of the linear layer's activations), and out is rounded
+ * once.  scratch: anima_hip_kv4_attention_scratch_bytes() bytes, 16-byte aligned
+ * (0: none needed), for the partial results of a cache whose keys are shared out
+ * over workgroups, joined in a fixed order. */
 size_t anima_hip_kv4_attention_scratch_bytes(int B, int S_q, int H, int H_kv, int D, int S_max,
                                              int dtype);
 bool anima_hip_kv4_attention_dev(const void *q, int dtype, const int64_t *q_strides,
