@@ -84,10 +84,10 @@ __device__ __forceinline__ int scale_byte(unsigned top)
 }
 
 // x as `N` bf16 terms whose sum is x exactly (three terms: 3 x 8 bits; below 2^-110,
-// where the last of them lie under bf16's smallest number 2^-133, x cut off to a
-// multiple of it): each term is the leading eight bits of what is left, by truncation.  An infinity
-// is its own first term, with no NaN behind it (INF: there may be one).  Terms
-// are packed in pairs.
+// where the last bits lie under bf16's smallest number 2^-133, x cut off to a
+// multiple of it): each term is the leading eight bits of what is left, by
+// truncation.  An infinity is its own first term, with no NaN behind it (INF:
+// there may be one).  Terms are packed in pairs.
 template <int N, bool INF = true>
 __device__ __forceinline__ void terms2(float x0, float x1, unsigned (&t)[N])
 {

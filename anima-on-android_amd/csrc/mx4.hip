@@ -1,8 +1,9 @@
 // MX4 rows (mx4.h): packing, unpacking and the append to a 4-bit K/V cache.
 // All three only move data (about 3 operations per element), so they are bound
 // by HBM, and by their launch where the rows are few: 268 M values pack in 147 us
-// from bf16 (4.6 TB/s) and 244 from f32 (5.0), unpack to f32 in 240 (5.1), and
-// are appended from bf16 in 183 (3.7: the loads wait for the start positions);
+// from bf16 (4.6 TB/s) and 244 from f32 (5.0), unpack to f32 in 240 (5.1) and to bf16
+// in 129 (5.3), and are appended from f32 in 234 (5.2) and from bf16 in 183 (3.7: a
+// thread's one load of 16 bytes waits for the start position and the count);
 // 2048 x 2048 take 4.0 and 5.3 us.  A thread takes eight consecutive elements, 16 or
 // 32 bytes of values against 4 bytes of codes, and four neighbouring lanes hold
 // one group, whose largest magnitude they find with two lane exchanges.  Unpacking,

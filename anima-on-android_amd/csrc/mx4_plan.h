@@ -106,6 +106,8 @@ inline LinPlan lin_plan(int M, int N, int K, bool f32, bool staged)
     // (rows x terms x K): bf16 0.7 at 22000, 0.95 at 88000, 1.3 at 131000; f32 at 3 to 8
     // rows 0.6 to 0.8 at 49000, 0.9 at 132000, 1.1 at 197000, at 12 rows 0.8 at 51000,
     // 1.0 at 74000, 1.2 at 147000, at 16 rows 0.7 at 25000, 1.1 at 49000, 2 at 264000.
+    // The limits are for K a multiple of 128: other K stay here at any size (f32, 16 rows,
+    // N 2048: 39.8 us at K = 8200, where 8192 takes 13.5 by staged tiles).
     const int64_t limit = !f32 ? 90000 : M <= 8 ? 150000 : M <= 12 ? 100000 : 40000;
     if (M <= kFewRows && (!staged || K % 128 || int64_t(M) * (f32 ? 3 : 1) * K <= limit))
         return pl;
@@ -191,6 +193,10 @@ constexpr Rate kRates[2][2] = {{{{0.64, 1.79, 1.51}, {0.52, 0.82, 0.98}},
 // further: 2048 rows of 512 keys, 4 K/V heads, take 10.8 us by it and 18.7 by the
 // tile kernel (bf16); 4096 x 512 keys, 32 heads, 50 us by the tile kernel against 141
 // by the first token kernel.
+// The lengths are the device's, so the plan is for a full cache.  One that holds little of
+// its capacity is shared out too far: 16 heads on 4 of 128, bf16, 512 tokens in caches of
+// 512, 4096 and 32768, by one query 9.3, 10.3 and 10.9 us, by 64 10.0, 12.2 and 20.4, by
+// 512 11.7, 24.2 and 32.7.
 inline AttnPlan attn_plan(int B, int S_q, int H, int H_kv, int D, int S_max, bool f32,
                           bool causal)
 {
