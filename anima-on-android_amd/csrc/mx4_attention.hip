@@ -120,10 +120,11 @@ __device__ __forceinline__ float base_shift(float mx, float scale2)
 // What takes probabilities and their sums from the maximum `from` to `to`, both raw scores:
 // waves, splits and the steps of one wave meet at their distance, which stays exact where
 // their scaled values have lost it, and at the shifts their exponents hold (up to 0.5).
+// Halves, whose distance is always a number: the scale may be small, or 0.
 template <int NT>
 __device__ __forceinline__ float rebase(float from, float to, float scale2)
 {
-    return __builtin_amdgcn_exp2f((from - to) * scale2 +
+    return __builtin_amdgcn_exp2f(2.0f * ((0.5f * from - 0.5f * to) * scale2) +
                                   (base_shift<NT>(to, scale2) - base_shift<NT>(from, scale2)));
 }
 
@@ -540,7 +541,9 @@ __global__ __launch_bounds__(kTokWaves * 64, 2) void kv4_token_kernel(AttnArgs a
         jm = fmaxf(jm, sm[i][jr]);
 #pragma unroll
     for (int i = 0; i < kTokWaves; ++i) {
-        w[i] = sl[i][jr] == 0.0f ? 0.0f : sm[i][jr] == jm ? 1.0f : rebase<NT>(sm[i][jr], jm, scale2);
+        w[i] = sl[i][jr] == 0.0f  ? 0.0f
+               : sm[i][jr] == jm ? 1.0f
+                                 : rebase<NT>(sm[i][jr], jm, scale2);
         jl += w[i] * sl[i][jr];
     }
     const float inv = jl == 0.0f ? 0.0f : 1.0f / jl;
@@ -944,9 +947,9 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void kv4_tile_kernel(AttnArgs a
 }
 
 // O = sum_s w_s P_s / sum_s w_s, w_s = l_s rebase(m_s, max m), over the splits (at most
-// 64); one of which no key was seen has l_s = 0.  PER waves per row: in each, lane s weighs split s;
-// wave w adds the splits w, w + PER, .., at most 16, its loads all in flight,
-// D / 64 dimensions per lane, and the waves' sums are added in their order.
+// 64); one of which no key was seen has l_s = 0.  PER waves per row: in each, lane s
+// weighs split s; wave w adds the splits w, w + PER, .., at most 16, its loads all in
+// flight, D / 64 dimensions per lane, and the waves' sums are added in their order.
 template <typename T, int D, int PER>
 __global__ __launch_bounds__(256) void kv4_join_kernel(AttnArgs a)
 {
