@@ -138,7 +138,8 @@ __device__ __forceinline__ float weighed(float w, float x)
 
 struct AttnArgs {
     Kv4Attention p;
-    float scale2;   // softmax scale * log2(e)
+    float scale2;   // softmax scale * log2(e) / q_factor, not negative
+    float q_factor;  // on the queries: the scale's sign, and for f32 part of a tiny scale
     int group;      // H / H_kv
     int rows;       // S_q * group
     int tiles;      // query tiles of a K/V head
@@ -165,8 +166,8 @@ struct Seq {
     }
 };
 
-// A query row's eight values from d as bf16 terms, negated or not.
-__device__ __forceinline__ void q_terms(const uint16_t *q, bool wide, bool neg, bf16x8 (&t)[1])
+// A query row's eight values from d times the factor (bf16: 1 or -1) as bf16 terms.
+__device__ __forceinline__ void q_terms(const uint16_t *q, bool wide, float factor, bf16x8 (&t)[1])
 {
     u32x4 u;
     if (wide)
@@ -176,7 +177,7 @@ __device__ __forceinline__ void q_terms(const uint16_t *q, bool wide, bool neg, 
         for (int i = 0; i < 4; ++i)
             u[i] = unsigned(q[2 * i]) | unsigned(q[2 * i + 1]) << 16;
     }
-    t[0] = __builtin_bit_cast(bf16x8, neg ? u ^ 0x80008000u : u);
+    t[0] = __builtin_bit_cast(bf16x8, factor < 0.0f ? u ^ 0x80008000u : u);
 }
 
 template <bool INF = true>
@@ -196,12 +197,12 @@ __device__ __forceinline__ void terms8(const float (&x)[8], bf16x8 (&t)[3])
         t[j] = __builtin_bit_cast(bf16x8, u[j]);
 }
 
-__device__ __forceinline__ void q_terms(const float *q, bool, bool neg, bf16x8 (&t)[3])
+__device__ __forceinline__ void q_terms(const float *q, bool, float factor, bf16x8 (&t)[3])
 {
     float x[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-        x[i] = neg ? -q[i] : q[i];
+        x[i] = q[i] * factor;
     terms8(x, t);
 }
 
@@ -306,8 +307,8 @@ __global__ __launch_bounds__(kTokWaves * 64, 2) void kv4_token_kernel(AttnArgs a
     // This lane's query rows (column n of the accumulators).  Rows past the last
     // read that one and are not written; a column's values stay its own.
     const Seq seq(p, b, hk);
-    // Scores are kept unscaled; the sign of the scale goes into the queries.
-    const float scale2 = fabsf(a.scale2);
+    // Scores are kept unscaled; the sign of the scale is in the queries.
+    const float scale2 = a.scale2;
     bf16x8 qf[RB][STEPS][NT];
     int limit[RB], most = 0, least = INT32_MAX;
 #pragma unroll
@@ -321,7 +322,7 @@ __global__ __launch_bounds__(kTokWaves * 64, 2) void kv4_token_kernel(AttnArgs a
                            ((p.qs.b | p.qs.h | p.qs.s) & 7)) == 0;
 #pragma unroll
         for (int st = 0; st < STEPS; ++st)
-            q_terms(qr + g * (D / 4) + 8 * st, wide, a.scale2 < 0.0f, qf[rb][st]);
+            q_terms(qr + g * (D / 4) + 8 * st, wide, a.q_factor, qf[rb][st]);
         const bool live = row < a.rows && s < seq.nq;
         limit[rb] = live ? seq.limit(p, s) : 0;
         most = max(most, limit[rb]);
@@ -625,8 +626,8 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void kv4_tile_kernel(AttnArgs a
     const int per = (steps + a.splits - 1) / a.splits;
     const int first = min(split * per, steps), end = min(first + per, steps);
 
-    // Scores are kept unscaled; the sign of the scale goes into the queries.
-    const float scale2 = fabsf(a.scale2);
+    // Scores are kept unscaled; the sign of the scale is in the queries.
+    const float scale2 = a.scale2;
     bf16x8 qf[KSTEPS][NT];
     {
         const T *q = static_cast<const T *>(p.q);
@@ -635,7 +636,7 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void kv4_tile_kernel(AttnArgs a
                            ((p.qs.b | p.qs.h | p.qs.s) & 7)) == 0;
 #pragma unroll
         for (int ks = 0; ks < KSTEPS; ++ks)
-            q_terms(qr + 16 * ks + 8 * half, wide, a.scale2 < 0.0f, qf[ks]);
+            q_terms(qr + 16 * ks + 8 * half, wide, a.q_factor, qf[ks]);
     }
 
     // What this thread decodes of a tile: D / 4 codes of one key's K, and V of
@@ -983,7 +984,7 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(AttnArgs a)
     const float w =
         ml.y == 0.0f
             ? 0.0f
-            : (ml.x == m ? 1.0f : rebase<kTerms<T>>(ml.x, m, fabsf(a.scale2))) * ml.y;
+            : (ml.x == m ? 1.0f : rebase<kTerms<T>>(ml.x, m, a.scale2)) * ml.y;
     float l = w;
 #pragma unroll
     for (int o = 32; o; o >>= 1)
@@ -1068,7 +1069,15 @@ bool launch_kv4_attention(const Kv4Attention &p, void *scratch, size_t scratch_b
                                   p.causal);
     AttnArgs a{};
     a.p = p;
-    a.scale2 = p.scale * kLog2e;
+    a.scale2 = std::fabs(p.scale * kLog2e);
+    a.q_factor = p.scale < 0.0f ? -1.0f : 1.0f;
+    // f32 queries' exponents take the distance of two scores.  One past f32's range is a
+    // weight of 0 under scales from 2^9 / 2^128 on, but not under smaller ones or 0: part of
+    // those goes into the queries, whose bits lost by it count for less than 2^-50.
+    if (p.type == kMx4F32 && a.scale2 < 0x1p-119f) {
+        a.scale2 *= 0x1p64f;
+        a.q_factor *= 0x1p-64f;
+    }
     a.group = p.H / p.H_kv;
     a.rows = p.S_q * a.group;
     a.tiles = pl.tiles;

@@ -180,8 +180,8 @@ def test_rising_scores_keep_their_distances(dtype, Bn, S_q, H, H_kv, D, S, kerne
         check_exact_scores(cache, q, raw, dtype, scale)
 
 
-@pytest.mark.parametrize("dtype,Bn,S_q,H,H_kv,D,S,kernel,blocks,splits", [c for c in SHAPES if c[0] == B])
-@pytest.mark.parametrize("scale", [0.0, 2.0 ** -126])
+@EACH
+@pytest.mark.parametrize("scale", [0.0, 2.0 ** -126, -2.0 ** -126])
 def test_distances_past_the_range(dtype, Bn, S_q, H, H_kv, D, S, kernel, blocks, splits, scale):
     """Scores of 1.5 * 2^127 and its negative, whose distance f32 does not hold: under a scale of zero
     all keys weigh the same, and under a small one the lower ones e^-6 of the one higher key."""
@@ -193,6 +193,6 @@ def test_distances_past_the_range(dtype, Bn, S_q, H, H_kv, D, S, kernel, blocks,
     v[..., ::2] = np.where(key // 32 % 2, 1, -1)[None, None, :, None]
     cache = kv4.Cache.of(k, v)
     q = np.zeros((Bn, S_q, H, D))
-    q[..., 0] = 2.0 ** 64
+    q[..., 0] = 2.0 ** 64 * (1 if scale >= 0 else -1)
     raw, q = ref.typed(q, dtype)
     check_exact_scores(cache, q, raw, dtype, scale)
