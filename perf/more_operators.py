@@ -8,8 +8,9 @@ A row of K elements has ceil(K / 128) * 128 bytes of codes, zero past K, and cei
 scale bytes, zero past its groups.
 
 Packing: the scale is the smallest power of two by which the largest magnitude a of a group is at
-most 448 (2^E <= a < 2^(E+1): byte E - 8 + 127, one more where a > 1.75 * 2^E), at least byte 2;
-elements round to nearest, ties to even.  A group with an infinity or a NaN gets 255.
+most 448 (2^E <= a < 2^(E+1): byte E - 8 + 127, one more where a > 1.75 * 2^E), kept within bytes
+10 .. 246, so that every value is zero or a normal bf16 number; elements round to nearest, ties to
+even, and saturate at 448.  A group with an infinity or a NaN gets 255.
 
 Kinds:
 
@@ -268,17 +269,17 @@ def plain_pack(x):
     x = torch.nn.functional.pad(x.float(), (0, groups * 128 - K)).reshape(rows, groups, 128)
     a = x.abs().amax(-1)
     m, e = torch.frexp(a)  # a = m 2^e, m in [0.5, 1)
-    byte = torch.where(a > 0, e + 118 + (m > 0.875).int(), 2).clamp(2, 247)
+    byte = torch.where(a > 0, e + 118 + (m > 0.875).int(), 10).clamp(10, 246)
     finite = torch.isfinite(a)
     byte = torch.where(finite, byte, 255)
-    y = torch.where(finite[..., None], x * _power(254 - byte.clamp(max=247))[..., None], 0.0)
+    y = torch.where(finite[..., None], x * _power(254 - byte.clamp(max=246))[..., None], 0.0)
     # The last place of an e4m3 number is 2^-3 of its power of two, 2^-9 at least.
     _, e = torch.frexp(y)
     e = (e - 1).clamp(min=-6)
     steps = torch.round(y.abs() * _power(130 - e)).int()  # ties to even
     up = steps >> 4  # rounded up to the next power of two
     steps, e = torch.where(up > 0, 8, steps), e + up
-    code = torch.where(steps >= 8, (e + 7) * 8 + steps - 8, steps)
+    code = torch.where(steps >= 8, (e + 7) * 8 + steps - 8, steps).clamp(max=126)
     code = code + 128 * torch.signbit(y).int()
     scales = torch.nn.functional.pad(byte, (0, _scale_bytes(K) - groups))
     return code.reshape(rows, -1).to(torch.uint8), scales.to(torch.uint8)
@@ -359,7 +360,7 @@ def _exact_rounded(x):
     top = g.abs().max(-1, keepdim=True).values
     power = torch.tensor([2.0 ** (k - 127) for k in range(256)], dtype=torch.float64, device=DEV)
     # The first power of two by which `top` is at most 448.
-    unit = power[torch.searchsorted(448.0 * power, top).clamp(2, 247)]
+    unit = power[torch.searchsorted(448.0 * power, top).clamp(10, 246)]
     number = torch.tensor([(c & 7) * 2.0 ** -9 if c < 8 else (8 + (c & 7)) * 2.0 ** ((c >> 3) - 10)
                            for c in range(127)], dtype=torch.float64, device=DEV)
     mag = g.abs() / unit
