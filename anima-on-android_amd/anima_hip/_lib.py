@@ -87,6 +87,15 @@ SIGNATURES = {
     "anima_hip_kv4_attention_scratch_bytes": (ct.c_size_t, [_I] * 7),
     "anima_hip_kv4_attention_dev": (_B, [_P, _I, _I64P] + [_P] * 7 + [_I64P] + [_I] * 7
                                     + [_F, _B, _P, ct.c_size_t, _P]),
+    "anima_hip_fp8_pack_dev": (_B, [_P, ct.c_int64, _I, _P, _P, ct.c_int64, _I, _P]),
+    "anima_hip_fp8_unpack_dev": (_B, [_P, _P, _P, ct.c_int64, _I, ct.c_int64, _I, _P]),
+    "anima_hip_add_rmsnorm_fp8_dev": (_B, [_P, ct.c_int64, _P, ct.c_int64, _P, _F, _I, _P,
+                                           ct.c_int64, _P, ct.c_int64, _P, _P, ct.c_int64, _I,
+                                           _P]),
+    "anima_hip_linear_fp8_scratch_bytes": (ct.c_size_t, [_I] * 4),
+    "anima_hip_linear_fp8_dev": (_B, [_P] * 5 + [ct.c_int64] + [_I] * 4 + [_P, ct.c_size_t, _P]),
+    "anima_hip_rope_axes_dev": (_B, [_P, _I64P, _P, _I64P, _I] * 2
+                                + [_P, ct.c_int64, _P, _P, _P] + [_I] * 6 + [_B, _B, _P]),
     "anima_hip_last_call_ms": (_B, [ct.POINTER(_F), ct.POINTER(_F)]),
     "anima_hip_malloc": (_P, [ct.c_size_t]),
     "anima_hip_free": (None, [_P]),

@@ -1741,6 +1741,203 @@ bool anima_hip_kv4_attention_dev(const void *q, int dtype, const int64_t *q_stri
     return launch_kv4_attention(p, scratch, scratch_bytes, pick_stream(stream));
 }
 
+namespace {
+// Rows of K values ld apart, for an argument called `name`.
+bool check_rows(const std::string &who, const char *name, const void *x, int64_t ld, Mx4Type t,
+                int64_t rows, int K)
+{
+    if (rows > 1 && ld < K)
+        return fail(who + ": row stride of " + name + " shorter than a row");
+    if (!elem_aligned(x, t))
+        return fail(who + ": " + name + " must be aligned to its type");
+    return true;
+}
+}  // namespace
+
+bool anima_hip_fp8_pack_dev(const void *x, int64_t ldx, int dtype, uint8_t *codes, uint8_t *scales,
+                            int64_t rows, int K, void *stream)
+{
+    Mx4Type t;
+    if (!check_mx4_rows("fp8_pack_dev", x, ldx, dtype, codes, scales, rows, K, t))
+        return false;
+    if (!ready_for_device_call())
+        return false;
+    return launch_fp8_pack(x, ldx, t, codes, scales, rows, K, pick_stream(stream));
+}
+
+bool anima_hip_fp8_unpack_dev(const uint8_t *codes, const uint8_t *scales, void *x, int64_t ldx,
+                              int dtype, int64_t rows, int K, void *stream)
+{
+    Mx4Type t;
+    if (!check_mx4_rows("fp8_unpack_dev", x, ldx, dtype, codes, scales, rows, K, t))
+        return false;
+    if (!ready_for_device_call())
+        return false;
+    return launch_fp8_unpack(codes, scales, x, ldx, t, rows, K, pick_stream(stream));
+}
+
+bool anima_hip_add_rmsnorm_fp8_dev(const void *x, int64_t ldx, const void *residual, int64_t ldr,
+                                   const float *w, float eps, int dtype, void *sum, int64_t ldsum,
+                                   void *y, int64_t ldy, uint8_t *codes, uint8_t *scales,
+                                   int64_t rows, int K, void *stream)
+{
+    const std::string who = "add_rmsnorm_fp8_dev";
+    AddRmsNorm a;
+    if (!mx4_type("add_rmsnorm_fp8_dev", dtype, a.type))
+        return false;
+    if (rows < 0 || K < 0 || K > kMx4MaxDim)
+        return fail(who + ": rows must not be negative, K between 0 and 2^30");
+    if (!(eps >= 0.0f) || !std::isfinite(eps))
+        return fail(who + ": eps must be finite and not negative");
+    if (!codes != !scales)
+        return fail(who + ": codes and scales must be given together");
+    if (!sum && !y && !codes)
+        return fail(who + ": no output");
+    if (rows > 0 && K > 0) {
+        if (!x)
+            return fail(who + ": null pointer");
+        if (!check_rows(who, "x", x, ldx, a.type, rows, K) ||
+            (residual && !check_rows(who, "residual", residual, ldr, a.type, rows, K)) ||
+            (sum && !check_rows(who, "sum", sum, ldsum, a.type, rows, K)) ||
+            (y && !check_rows(who, "y", y, ldy, a.type, rows, K)))
+            return false;
+        if (reinterpret_cast<uintptr_t>(w) & 3u)
+            return fail(who + ": w must be aligned to its type");
+        if (sum && sum == y)
+            return fail(who + ": sum and y must be different arrays");
+        if (codes && !check_mx4("add_rmsnorm_fp8_dev", codes, scales))
+            return false;
+    }
+    a.x = x;
+    a.residual = residual;
+    a.w = w;
+    a.sum = sum;
+    a.y = y;
+    a.codes = codes;
+    a.scales = scales;
+    a.ldx = ldx;
+    a.ldr = ldr;
+    a.ldsum = ldsum;
+    a.ldy = ldy;
+    a.rows = rows;
+    a.K = K;
+    a.eps = eps;
+    if (!ready_for_device_call())
+        return false;
+    return launch_add_rmsnorm_fp8(a, pick_stream(stream));
+}
+
+size_t anima_hip_linear_fp8_scratch_bytes(int M, int N, int K, int dtype)
+{
+    if (dtype != ANIMA_HIP_DTYPE_F32 && dtype != ANIMA_HIP_DTYPE_BF16)
+        return 0;
+    if (M > kMx4MaxDim || N > kMx4MaxDim || K > kMx4MaxDim)
+        return 0;
+    return linear_fp8_scratch_bytes(M, N, K, Mx4Type(dtype));
+}
+
+bool anima_hip_linear_fp8_dev(const uint8_t *a_codes, const uint8_t *a_scales,
+                              const uint8_t *w_codes, const uint8_t *w_scales, void *c, int64_t ldc,
+                              int M, int N, int K, int dtype, void *scratch, size_t scratch_bytes,
+                              void *stream)
+{
+    Fp8Linear p;
+    if (!mx4_type("linear_fp8_dev", dtype, p.type))
+        return false;
+    if (M < 0 || N < 0 || K < 0 || M > kMx4MaxDim || N > kMx4MaxDim || K > kMx4MaxDim)
+        return fail("linear_fp8_dev: M, N and K must be between 0 and 2^30");
+    if (M > 0 && N > 0) {
+        if (!c)
+            return fail("linear_fp8_dev: null pointer");
+        if (!check_rows("linear_fp8_dev", "c", c, ldc, p.type, M, N))
+            return false;
+        if (K > 0 && (!check_mx4("linear_fp8_dev", a_codes, a_scales) ||
+                      !check_mx4("linear_fp8_dev", w_codes, w_scales)))
+            return false;
+    }
+    p.a = a_codes;
+    p.a_scales = a_scales;
+    p.w = w_codes;
+    p.w_scales = w_scales;
+    p.c = c;
+    p.ldc = ldc;
+    p.M = M;
+    p.N = N;
+    p.K = K;
+    if (!ready_for_device_call())
+        return false;
+    return launch_linear_fp8(p, scratch, scratch_bytes, pick_stream(stream));
+}
+
+namespace {
+// No two rows of an output [B, H, S, D] share an element along one axis.
+bool rows_apart(const Strides &s, int B, int H, int S, int D)
+{
+    const auto ok = [&](int n, int64_t stride) { return n <= 1 || stride >= D || stride <= -D; };
+    return ok(B, s.b) && ok(H, s.h) && ok(S, s.s);
+}
+}  // namespace
+
+bool anima_hip_rope_axes_dev(const void *q, const int64_t *q_strides, void *q_out,
+                             const int64_t *qo_strides, int H_q, const void *k,
+                             const int64_t *k_strides, void *k_out, const int64_t *ko_strides,
+                             int H_k, const int32_t *positions, int64_t pos_batch_stride,
+                             const int32_t *counts, const double *freqs, const uint8_t *pair_axis,
+                             int axes, int pairs, int B, int S, int D, int dtype, bool interleaved,
+                             bool inverse, void *stream)
+{
+    const std::string who = "rope_axes_dev";
+    RopeAxes a;
+    if (!mx4_type("rope_axes_dev", dtype, a.type))
+        return false;
+    if (B < 0 || S < 0 || H_q < 0 || H_k < 0)
+        return fail(who + ": B, S, H_q and H_k must not be negative");
+    if (H_q > 2048 || H_k > 2048)
+        return fail(who + ": H_q and H_k must be at most 2048");
+    if (D < 2 || D > 1024 || pairs < 1 || pairs > D / 2)
+        return fail(who + ": D must be between 2 and 1024, pairs between 1 and D / 2");
+    if (axes < 1 || axes > 256)
+        return fail(who + ": axes must be between 1 and 256");
+    a.qs = from_array(q_strides, H_q, S, D);
+    a.ks = from_array(k_strides, H_k, S, D);
+    a.qos = from_array(qo_strides, H_q, S, D);
+    a.kos = from_array(ko_strides, H_k, S, D);
+    if (B > 0 && S > 0 && H_q + H_k > 0) {
+        if ((H_q > 0 && (!q || !q_out)) || (H_k > 0 && (!k || !k_out)) || !positions || !freqs)
+            return fail(who + ": null pointer");
+        if ((H_q > 0 && (!elem_aligned(q, a.type) || !elem_aligned(q_out, a.type))) ||
+            (H_k > 0 && (!elem_aligned(k, a.type) || !elem_aligned(k_out, a.type))) ||
+            (reinterpret_cast<uintptr_t>(positions) & 3u) ||
+            (reinterpret_cast<uintptr_t>(counts) & 3u) ||
+            (reinterpret_cast<uintptr_t>(freqs) & 7u))
+            return fail(who + ": arrays must be aligned to their type");
+        if ((H_q > 0 && !rows_apart(a.qos, B, H_q, S, D)) ||
+            (H_k > 0 && !rows_apart(a.kos, B, H_k, S, D)))
+            return fail(who + ": rows of an output overlap");
+    }
+    a.q = q;
+    a.q_out = q_out;
+    a.H_q = H_q;
+    a.k = k;
+    a.k_out = k_out;
+    a.H_k = H_k;
+    a.positions = positions;
+    a.pos_batch = pos_batch_stride;
+    a.counts = counts;
+    a.freqs = freqs;
+    a.pair_axis = pair_axis;
+    a.axes = axes;
+    a.pairs = pairs;
+    a.B = B;
+    a.S = S;
+    a.D = D;
+    a.interleaved = interleaved;
+    a.inverse = inverse;
+    if (!ready_for_device_call())
+        return false;
+    return launch_rope_axes(a, pick_stream(stream));
+}
+
 size_t anima_hip_attention_scratch_bytes(int B, int S_q, int Bk, int S_kv, int H, int D,
                                          int mode)
 {

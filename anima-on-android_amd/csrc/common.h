@@ -507,6 +507,55 @@ size_t kv4_attention_scratch_bytes(int B, int S_q, int H, int H_kv, int D, int S
 bool launch_kv4_attention(const Kv4Attention &p, void *scratch, size_t scratch_bytes,
                           hipStream_t st);
 
+// ---- 8-bit rows (FP8: e4m3 elements, one e8m0 scale byte per 128; layout in
+// fp8.h).  Types of values as Mx4Type. ----
+__host__ __device__ inline int64_t fp8_groups(int K) { return (int64_t(K) + 127) / 128; }
+__host__ __device__ inline int64_t fp8_scale_bytes(int K) { return (int64_t(K) + 511) / 512 * 4; }
+// Rows of x [rows][ldx] to codes [rows][128 fp8_groups(K)] and scales
+// [rows][fp8_scale_bytes(K)], and back (fp8.hip).
+bool launch_fp8_pack(const void *x, int64_t ldx, Mx4Type type, uint8_t *codes, uint8_t *scales,
+                     int64_t rows, int K, hipStream_t st);
+bool launch_fp8_unpack(const uint8_t *codes, const uint8_t *scales, void *x, int64_t ldx,
+                       Mx4Type type, int64_t rows, int K, hipStream_t st);
+// h = x + residual; sum = h, y = h / sqrt(mean(h^2) + eps) * w, codes and scales
+// = y in 8-bit rows (fp8.hip).  residual, w, sum, y, codes with scales: optional.
+struct AddRmsNorm {
+    const void *x = nullptr, *residual = nullptr;
+    const float *w = nullptr;
+    void *sum = nullptr, *y = nullptr;
+    uint8_t *codes = nullptr, *scales = nullptr;
+    int64_t ldx = 0, ldr = 0, ldsum = 0, ldy = 0, rows = 0;
+    int K = 0;
+    float eps = 1e-6f;
+    Mx4Type type = kMx4F32;
+};
+bool launch_add_rmsnorm_fp8(const AddRmsNorm &a, hipStream_t st);
+// C[M,N] = A[M,K] . W[N,K]^T, A and W in 8-bit rows, C f32 or bf16
+// (fp8_linear.hip).
+struct Fp8Linear {
+    const uint8_t *a = nullptr, *a_scales = nullptr, *w = nullptr, *w_scales = nullptr;
+    void *c = nullptr;
+    int64_t ldc = 0;
+    int M = 0, N = 0, K = 0;
+    Mx4Type type = kMx4F32;  // of C
+};
+size_t linear_fp8_scratch_bytes(int M, int N, int K, Mx4Type type);
+bool launch_linear_fp8(const Fp8Linear &p, void *scratch, size_t scratch_bytes, hipStream_t st);
+// Queries and keys turned by their tokens' positions (rope_axes.hip).
+struct RopeAxes {
+    const void *q = nullptr, *k = nullptr;
+    void *q_out = nullptr, *k_out = nullptr;
+    Strides qs, ks, qos, kos;
+    const int32_t *positions = nullptr, *counts = nullptr;  // device
+    const double *freqs = nullptr;                          // device
+    const uint8_t *pair_axis = nullptr;                     // device
+    int64_t pos_batch = 0;
+    int H_q = 0, H_k = 0, axes = 1, pairs = 0, B = 0, S = 0, D = 0;
+    Mx4Type type = kMx4F32;
+    bool interleaved = false, inverse = false;
+};
+bool launch_rope_axes(const RopeAxes &a, hipStream_t st);
+
 // ---- Element-wise and row operators (ops.hip), device pointers ----
 // GELU (exact erf form), SiLU, LayerNorm without affine over rows of D,
 // softmax over rows of D, and C[i][j] += bias[j] for an M x N matrix.

@@ -1,0 +1,166 @@
+// 8-bit rows (FP8): every 128 consecutive elements of a row share one scale
+// byte s, an e8m0 number 2^(s - 127) with 255 for NaN; an element is an e4m3
+// code (OCP: sign, four bits of exponent with bias 7, three of mantissa; no
+// infinity, largest 448).  A row of K elements takes ceil(K / 128) * 128 bytes
+// of codes, zero past K, and ceil(K / 512) * 4 scale bytes, zero past its
+// groups, so that a dword holds four groups' scales at any row.
+//
+// The scale is the smallest power of two by which the group's largest magnitude
+// is at most 448, so that an element is scaled exactly and rounded once.  A
+// power of two rather than the quotient by 448: the MFMA takes e8m0 scales by
+// itself, and what a scale between two powers of two would gain is none of an
+// element's four significant bits, only half a power of two of range.
+#pragma once
+
+#include "flash_tile.h"
+
+namespace anima_hip {
+namespace fp8 {
+
+using flash_tile::bf16x2;
+using flash_tile::bf16x8;
+using flash_tile::f32x2;
+using flash_tile::f32x4;
+using flash_tile::u32x4;
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kGroup = 128;     // elements per scale
+constexpr int kNanScale = 255;  // scale byte of a group that held an infinity or a NaN
+// Scale bytes the packer writes: 2^-117 keeps the smallest element, 2^-9, a normal
+// bf16 number, 2^119 keeps the largest, 448, finite (1.75 * 2^127).
+constexpr int kMinScale = 10, kMaxScale = 246;
+
+// Scale byte of a group whose largest |x| has the bits `top` (as unsigned
+// integers, magnitudes order like the numbers, NaN above infinity).
+__device__ __forceinline__ int scale_byte(unsigned top)
+{
+    if (top >= 0x7F800000u)
+        return kNanScale;
+    const int e = int(top >> 23) - 8 + ((top & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+    return min(max(e, kMinScale), kMaxScale);
+}
+
+// 2^(127 - byte) for a byte the packer writes: what elements are multiplied by.
+__device__ __forceinline__ float unscale_of(int byte) { return __uint_as_float((254u - byte) << 23); }
+
+// The scale as the conversions take it: only the exponent field counts.
+__device__ __forceinline__ float scale_of(unsigned byte) { return __uint_as_float(byte << 23); }
+
+// Four values over their scale as codes, round to nearest even.  Only groups at
+// the largest scale reach past 448; there elements saturate.
+__device__ __forceinline__ unsigned encode4(float x0, float x1, float x2, float x3, float unscale)
+{
+    const auto in = [&](float x) { return __builtin_amdgcn_fmed3f(x * unscale, -448.0f, 448.0f); };
+    int r = 0;
+    r = __builtin_amdgcn_cvt_pk_fp8_f32(in(x0), in(x1), r, false);
+    r = __builtin_amdgcn_cvt_pk_fp8_f32(in(x2), in(x3), r, true);
+    return unsigned(r);
+}
+
+// Largest of v over the 16 lanes of a DPP row, in all of them.
+__device__ __forceinline__ unsigned row16_max(unsigned v)
+{
+    v = max(v, unsigned(__builtin_amdgcn_update_dpp(0, int(v), 0x128, 0xF, 0xF, false)));  // row_ror:8
+    v = max(v, unsigned(__builtin_amdgcn_update_dpp(0, int(v), 0x124, 0xF, 0xF, false)));
+    v = max(v, unsigned(__builtin_amdgcn_update_dpp(0, int(v), 0x122, 0xF, 0xF, false)));
+    v = max(v, unsigned(__builtin_amdgcn_update_dpp(0, int(v), 0x121, 0xF, 0xF, false)));
+    return v;
+}
+
+// One group over the 16 lanes of a DPP row, eight elements each, group g of `groups`
+// of its row.  All 16 lanes come here together.  Groups with an infinity or a NaN
+// have zero codes, so that packing is a function of the values alone.
+__device__ __forceinline__ void pack_group(const float (&x)[8], uint8_t *row_codes,
+                                           uint8_t *row_scales, int g, int groups, int piece)
+{
+    unsigned top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+    top = row16_max(top);
+    const int s = scale_byte(top);
+    u32x2 c = {0u, 0u};
+    if (s != kNanScale) {
+        const float u = unscale_of(s);
+        c[0] = encode4(x[0], x[1], x[2], x[3], u);
+        c[1] = encode4(x[4], x[5], x[6], x[7], u);
+    }
+    *reinterpret_cast<u32x2 *>(row_codes + int64_t(g) * kGroup + 8 * piece) = c;
+    // The last group's lanes write the zeros past it too.
+    if (piece == 0 || (g == groups - 1 && piece < 4 - (g & 3)))
+        row_scales[g + piece] = piece == 0 ? uint8_t(s) : uint8_t(0);
+}
+
+// Elements k0 .. k0+7 of a row of K; zero past its end.  `vec`: 16-byte loads
+// of a whole piece.
+__device__ __forceinline__ void load8(const float *row, int k0, int K, bool vec, float (&x)[8])
+{
+    if (vec && k0 + 8 <= K) {
+        const f32x4 a = *reinterpret_cast<const f32x4 *>(row + k0);
+        const f32x4 b = *reinterpret_cast<const f32x4 *>(row + k0 + 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[i] = a[i];
+            x[4 + i] = b[i];
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        x[i] = k0 + i < K ? row[k0 + i] : 0.0f;
+}
+
+__device__ __forceinline__ void load8(const uint16_t *row, int k0, int K, bool vec, float (&x)[8])
+{
+    if (vec && k0 + 8 <= K) {
+        const u32x4 a = *reinterpret_cast<const u32x4 *>(row + k0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = __uint_as_float(a[i] << 16);
+            x[2 * i + 1] = __uint_as_float(a[i] & 0xFFFF0000u);
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        x[i] = k0 + i < K ? __uint_as_float(unsigned(row[k0 + i]) << 16) : 0.0f;
+}
+
+// The same elements stored, rounded to the row's type.
+__device__ __forceinline__ void store8(float *row, int k0, int K, bool vec, const float (&x)[8])
+{
+    if (vec && k0 + 8 <= K) {
+        *reinterpret_cast<f32x4 *>(row + k0) = f32x4{x[0], x[1], x[2], x[3]};
+        *reinterpret_cast<f32x4 *>(row + k0 + 4) = f32x4{x[4], x[5], x[6], x[7]};
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (k0 + i < K)
+            row[k0 + i] = x[i];
+}
+
+__device__ __forceinline__ unsigned bf16_pair(float lo, float hi)
+{
+    return __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{lo, hi}, bf16x2));
+}
+
+__device__ __forceinline__ void store8(uint16_t *row, int k0, int K, bool vec, const float (&x)[8])
+{
+    u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        w[i] = bf16_pair(x[2 * i], x[2 * i + 1]);
+    if (vec && k0 + 8 <= K) {
+        *reinterpret_cast<u32x4 *>(row + k0) = w;
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (k0 + i < K)
+            row[k0 + i] = uint16_t(w[i >> 1] >> (16 * (i & 1)));
+}
+
+}  // namespace fp8
+}  // namespace anima_hip

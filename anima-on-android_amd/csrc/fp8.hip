@@ -1,0 +1,340 @@
+// 8-bit rows (fp8.h): packing and unpacking, and the root-mean-square norm that
+// adds the residual and writes its result in 8-bit rows.
+#include "fp8.h"
+
+#include <algorithm>
+
+namespace anima_hip {
+namespace {
+
+using namespace fp8;
+
+template <typename T>
+__global__ __launch_bounds__(256) void fp8_pack_kernel(const T *x, int64_t ldx, uint8_t *codes,
+                                                       uint8_t *scales, unsigned groups,
+                                                       unsigned total, int K, bool vec)
+{
+    const unsigned gi = blockIdx.x * 16u + (threadIdx.x >> 4);
+    if (gi >= total)
+        return;  // all 16 lanes of a group
+    const int piece = threadIdx.x & 15;
+    const unsigned row = gi / groups;
+    const int g = int(gi - row * groups);
+    float v[8];
+    load8(x + int64_t(row) * ldx, g * kGroup + 8 * piece, K, vec, v);
+    pack_group(v, codes + int64_t(row) * groups * kGroup,
+               scales + int64_t(row) * fp8_scale_bytes(K), g, int(groups), piece);
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void fp8_unpack_kernel(const uint8_t *codes,
+                                                         const uint8_t *scales, T *x, int64_t ldx,
+                                                         unsigned groups, unsigned total, int K,
+                                                         bool vec)
+{
+    const unsigned gi = blockIdx.x * 16u + (threadIdx.x >> 4);
+    if (gi >= total)
+        return;
+    const int piece = threadIdx.x & 15;
+    const unsigned row = gi / groups;
+    const int g = int(gi - row * groups);
+    const int byte = scales[int64_t(row) * fp8_scale_bytes(K) + g];
+    const u32x2 c = *reinterpret_cast<const u32x2 *>(codes + int64_t(gi) * kGroup + 8 * piece);
+    // 2^(byte - 127), subnormal for byte 0, NaN for 255.
+    const float s = byte == 0 ? __uint_as_float(0x400000u)
+                    : byte == kNanScale ? __uint_as_float(0x7FC00000u) : scale_of(byte);
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(int(c[i]), false);
+        const f32x2 hi = __builtin_amdgcn_cvt_pk_f32_fp8(int(c[i]), true);
+        v[4 * i] = lo[0] * s;
+        v[4 * i + 1] = lo[1] * s;
+        v[4 * i + 2] = hi[0] * s;
+        v[4 * i + 3] = hi[1] * s;
+    }
+    store8(x + int64_t(row) * ldx, g * kGroup + 8 * piece, K, vec, v);
+}
+
+// ------------------------------------------------------------------ norm
+
+struct NormArgs {
+    const void *x, *r;
+    const float *w;
+    void *sum, *y;
+    uint8_t *codes, *scales;
+    int64_t ldx, ldr, lds, ldy, rows;
+    int K;
+    float eps;
+    bool vec;  // 16-byte accesses of whole pieces
+};
+
+// Sum of v over the wave, in all lanes.
+__device__ __forceinline__ double wave_sum(double v)
+{
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1)
+        v += __shfl_xor(v, m);
+    return v;
+}
+
+// 1 / sqrt(m): the hardware's estimate and two Newton steps; its own value where
+// the steps have none (m zero or infinite).
+__device__ __forceinline__ double inv_sqrt(double m)
+{
+    double r = __builtin_amdgcn_rsq(m);
+    if (m > 0.0 && m < __builtin_inf()) {
+        r = r * fma(-0.5 * m * r, r, 1.5);
+        r = r * fma(-0.5 * m * r, r, 1.5);
+    }
+    return r;
+}
+
+// h = x + r of a piece, zero past K.
+template <typename T>
+__device__ __forceinline__ void load_sum(const NormArgs &p, int64_t row, int k0, float (&h)[8])
+{
+    load8(static_cast<const T *>(p.x) + row * p.ldx, k0, p.K, p.vec, h);
+    if (p.r) {
+        float r[8];
+        load8(static_cast<const T *>(p.r) + row * p.ldr, k0, p.K, p.vec, r);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            h[i] += r[i];
+    }
+}
+
+__device__ __forceinline__ void load_weight(const NormArgs &p, int k0, float (&w)[8])
+{
+    if (p.w) {
+        load8(p.w, k0, p.K, p.vec, w);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        w[i] = 1.0f;
+}
+
+// A piece of the results.  The 16 lanes of a group come here together.
+template <typename T>
+__device__ __forceinline__ void store_normed(const NormArgs &p, int64_t row, int piece,
+                                             const float (&h)[8], double inv, int groups)
+{
+    const int k0 = 8 * piece;
+    if (p.sum)
+        store8(static_cast<T *>(p.sum) + row * p.lds, k0, p.K, p.vec, h);
+    float w[8], y[8];
+    load_weight(p, k0, w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        y[i] = k0 + i < p.K ? float(double(h[i]) * inv) * w[i] : 0.0f;
+    if (p.y)
+        store8(static_cast<T *>(p.y) + row * p.ldy, k0, p.K, p.vec, y);
+    if (p.codes)
+        pack_group(y, p.codes + row * groups * kGroup, p.scales + row * fp8_scale_bytes(p.K),
+                   piece >> 4, groups, piece & 15);
+}
+
+// A row's threads (64, 256 or 1024) hold it in registers, PIECES times eight
+// elements each, so x and r are read once.
+template <typename T, int THREADS, int PIECES>
+__global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void add_rmsnorm_kernel(NormArgs p)
+{
+    constexpr int WAVES = THREADS / 64;
+    const int tid = threadIdx.x % THREADS;
+    const int64_t row = THREADS < 256 ? int64_t(blockIdx.x) * (256 / THREADS) +
+                                            threadIdx.x / THREADS
+                                      : int64_t(blockIdx.x);
+    if (row >= p.rows)
+        return;  // whole waves: one wave per row where a workgroup has several
+    const int groups = int(fp8_groups(p.K));
+    float h[PIECES][8];
+    double ss = 0.0;
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j) {
+        load_sum<T>(p, row, 8 * (j * THREADS + tid), h[j]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            ss = fma(double(h[j][i]), double(h[j][i]), ss);
+    }
+    ss = wave_sum(ss);
+    if constexpr (WAVES > 1) {
+        __shared__ double part[WAVES];
+        if ((tid & 63) == 0)
+            part[tid >> 6] = ss;
+        __syncthreads();
+        ss = part[0];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w)
+            ss += part[w];
+    }
+    const double inv = inv_sqrt(ss / p.K + double(p.eps));
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j)
+        if (((j * THREADS + tid) >> 4) < groups)
+            store_normed<T>(p, row, j * THREADS + tid, h[j], inv, groups);
+}
+
+// Longer rows: a workgroup reads its row twice.  Writes follow the second read
+// of the same elements by the same thread, so that outputs may be the inputs.
+template <typename T>
+__global__ __launch_bounds__(1024) void add_rmsnorm_long_kernel(NormArgs p)
+{
+    __shared__ double part[16];
+    const int64_t row = blockIdx.x;
+    const int tid = threadIdx.x;
+    const int groups = int(fp8_groups(p.K));
+    const int pieces = groups * 16;
+    double ss = 0.0;
+    for (int piece = tid; piece < pieces; piece += 1024) {
+        float h[8];
+        load_sum<T>(p, row, 8 * piece, h);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            ss = fma(double(h[i]), double(h[i]), ss);
+    }
+    ss = wave_sum(ss);
+    if ((tid & 63) == 0)
+        part[tid >> 6] = ss;
+    __syncthreads();
+    ss = part[0];
+#pragma unroll
+    for (int w = 1; w < 16; ++w)
+        ss += part[w];
+    const double inv = inv_sqrt(ss / p.K + double(p.eps));
+    for (int piece = tid; piece < pieces; piece += 1024) {
+        float h[8];
+        load_sum<T>(p, row, 8 * piece, h);
+        store_normed<T>(p, row, piece, h, inv, groups);
+    }
+}
+
+// Pieces of eight elements can move as 16-byte accesses: base, and every
+// stride in elements.
+bool wide(const void *p, int64_t ld, Mx4Type t)
+{
+    return flash_tile::aligned(p, 16) && ld % (t == kMx4F32 ? 4 : 8) == 0;
+}
+
+// Groups of a call, 16 threads each, in one launch of at most 2^32 threads.
+bool group_count(const char *who, int64_t rows, int64_t groups, unsigned &total)
+{
+    constexpr int64_t most = (int64_t(1) << 28) - 16;
+    if (groups > 0 && rows > most / groups)
+        return fail(std::string(who) + ": too many elements");
+    total = unsigned(rows * groups);
+    return true;
+}
+
+// The runtime counts the threads of a launch in 32 bits.
+bool norm_grid(int64_t blocks, int threads, dim3 &grid)
+{
+    if (blocks > UINT32_MAX / threads)
+        return fail("add_rmsnorm_fp8_dev: too many rows for one launch");
+    grid = dim3(unsigned(blocks));
+    return true;
+}
+
+template <typename T, int THREADS>
+bool run_norm(const NormArgs &p, int pieces, hipStream_t st)
+{
+    constexpr int PER = THREADS < 256 ? 256 / THREADS : 1;  // rows of a workgroup
+    const dim3 block(THREADS < 256 ? 256 : THREADS);
+    dim3 grid;
+    if (!norm_grid((p.rows + PER - 1) / PER, block.x, grid))
+        return false;
+    if (pieces <= 1)
+        hipLaunchKernelGGL((add_rmsnorm_kernel<T, THREADS, 1>), grid, block, 0, st, p);
+    else if (pieces <= 2)
+        hipLaunchKernelGGL((add_rmsnorm_kernel<T, THREADS, 2>), grid, block, 0, st, p);
+    else
+        hipLaunchKernelGGL((add_rmsnorm_kernel<T, THREADS, 4>), grid, block, 0, st, p);
+    return hip_ok(hipGetLastError(), "add_rmsnorm_kernel launch");
+}
+
+template <typename T>
+bool launch_norm(const NormArgs &p, hipStream_t st)
+{
+    const auto pieces = [&](int threads) { return (p.K + 8 * threads - 1) / (8 * threads); };
+    if (pieces(64) <= 1)
+        return run_norm<T, 64>(p, pieces(64), st);
+    if (pieces(256) <= 4)
+        return run_norm<T, 256>(p, pieces(256), st);
+    if (pieces(1024) <= 4)
+        return run_norm<T, 1024>(p, pieces(1024), st);
+    dim3 grid;
+    if (!norm_grid(p.rows, 1024, grid))
+        return false;
+    hipLaunchKernelGGL(add_rmsnorm_long_kernel<T>, grid, dim3(1024), 0, st, p);
+    return hip_ok(hipGetLastError(), "add_rmsnorm_long_kernel launch");
+}
+
+}  // namespace
+
+bool launch_fp8_pack(const void *x, int64_t ldx, Mx4Type type, uint8_t *codes, uint8_t *scales,
+                     int64_t rows, int K, hipStream_t st)
+{
+    const unsigned groups = unsigned(fp8_groups(K));
+    unsigned total = 0;
+    if (!group_count("fp8_pack_dev", rows, groups, total))
+        return false;
+    if (total == 0)
+        return true;
+    const dim3 grid((total + 15) / 16), block(256);
+    const bool vec = wide(x, ldx, type);
+    if (type == kMx4F32)
+        hipLaunchKernelGGL(fp8_pack_kernel<float>, grid, block, 0, st,
+                           static_cast<const float *>(x), ldx, codes, scales, groups, total, K, vec);
+    else
+        hipLaunchKernelGGL(fp8_pack_kernel<uint16_t>, grid, block, 0, st,
+                           static_cast<const uint16_t *>(x), ldx, codes, scales, groups, total, K,
+                           vec);
+    return hip_ok(hipGetLastError(), "fp8_pack_kernel launch");
+}
+
+bool launch_fp8_unpack(const uint8_t *codes, const uint8_t *scales, void *x, int64_t ldx,
+                       Mx4Type type, int64_t rows, int K, hipStream_t st)
+{
+    const unsigned groups = unsigned(fp8_groups(K));
+    unsigned total = 0;
+    if (!group_count("fp8_unpack_dev", rows, groups, total))
+        return false;
+    if (total == 0)
+        return true;
+    const dim3 grid((total + 15) / 16), block(256);
+    const bool vec = wide(x, ldx, type);
+    if (type == kMx4F32)
+        hipLaunchKernelGGL(fp8_unpack_kernel<float>, grid, block, 0, st, codes, scales,
+                           static_cast<float *>(x), ldx, groups, total, K, vec);
+    else
+        hipLaunchKernelGGL(fp8_unpack_kernel<uint16_t>, grid, block, 0, st, codes, scales,
+                           static_cast<uint16_t *>(x), ldx, groups, total, K, vec);
+    return hip_ok(hipGetLastError(), "fp8_unpack_kernel launch");
+}
+
+bool launch_add_rmsnorm_fp8(const AddRmsNorm &a, hipStream_t st)
+{
+    if (a.rows <= 0 || a.K <= 0)
+        return true;
+    NormArgs p{};
+    p.x = a.x;
+    p.r = a.residual;
+    p.w = a.w;
+    p.sum = a.sum;
+    p.y = a.y;
+    p.codes = a.codes;
+    p.scales = a.scales;
+    p.ldx = a.ldx;
+    p.ldr = a.ldr;
+    p.lds = a.ldsum;
+    p.ldy = a.ldy;
+    p.rows = a.rows;
+    p.K = a.K;
+    p.eps = a.eps;
+    p.vec = wide(a.x, a.ldx, a.type) && (!a.residual || wide(a.residual, a.ldr, a.type)) &&
+            (!a.sum || wide(a.sum, a.ldsum, a.type)) && (!a.y || wide(a.y, a.ldy, a.type)) &&
+            (!a.w || flash_tile::aligned(a.w, 16));
+    return a.type == kMx4F32 ? launch_norm<float>(p, st) : launch_norm<uint16_t>(p, st);
+}
+
+}  // namespace anima_hip

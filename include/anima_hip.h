@@ -651,6 +651,89 @@ bool anima_hip_kv4_attention_dev(const void *q, int dtype, const int64_t *q_stri
                                  int D, int S_max, float scale, bool is_causal, void *scratch,
                                  size_t scratch_bytes, void *stream);
 
+/* ---- 8-bit rows (FP8) ----
+ * Operands of products in 8-bit floating point.  No counterpart in the
+ * reference.  Every 128 consecutive elements of a row share one scale byte s,
+ * standing for 2^(s - 127) (255: the group is NaN); an element is an e4m3 number
+ * (OCP: sign, four exponent bits with bias 7, three of mantissa; no infinity,
+ * largest 448).  A row of K elements takes ceil(K / 128) * 128 bytes of codes,
+ * zero past K, and ceil(K / 512) * 4 scale bytes, zero past its groups; rows
+ * follow one another without gaps.  Codes are 16-byte aligned, scales 4-byte
+ * aligned.  dtype of values: ANIMA_HIP_DTYPE_F32 or ANIMA_HIP_DTYPE_BF16.
+ * Nothing is allocated; all entries are asynchronous on `stream` and may be
+ * captured into a HIP graph.  A call that would take more than 2^32 threads
+ * (from 2^35 values on) is refused. */
+
+/* x [rows][ldx] (K elements of each row) to FP8 rows.  The scale is the smallest
+ * power of two by which the group's largest magnitude a is at most 448: with
+ * 2^E <= a < 2^(E+1) byte E - 8 + 127, one more where a > 1.75 * 2^E, kept
+ * within 10 .. 246; elements round to nearest, ties to even, and saturate at 448
+ * (which only the largest scale lets them reach).  Every value is zero or a
+ * normal bf16 number.  A group that holds an infinity or a NaN gets scale 255
+ * and zero codes. */
+bool anima_hip_fp8_pack_dev(const void *x, int64_t ldx, int dtype, uint8_t *codes, uint8_t *scales,
+                            int64_t rows, int K, void *stream);
+/* The values of FP8 rows as the packer writes them, each exact in either type;
+ * other scale bytes stand for their power of two, and values past f32 are infinite. */
+bool anima_hip_fp8_unpack_dev(const uint8_t *codes, const uint8_t *scales, void *x, int64_t ldx,
+                              int dtype, int64_t rows, int K, void *stream);
+
+/* Root-mean-square norm over rows of K elements, with the residual's addition:
+ *   h = x + residual,  sum = h,  y = h / sqrt(mean(h^2) + eps) * w,
+ * and y as FP8 rows.  x, residual, sum and y are of `dtype`, rows ldx, ldr,
+ * ldsum and ldy elements apart; w is f32 [K].  residual, w (NULL: 1), sum, y, and
+ * codes with scales may each be NULL; one output at least is given.  h is
+ * taken in f32 (sum is its rounding, and the norm is of h itself), the sum of
+ * squares and its root in 64 bits, so that no h is too large or too small for
+ * them; each output is rounded once.  An infinity in a row makes its own element
+ * NaN and the others 0.  sum and y may be x or residual themselves (at the same
+ * stride), not each other. */
+bool anima_hip_add_rmsnorm_fp8_dev(const void *x, int64_t ldx, const void *residual, int64_t ldr,
+                                   const float *w, float eps, int dtype, void *sum, int64_t ldsum,
+                                   void *y, int64_t ldy, uint8_t *codes, uint8_t *scales,
+                                   int64_t rows, int K, void *stream);
+
+/* C[M,N] = A[M,K] . W[N,K]^T, A and W in FP8 rows of K elements, C of `dtype`,
+ * rows ldc elements apart: anima_hip_linear_dev with both operands in 8 bits.
+ * C in f32: products are exact and sums f32.  C in bf16: on the fp8 MFMA, whose
+ * adder cuts the products of eight neighbouring elements off at 2^-13 of the
+ * power of two of the largest of them and adds the eights in f32 (below
+ * 7 * 2^-13 of that product in each eight, about 1.5e-5 of the result on normal
+ * values), rounded to bf16 once.  Products of scales below 2^-149 count as zero.
+ * scratch: anima_hip_linear_fp8_scratch_bytes(M, N, K, dtype) bytes, 16-byte
+ * aligned (0: none needed), for the partial sums of a product split over K,
+ * added in a fixed order; calls that overlap in time need scratch of their own. */
+size_t anima_hip_linear_fp8_scratch_bytes(int M, int N, int K, int dtype);
+bool anima_hip_linear_fp8_dev(const uint8_t *a_codes, const uint8_t *a_scales,
+                              const uint8_t *w_codes, const uint8_t *w_scales, void *c, int64_t ldc,
+                              int M, int N, int K, int dtype, void *scratch, size_t scratch_bytes,
+                              void *stream);
+
+/* Rotary positions with several axes: q [B, H_q, S, D] and k [B, H_k, S, D] of
+ * `dtype` turned by their tokens' positions into q_out and k_out, all views
+ * through {batch, head, token} strides (NULL: contiguous).  Either of q and k may
+ * have no heads.  Pair p < pairs of a row, elements (p, p + pairs) or,
+ * interleaved, (2p, 2p + 1), turns by positions[axis] * freqs[p] with axis =
+ * pair_axis[p]: (a, b) -> (a cos - b sin, b cos + a sin); inverse: by the
+ * negative angle, which undoes the turn and takes gradients back through it.
+ * Elements from 2 * pairs on are copied.  This is the rotation of
+ * anima_hip_qk_prologue_dev (anima_rt/include/cpu/rope_kernel.h:65-97) with
+ * positions in place of a table.  positions: int32 [B][S][axes] on the device,
+ * batch entries pos_batch_stride elements apart (0: one for all); freqs: radians
+ * per position, f64 [pairs] on the device; pair_axis: uint8 [pairs] on the device
+ * (values from axes on count as the last axis), or NULL for axis 0.  counts: int32
+ * [B] on the device, tokens of each sequence, or NULL for S; rows of tokens from
+ * counts[b] on are not written.  Angles are taken in 64 bits, the turn in f32, and
+ * outputs rounded once.  An output may be its own input (same strides); other
+ * overlaps are not allowed.  D at most 1024, heads at most 2048 each. */
+bool anima_hip_rope_axes_dev(const void *q, const int64_t *q_strides, void *q_out,
+                             const int64_t *qo_strides, int H_q, const void *k,
+                             const int64_t *k_strides, void *k_out, const int64_t *ko_strides,
+                             int H_k, const int32_t *positions, int64_t pos_batch_stride,
+                             const int32_t *counts, const double *freqs, const uint8_t *pair_axis,
+                             int axes, int pairs, int B, int S, int D, int dtype, bool interleaved,
+                             bool inverse, void *stream);
+
 /* Timing hook: device time of the last completed host-pointer call (the
  * anima_rt_run_* drop-ins, anima_hip_sdpa, anima_hip_attention,
  * anima_hip_cross_attention), from HIP events on the library's streams:
