@@ -56,6 +56,16 @@ __device__ __forceinline__ void dma16s(const void *base, unsigned voff, u16 *lds
                  : "s"(m0), "v"(voff), "s"(base)
                  : "memory", "m0");
 }
+// One dword per lane to the 256-byte LDS window at `lds`, addressed the same way.
+__device__ __forceinline__ void dma4s(const void *base, unsigned voff, u16 *lds)
+{
+    const unsigned m0 = static_cast<unsigned>(
+        reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void *)lds));
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2"
+                 :
+                 : "s"(m0), "v"(voff), "s"(base)
+                 : "memory", "m0");
+}
 #pragma clang diagnostic pop
 
 // s_waitcnt vmcnt(N) (expcnt and lgkmcnt unconstrained).

@@ -521,21 +521,6 @@ struct Staged {
     static_assert((S - 2) * OPS < 16, "counted by vmcnt");
 };
 
-// One dword per lane from base + voff to the 256-byte LDS window at `lds`, as
-// flash_tile::dma16s copies 16 bytes.
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-__device__ __forceinline__ void dma4s(const void *base, unsigned voff, u16 *lds)
-{
-    const unsigned m0 = static_cast<unsigned>(
-        reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void *)lds));
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2"
-                 :
-                 : "s"(m0), "v"(voff), "s"(base)
-                 : "memory", "m0");
-}
-#pragma clang diagnostic pop
-
 template <typename T, int MB, int NB, int WM, int WN, int KS, int S, int CM>
 __global__ __launch_bounds__(WM *WN *KS * 64) void linear_staged_kernel(LinArgs p)
 {
