@@ -14,6 +14,7 @@
 #include "fp8_plan.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace anima_hip {
 namespace {
@@ -27,7 +28,6 @@ using flash_tile::f32x16;
 using flash_tile::mfma_bf16;
 using flash_tile::ring_barrier;
 using flash_tile::u16;
-using flash_tile::wait_vmcnt;
 using flash_tile::xcd_major_block;
 
 struct LinArgs {
@@ -42,6 +42,18 @@ struct LinArgs {
 __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c)
 {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// Waits until the fp8 MFMAs before it have written their results.  The compiler's
+// own wait before a vector instruction reads them is that of shorter MFMAs (a
+// 32x32x64 product of fp8 takes 16 passes, and it waits for 8: the last registers were
+// read before they were written), so every reader comes behind one of these, 32 wait
+// states, in the block of the MFMAs.
+__device__ __forceinline__ void mfma_drain()
+{
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
 }
 
 // Eight codes as bf16, times their scale.
@@ -165,6 +177,8 @@ __global__ __launch_bounds__(WAVES * 64) void fp8_few_kernel(LinArgs p)
             load(grp + WAVES, next);
         multiply(cur);
         cur = next;
+        if constexpr (!EXACT)
+            mfma_drain();
     }
     if constexpr (WAVES > 1) {
         // The waves' sums in wave order.
@@ -200,51 +214,56 @@ __global__ __launch_bounds__(WAVES * 64) void fp8_few_kernel(LinArgs p)
 // LDS at the end).  C^T on 32x32 MFMAs, W the first operand, so that a lane's four
 // consecutive accumulators are four columns of one row.
 //
-// Rows of both operands, 128 CM bytes at a time, and the dwords of their scales reach
-// LDS by DMA through S stages; 16-byte pieces are placed by piece ^ swizzle(row) against
-// bank conflicts.  Fragments of a step are read while the MFMAs of the step before run; a
-// chunk's first ones under the last step of the chunk before, behind the barrier that
-// ends it.
-template <typename T, int MB, int NB, int WM, int WN, int KS, int S, int CM>
+// Rows of both operands reach LDS by DMA, KC bytes at a time through S stages; 16-byte
+// pieces are placed by piece ^ swizzle(row) against bank conflicts.  Their scales
+// come once for a section of SEC groups: a dword per row and chunk costs as many requests as the
+// rows themselves.  Fragments of a step are read while the MFMAs of the step before
+// run; a chunk's first ones under the last step of the chunk before, behind the barrier
+// that ends it.
+template <typename T, int MB, int NB, int WM, int WN, int KS, int S, int KC, int SEC>
 struct Staged {
     static constexpr int WAVES = WM * WN * KS, THREADS = WAVES * 64;
     static constexpr int BM = 32 * MB * WM, BN = 32 * NB * WN;
-    static constexpr int KC = 128 * CM;  // bytes of a row in a chunk
     static constexpr int STEP = sizeof(T) == 4 ? 32 : 64;  // elements of K
     static constexpr int STEPS = KC / STEP, SHARE = STEPS / KS;
-    // LDS in bytes: A, W, a dword of scales for each row of both.
-    static constexpr int A_BY = BM * KC, W_BY = BN * KC;
-    static constexpr int AS_WIN = (BM + 63) / 64, WS_WIN = (BN + 63) / 64;
-    static constexpr int STAGE = A_BY + W_BY + (AS_WIN + WS_WIN) * 256;
-    // 1 KiB windows (scales: 256 bytes) per chunk, and per wave; a wave without
-    // one copies the last again, so that all count the same.
-    static constexpr int A_WIN = A_BY / 1024, W_WIN = W_BY / 1024, S_WIN = AS_WIN + WS_WIN;
-    static constexpr int A_OPS = (A_WIN + WAVES - 1) / WAVES;
-    static constexpr int W_OPS = (W_WIN + WAVES - 1) / WAVES;
-    static constexpr int S_OPS = (S_WIN + WAVES - 1) / WAVES;
-    static constexpr int OPS = A_OPS + W_OPS + S_OPS;
+    // LDS in bytes: S stages of A and W, then scales: rows of both by 16 groups, SEC / 16
+    // times.
+    static constexpr int A_BY = BM * KC, STAGE = A_BY + BN * KC;
+    static constexpr int ROWS = BM + BN, SCALES = S * STAGE;
+    // 1 KiB windows per chunk, and per wave; a wave without one copies the last again,
+    // so that all count the same.
+    static constexpr int A_WIN = A_BY / 1024, WIN = STAGE / 1024;
+    static constexpr int OPS = (WIN + WAVES - 1) / WAVES;
     // The epilogue's rows of one 32-row block per wave, and the shares' sums.
     static constexpr int PITCH = 32 * NB + 16 / int(sizeof(T));
     static constexpr int OUT_BY = WAVES / KS * 32 * PITCH * int(sizeof(T));
     static constexpr int RED_BY = (KS - 1) * (WAVES / KS) * MB * NB * 4096;
     static constexpr int MAX2 = RED_BY > OUT_BY ? RED_BY : OUT_BY;
-    static constexpr int LDS = S * STAGE > MAX2 ? S * STAGE : MAX2;
-    static_assert(STEPS % KS == 0 && LDS <= 163840, "160 KiB of LDS");
-    static_assert(S >= 2 && (S - 2) * OPS < 16, "counted by vmcnt");
+    static constexpr int USED = SCALES + ROWS * SEC;
+    static constexpr int LDS = USED > MAX2 ? USED : MAX2;
+    static_assert(STEPS % KS == 0 && SEC % 16 == 0 && LDS <= 163840, "160 KiB of LDS");
+    static_assert(S >= 2 && (S - 2) * OPS < 64, "counted by vmcnt");
 };
 
-// Place of piece `i` of a staged row, so that the 16 rows of a ds_read_b128 quarter
+// Place of a piece of a staged row, so that the 16 rows of a ds_read_b128 quarter
 // touch distinct banks.
-template <int CM>
+template <int KC>
 __device__ __forceinline__ int swizzle(int row)
 {
-    return CM == 1 ? (row & 7) ^ (row >> 3 & 1) : row & 15;
+    return KC == 128 ? (row & 7) ^ (row >> 3 & 1) : row & 15;
 }
 
-template <typename T, int MB, int NB, int WM, int WN, int KS, int S, int CM>
+// s_waitcnt vmcnt(N), N < 64.
+template <int N>
+__device__ __forceinline__ void wait_copies()
+{
+    __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | (N >> 4) << 14);
+}
+
+template <typename T, int MB, int NB, int WM, int WN, int KS, int S, int KC, int SEC>
 __global__ __launch_bounds__(WM *WN *KS * 64) void fp8_staged_kernel(LinArgs p)
 {
-    using G = Staged<T, MB, NB, WM, WN, KS, S, CM>;
+    using G = Staged<T, MB, NB, WM, WN, KS, S, KC, SEC>;
     constexpr bool EXACT = sizeof(T) == 4;
     __shared__ __attribute__((aligned(16))) uint8_t smem[G::LDS];
 
@@ -261,56 +280,52 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void fp8_staged_kernel(LinArgs p)
     const int bm = min(4, p.tiles_m - 4 * band);
     const int tn = in_band / bm, tm = 4 * band + in_band - tn * bm;
     const int row0 = tm * G::BM, col0 = tn * G::BN;
-    // Chunks of this split.
-    const int c0 = split * (p.per_split / CM), c1 = min(c0 + p.per_split / CM, p.groups / CM);
+    const int g0 = split * p.per_split, g1 = min(g0 + p.per_split, p.groups);
 
     // This lane's part of each copy, in bytes from the tile's first row; rows past
     // M or N read the last one again (their results are not stored).
-    constexpr int ROWS = 8 / CM, PIECES = 8 * CM;  // of a window, of a row
+    constexpr int WROWS = 1024 / KC, PIECES = KC / 16;  // of a window, of a row
     const int64_t pitch = int64_t(p.groups) * kGroup;
-    unsigned aoff[G::A_OPS], woff[G::W_OPS], soff[G::S_OPS];
-    int adst[G::A_OPS], wdst[G::W_OPS], sdst[G::S_OPS];
-    bool swin[G::S_OPS];  // scales of W
+    const uint8_t *const a0 = p.a + row0 * pitch, *const w0 = p.w + col0 * pitch;
+    unsigned doff[G::OPS];
+    int ddst[G::OPS];
+    bool dw[G::OPS];
 #pragma unroll
-    for (int i = 0; i < G::A_OPS; ++i) {
-        const int w = min(i * G::WAVES + wave, G::A_WIN - 1);
-        const int r = w * ROWS + lane / PIECES;
-        aoff[i] = unsigned((min(row0 + r, p.M - 1) - row0) * pitch +
-                           16 * (lane % PIECES ^ swizzle<CM>(r)));
-        adst[i] = w * 1024;
+    for (int i = 0; i < G::OPS; ++i) {
+        const int w = min(i * G::WAVES + wave, G::WIN - 1);
+        dw[i] = w >= G::A_WIN;
+        const int r = (dw[i] ? w - G::A_WIN : w) * WROWS + lane / PIECES;
+        const int at = dw[i] ? min(col0 + r, p.N - 1) - col0 : min(row0 + r, p.M - 1) - row0;
+        doff[i] = unsigned(at * pitch + 16 * (lane % PIECES ^ swizzle<KC>(r)));
+        ddst[i] = w * 1024;
     }
+    // Part i of `parts` of chunk c's copies.
+    auto copies = [&](int c, unsigned stage, int i, int parts) {
 #pragma unroll
-    for (int i = 0; i < G::W_OPS; ++i) {
-        const int w = min(i * G::WAVES + wave, G::W_WIN - 1);
-        const int r = w * ROWS + lane / PIECES;
-        woff[i] = unsigned((min(col0 + r, p.N - 1) - col0) * pitch +
-                           16 * (lane % PIECES ^ swizzle<CM>(r)));
-        wdst[i] = G::A_BY + w * 1024;
-    }
+        for (int k = G::OPS * i / parts; k < G::OPS * (i + 1) / parts; ++k)
+            dma16s((dw[k] ? w0 : a0) + int64_t(c) * KC, doff[k],
+                   reinterpret_cast<u16 *>(smem + stage + ddst[k]));
+    };
+    // The scales of groups g .. ge - 1, g a multiple of 16: windows of 16 rows by four
+    // dwords, past a row's end its last one again.
+    auto scales = [&](int g, int ge) {
+        for (int sub = 0; g + 16 * sub < ge; ++sub)
 #pragma unroll
-    for (int i = 0; i < G::S_OPS; ++i) {
-        const int w = min(i * G::WAVES + wave, G::S_WIN - 1);
-        swin[i] = w >= G::AS_WIN;
-        const int r = (swin[i] ? w - G::AS_WIN : w) * 64 + lane;
-        soff[i] = unsigned((swin[i] ? min(col0 + r, p.N - 1) - col0 : min(row0 + r, p.M - 1) - row0) *
-                           p.sg);
-        sdst[i] = G::A_BY + G::W_BY + w * 256;
-    }
-    const uint8_t *a0 = p.a + row0 * pitch, *w0 = p.w + col0 * pitch;
-    const uint8_t *as0 = p.as + int64_t(row0) * p.sg, *ws0 = p.ws + int64_t(col0) * p.sg;
-    auto dma = [&](int c, int stage) {
-        uint8_t *dst = smem + stage * G::STAGE;
-#pragma unroll
-        for (int i = 0; i < G::A_OPS; ++i)
-            dma16s(a0 + int64_t(c) * G::KC, aoff[i], reinterpret_cast<u16 *>(dst + adst[i]));
-#pragma unroll
-        for (int i = 0; i < G::W_OPS; ++i)
-            dma16s(w0 + int64_t(c) * G::KC, woff[i], reinterpret_cast<u16 *>(dst + wdst[i]));
-        // The scales of the four groups that the chunk is among.
-#pragma unroll
-        for (int i = 0; i < G::S_OPS; ++i)
-            dma4s((swin[i] ? ws0 : as0) + (c * CM & ~3), soff[i],
-                  reinterpret_cast<u16 *>(dst + sdst[i]));
+            for (int i = 0; i < (G::ROWS / 16 + G::WAVES - 1) / G::WAVES; ++i) {
+                const int w = i * G::WAVES + wave;
+                if (w * 16 >= G::ROWS)
+                    continue;
+                const bool is_w = w * 16 >= G::BM;
+                const int r = w * 16 + lane / 4 - (is_w ? G::BM : 0);
+                const int at = is_w ? min(col0 + r, p.N - 1) - col0
+                                    : min(row0 + r, p.M - 1) - row0;
+                const unsigned off = unsigned(at * p.sg + min(g + 16 * sub + lane % 4 * 4, p.sg - 4));
+                dma4s(is_w ? p.ws + int64_t(col0) * p.sg : p.as + int64_t(row0) * p.sg, off,
+                      reinterpret_cast<u16 *>(smem + G::SCALES + (sub * G::ROWS + w * 16) * 16));
+            }
+    };
+    auto after = [&](unsigned stage) {
+        return stage == (S - 1) * G::STAGE ? 0u : stage + G::STAGE;
     };
 
     f32x16 acc[MB][NB];
@@ -324,44 +339,71 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void fp8_staged_kernel(LinArgs p)
 
     unsigned sa[MB], sw[NB];  // scales of a chunk from its first group's on
     unsigned ao = 0, wo = 0;  // rows (wm MB) 32 + col and (wn NB) 32 + col of a chunk
-    // Chunk c's scales go to na and nw.
+    unsigned stage = 0, fill = 0;  // of the chunk in work, and to copy to
+    int first = 0;                 // group of the section's first chunk
+    constexpr int CG = KC / kGroup;  // groups of a chunk
+    // Chunk c is there, at `stage`, and its scales in na and nw; `fill` is free.
     auto enter = [&](int c, unsigned (&na)[MB], unsigned (&nw)[NB]) {
-        // Chunk c has landed when at most the S - 2 behind it are on their way.
-        if (c + S - 2 < c1)
-            wait_vmcnt<(S - 2) * G::OPS>();
-        else
-            wait_vmcnt<0>();
         ring_barrier();  // for every wave; and all have left the stage before it
-        if (c + S - 1 < c1)
-            dma(c + S - 1, (c + S - 1 - c0) % S);
-        const unsigned base = (c - c0) % S * G::STAGE;
-        ao = base + (wm * 32 * MB + col) * G::KC;
-        wo = base + G::A_BY + (wn * 32 * NB + col) * G::KC;
+        ao = stage + (wm * 32 * MB + col) * KC;
+        wo = stage + G::A_BY + (wn * 32 * NB + col) * KC;
         asm volatile("" : "+v"(ao), "+v"(wo));
-        const unsigned *s = reinterpret_cast<const unsigned *>(smem + base + G::A_BY + G::W_BY);
-        const int shift = c * CM % 4 * 8;
+        const int g = c * CG - first, shift = g % 4 * 8;
+        const uint8_t *s = smem + G::SCALES + g / 16 * (G::ROWS * 16) + (g % 16 & ~3) + col * 16;
 #pragma unroll
         for (int i = 0; i < MB; ++i)
-            na[i] = s[(wm * MB + i) * 32 + col] >> shift;
+            na[i] = *reinterpret_cast<const unsigned *>(s + (wm * MB + i) * 512) >> shift;
 #pragma unroll
         for (int j = 0; j < NB; ++j)
-            nw[j] = s[G::AS_WIN * 64 + (wn * NB + j) * 32 + col] >> shift;
+            nw[j] = *reinterpret_cast<const unsigned *>(s + G::BM * 16 + (wn * NB + j) * 512) >>
+                    shift;
     };
     // 16 bytes of row col of block b; the swizzle depends on col alone.
     auto piece = [&](unsigned row, int b, int i) {
-        return *reinterpret_cast<const u32x4 *>(smem + row + 32 * b * G::KC +
-                                                16 * (i ^ swizzle<CM>(col)));
+        return *reinterpret_cast<const u32x4 *>(smem + row + 32 * b * KC +
+                                                16 * (i ^ swizzle<KC>(col)));
     };
     // This wave's steps of a chunk: share * SHARE .. .
     auto step_of = [&](int i) { return KS == 1 ? i : share * G::SHARE + i; };
     constexpr int LAST = G::SHARE - 1;
-    if (c0 < c1) {
+    // What a chunk is followed by: another and copies to make, another, nothing.
+    using Copy = std::integral_constant<int, 2>;
+    using More = std::integral_constant<int, 1>;
+    using Last = std::integral_constant<int, 0>;
+
+    // The chunks c0 .. c1 - 1 of a section: chunk c by work(c, what follows).
+    auto section = [&](int c0, int c1, auto &&begin, auto &&work) {
+        first = c0 * CG & ~15;
+        scales(first, c1 * CG);
 #pragma unroll
         for (int i = 0; i < S - 1; ++i)
             if (c0 + i < c1)
-                dma(c0 + i, i);
+                copies(c0 + i, i * G::STAGE, 0, 1);
+        stage = 0;
+        fill = (S - 1) * G::STAGE;
+        if (c0 + S - 1 < c1)
+            wait_copies<(S - 2) * G::OPS>();
+        else
+            wait_copies<0>();
         enter(c0, sa, sw);
-    }
+        if (c0 + S - 1 < c1)
+            copies(c0 + S - 1, fill, 0, 1);
+        begin();
+        int c = c0;
+        for (; c + S < c1; ++c)
+            work(c, Copy{});
+        for (; c + 1 < c1; ++c)
+            work(c, More{});
+        work(c, Last{});
+    };
+    // To the next chunk, c.
+    auto turn = [&](int c, auto follows, unsigned (&na)[MB], unsigned (&nw)[NB]) {
+        // It has landed when at most the S - 2 behind it are on their way.
+        wait_copies<decltype(follows)::value == 2 ? (S - 2) * G::OPS : 0>();
+        stage = after(stage);
+        fill = after(fill);
+        enter(c, na, nw);
+    };
 
     if constexpr (EXACT) {
         // A step is 32 elements: 16 of each half, two bf16 MFMAs.  A fragment's
@@ -372,64 +414,66 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void fp8_staged_kernel(LinArgs p)
             v[0] = decode8(x[0], x[1], f);
             v[1] = decode8(x[2], x[3], f);
         };
-        if (c0 < c1) {
+        auto begin = [&]() {
 #pragma unroll
             for (int j = 0; j < NB; ++j)
                 rw[j] = piece(wo, j, 2 * step_of(0) + half);
 #pragma unroll
             for (int i = 0; i < MB; ++i)
                 ra[i] = piece(ao, i, 2 * step_of(0) + half);
-        }
-        for (int c = c0; c < c1; ++c) {
+        };
+        auto work = [&](int c, auto follows) {
+            constexpr int FOLLOWS = decltype(follows)::value;
 #pragma unroll
             for (int st = 0; st < G::SHARE; ++st) {
                 const int byte = step_of(st) / 4 * 8;  // of the step's group
                 const int next = step_of(st < LAST ? st + 1 : 0);
-                bf16x8 wv[NB][2];
+                const bool last = st == LAST;
+                bf16x8 wv[NB][2], av[MB][2];
 #pragma unroll
                 for (int j = 0; j < NB; ++j)
                     decode2(rw[j], sw[j] >> byte, wv[j]);
-                if (st < LAST) {
+                if (last) {
+                    // Decoded whole, so that the next chunk's first fragments can come in
+                    // under the products.
+#pragma unroll
+                    for (int i = 0; i < MB; ++i)
+                        decode2(ra[i], sa[i] >> byte, av[i]);
+                    if constexpr (FOLLOWS > 0)
+                        turn(c + 1, follows, sa, sw);
+                }
+                if (!last || FOLLOWS > 0) {
 #pragma unroll
                     for (int j = 0; j < NB; ++j)
                         rw[j] = piece(wo, j, 2 * next + half);
+                    if (last)
 #pragma unroll
-                    for (int i = 0; i < MB; ++i) {
-                        bf16x8 av[2];
-                        decode2(ra[i], sa[i] >> byte, av);
-                        ra[i] = piece(ao, i, 2 * next + half);
-#pragma unroll
-                        for (int q = 0; q < 2; ++q)
-#pragma unroll
-                            for (int j = 0; j < NB; ++j)
-                                acc[i][j] = mfma_bf16(wv[j][q], av[q], acc[i][j]);
-                    }
-                    continue;
+                        for (int i = 0; i < MB; ++i)
+                            ra[i] = piece(ao, i, 2 * next + half);
                 }
-                // The chunk's last step is decoded whole, so that the next chunk's first
-                // fragments can come in under its products (past the last chunk: its own
-                // first ones again, which nothing uses).
-                bf16x8 av[MB][2];
-#pragma unroll
-                for (int i = 0; i < MB; ++i)
-                    decode2(ra[i], sa[i] >> byte, av[i]);
-                if (c + 1 < c1)
-                    enter(c + 1, sa, sw);
-#pragma unroll
-                for (int j = 0; j < NB; ++j)
-                    rw[j] = piece(wo, j, 2 * next + half);
-#pragma unroll
-                for (int i = 0; i < MB; ++i)
-                    ra[i] = piece(ao, i, 2 * next + half);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int i = 0; i < MB; ++i)
+                for (int i = 0; i < MB; ++i) {
+                    if (!last) {
+                        decode2(ra[i], sa[i] >> byte, av[i]);
+                        ra[i] = piece(ao, i, 2 * next + half);
+                    }
 #pragma unroll
                     for (int q = 0; q < 2; ++q)
 #pragma unroll
                         for (int j = 0; j < NB; ++j)
                             acc[i][j] = mfma_bf16(wv[j][q], av[i][q], acc[i][j]);
+                    if (last && FOLLOWS == 2) {
+                        copies(c + S, fill, i, MB);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
             }
+        };
+        for (int g = g0; g < g1; g += SEC - g % 16) {
+            if (g > g0)
+                __syncthreads();
+            section(g / CG, min(g1, g + SEC - g % 16) / CG, begin, work);
         }
     } else {
         // A step is 64 elements, 32 of each half, one fp8 MFMA.  The fragments of W
@@ -444,40 +488,44 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void fp8_staged_kernel(LinArgs p)
             return __builtin_bit_cast(i32x8,
                                       __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
         };
-        if (c0 < c1) {
+        auto begin = [&]() {
 #pragma unroll
             for (int j = 0; j < NB; ++j)
                 fw[0][j] = read(wo, j, step_of(0));
 #pragma unroll
             for (int i = 0; i < MB; ++i)
                 fa[0][i] = read(ao, i, step_of(0));
-        }
-        for (int c = c0; c < c1; ++c) {
+        };
+        auto work = [&](int c, auto follows) {
+            constexpr int FOLLOWS = decltype(follows)::value;
+            unsigned na[MB], nw[NB];
 #pragma unroll
             for (int st = 0; st < G::SHARE; ++st) {
                 const int now = G::SHARE == 1 ? 0 : st & 1, nxt = now ^ 1;
                 const int na_set = ONE ? 0 : nxt, a_set = ONE ? 0 : now;
                 const int byte = step_of(st) / 2 * 8;  // of the step's group
                 const int next = step_of(st < LAST ? st + 1 : 0);
-                // Past the last chunk: its own first step again, which nothing uses.
-                unsigned na[MB], nw[NB];
+                const bool last = st == LAST, go = !last || FOLLOWS > 0;
+                // What the next step's fragments need: with more than one block of rows it
+                // runs under the products of the first.
+                auto ahead = [&]() {
+                    if constexpr (FOLLOWS > 0)
+                        if (last)
+                            turn(c + 1, follows, na, nw);
+                    if (go) {
 #pragma unroll
-                for (int i = 0; i < MB; ++i)
-                    na[i] = sa[i];
+                        for (int j = 0; j < NB; ++j)
+                            fw[nxt][j] = read(wo, j, next);
+                        if constexpr (!ONE) {
 #pragma unroll
-                for (int j = 0; j < NB; ++j)
-                    nw[j] = sw[j];
-                if (st == LAST && c + 1 < c1)
-                    enter(c + 1, na, nw);
-#pragma unroll
-                for (int j = 0; j < NB; ++j)
-                    fw[nxt][j] = read(wo, j, next);
-                if constexpr (!ONE) {
-#pragma unroll
-                    for (int i = 0; i < MB; ++i)
-                        fa[na_set][i] = read(ao, i, next);
-                }
-                __builtin_amdgcn_sched_barrier(0);
+                            for (int i = 0; i < MB; ++i)
+                                fa[na_set][i] = read(ao, i, next);
+                        }
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                };
+                if constexpr (MB == 1)
+                    ahead();
 #pragma unroll
                 for (int i = 0; i < MB; ++i) {
 #pragma unroll
@@ -485,30 +533,42 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void fp8_staged_kernel(LinArgs p)
                         acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
                             fw[now][j], fa[a_set][i], acc[i][j], 0, 0, 0, int(sw[j] >> byte), 0,
                             int(sa[i] >> byte));
-                    if constexpr (ONE) {
-                        fa[0][i] = read(ao, i, next);
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (MB > 1 && i == 0)
+                        ahead();
+                    if (last && FOLLOWS == 2)
+                        copies(c + S, fill, i, MB);
+                    if constexpr (ONE)
+                        if (go)
+                            fa[0][i] = read(ao, i, next);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-                if (st == LAST) {
+            }
+            if constexpr (FOLLOWS == 0)
+                mfma_drain();
+            else {
 #pragma unroll
-                    for (int i = 0; i < MB; ++i)
-                        sa[i] = na[i];
+                for (int i = 0; i < MB; ++i)
+                    sa[i] = na[i];
+#pragma unroll
+                for (int j = 0; j < NB; ++j)
+                    sw[j] = nw[j];
+                if constexpr (G::SHARE % 2 == 1) {
 #pragma unroll
                     for (int j = 0; j < NB; ++j)
-                        sw[j] = nw[j];
-                }
-                if (G::SHARE % 2 == 1 && st == LAST) {
-#pragma unroll
-                    for (int j = 0; j < NB; ++j)
-                        fw[0][j] = fw[nxt][j];
+                        fw[0][j] = fw[1][j];
                     if constexpr (!ONE) {
 #pragma unroll
                         for (int i = 0; i < MB; ++i)
-                            fa[0][i] = fa[na_set][i];
+                            fa[0][i] = fa[1][i];
                     }
                 }
             }
+        };
+        for (int g = g0; g < g1; g += SEC - g % 16) {
+            if (g > g0)
+                __syncthreads();
+            section(g / CG, min(g1, g + SEC - g % 16) / CG, begin, work);
         }
     }
 
@@ -642,34 +702,36 @@ __global__ __launch_bounds__(256) void fp8_sum_kernel(const float *part, T *c, i
 
 // Shapes of the staged kernel, MB, NB, WM, WN, KS, S, and of the same with two groups
 // at once.
-#define STAGED_BF16(X, cm) \
-    X(cm, 0, 4, 4, 2, 2, 1, 2) X(cm, 1, 3, 4, 2, 2, 1, 2) X(cm, 2, 2, 4, 2, 2, 1, 3) \
-    X(cm, 3, 2, 2, 2, 2, 1, 3) X(cm, 4, 1, 2, 2, 2, 1, 3) X(cm, 5, 1, 1, 2, 2, 1, 4) \
-    X(cm, 6, 1, 1, 1, 2, 2, 4)
-#define PAIRED_BF16(X, cm) \
-    X(cm, 4, 1, 2, 2, 2, 2, 2) X(cm, 5, 1, 1, 2, 2, 2, 3) X(cm, 6, 1, 1, 1, 2, 4, 3)
-#define STAGED_F32(X, cm) \
-    X(cm, 0, 2, 4, 4, 2, 1, 2) X(cm, 1, 1, 4, 4, 2, 1, 3) X(cm, 2, 2, 2, 2, 2, 1, 3) \
-    X(cm, 3, 1, 2, 2, 2, 1, 3) X(cm, 4, 1, 1, 2, 2, 1, 4) X(cm, 5, 1, 1, 1, 2, 2, 4)
-#define PAIRED_F32(X, cm) \
-    X(cm, 3, 1, 2, 2, 2, 2, 2) X(cm, 4, 1, 1, 2, 2, 2, 3) X(cm, 5, 1, 1, 1, 2, 4, 3)
+#define STAGED_BF16(X) \
+    X(0, 4, 4, 2, 2, 1, 2, 128, 64) X(1, 3, 2, 2, 4, 1, 2, 128, 64) X(2, 2, 4, 2, 2, 1, 3, 128, 32) \
+    X(3, 2, 2, 2, 2, 1, 3, 128, 32) X(4, 1, 2, 2, 2, 1, 3, 128, 16) X(5, 1, 1, 2, 2, 1, 4, 128, 32) \
+    X(6, 1, 1, 1, 2, 2, 4, 128, 32)
+#define PAIRED_BF16(X) \
+    X(4, 1, 2, 2, 2, 2, 2, 256, 32) X(5, 1, 1, 2, 2, 2, 3, 256, 32) X(6, 1, 1, 1, 2, 4, 3, 256, 32)
+#define STAGED_F32(X) \
+    X(0, 2, 4, 4, 2, 1, 2, 128, 64) X(1, 1, 4, 4, 2, 1, 3, 128, 32) X(2, 2, 2, 2, 2, 1, 3, 128, 32) \
+    X(3, 1, 2, 2, 2, 1, 3, 128, 16) X(4, 1, 1, 2, 2, 1, 4, 128, 32) X(5, 1, 1, 1, 2, 2, 4, 128, 32)
+#define PAIRED_F32(X) \
+    X(3, 1, 2, 2, 2, 2, 2, 256, 32) X(4, 1, 1, 2, 2, 2, 3, 256, 32) X(5, 1, 1, 1, 2, 4, 3, 256, 32)
 
-#define SHAPE_CHECK(table, i, mb, nb, wm, wn, cm) \
+#define SHAPE_CHECK(table, i, mb, nb, wm, wn, kc) \
     static_assert(table[i].bm == 32 * mb * wm && table[i].bn == 32 * nb * wn && \
-                  (cm == 1 || table[i].pairs), "shape table");
-#define CHECK_BF16(cm, i, mb, nb, wm, wn, ks, s) SHAPE_CHECK(kBf16Shapes, i, mb, nb, wm, wn, cm)
-#define CHECK_F32(cm, i, mb, nb, wm, wn, ks, s) SHAPE_CHECK(kF32Shapes, i, mb, nb, wm, wn, cm)
-STAGED_BF16(CHECK_BF16, 1)
-PAIRED_BF16(CHECK_BF16, 2)
-STAGED_F32(CHECK_F32, 1)
-PAIRED_F32(CHECK_F32, 2)
+                  (kc == 128 || table[i].pairs), "shape table");
+#define CHECK_BF16(i, mb, nb, wm, wn, ks, s, kc, sec) \
+    SHAPE_CHECK(kBf16Shapes, i, mb, nb, wm, wn, kc)
+#define CHECK_F32(i, mb, nb, wm, wn, ks, s, kc, sec) \
+    SHAPE_CHECK(kF32Shapes, i, mb, nb, wm, wn, kc)
+STAGED_BF16(CHECK_BF16)
+PAIRED_BF16(CHECK_BF16)
+STAGED_F32(CHECK_F32)
+PAIRED_F32(CHECK_F32)
 
 constexpr int kPairs = 16;  // beside a shape's number: two groups at once
-#define STAGED_CASE(cm, i, mb, nb, wm, wn, ks, s)                                                \
-    case i + (cm == 2 ? kPairs : 0):                                                             \
+#define STAGED_CASE(i, mb, nb, wm, wn, ks, s, kc, sec)                                           \
+    case i + (kc == 256 ? kPairs : 0):                                                           \
         if (!launch_fits(blocks, wm * wn * ks * 64))                                             \
             return fail("linear_fp8_dev: too many tiles for one launch");                        \
-        hipLaunchKernelGGL((fp8_staged_kernel<T, mb, nb, wm, wn, ks, s, cm>),                    \
+        hipLaunchKernelGGL((fp8_staged_kernel<T, mb, nb, wm, wn, ks, s, kc, sec>),               \
                            dim3(unsigned(blocks)), dim3(wm * wn * ks * 64), 0, st, p);           \
         break;
 
@@ -683,13 +745,13 @@ bool run_staged(LinArgs p, const LinPlan &pl, hipStream_t st)
     const int shape = pl.shape + (pl.pairs ? kPairs : 0);
     if constexpr (sizeof(T) == 2) {
         switch (shape) {
-            STAGED_BF16(STAGED_CASE, 1)
-            PAIRED_BF16(STAGED_CASE, 2)
+            STAGED_BF16(STAGED_CASE)
+            PAIRED_BF16(STAGED_CASE)
         }
     } else {
         switch (shape) {
-            STAGED_F32(STAGED_CASE, 1)
-            PAIRED_F32(STAGED_CASE, 2)
+            STAGED_F32(STAGED_CASE)
+            PAIRED_F32(STAGED_CASE)
         }
     }
     if (!hip_ok(hipGetLastError(), "fp8_staged_kernel launch"))
