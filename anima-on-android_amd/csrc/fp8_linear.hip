@@ -28,7 +28,6 @@ using flash_tile::f32x16;
 using flash_tile::mfma_bf16;
 using flash_tile::ring_barrier;
 using flash_tile::u16;
-using flash_tile::xcd_major_block;
 
 struct LinArgs {
     const uint8_t *a, *as, *w, *ws;
@@ -36,7 +35,7 @@ struct LinArgs {
     float *part;  // split K: f32 planes [splits][M][N]
     int64_t ldc;
     int M, N, groups, sg;  // sg: scale bytes of a row
-    int tiles_m, tiles_n, per_split;  // staged: tiles, and groups of one split
+    int tiles_m, tiles_n, splits, per_split;  // staged: tiles, and splits of K by groups
 };
 
 __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c)
@@ -234,14 +233,19 @@ struct Staged {
     // so that all count the same.
     static constexpr int A_WIN = A_BY / 1024, WIN = STAGE / 1024;
     static constexpr int OPS = (WIN + WAVES - 1) / WAVES;
-    // The epilogue's rows of one 32-row block per wave, and the shares' sums.
-    static constexpr int PITCH = 32 * NB + 16 / int(sizeof(T));
+    // The epilogue's rows, in the last stage: 32 of them by the columns of JB blocks (128
+    // bytes or more) per wave at a time.  The shares' sums take all of the stages.
+    static constexpr int JB = sizeof(T) == 4 ? 1 : NB;
+    static constexpr int PITCH = 32 * JB + 16 / int(sizeof(T));
     static constexpr int OUT_BY = WAVES / KS * 32 * PITCH * int(sizeof(T));
     static constexpr int RED_BY = (KS - 1) * (WAVES / KS) * MB * NB * 4096;
-    static constexpr int MAX2 = RED_BY > OUT_BY ? RED_BY : OUT_BY;
     static constexpr int USED = SCALES + ROWS * SEC;
-    static constexpr int LDS = USED > MAX2 ? USED : MAX2;
+    static constexpr int LDS = USED > RED_BY ? USED : RED_BY;
+    // Tiles in turn, the next one's first chunks coming in under the epilogue.
+    static constexpr bool TURNS = KS == 1 && OUT_BY <= STAGE;
+    static constexpr int OUT = TURNS ? (S - 1) * STAGE : 0;
     static_assert(STEPS % KS == 0 && SEC % 16 == 0 && LDS <= 163840, "160 KiB of LDS");
+    static_assert(OUT + OUT_BY <= SCALES, "the epilogue's rows fit the stages");
     static_assert(S >= 2 && (S - 2) * OPS < 64, "counted by vmcnt");
 };
 
@@ -271,34 +275,42 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void fp8_staged_kernel(LinArgs p)
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave % WM, wn = wave / WM % WN, share = wave / (WM * WN);
     const int col = lane & 31, half = lane >> 5;
-    const int tiles = p.tiles_m * p.tiles_n;
-    const int blk = xcd_major_block();
-    const int split = blk / tiles, t = blk - split * tiles;
-    // Four M tiles by all N tiles at a time, M inside: the 32 CUs of an XCD work
-    // on about 4 x 8 tiles.
-    const int band = t / (4 * p.tiles_n), in_band = t - band * 4 * p.tiles_n;
-    const int bm = min(4, p.tiles_m - 4 * band);
-    const int tn = in_band / bm, tm = 4 * band + in_band - tn * bm;
-    const int row0 = tm * G::BM, col0 = tn * G::BN;
-    const int g0 = split * p.per_split, g1 = min(g0 + p.per_split, p.groups);
-
-    // This lane's part of each copy, in bytes from the tile's first row; rows past
-    // M or N read the last one again (their results are not stored).
     constexpr int WROWS = 1024 / KC, PIECES = KC / 16;  // of a window, of a row
     const int64_t pitch = int64_t(p.groups) * kGroup;
-    const uint8_t *const a0 = p.a + row0 * pitch, *const w0 = p.w + col0 * pitch;
+
+    // The tile and split in work, and this lane's part of each copy, in bytes from the
+    // tile's first row; rows past M or N read the last one again (their results are not
+    // stored).
+    int row0, col0, split, g0, g1;
+    const uint8_t *a0, *w0;
     unsigned doff[G::OPS];
     int ddst[G::OPS];
     bool dw[G::OPS];
+    auto take = [&](int item) {
+        const int tiles = p.tiles_m * p.tiles_n;
+        split = item / tiles;
+        const int t = item - split * tiles;
+        // Four M tiles by all N tiles at a time, M inside: the 32 CUs of an XCD work
+        // on about 4 x 8 tiles.
+        const int band = t / (4 * p.tiles_n), in_band = t - band * 4 * p.tiles_n;
+        const int bm = min(4, p.tiles_m - 4 * band);
+        const int tn = in_band / bm, tm = 4 * band + in_band - tn * bm;
+        row0 = tm * G::BM;
+        col0 = tn * G::BN;
+        g0 = split * p.per_split;
+        g1 = min(g0 + p.per_split, p.groups);
+        a0 = p.a + row0 * pitch;
+        w0 = p.w + col0 * pitch;
 #pragma unroll
-    for (int i = 0; i < G::OPS; ++i) {
-        const int w = min(i * G::WAVES + wave, G::WIN - 1);
-        dw[i] = w >= G::A_WIN;
-        const int r = (dw[i] ? w - G::A_WIN : w) * WROWS + lane / PIECES;
-        const int at = dw[i] ? min(col0 + r, p.N - 1) - col0 : min(row0 + r, p.M - 1) - row0;
-        doff[i] = unsigned(at * pitch + 16 * (lane % PIECES ^ swizzle<KC>(r)));
-        ddst[i] = w * 1024;
-    }
+        for (int i = 0; i < G::OPS; ++i) {
+            const int w = min(i * G::WAVES + wave, G::WIN - 1);
+            dw[i] = w >= G::A_WIN;
+            const int r = (dw[i] ? w - G::A_WIN : w) * WROWS + lane / PIECES;
+            const int at = dw[i] ? min(col0 + r, p.N - 1) - col0 : min(row0 + r, p.M - 1) - row0;
+            doff[i] = unsigned(at * pitch + 16 * (lane % PIECES ^ swizzle<KC>(r)));
+            ddst[i] = w * 1024;
+        }
+    };
     // Part i of `parts` of chunk c's copies.
     auto copies = [&](int c, unsigned stage, int i, int parts) {
 #pragma unroll
@@ -329,14 +341,6 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void fp8_staged_kernel(LinArgs p)
     };
 
     f32x16 acc[MB][NB];
-#pragma unroll
-    for (int i = 0; i < MB; ++i)
-#pragma unroll
-        for (int j = 0; j < NB; ++j)
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-                acc[i][j][r] = 0.0f;
-
     unsigned sa[MB], sw[NB];  // scales of a chunk from its first group's on
     unsigned ao = 0, wo = 0;  // rows (wm MB) 32 + col and (wn NB) 32 + col of a chunk
     unsigned stage = 0, fill = 0;  // of the chunk in work, and to copy to
@@ -371,20 +375,23 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void fp8_staged_kernel(LinArgs p)
     using More = std::integral_constant<int, 1>;
     using Last = std::integral_constant<int, 0>;
 
-    // The chunks c0 .. c1 - 1 of a section: chunk c by work(c, what follows).
-    auto section = [&](int c0, int c1, auto &&begin, auto &&work) {
-        first = c0 * CG & ~15;
-        scales(first, c1 * CG);
+    // The section from group g on: its end, its first copies, and its chunks, chunk c
+    // by work(c, what follows).
+    auto end = [&](int g) { return min(g1, (g & ~15) + SEC); };
+    auto start = [&](int g) {
+        const int c0 = g / CG, c1 = end(g) / CG;
+        scales(g & ~15, end(g));
 #pragma unroll
         for (int i = 0; i < S - 1; ++i)
             if (c0 + i < c1)
                 copies(c0 + i, i * G::STAGE, 0, 1);
+    };
+    auto run = [&](int g, auto &&begin, auto &&work) {
+        const int c0 = g / CG, c1 = end(g) / CG;
+        first = g & ~15;
         stage = 0;
         fill = (S - 1) * G::STAGE;
-        if (c0 + S - 1 < c1)
-            wait_copies<(S - 2) * G::OPS>();
-        else
-            wait_copies<0>();
+        wait_copies<0>();
         enter(c0, sa, sw);
         if (c0 + S - 1 < c1)
             copies(c0 + S - 1, fill, 0, 1);
@@ -396,6 +403,23 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void fp8_staged_kernel(LinArgs p)
             work(c, More{});
         work(c, Last{});
     };
+    // All sections of a tile; the first one's copies are on their way.
+    auto product = [&](auto &&begin, auto &&work) {
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    acc[i][j][r] = 0.0f;
+        for (int g = g0; g < g1; g = end(g)) {
+            if (g > g0) {
+                __syncthreads();
+                start(g);
+            }
+            run(g, begin, work);
+        }
+    };
     // To the next chunk, c.
     auto turn = [&](int c, auto follows, unsigned (&na)[MB], unsigned (&nw)[NB]) {
         // It has landed when at most the S - 2 behind it are on their way.
@@ -403,6 +427,138 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void fp8_staged_kernel(LinArgs p)
         stage = after(stage);
         fill = after(fill);
         enter(c, na, nw);
+    };
+
+    // A tile's results.
+    auto finish = [&](int trow0, int tcol0, int tsplit) {
+        if constexpr (KS > 1) {
+            // The shares' sums, in their order.
+            f32x4 *red = reinterpret_cast<f32x4 *>(smem);
+            constexpr int BLOCKS = WM * WN * MB * NB;
+            const int w0i = wave % (WM * WN);
+            if (share > 0)
+#pragma unroll
+                for (int i = 0; i < MB; ++i)
+#pragma unroll
+                    for (int j = 0; j < NB; ++j)
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+                            red[(((share - 1) * BLOCKS + (w0i * MB + i) * NB + j) * 4 + q) * 64 + lane] =
+                                f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
+                                      acc[i][j][4 * q + 3]};
+            __syncthreads();
+            if (share == 0)
+#pragma unroll
+                for (int k = 0; k < KS - 1; ++k)
+#pragma unroll
+                    for (int i = 0; i < MB; ++i)
+#pragma unroll
+                        for (int j = 0; j < NB; ++j)
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) {
+                                const f32x4 v =
+                                    red[((k * BLOCKS + (w0i * MB + i) * NB + j) * 4 + q) * 64 + lane];
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    acc[i][j][4 * q + e] += v[e];
+                            }
+            __syncthreads();
+            if (share > 0)
+                return;
+        }
+
+        // Lane (col, half): row col of its blocks, columns acc_row(r, half).
+        const int m0 = trow0 + wm * MB * 32, n0 = tcol0 + wn * 32 * NB;
+        if (p.part) {
+            float *plane = p.part + int64_t(tsplit) * p.M * p.N;
+            const bool wide = p.N % 4 == 0;
+#pragma unroll
+            for (int i = 0; i < MB; ++i) {
+                const int m = m0 + i * 32 + col;
+                if (m >= p.M)
+                    continue;
+#pragma unroll
+                for (int j = 0; j < NB; ++j)
+#pragma unroll
+                    for (int r = 0; r < 16; r += 4)
+                        store4(plane + int64_t(m) * p.N, n0 + 32 * j + acc_row(r, half), p.N, wide,
+                               f32x4{acc[i][j][r], acc[i][j][r + 1], acc[i][j][r + 2],
+                                     acc[i][j][r + 3]});
+            }
+            return;
+        }
+        // Through LDS, so that rows go out in runs of 32 JB columns.
+        T *so = reinterpret_cast<T *>(smem + G::OUT) + (wave % (WM * WN)) * 32 * G::PITCH;
+        constexpr int JB = G::JB, E = 16 / int(sizeof(T));  // elements of a 16-byte piece
+        constexpr int RUN = 32 * JB / E;                    // pieces of a run
+        const bool wide = (reinterpret_cast<uintptr_t>(p.c) & 15) == 0 && p.ldc % E == 0 &&
+                          n0 + 32 * NB <= p.N;
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+            for (int jb = 0; jb < NB; jb += JB) {
+#pragma unroll
+                for (int j = 0; j < JB; ++j)
+#pragma unroll
+                    for (int r = 0; r < 16; r += 4)
+                        store4(so + col * G::PITCH, 32 * j + acc_row(r, half), 32 * JB, true,
+                               f32x4{acc[i][jb + j][r], acc[i][jb + j][r + 1],
+                                     acc[i][jb + j][r + 2], acc[i][jb + j][r + 3]});
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                for (int q = 0; q < RUN / 2; ++q) {
+                    const int f = q * 64 + lane, r = f / RUN, piece = f % RUN;
+                    const int m = m0 + i * 32 + r;
+                    const u32x4 v = *reinterpret_cast<const u32x4 *>(so + r * G::PITCH + E * piece);
+                    if (m >= p.M)
+                        continue;
+                    const int nn = n0 + 32 * jb + E * piece;
+                    T *dst = static_cast<T *>(p.c) + int64_t(m) * p.ldc + nn;
+                    if (wide)
+                        __builtin_nontemporal_store(v, reinterpret_cast<u32x4 *>(dst));
+                    else
+#pragma unroll
+                        for (int e = 0; e < E; ++e)
+                            if (nn + e < p.N) {
+                                if constexpr (EXACT)
+                                    dst[e] = __uint_as_float(v[e]);
+                                else
+                                    dst[e] = u16(v[e >> 1] >> (16 * (e & 1)));
+                            }
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+            }
+    };
+    // The tiles of this workgroup in turn: XCD x = blockIdx % 8 has a contiguous range of
+    // them, and its workgroups take every so many-th.
+    auto tile = [&](auto &&begin, auto &&work) {
+        const unsigned items = unsigned(p.tiles_m * p.tiles_n) * p.splits;
+        const unsigned x = blockIdx.x % kXcds, q = items / kXcds, r = items % kXcds;
+        const unsigned from = x * q + min(x, r), to = from + q + (x < r ? 1 : 0);
+        const unsigned step = (gridDim.x - x + kXcds - 1) / kXcds;
+        unsigned item = from + blockIdx.x / kXcds;
+        if (item >= to)
+            return;
+        take(int(item));
+        if (g0 < g1)
+            start(g0);
+        for (;;) {
+            product(begin, work);
+            const int trow0 = row0, tcol0 = col0, tsplit = split;
+            item += step;
+            const bool more = G::TURNS && item < to;
+            __syncthreads();  // every wave has left the stages
+            if (more) {
+                take(int(item));
+                if (g0 < g1)
+                    start(g0);
+            }
+            finish(trow0, tcol0, tsplit);
+            if (!more)
+                return;
+        }
     };
 
     if constexpr (EXACT) {
@@ -470,11 +626,7 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void fp8_staged_kernel(LinArgs p)
                 }
             }
         };
-        for (int g = g0; g < g1; g += SEC - g % 16) {
-            if (g > g0)
-                __syncthreads();
-            section(g / CG, min(g1, g + SEC - g % 16) / CG, begin, work);
-        }
+        tile(begin, work);
     } else {
         // A step is 64 elements, 32 of each half, one fp8 MFMA.  The fragments of W
         // have two sets of registers; those of A too in small blocks, and in large ones
@@ -565,109 +717,7 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void fp8_staged_kernel(LinArgs p)
                 }
             }
         };
-        for (int g = g0; g < g1; g += SEC - g % 16) {
-            if (g > g0)
-                __syncthreads();
-            section(g / CG, min(g1, g + SEC - g % 16) / CG, begin, work);
-        }
-    }
-
-    __syncthreads();
-    if constexpr (KS > 1) {
-        // The shares' sums, in their order.
-        f32x4 *red = reinterpret_cast<f32x4 *>(smem);
-        constexpr int BLOCKS = WM * WN * MB * NB;
-        const int w0i = wave % (WM * WN);
-        if (share > 0)
-#pragma unroll
-            for (int i = 0; i < MB; ++i)
-#pragma unroll
-                for (int j = 0; j < NB; ++j)
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        red[(((share - 1) * BLOCKS + (w0i * MB + i) * NB + j) * 4 + q) * 64 + lane] =
-                            f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
-                                  acc[i][j][4 * q + 3]};
-        __syncthreads();
-        if (share == 0)
-#pragma unroll
-            for (int k = 0; k < KS - 1; ++k)
-#pragma unroll
-                for (int i = 0; i < MB; ++i)
-#pragma unroll
-                    for (int j = 0; j < NB; ++j)
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            const f32x4 v =
-                                red[((k * BLOCKS + (w0i * MB + i) * NB + j) * 4 + q) * 64 + lane];
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                acc[i][j][4 * q + e] += v[e];
-                        }
-        __syncthreads();
-        if (share > 0)
-            return;
-    }
-
-    // Lane (col, half): row col of its blocks, columns acc_row(r, half).
-    const int n0 = col0 + wn * 32 * NB;
-    if (p.part) {
-        float *plane = p.part + int64_t(split) * p.M * p.N;
-        const bool wide = p.N % 4 == 0;
-#pragma unroll
-        for (int i = 0; i < MB; ++i) {
-            const int m = row0 + (wm * MB + i) * 32 + col;
-            if (m >= p.M)
-                continue;
-#pragma unroll
-            for (int j = 0; j < NB; ++j)
-#pragma unroll
-                for (int r = 0; r < 16; r += 4)
-                    store4(plane + int64_t(m) * p.N, n0 + 32 * j + acc_row(r, half), p.N, wide,
-                           f32x4{acc[i][j][r], acc[i][j][r + 1], acc[i][j][r + 2],
-                                 acc[i][j][r + 3]});
-        }
-        return;
-    }
-    // Through LDS, so that rows go out in runs of 32 NB columns.
-    T *so = reinterpret_cast<T *>(smem) + (wave % (WM * WN)) * 32 * G::PITCH;
-    constexpr int E = 16 / int(sizeof(T));  // elements of a 16-byte piece
-    constexpr int OUT = 32 * NB / E;        // pieces of a row
-    const bool wide = (reinterpret_cast<uintptr_t>(p.c) & 15) == 0 && p.ldc % E == 0 &&
-                      n0 + 32 * NB <= p.N;
-#pragma unroll
-    for (int i = 0; i < MB; ++i) {
-#pragma unroll
-        for (int j = 0; j < NB; ++j)
-#pragma unroll
-            for (int r = 0; r < 16; r += 4)
-                store4(so + col * G::PITCH, 32 * j + acc_row(r, half), 32 * NB, true,
-                       f32x4{acc[i][j][r], acc[i][j][r + 1], acc[i][j][r + 2], acc[i][j][r + 3]});
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int q = 0; q < OUT / 2; ++q) {
-            const int f = q * 64 + lane, r = f / OUT, piece = f % OUT;
-            const int m = row0 + (wm * MB + i) * 32 + r;
-            const u32x4 v = *reinterpret_cast<const u32x4 *>(so + r * G::PITCH + E * piece);
-            if (m >= p.M)
-                continue;
-            const int nn = n0 + E * piece;
-            T *dst = static_cast<T *>(p.c) + int64_t(m) * p.ldc + nn;
-            if (wide)
-                __builtin_nontemporal_store(v, reinterpret_cast<u32x4 *>(dst));
-            else
-#pragma unroll
-                for (int e = 0; e < E; ++e)
-                    if (nn + e < p.N) {
-                        if constexpr (EXACT)
-                            dst[e] = __uint_as_float(v[e]);
-                        else
-                            dst[e] = u16(v[e >> 1] >> (16 * (e & 1)));
-                    }
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+        tile(begin, work);
     }
 }
 
@@ -729,19 +779,30 @@ PAIRED_F32(CHECK_F32)
 constexpr int kPairs = 16;  // beside a shape's number: two groups at once
 #define STAGED_CASE(i, mb, nb, wm, wn, ks, s, kc, sec)                                           \
     case i + (kc == 256 ? kPairs : 0):                                                           \
-        if (!launch_fits(blocks, wm * wn * ks * 64))                                             \
-            return fail("linear_fp8_dev: too many tiles for one launch");                        \
-        hipLaunchKernelGGL((fp8_staged_kernel<T, mb, nb, wm, wn, ks, s, kc, sec>),               \
-                           dim3(unsigned(blocks)), dim3(wm * wn * ks * 64), 0, st, p);           \
+        launch_staged<T, mb, nb, wm, wn, ks, s, kc, sec>(p, items, st);                          \
         break;
+
+template <typename T, int MB, int NB, int WM, int WN, int KS, int S, int KC, int SEC>
+void launch_staged(const LinArgs &p, int64_t items, hipStream_t st)
+{
+    using G = Staged<T, MB, NB, WM, WN, KS, S, KC, SEC>;
+    // As many workgroups as the CUs hold at once, where they take tiles in turn.
+    constexpr int64_t room = 256 * (163840 / G::LDS < 2 ? 1 : 2);
+    const dim3 grid(unsigned(G::TURNS ? std::min(items, room) : items));
+    hipLaunchKernelGGL((fp8_staged_kernel<T, MB, NB, WM, WN, KS, S, KC, SEC>), grid,
+                       dim3(G::THREADS), 0, st, p);
+}
 
 template <typename T>
 bool run_staged(LinArgs p, const LinPlan &pl, hipStream_t st)
 {
     p.tiles_m = pl.tiles_m;
     p.tiles_n = pl.tiles_n;
+    p.splits = pl.splits;
     p.per_split = pl.per_split;
-    const int64_t blocks = int64_t(pl.tiles_m) * pl.tiles_n * pl.splits;
+    const int64_t items = int64_t(pl.tiles_m) * pl.tiles_n * pl.splits;
+    if (!launch_fits(items, 512))
+        return fail("linear_fp8_dev: too many tiles for one launch");
     const int shape = pl.shape + (pl.pairs ? kPairs : 0);
     if constexpr (sizeof(T) == 2) {
         switch (shape) {
