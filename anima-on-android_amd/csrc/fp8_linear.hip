@@ -215,47 +215,53 @@ __global__ __launch_bounds__(WAVES * 64) void fp8_few_kernel(LinArgs p)
 //
 // Rows of both operands reach LDS by DMA, KC bytes at a time through S stages; 16-byte
 // pieces are placed by piece ^ swizzle(row) against bank conflicts.  Their scales
-// come once for a section of SEC groups: a dword per row and chunk costs as many requests as the
-// rows themselves.  Fragments of a step are read while the MFMAs of the step before
-// run; a chunk's first ones under the last step of the chunk before, behind the barrier
-// that ends it.
-template <typename T, int MB, int NB, int WM, int WN, int KS, int S, int KC, int SEC>
+// come in sections of 16 groups, two at a time.  Fragments of a step are read
+// while the MFMAs of the step before run; a chunk's first ones under the last step of
+// the chunk before, behind the barrier that ends it.
+//
+// With KS = 1 a workgroup takes several tiles in turn, the next one's first chunks coming
+// in while this one's results go out (4608 x 8192 x 2048: 82 us, so 75).
+template <typename T, int MB, int NB, int WM, int WN, int KS, int S, int KC>
 struct Staged {
+    static constexpr bool TURN = KS == 1;
     static constexpr int WAVES = WM * WN * KS, THREADS = WAVES * 64;
     static constexpr int BM = 32 * MB * WM, BN = 32 * NB * WN;
     static constexpr int STEP = sizeof(T) == 4 ? 32 : 64;  // elements of K
     static constexpr int STEPS = KC / STEP, SHARE = STEPS / KS;
-    // LDS in bytes: S stages of A and W, then scales: rows of both by 16 groups, SEC / 16
-    // times.
+    // LDS in bytes: S stages of A and W, then two sections of scales, 16 bytes a row.
     static constexpr int A_BY = BM * KC, STAGE = A_BY + BN * KC;
-    static constexpr int ROWS = BM + BN, SCALES = S * STAGE;
+    static constexpr int ROWS = BM + BN, SCALES = S * STAGE, SECTION = ROWS * 16;
     // 1 KiB windows per chunk, and per wave; a wave without one copies the last again,
     // so that all count the same.
     static constexpr int A_WIN = A_BY / 1024, WIN = STAGE / 1024;
     static constexpr int OPS = (WIN + WAVES - 1) / WAVES;
     // The epilogue's rows, in the last stage: 32 of them by the columns of JB blocks (128
-    // bytes or more) per wave at a time.  The shares' sums take all of the stages.
+    // bytes or more) per wave at a time.  The shares' sums take all of LDS.
     static constexpr int JB = sizeof(T) == 4 ? 1 : NB;
-    static constexpr int PITCH = 32 * JB + 16 / int(sizeof(T));
-    static constexpr int OUT_BY = WAVES / KS * 32 * PITCH * int(sizeof(T));
+    static constexpr int OUT_ROW = 32 * JB * int(sizeof(T));
+    static constexpr int OUT = TURN ? (S - 1) * STAGE : 0;
+    static constexpr int OUT_BY = WAVES / KS * 32 * OUT_ROW;
     static constexpr int RED_BY = (KS - 1) * (WAVES / KS) * MB * NB * 4096;
-    static constexpr int USED = SCALES + ROWS * SEC;
+    static constexpr int USED = SCALES + 2 * SECTION;
     static constexpr int LDS = USED > RED_BY ? USED : RED_BY;
-    // Tiles in turn, the next one's first chunks coming in under the epilogue.
-    static constexpr bool TURNS = KS == 1 && OUT_BY <= STAGE;
-    static constexpr int OUT = TURNS ? (S - 1) * STAGE : 0;
-    static_assert(STEPS % KS == 0 && SEC % 16 == 0 && LDS <= 163840, "160 KiB of LDS");
+    // Workgroups that a CU holds at once.
+    static constexpr int ROOM = LDS <= 81920 && THREADS <= 256 ? 2 : 1;
+    static_assert(STEPS % KS == 0 && LDS <= 163840, "160 KiB of LDS");
     static_assert(OUT + OUT_BY <= SCALES, "the epilogue's rows fit the stages");
     static_assert(S >= 2 && (S - 2) * OPS < 64, "counted by vmcnt");
 };
 
-// Place of a piece of a staged row, so that the 16 rows of a ds_read_b128 quarter
-// touch distinct banks.
-template <int KC>
+// Place of a 16-byte piece of a row of ROW bytes in LDS, so that the 16 rows of a
+// ds_read_b128 quarter touch distinct banks.
+template <int ROW>
 __device__ __forceinline__ int swizzle(int row)
 {
-    return KC == 128 ? (row & 7) ^ (row >> 3 & 1) : row & 15;
+    return ROW == 64 ? row >> 2 & 3 : ROW == 128 ? (row & 7) ^ (row >> 3 & 1) : row & 15;
 }
+
+// The compiler gives up inlining bodies used several times, and with them the scalar
+// registers that the copies' addresses need.
+#define INLINED __attribute__((always_inline))
 
 // s_waitcnt vmcnt(N), N < 64.
 template <int N>
@@ -264,11 +270,12 @@ __device__ __forceinline__ void wait_copies()
     __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | (N >> 4) << 14);
 }
 
-template <typename T, int MB, int NB, int WM, int WN, int KS, int S, int KC, int SEC>
+template <typename T, int MB, int NB, int WM, int WN, int KS, int S, int KC>
 __global__ __launch_bounds__(WM *WN *KS * 64) void fp8_staged_kernel(LinArgs p)
 {
-    using G = Staged<T, MB, NB, WM, WN, KS, S, KC, SEC>;
+    using G = Staged<T, MB, NB, WM, WN, KS, S, KC>;
     constexpr bool EXACT = sizeof(T) == 4;
+    constexpr int CG = KC / kGroup;  // groups of a chunk
     __shared__ __attribute__((aligned(16))) uint8_t smem[G::LDS];
 
     const int tid = threadIdx.x, lane = tid & 63;
@@ -278,15 +285,15 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void fp8_staged_kernel(LinArgs p)
     constexpr int WROWS = 1024 / KC, PIECES = KC / 16;  // of a window, of a row
     const int64_t pitch = int64_t(p.groups) * kGroup;
 
-    // The tile and split in work, and this lane's part of each copy, in bytes from the
+    // The tile and split in work, its chunks, and this lane's part of each copy in bytes from the
     // tile's first row; rows past M or N read the last one again (their results are not
     // stored).
-    int row0, col0, split, g0, g1;
-    const uint8_t *a0, *w0;
+    int row0, col0, split, c0, c1;
+    const uint8_t *a0, *w0, *as0, *ws0;
     unsigned doff[G::OPS];
     int ddst[G::OPS];
     bool dw[G::OPS];
-    auto take = [&](int item) {
+    auto take = [&](int item) INLINED {
         const int tiles = p.tiles_m * p.tiles_n;
         split = item / tiles;
         const int t = item - split * tiles;
@@ -297,10 +304,12 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void fp8_staged_kernel(LinArgs p)
         const int tn = in_band / bm, tm = 4 * band + in_band - tn * bm;
         row0 = tm * G::BM;
         col0 = tn * G::BN;
-        g0 = split * p.per_split;
-        g1 = min(g0 + p.per_split, p.groups);
+        c0 = split * p.per_split / CG;
+        c1 = min((split + 1) * p.per_split, p.groups) / CG;
         a0 = p.a + row0 * pitch;
         w0 = p.w + col0 * pitch;
+        as0 = p.as + int64_t(row0) * p.sg;
+        ws0 = p.ws + int64_t(col0) * p.sg;
 #pragma unroll
         for (int i = 0; i < G::OPS; ++i) {
             const int w = min(i * G::WAVES + wave, G::WIN - 1);
@@ -312,48 +321,59 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void fp8_staged_kernel(LinArgs p)
         }
     };
     // Part i of `parts` of chunk c's copies.
-    auto copies = [&](int c, unsigned stage, int i, int parts) {
+    auto copies = [&](int c, unsigned stage, int i, int parts) INLINED {
 #pragma unroll
         for (int k = G::OPS * i / parts; k < G::OPS * (i + 1) / parts; ++k)
             dma16s((dw[k] ? w0 : a0) + int64_t(c) * KC, doff[k],
-                   reinterpret_cast<u16 *>(smem + stage + ddst[k]));
+                   reinterpret_cast<u16 *>(
+                       smem + __builtin_amdgcn_readfirstlane(int(stage) + ddst[k])));
     };
-    // The scales of groups g .. ge - 1, g a multiple of 16: windows of 16 rows by four
-    // dwords, past a row's end its last one again.
-    auto scales = [&](int g, int ge) {
-        for (int sub = 0; g + 16 * sub < ge; ++sub)
+    // Section s of the scales, groups 16 s on: windows of 16 rows by four dwords, so that a
+    // row is one request (a dword of each of 64 rows costs 64), past a row's end its
+    // last dword again.
+    auto scales = [&](int section) INLINED {
+        const int s = __builtin_amdgcn_readfirstlane(section);
 #pragma unroll
-            for (int i = 0; i < (G::ROWS / 16 + G::WAVES - 1) / G::WAVES; ++i) {
-                const int w = i * G::WAVES + wave;
-                if (w * 16 >= G::ROWS)
-                    continue;
-                const bool is_w = w * 16 >= G::BM;
-                const int r = w * 16 + lane / 4 - (is_w ? G::BM : 0);
-                const int at = is_w ? min(col0 + r, p.N - 1) - col0
-                                    : min(row0 + r, p.M - 1) - row0;
-                const unsigned off = unsigned(at * p.sg + min(g + 16 * sub + lane % 4 * 4, p.sg - 4));
-                dma4s(is_w ? p.ws + int64_t(col0) * p.sg : p.as + int64_t(row0) * p.sg, off,
-                      reinterpret_cast<u16 *>(smem + G::SCALES + (sub * G::ROWS + w * 16) * 16));
-            }
+        for (int i = 0; i < (G::ROWS / 16 + G::WAVES - 1) / G::WAVES; ++i) {
+            const int w = min(i * G::WAVES + wave, G::ROWS / 16 - 1);
+            const bool is_w = w * 16 >= G::BM;
+            const int r = w * 16 + lane / 4 - (is_w ? G::BM : 0);
+            const int at = is_w ? min(col0 + r, p.N - 1) - col0 : min(row0 + r, p.M - 1) - row0;
+            dma4s(is_w ? ws0 : as0, unsigned(at * p.sg + min(16 * s + lane % 4 * 4, p.sg - 4)),
+                  reinterpret_cast<u16 *>(smem + __builtin_amdgcn_readfirstlane(
+                                                     G::SCALES + (s & 1) * G::SECTION + w * 256)));
+        }
     };
-    auto after = [&](unsigned stage) {
+    // The first copies of the tile.
+    auto start = [&]() INLINED {
+        if (c0 >= c1)
+            return;
+        const int s = c0 * CG / 16;
+        scales(s);
+        if (16 * (s + 1) < p.groups)
+            scales(s + 1);
+#pragma unroll
+        for (int i = 0; i < S - 1; ++i)
+            if (c0 + i < c1)
+                copies(c0 + i, i * G::STAGE, 0, 1);
+    };
+    auto after = [&](unsigned stage) INLINED {
         return stage == (S - 1) * G::STAGE ? 0u : stage + G::STAGE;
     };
 
     f32x16 acc[MB][NB];
     unsigned sa[MB], sw[NB];  // scales of a chunk from its first group's on
     unsigned ao = 0, wo = 0;  // rows (wm MB) 32 + col and (wn NB) 32 + col of a chunk
-    unsigned stage = 0, fill = 0;  // of the chunk in work, and to copy to
-    int first = 0;                 // group of the section's first chunk
-    constexpr int CG = KC / kGroup;  // groups of a chunk
-    // Chunk c is there, at `stage`, and its scales in na and nw; `fill` is free.
-    auto enter = [&](int c, unsigned (&na)[MB], unsigned (&nw)[NB]) {
-        ring_barrier();  // for every wave; and all have left the stage before it
+    unsigned stage = 0;       // of the chunk in work
+    // Chunk c is there, at `stage`, and its scales in na and nw; every wave has left the
+    // stage before it.
+    auto enter = [&](int c, unsigned (&na)[MB], unsigned (&nw)[NB]) INLINED {
+        ring_barrier();
         ao = stage + (wm * 32 * MB + col) * KC;
         wo = stage + G::A_BY + (wn * 32 * NB + col) * KC;
         asm volatile("" : "+v"(ao), "+v"(wo));
-        const int g = c * CG - first, shift = g % 4 * 8;
-        const uint8_t *s = smem + G::SCALES + g / 16 * (G::ROWS * 16) + (g % 16 & ~3) + col * 16;
+        const int g = c * CG, shift = g % 4 * 8;
+        const uint8_t *s = smem + G::SCALES + (g / 16 & 1) * G::SECTION + (g % 16 & ~3) + col * 16;
 #pragma unroll
         for (int i = 0; i < MB; ++i)
             na[i] = *reinterpret_cast<const unsigned *>(s + (wm * MB + i) * 512) >> shift;
@@ -363,48 +383,32 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void fp8_staged_kernel(LinArgs p)
                     shift;
     };
     // 16 bytes of row col of block b; the swizzle depends on col alone.
-    auto piece = [&](unsigned row, int b, int i) {
+    auto piece = [&](unsigned row, int b, int i) INLINED {
         return *reinterpret_cast<const u32x4 *>(smem + row + 32 * b * KC +
                                                 16 * (i ^ swizzle<KC>(col)));
     };
     // This wave's steps of a chunk: share * SHARE .. .
-    auto step_of = [&](int i) { return KS == 1 ? i : share * G::SHARE + i; };
+    auto step_of = [&](int i) INLINED { return KS == 1 ? i : share * G::SHARE + i; };
     constexpr int LAST = G::SHARE - 1;
-    // What a chunk is followed by: another and copies to make, another, nothing.
-    using Copy = std::integral_constant<int, 2>;
-    using More = std::integral_constant<int, 1>;
-    using Last = std::integral_constant<int, 0>;
 
-    // The section from group g on: its end, its first copies, and its chunks, chunk c
-    // by work(c, what follows).
-    auto end = [&](int g) { return min(g1, (g & ~15) + SEC); };
-    auto start = [&](int g) {
-        const int c0 = g / CG, c1 = end(g) / CG;
-        scales(g & ~15, end(g));
-#pragma unroll
-        for (int i = 0; i < S - 1; ++i)
-            if (c0 + i < c1)
-                copies(c0 + i, i * G::STAGE, 0, 1);
+    // What follows a chunk: nothing, another, or another and the copies for S chunks on.
+    enum { kEnd, kMore, kCopy };
+    using End = std::integral_constant<int, kEnd>;
+    using More = std::integral_constant<int, kMore>;
+    using Copy = std::integral_constant<int, kCopy>;
+    // To the next chunk, c: it has landed when at most the S - 2 behind it are on their
+    // way.
+    auto turn = [&](int c, auto follows, unsigned (&na)[MB], unsigned (&nw)[NB]) INLINED {
+        wait_copies<decltype(follows)::value == kCopy ? (S - 2) * G::OPS : 0>();
+        stage = after(stage);
+        enter(c, na, nw);
     };
-    auto run = [&](int g, auto &&begin, auto &&work) {
-        const int c0 = g / CG, c1 = end(g) / CG;
-        first = g & ~15;
-        stage = 0;
-        fill = (S - 1) * G::STAGE;
-        wait_copies<0>();
-        enter(c0, sa, sw);
-        if (c0 + S - 1 < c1)
-            copies(c0 + S - 1, fill, 0, 1);
-        begin();
-        int c = c0;
-        for (; c + S < c1; ++c)
-            work(c, Copy{});
-        for (; c + 1 < c1; ++c)
-            work(c, More{});
-        work(c, Last{});
-    };
-    // All sections of a tile; the first one's copies are on their way.
-    auto product = [&](auto &&begin, auto &&work) {
+    // The stage that copies for S chunks on go to, behind the turn: that of the chunk before.
+    auto fill = [&]() INLINED { return stage == 0 ? (S - 1) * G::STAGE : stage - G::STAGE; };
+
+    // All chunks of a tile, chunk c by work(c, what follows); its first copies are on
+    // their way, and the stores of the tile before behind them.
+    auto product = [&](auto &&begin, auto &&work) INLINED {
 #pragma unroll
         for (int i = 0; i < MB; ++i)
 #pragma unroll
@@ -412,25 +416,35 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void fp8_staged_kernel(LinArgs p)
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
                     acc[i][j][r] = 0.0f;
-        for (int g = g0; g < g1; g = end(g)) {
-            if (g > g0) {
-                __syncthreads();
-                start(g);
-            }
-            run(g, begin, work);
+        if (c0 >= c1)
+            return;
+        stage = 0;
+        if (!G::TURN && c0 + S - 1 < c1)
+            wait_copies<(S - 2) * G::OPS>();
+        else
+            wait_copies<0>();
+        enter(c0, sa, sw);
+        if (c0 + S - 1 < c1)
+            copies(c0 + S - 1, (S - 1) * G::STAGE, 0, 1);
+        begin();
+        int c = c0;
+        int section = c0 * CG / 16;
+        while (c + S < c1) {
+            // To the end of the section; the one after next takes its place then.
+            const int e = min((section + 1) * 16 / CG, c1 - S);
+            for (; c < e; ++c)
+                work(c, Copy{});
+            ++section;
+            if (c + S < c1 && 16 * (section + 1) < p.groups)
+                scales(section + 1);
         }
-    };
-    // To the next chunk, c.
-    auto turn = [&](int c, auto follows, unsigned (&na)[MB], unsigned (&nw)[NB]) {
-        // It has landed when at most the S - 2 behind it are on their way.
-        wait_copies<decltype(follows)::value == 2 ? (S - 2) * G::OPS : 0>();
-        stage = after(stage);
-        fill = after(fill);
-        enter(c, na, nw);
+        for (; c + 1 < c1; ++c)
+            work(c, More{});
+        work(c, End{});
     };
 
     // A tile's results.
-    auto finish = [&](int trow0, int tcol0, int tsplit) {
+    auto finish = [&](int m0, int n0, int plane_of) INLINED {
         if constexpr (KS > 1) {
             // The shares' sums, in their order.
             f32x4 *red = reinterpret_cast<f32x4 *>(smem);
@@ -443,9 +457,9 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void fp8_staged_kernel(LinArgs p)
                     for (int j = 0; j < NB; ++j)
 #pragma unroll
                         for (int q = 0; q < 4; ++q)
-                            red[(((share - 1) * BLOCKS + (w0i * MB + i) * NB + j) * 4 + q) * 64 + lane] =
-                                f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
-                                      acc[i][j][4 * q + 3]};
+                            red[(((share - 1) * BLOCKS + (w0i * MB + i) * NB + j) * 4 + q) * 64 +
+                                lane] = f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1],
+                                              acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
             __syncthreads();
             if (share == 0)
 #pragma unroll
@@ -457,7 +471,8 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void fp8_staged_kernel(LinArgs p)
 #pragma unroll
                             for (int q = 0; q < 4; ++q) {
                                 const f32x4 v =
-                                    red[((k * BLOCKS + (w0i * MB + i) * NB + j) * 4 + q) * 64 + lane];
+                                    red[((k * BLOCKS + (w0i * MB + i) * NB + j) * 4 + q) * 64 +
+                                        lane];
 #pragma unroll
                                 for (int e = 0; e < 4; ++e)
                                     acc[i][j][4 * q + e] += v[e];
@@ -466,11 +481,11 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void fp8_staged_kernel(LinArgs p)
             if (share > 0)
                 return;
         }
-
         // Lane (col, half): row col of its blocks, columns acc_row(r, half).
-        const int m0 = trow0 + wm * MB * 32, n0 = tcol0 + wn * 32 * NB;
+        m0 += wm * MB * 32;
+        n0 += wn * NB * 32;
         if (p.part) {
-            float *plane = p.part + int64_t(tsplit) * p.M * p.N;
+            float *plane = p.part + int64_t(plane_of) * p.M * p.N;
             const bool wide = p.N % 4 == 0;
 #pragma unroll
             for (int i = 0; i < MB; ++i) {
@@ -487,12 +502,12 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void fp8_staged_kernel(LinArgs p)
             }
             return;
         }
-        // Through LDS, so that rows go out in runs of 32 JB columns.
-        T *so = reinterpret_cast<T *>(smem + G::OUT) + (wave % (WM * WN)) * 32 * G::PITCH;
-        constexpr int JB = G::JB, E = 16 / int(sizeof(T));  // elements of a 16-byte piece
-        constexpr int RUN = 32 * JB / E;                    // pieces of a run
-        const bool wide = (reinterpret_cast<uintptr_t>(p.c) & 15) == 0 && p.ldc % E == 0 &&
-                          n0 + 32 * NB <= p.N;
+        // Through LDS, so that rows go out in runs of 32 JB columns; pieces of 16 bytes are
+        // placed as in the stages.
+        constexpr int JB = G::JB, ROW = G::OUT_ROW;
+        constexpr int RUN = ROW / 16, E = 16 / int(sizeof(T));  // pieces of a row, their elements
+        uint8_t *so = smem + G::OUT + wave % (WM * WN) * (32 * ROW);
+        const bool wide = (reinterpret_cast<uintptr_t>(p.c) & 15) == 0 && p.ldc % E == 0;
 #pragma unroll
         for (int i = 0; i < MB; ++i)
 #pragma unroll
@@ -500,22 +515,25 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void fp8_staged_kernel(LinArgs p)
 #pragma unroll
                 for (int j = 0; j < JB; ++j)
 #pragma unroll
-                    for (int r = 0; r < 16; r += 4)
-                        store4(so + col * G::PITCH, 32 * j + acc_row(r, half), 32 * JB, true,
-                               f32x4{acc[i][jb + j][r], acc[i][jb + j][r + 1],
-                                     acc[i][jb + j][r + 2], acc[i][jb + j][r + 3]});
+                    for (int q = 0; q < 16; q += 4) {
+                        const f32x16 &v = acc[i][jb + j];
+                        const int at = (32 * j + acc_row(q, half)) * int(sizeof(T));
+                        store4(reinterpret_cast<T *>(so + col * ROW +
+                                                     ((at / 16) ^ swizzle<ROW>(col)) * 16 + at % 16),
+                               0, 4, true, f32x4{v[q], v[q + 1], v[q + 2], v[q + 3]});
+                    }
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                 __builtin_amdgcn_wave_barrier();
 #pragma unroll
                 for (int q = 0; q < RUN / 2; ++q) {
-                    const int f = q * 64 + lane, r = f / RUN, piece = f % RUN;
-                    const int m = m0 + i * 32 + r;
-                    const u32x4 v = *reinterpret_cast<const u32x4 *>(so + r * G::PITCH + E * piece);
+                    const int f = q * 64 + lane, r = f / RUN, pc = f % RUN;
+                    const u32x4 v =
+                        *reinterpret_cast<const u32x4 *>(so + r * ROW + (pc ^ swizzle<ROW>(r)) * 16);
+                    const int m = m0 + i * 32 + r, nn = n0 + 32 * jb + E * pc;
                     if (m >= p.M)
                         continue;
-                    const int nn = n0 + 32 * jb + E * piece;
                     T *dst = static_cast<T *>(p.c) + int64_t(m) * p.ldc + nn;
-                    if (wide)
+                    if (wide && nn + E <= p.N)
                         __builtin_nontemporal_store(v, reinterpret_cast<u32x4 *>(dst));
                     else
 #pragma unroll
@@ -531,31 +549,27 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void fp8_staged_kernel(LinArgs p)
                 __builtin_amdgcn_wave_barrier();
             }
     };
-    // The tiles of this workgroup in turn: XCD x = blockIdx % 8 has a contiguous range of
-    // them, and its workgroups take every so many-th.
-    auto tile = [&](auto &&begin, auto &&work) {
+    // The tiles of this workgroup: XCD x = blockIdx % 8 has a contiguous range of them, and
+    // its workgroups take every so many-th.
+    auto tiles = [&](auto &&begin, auto &&work) INLINED {
         const unsigned items = unsigned(p.tiles_m * p.tiles_n) * p.splits;
         const unsigned x = blockIdx.x % kXcds, q = items / kXcds, r = items % kXcds;
-        const unsigned from = x * q + min(x, r), to = from + q + (x < r ? 1 : 0);
+        const unsigned to = x * q + min(x, r) + q + (x < r ? 1 : 0);
         const unsigned step = (gridDim.x - x + kXcds - 1) / kXcds;
-        unsigned item = from + blockIdx.x / kXcds;
-        if (item >= to)
-            return;
-        take(int(item));
-        if (g0 < g1)
-            start(g0);
+        unsigned item = x * q + min(x, r) + blockIdx.x / kXcds;
+        take(__builtin_amdgcn_readfirstlane(int(item)));
+        start();
         for (;;) {
             product(begin, work);
-            const int trow0 = row0, tcol0 = col0, tsplit = split;
+            const int m0 = row0, n0 = col0, plane_of = split;
             item += step;
-            const bool more = G::TURNS && item < to;
+            const bool more = G::TURN && item < to;
             __syncthreads();  // every wave has left the stages
             if (more) {
-                take(int(item));
-                if (g0 < g1)
-                    start(g0);
+                take(__builtin_amdgcn_readfirstlane(int(item)));
+                start();
             }
-            finish(trow0, tcol0, tsplit);
+            finish(m0, n0, plane_of);
             if (!more)
                 return;
         }
@@ -565,12 +579,12 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void fp8_staged_kernel(LinArgs p)
         // A step is 32 elements: 16 of each half, two bf16 MFMAs.  A fragment's
         // registers are free once it is decoded, and take the next step's then.
         u32x4 ra[MB], rw[NB];
-        auto decode2 = [&](const u32x4 &x, unsigned scale, bf16x8 (&v)[2]) {
+        auto decode2 = [&](const u32x4 &x, unsigned scale, bf16x8 (&v)[2]) INLINED {
             const float f = scale_of(scale & 255u);
             v[0] = decode8(x[0], x[1], f);
             v[1] = decode8(x[2], x[3], f);
         };
-        auto begin = [&]() {
+        auto begin = [&]() INLINED {
 #pragma unroll
             for (int j = 0; j < NB; ++j)
                 rw[j] = piece(wo, j, 2 * step_of(0) + half);
@@ -578,8 +592,8 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void fp8_staged_kernel(LinArgs p)
             for (int i = 0; i < MB; ++i)
                 ra[i] = piece(ao, i, 2 * step_of(0) + half);
         };
-        auto work = [&](int c, auto follows) {
-            constexpr int FOLLOWS = decltype(follows)::value;
+        tiles(begin, [&](int c, auto follows) INLINED {
+            constexpr int F = decltype(follows)::value;
 #pragma unroll
             for (int st = 0; st < G::SHARE; ++st) {
                 const int byte = step_of(st) / 4 * 8;  // of the step's group
@@ -595,10 +609,10 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void fp8_staged_kernel(LinArgs p)
 #pragma unroll
                     for (int i = 0; i < MB; ++i)
                         decode2(ra[i], sa[i] >> byte, av[i]);
-                    if constexpr (FOLLOWS > 0)
+                    if constexpr (F > kEnd)
                         turn(c + 1, follows, sa, sw);
                 }
-                if (!last || FOLLOWS > 0) {
+                if (!last || F > kEnd) {
 #pragma unroll
                     for (int j = 0; j < NB; ++j)
                         rw[j] = piece(wo, j, 2 * next + half);
@@ -619,28 +633,27 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void fp8_staged_kernel(LinArgs p)
 #pragma unroll
                         for (int j = 0; j < NB; ++j)
                             acc[i][j] = mfma_bf16(wv[j][q], av[i][q], acc[i][j]);
-                    if (last && FOLLOWS == 2) {
-                        copies(c + S, fill, i, MB);
+                    if (last && F >= kCopy) {
+                        copies(c + S, fill(), i, MB);
                         __builtin_amdgcn_sched_barrier(0);
                     }
                 }
             }
-        };
-        tile(begin, work);
+        });
     } else {
         // A step is 64 elements, 32 of each half, one fp8 MFMA.  The fragments of W
         // have two sets of registers; those of A too in small blocks, and in large ones
         // one, a block of rows' next fragment read behind its last product.
-        constexpr bool ONE = MB * NB >= 8;
+        constexpr bool ONE = MB * NB >= 6;
         constexpr int SETS = ONE ? 1 : 2;
         i32x8 fa[SETS][MB], fw[2][NB];
-        auto read = [&](unsigned row, int b, int st) {
+        auto read = [&](unsigned row, int b, int st) INLINED {
             const u32x4 x = piece(row, b, 4 * st + 2 * half);
             const u32x4 y = piece(row, b, 4 * st + 2 * half + 1);
             return __builtin_bit_cast(i32x8,
                                       __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
         };
-        auto begin = [&]() {
+        auto begin = [&]() INLINED {
 #pragma unroll
             for (int j = 0; j < NB; ++j)
                 fw[0][j] = read(wo, j, step_of(0));
@@ -648,55 +661,69 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void fp8_staged_kernel(LinArgs p)
             for (int i = 0; i < MB; ++i)
                 fa[0][i] = read(ao, i, step_of(0));
         };
-        auto work = [&](int c, auto follows) {
-            constexpr int FOLLOWS = decltype(follows)::value;
+        tiles(begin, [&](int c, auto follows) INLINED {
+            constexpr int F = decltype(follows)::value;
             unsigned na[MB], nw[NB];
 #pragma unroll
             for (int st = 0; st < G::SHARE; ++st) {
                 const int now = G::SHARE == 1 ? 0 : st & 1, nxt = now ^ 1;
-                const int na_set = ONE ? 0 : nxt, a_set = ONE ? 0 : now;
                 const int byte = step_of(st) / 2 * 8;  // of the step's group
                 const int next = step_of(st < LAST ? st + 1 : 0);
-                const bool last = st == LAST, go = !last || FOLLOWS > 0;
-                // What the next step's fragments need: with more than one block of rows it
-                // runs under the products of the first.
-                auto ahead = [&]() {
-                    if constexpr (FOLLOWS > 0)
+                const bool last = st == LAST, go = !last || F > kEnd;
+                auto mfma = [&](int i, int j) INLINED {
+                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+                        fw[now][j], fa[ONE ? 0 : now][i], acc[i][j], 0, 0, 0, int(sw[j] >> byte),
+                        0, int(sa[i] >> byte));
+                };
+                if constexpr (ONE) {
+                    // Between the products: the turn to the next chunk behind the first one,
+                    // then the next fragments, those of A behind their last product, and the
+                    // copies, one or two each (in lumps the products wait for them: 192 x
+                    // 256 by four waves 88 us, so 76).
+                    constexpr int N = MB * NB;
+#pragma unroll
+                    for (int k = 0; k < N; ++k) {
+                        const int i = k / NB, j = k % NB;
+                        mfma(i, j);
+                        __builtin_amdgcn_sched_barrier(0);
+                        if constexpr (F > kEnd)
+                            if (last && k == 0)
+                                turn(c + 1, follows, na, nw);
+                        if (go && k < NB)
+                            fw[nxt][k] = read(wo, k, next);
+                        if (last && F >= kCopy)
+                            copies(c + S, fill(), k, N);
+                        if (go && j == NB - 1)
+                            fa[0][i] = read(ao, i, next);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                } else {
+                    // Small blocks: all of the next step's fragments before its products.
+                    if constexpr (F > kEnd)
                         if (last)
                             turn(c + 1, follows, na, nw);
                     if (go) {
 #pragma unroll
                         for (int j = 0; j < NB; ++j)
                             fw[nxt][j] = read(wo, j, next);
-                        if constexpr (!ONE) {
 #pragma unroll
-                            for (int i = 0; i < MB; ++i)
-                                fa[na_set][i] = read(ao, i, next);
-                        }
+                        for (int i = 0; i < MB; ++i)
+                            fa[nxt][i] = read(ao, i, next);
                     }
                     __builtin_amdgcn_sched_barrier(0);
-                };
-                if constexpr (MB == 1)
-                    ahead();
 #pragma unroll
-                for (int i = 0; i < MB; ++i) {
+                    for (int i = 0; i < MB; ++i) {
 #pragma unroll
-                    for (int j = 0; j < NB; ++j)
-                        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-                            fw[now][j], fa[a_set][i], acc[i][j], 0, 0, 0, int(sw[j] >> byte), 0,
-                            int(sa[i] >> byte));
-                    __builtin_amdgcn_sched_barrier(0);
-                    if (MB > 1 && i == 0)
-                        ahead();
-                    if (last && FOLLOWS == 2)
-                        copies(c + S, fill, i, MB);
-                    if constexpr (ONE)
-                        if (go)
-                            fa[0][i] = read(ao, i, next);
-                    __builtin_amdgcn_sched_barrier(0);
+                        for (int j = 0; j < NB; ++j)
+                            mfma(i, j);
+                        __builtin_amdgcn_sched_barrier(0);
+                        if (last && F >= kCopy)
+                            copies(c + S, fill(), i, MB);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
                 }
             }
-            if constexpr (FOLLOWS == 0)
+            if constexpr (F == kEnd)
                 mfma_drain();
             else {
 #pragma unroll
@@ -716,8 +743,7 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void fp8_staged_kernel(LinArgs p)
                     }
                 }
             }
-        };
-        tile(begin, work);
+        });
     }
 }
 
@@ -753,23 +779,27 @@ __global__ __launch_bounds__(256) void fp8_sum_kernel(const float *part, T *c, i
 // Shapes of the staged kernel, MB, NB, WM, WN, KS, S, and of the same with two groups
 // at once.
 #define STAGED_BF16(X) \
-    X(0, 4, 4, 2, 2, 1, 2, 128, 64) X(1, 3, 2, 2, 4, 1, 2, 128, 64) X(2, 2, 4, 2, 2, 1, 3, 128, 32) \
-    X(3, 2, 2, 2, 2, 1, 3, 128, 32) X(4, 1, 2, 2, 2, 1, 3, 128, 16) X(5, 1, 1, 2, 2, 1, 4, 128, 32) \
-    X(6, 1, 1, 1, 2, 2, 4, 128, 32)
+    X(0, 4, 4, 2, 2, 1, 2, 128) X(1, 3, 2, 2, 4, 1, 2, 128) \
+    X(2, 2, 4, 2, 2, 1, 2, 128) X(3, 2, 2, 2, 2, 1, 2, 128) \
+    X(4, 1, 2, 2, 2, 1, 3, 128) X(5, 1, 1, 2, 2, 1, 4, 128) \
+    X(6, 1, 1, 1, 2, 2, 4, 128)
 #define PAIRED_BF16(X) \
-    X(4, 1, 2, 2, 2, 2, 2, 256, 32) X(5, 1, 1, 2, 2, 2, 3, 256, 32) X(6, 1, 1, 1, 2, 4, 3, 256, 32)
+    X(4, 1, 2, 2, 2, 2, 2, 256) X(5, 1, 1, 2, 2, 2, 3, 256) \
+    X(6, 1, 1, 1, 2, 4, 3, 256)
 #define STAGED_F32(X) \
-    X(0, 2, 4, 4, 2, 1, 2, 128, 64) X(1, 1, 4, 4, 2, 1, 3, 128, 32) X(2, 2, 2, 2, 2, 1, 3, 128, 32) \
-    X(3, 1, 2, 2, 2, 1, 3, 128, 16) X(4, 1, 1, 2, 2, 1, 4, 128, 32) X(5, 1, 1, 1, 2, 2, 4, 128, 32)
+    X(0, 2, 4, 4, 2, 1, 2, 128) X(1, 1, 4, 4, 2, 1, 3, 128) \
+    X(2, 2, 2, 2, 2, 1, 2, 128) X(3, 1, 2, 2, 2, 1, 3, 128) \
+    X(4, 1, 1, 2, 2, 1, 4, 128) X(5, 1, 1, 1, 2, 2, 4, 128)
 #define PAIRED_F32(X) \
-    X(3, 1, 2, 2, 2, 2, 2, 256, 32) X(4, 1, 1, 2, 2, 2, 3, 256, 32) X(5, 1, 1, 1, 2, 4, 3, 256, 32)
+    X(3, 1, 2, 2, 2, 2, 2, 256) X(4, 1, 1, 2, 2, 2, 3, 256) \
+    X(5, 1, 1, 1, 2, 4, 3, 256)
 
 #define SHAPE_CHECK(table, i, mb, nb, wm, wn, kc) \
     static_assert(table[i].bm == 32 * mb * wm && table[i].bn == 32 * nb * wn && \
                   (kc == 128 || table[i].pairs), "shape table");
-#define CHECK_BF16(i, mb, nb, wm, wn, ks, s, kc, sec) \
+#define CHECK_BF16(i, mb, nb, wm, wn, ks, s, kc) \
     SHAPE_CHECK(kBf16Shapes, i, mb, nb, wm, wn, kc)
-#define CHECK_F32(i, mb, nb, wm, wn, ks, s, kc, sec) \
+#define CHECK_F32(i, mb, nb, wm, wn, ks, s, kc) \
     SHAPE_CHECK(kF32Shapes, i, mb, nb, wm, wn, kc)
 STAGED_BF16(CHECK_BF16)
 PAIRED_BF16(CHECK_BF16)
@@ -777,19 +807,18 @@ STAGED_F32(CHECK_F32)
 PAIRED_F32(CHECK_F32)
 
 constexpr int kPairs = 16;  // beside a shape's number: two groups at once
-#define STAGED_CASE(i, mb, nb, wm, wn, ks, s, kc, sec)                                           \
+#define STAGED_CASE(i, mb, nb, wm, wn, ks, s, kc)                                           \
     case i + (kc == 256 ? kPairs : 0):                                                           \
-        launch_staged<T, mb, nb, wm, wn, ks, s, kc, sec>(p, items, st);                          \
+        launch_staged<T, mb, nb, wm, wn, ks, s, kc>(p, items, st);                         \
         break;
 
-template <typename T, int MB, int NB, int WM, int WN, int KS, int S, int KC, int SEC>
+template <typename T, int MB, int NB, int WM, int WN, int KS, int S, int KC>
 void launch_staged(const LinArgs &p, int64_t items, hipStream_t st)
 {
-    using G = Staged<T, MB, NB, WM, WN, KS, S, KC, SEC>;
+    using G = Staged<T, MB, NB, WM, WN, KS, S, KC>;
     // As many workgroups as the CUs hold at once, where they take tiles in turn.
-    constexpr int64_t room = 256 * (163840 / G::LDS < 2 ? 1 : 2);
-    const dim3 grid(unsigned(G::TURNS ? std::min(items, room) : items));
-    hipLaunchKernelGGL((fp8_staged_kernel<T, MB, NB, WM, WN, KS, S, KC, SEC>), grid,
+    const dim3 grid(unsigned(G::TURN ? std::min<int64_t>(items, 256 * G::ROOM) : items));
+    hipLaunchKernelGGL((fp8_staged_kernel<T, MB, NB, WM, WN, KS, S, KC>), grid,
                        dim3(G::THREADS), 0, st, p);
 }
 
