@@ -65,6 +65,12 @@ __device__ __forceinline__ bf16x8 decode8(unsigned lo, unsigned hi, float scale)
     return __builtin_bit_cast(bf16x8, v);
 }
 
+// Two 16-byte pieces of a row as one operand of the fp8 MFMA.
+__device__ __forceinline__ i32x8 whole(const u32x4 &x, const u32x4 &y)
+{
+    return __builtin_bit_cast(i32x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
 // Four consecutive columns of C from nn on.
 __device__ __forceinline__ void store4(float *row, int nn, int N, bool wide, f32x4 v)
 {
@@ -93,117 +99,94 @@ __device__ __forceinline__ void store4(uint16_t *row, int nn, int N, bool wide, 
 
 // ------------------------------------------------------------- few rows
 
-// A workgroup takes 16 weight rows and up to 16 MB rows of A; its waves share the
-// groups of K, and both operands go from memory to registers to the MFMA.  Lane (n, g)
-// holds bytes 16 g and 64 + 16 g on of row n's 128: the products' order within
-// a group is free as long as both operands have the same.
-template <typename T, int MB, int WAVES>
+// A workgroup takes 16 weight rows and 16 rows of A; its waves share the groups of K,
+// kDepth of them on their way at once, and both operands go from memory to registers to the
+// MFMA.  Lane (n, g) holds bytes 16 g and 64 + 16 g on of row n's 128: the products' order
+// within a group is free as long as both operands have the same.
+// For small products, bound by latency: 1 x 2048 x 2048 takes 4.1 us.  Its loads, 64 bytes
+// of each of 16 rows, keep less on its way than whole lines by DMA do, so long sums and
+// large weights go through the tiles whatever the rows (1 x 2048 x 8192: 9.9 us here, 8.3
+// there; 1 x 131072 x 2048: 50 and 47).
+
+constexpr int kDepth = 4;
+
+template <typename T, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void fp8_few_kernel(LinArgs p)
 {
     constexpr bool EXACT = sizeof(T) == 4;
-    __shared__ f32x4 red[WAVES > 1 ? WAVES * MB * 64 : 1];
+    __shared__ f32x4 red[WAVES > 1 ? WAVES * 64 : 1];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 15, g = lane >> 4;
-    const unsigned blocks_m = (unsigned(p.M) + 16 * MB - 1) / (16 * MB);
+    const unsigned blocks_m = (unsigned(p.M) + 15) / 16;
     const unsigned strip = blockIdx.x / blocks_m;
-    const int row0 = int(strip) * 16, m0 = int(blockIdx.x - strip * blocks_m) * (16 * MB);
-    const int wrow = min(row0 + n, p.N - 1);
-    int arow[MB];
-#pragma unroll
-    for (int i = 0; i < MB; ++i)
-        arow[i] = min(m0 + 16 * i + n, p.M - 1);
+    const int row0 = int(strip) * 16, m0 = int(blockIdx.x - strip * blocks_m) * 16;
+    const int wrow = min(row0 + n, p.N - 1), arow = min(m0 + n, p.M - 1);
 
     struct Piece {
-        u32x4 w[2], a[MB][2];
-        unsigned ws, as[MB];
+        u32x4 w[2], a[2];
+        unsigned ws, as;
     };
     auto load = [&](int grp, Piece &x) {
         const uint8_t *w = p.w + (int64_t(wrow) * p.groups + grp) * kGroup + 16 * g;
-        x.w[0] = *reinterpret_cast<const u32x4 *>(w);
-        x.w[1] = *reinterpret_cast<const u32x4 *>(w + 64);
-        x.ws = p.ws[int64_t(wrow) * p.sg + grp];
+        const uint8_t *a = p.a + (int64_t(arow) * p.groups + grp) * kGroup + 16 * g;
 #pragma unroll
-        for (int i = 0; i < MB; ++i) {
-            const uint8_t *a = p.a + (int64_t(arow[i]) * p.groups + grp) * kGroup + 16 * g;
-            x.a[i][0] = *reinterpret_cast<const u32x4 *>(a);
-            x.a[i][1] = *reinterpret_cast<const u32x4 *>(a + 64);
-            x.as[i] = p.as[int64_t(arow[i]) * p.sg + grp];
+        for (int h = 0; h < 2; ++h) {
+            x.w[h] = *reinterpret_cast<const u32x4 *>(w + 64 * h);
+            x.a[h] = *reinterpret_cast<const u32x4 *>(a + 64 * h);
         }
+        x.ws = p.ws[int64_t(wrow) * p.sg + grp];
+        x.as = p.as[int64_t(arow) * p.sg + grp];
     };
-    f32x4 acc[MB];
-#pragma unroll
-    for (int i = 0; i < MB; ++i)
-        acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     auto multiply = [&](const Piece &x) {
         if constexpr (EXACT) {
-            const float ws = scale_of(x.ws);
-            bf16x8 w[4];
+            const float ws = scale_of(x.ws), as = scale_of(x.as);
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                w[j] = decode8(x.w[j >> 1][2 * (j & 1)], x.w[j >> 1][2 * (j & 1) + 1], ws);
-#pragma unroll
-            for (int i = 0; i < MB; ++i) {
-                const float as = scale_of(x.as[i]);
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    acc[i] = mfma16(w[j],
-                                    decode8(x.a[i][j >> 1][2 * (j & 1)],
-                                            x.a[i][j >> 1][2 * (j & 1) + 1], as),
-                                    acc[i]);
-            }
+                acc = mfma16(decode8(x.w[j >> 1][2 * (j & 1)], x.w[j >> 1][2 * (j & 1) + 1], ws),
+                             decode8(x.a[j >> 1][2 * (j & 1)], x.a[j >> 1][2 * (j & 1) + 1], as),
+                             acc);
         } else {
-            i32x8 w;
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                w[j] = int(x.w[j >> 2][j & 3]);
-#pragma unroll
-            for (int i = 0; i < MB; ++i) {
-                i32x8 a;
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    a[j] = int(x.a[i][j >> 2][j & 3]);
-                acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-                    w, a, acc[i], 0, 0, 0, int(x.ws), 0, int(x.as[i]));
-            }
+            acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                whole(x.w[0], x.w[1]), whole(x.a[0], x.a[1]), acc, 0, 0, 0, int(x.ws), 0,
+                int(x.as));
         }
     };
-    Piece cur, next;
-    if (wave < p.groups)
-        load(wave, cur);
-    for (int grp = wave; grp < p.groups; grp += WAVES) {
-        if (grp + WAVES < p.groups)
-            load(grp + WAVES, next);
-        multiply(cur);
-        cur = next;
+    Piece ring[kDepth];
+#pragma unroll
+    for (int d = 0; d < kDepth; ++d)
+        if (wave + d * WAVES < p.groups)
+            load(wave + d * WAVES, ring[d]);
+    for (int grp = wave; grp < p.groups; grp += kDepth * WAVES) {
+#pragma unroll
+        for (int d = 0; d < kDepth; ++d) {
+            const int at = grp + d * WAVES;
+            if (at >= p.groups)
+                break;
+            multiply(ring[d]);
+            if (at + kDepth * WAVES < p.groups)
+                load(at + kDepth * WAVES, ring[d]);
+        }
         if constexpr (!EXACT)
             mfma_drain();
     }
     if constexpr (WAVES > 1) {
         // The waves' sums in wave order.
-#pragma unroll
-        for (int i = 0; i < MB; ++i)
-            red[(wave * MB + i) * 64 + lane] = acc[i];
+        red[wave * 64 + lane] = acc;
         __syncthreads();
+        if (wave > 0)
+            return;
+        acc = red[lane];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w)
+            acc += red[w * 64 + lane];
     }
+    // Lane (n, g): columns 4g .. 4g+3 of row n.
     const bool wide = (reinterpret_cast<uintptr_t>(p.c) & (4 * sizeof(T) - 1)) == 0 &&
                       p.ldc % 4 == 0;
-#pragma unroll
-    for (int i = 0; i < MB; ++i) {
-        if (wave != i % WAVES)
-            continue;
-        f32x4 sum = acc[i];
-        if constexpr (WAVES > 1) {
-            sum = red[i * 64 + lane];
-#pragma unroll
-            for (int w = 1; w < WAVES; ++w)
-                sum += red[(w * MB + i) * 64 + lane];
-        }
-        // Lane (n, g): columns 4g .. 4g+3 of row n.
-        const int m = m0 + 16 * i + n;
-        if (m < p.M)
-            store4(static_cast<T *>(p.c) + int64_t(m) * p.ldc, row0 + 4 * g, p.N, wide, sum);
-    }
+    if (m0 + n < p.M)
+        store4(static_cast<T *>(p.c) + int64_t(m0 + n) * p.ldc, row0 + 4 * g, p.N, wide, acc);
 }
 
 // --------------------------------------------------------- staged tiles
@@ -648,10 +631,7 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void fp8_staged_kernel(LinArgs p)
         constexpr int SETS = ONE ? 1 : 2;
         i32x8 fa[SETS][MB], fw[2][NB];
         auto read = [&](unsigned row, int b, int st) INLINED {
-            const u32x4 x = piece(row, b, 4 * st + 2 * half);
-            const u32x4 y = piece(row, b, 4 * st + 2 * half + 1);
-            return __builtin_bit_cast(i32x8,
-                                      __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+            return whole(piece(row, b, 4 * st + 2 * half), piece(row, b, 4 * st + 2 * half + 1));
         };
         auto begin = [&]() INLINED {
 #pragma unroll
@@ -776,40 +756,30 @@ __global__ __launch_bounds__(256) void fp8_sum_kernel(const float *part, T *c, i
 
 // -------------------------------------------------------------- launches
 
-// Shapes of the staged kernel, MB, NB, WM, WN, KS, S, and of the same with two groups
-// at once.
+// Shapes of the staged kernel: MB, NB, WM, WN, KS, S, KC.
 #define STAGED_BF16(X) \
-    X(0, 4, 4, 2, 2, 1, 2, 128) X(1, 3, 2, 2, 4, 1, 2, 128) \
-    X(2, 2, 4, 2, 2, 1, 2, 128) X(3, 2, 2, 2, 2, 1, 2, 128) \
-    X(4, 1, 2, 2, 2, 1, 3, 128) X(5, 1, 1, 2, 2, 1, 4, 128) \
-    X(6, 1, 1, 1, 2, 2, 4, 128)
-#define PAIRED_BF16(X) \
-    X(4, 1, 2, 2, 2, 2, 2, 256) X(5, 1, 1, 2, 2, 2, 3, 256) \
-    X(6, 1, 1, 1, 2, 4, 3, 256)
+    X(0, 4, 4, 2, 2, 1, 2, 128) X(1, 3, 2, 2, 4, 1, 2, 128) X(2, 2, 4, 2, 2, 1, 2, 128) \
+    X(3, 2, 2, 2, 2, 1, 2, 128) X(4, 2, 1, 2, 2, 1, 3, 128) X(5, 1, 2, 2, 2, 1, 3, 128) \
+    X(6, 1, 1, 2, 2, 1, 4, 128) X(7, 1, 1, 2, 2, 2, 3, 256) X(8, 1, 1, 1, 2, 2, 4, 128) \
+    X(9, 1, 1, 1, 2, 4, 3, 256)
 #define STAGED_F32(X) \
-    X(0, 2, 4, 4, 2, 1, 2, 128) X(1, 1, 4, 4, 2, 1, 3, 128) \
-    X(2, 2, 2, 2, 2, 1, 2, 128) X(3, 1, 2, 2, 2, 1, 3, 128) \
-    X(4, 1, 1, 2, 2, 1, 4, 128) X(5, 1, 1, 1, 2, 2, 4, 128)
-#define PAIRED_F32(X) \
-    X(3, 1, 2, 2, 2, 2, 2, 256) X(4, 1, 1, 2, 2, 2, 3, 256) \
-    X(5, 1, 1, 1, 2, 4, 3, 256)
+    X(0, 2, 4, 4, 2, 1, 2, 128) X(1, 3, 2, 2, 4, 1, 2, 128) X(2, 2, 2, 2, 4, 1, 2, 128) \
+    X(3, 2, 2, 2, 2, 1, 2, 128) X(4, 1, 2, 2, 2, 1, 3, 128) X(5, 1, 2, 2, 2, 2, 2, 256) \
+    X(6, 1, 1, 2, 2, 1, 4, 128) X(7, 1, 1, 2, 2, 2, 3, 256) X(8, 1, 1, 1, 2, 2, 4, 128) \
+    X(9, 1, 1, 1, 2, 4, 3, 256)
 
-#define SHAPE_CHECK(table, i, mb, nb, wm, wn, kc) \
+#define SHAPE_CHECK(table, T, i, mb, nb, wm, wn, ks, s, kc) \
     static_assert(table[i].bm == 32 * mb * wm && table[i].bn == 32 * nb * wn && \
-                  (kc == 128 || table[i].pairs), "shape table");
-#define CHECK_BF16(i, mb, nb, wm, wn, ks, s, kc) \
-    SHAPE_CHECK(kBf16Shapes, i, mb, nb, wm, wn, kc)
-#define CHECK_F32(i, mb, nb, wm, wn, ks, s, kc) \
-    SHAPE_CHECK(kF32Shapes, i, mb, nb, wm, wn, kc)
+                  table[i].groups == kc / kGroup && \
+                  table[i].room == Staged<T, mb, nb, wm, wn, ks, s, kc>::ROOM, "shape table");
+#define CHECK_BF16(...) SHAPE_CHECK(kBf16Shapes, uint16_t, __VA_ARGS__)
+#define CHECK_F32(...) SHAPE_CHECK(kF32Shapes, float, __VA_ARGS__)
 STAGED_BF16(CHECK_BF16)
-PAIRED_BF16(CHECK_BF16)
 STAGED_F32(CHECK_F32)
-PAIRED_F32(CHECK_F32)
 
-constexpr int kPairs = 16;  // beside a shape's number: two groups at once
-#define STAGED_CASE(i, mb, nb, wm, wn, ks, s, kc)                                           \
-    case i + (kc == 256 ? kPairs : 0):                                                           \
-        launch_staged<T, mb, nb, wm, wn, ks, s, kc>(p, items, st);                         \
+#define STAGED_CASE(i, mb, nb, wm, wn, ks, s, kc)                   \
+    case i:                                                         \
+        launch_staged<T, mb, nb, wm, wn, ks, s, kc>(p, items, st);  \
         break;
 
 template <typename T, int MB, int NB, int WM, int WN, int KS, int S, int KC>
@@ -832,18 +802,14 @@ bool run_staged(LinArgs p, const LinPlan &pl, hipStream_t st)
     const int64_t items = int64_t(pl.tiles_m) * pl.tiles_n * pl.splits;
     if (!launch_fits(items, 512))
         return fail("linear_fp8_dev: too many tiles for one launch");
-    const int shape = pl.shape + (pl.pairs ? kPairs : 0);
-    if constexpr (sizeof(T) == 2) {
-        switch (shape) {
+    if constexpr (sizeof(T) == 2)
+        switch (pl.shape) {
             STAGED_BF16(STAGED_CASE)
-            PAIRED_BF16(STAGED_CASE)
         }
-    } else {
-        switch (shape) {
+    else
+        switch (pl.shape) {
             STAGED_F32(STAGED_CASE)
-            PAIRED_F32(STAGED_CASE)
         }
-    }
     if (!hip_ok(hipGetLastError(), "fp8_staged_kernel launch"))
         return false;
     if (pl.splits == 1)
@@ -854,20 +820,18 @@ bool run_staged(LinArgs p, const LinPlan &pl, hipStream_t st)
     return hip_ok(hipGetLastError(), "fp8_sum_kernel launch");
 }
 
-template <typename T, int MB>
+template <typename T>
 bool run_few(const LinArgs &p, int waves, hipStream_t st)
 {
-    const int64_t strips = (p.N + 15) / 16, blocks_m = (p.M + 16 * MB - 1) / (16 * MB);
-    if (!launch_fits(strips * blocks_m, waves * 64))
+    const int64_t blocks = (int64_t(p.N) + 15) / 16 * ((int64_t(p.M) + 15) / 16);
+    if (!launch_fits(blocks, waves * 64))
         return fail("linear_fp8_dev: too many rows for one launch");
-    // Blocks of A rows inside: those of one strip read its weights at about the same time.
-    const dim3 grid(unsigned(strips * blocks_m));
+    const dim3 grid(static_cast<unsigned>(blocks));
     switch (waves) {
-    case 1: hipLaunchKernelGGL((fp8_few_kernel<T, MB, 1>), grid, dim3(64), 0, st, p); break;
-    case 2: hipLaunchKernelGGL((fp8_few_kernel<T, MB, 2>), grid, dim3(128), 0, st, p); break;
-    case 4: hipLaunchKernelGGL((fp8_few_kernel<T, MB, 4>), grid, dim3(256), 0, st, p); break;
-    case 8: hipLaunchKernelGGL((fp8_few_kernel<T, MB, 8>), grid, dim3(512), 0, st, p); break;
-    default: hipLaunchKernelGGL((fp8_few_kernel<T, MB, 16>), grid, dim3(1024), 0, st, p); break;
+    case 1: hipLaunchKernelGGL((fp8_few_kernel<T, 1>), grid, dim3(64), 0, st, p); break;
+    case 2: hipLaunchKernelGGL((fp8_few_kernel<T, 2>), grid, dim3(128), 0, st, p); break;
+    case 4: hipLaunchKernelGGL((fp8_few_kernel<T, 4>), grid, dim3(256), 0, st, p); break;
+    default: hipLaunchKernelGGL((fp8_few_kernel<T, 8>), grid, dim3(512), 0, st, p); break;
     }
     return hip_ok(hipGetLastError(), "fp8_few_kernel launch");
 }
@@ -875,11 +839,7 @@ bool run_few(const LinArgs &p, int waves, hipStream_t st)
 template <typename T>
 bool run_linear(const LinArgs &p, const LinPlan &pl, hipStream_t st)
 {
-    if (pl.staged)
-        return run_staged<T>(p, pl, st);
-    return pl.blocks == 1   ? run_few<T, 1>(p, pl.waves, st)
-           : pl.blocks == 2 ? run_few<T, 2>(p, pl.waves, st)
-                            : run_few<T, 4>(p, pl.waves, st);
+    return pl.staged ? run_staged<T>(p, pl, st) : run_few<T>(p, pl.waves, st);
 }
 
 }  // namespace
