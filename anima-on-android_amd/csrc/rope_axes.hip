@@ -7,21 +7,22 @@
 // the rest of a row is copied.
 //
 // Bound by HBM: every value is read and written once, against six operations a
-// pair.  A workgroup takes the tokens that give each thread about two vector
-// pairs, computes their angles' cosines and sines once for all heads into LDS, and turns
-// 16 bytes of either half of a pair per thread.
+// pair.  A workgroup takes the tokens that give each thread one chunk, up to 16 bytes of
+// either member of its pairs, and computes their angles' cosines and sines once for all
+// heads into LDS while the chunks are on their way.  2 x 4096 tokens of 32 f32 heads of
+// 128: 40 us, 6.7 TB/s (much of it from the last-level cache); 30003 tokens of 14 bf16 heads
+// of 64: 18.4 us, 5.8 TB/s.  Rows that no vector fits go by single elements, a third to a
+// half of that.
 #include "flash_tile.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace anima_hip {
 namespace {
 
-using flash_tile::aligned;
 using flash_tile::bf16x2;
 using flash_tile::f32x2;
-using flash_tile::f32x4;
-using flash_tile::u32x4;
 
 constexpr int kThreads = 256;
 constexpr int kTable = 1024;  // angles of a workgroup, most
@@ -48,46 +49,35 @@ struct RopeArgs {
     int S, axes, pairs, D, heads_q;
     int per_block;     // tokens of a workgroup
     Divisor items, chunks;  // of a token, of a head
+    Divisor pairs_by, sequence;  // by pairs, by S where a workgroup's tokens are more
     int turned;        // chunks of a head that turn; the rest are copied
     bool inverse;
 };
 
 template <typename T, int V>
-struct Vec;
-template <>
-struct Vec<float, 4> {
-    f32x4 v;
-    __device__ __forceinline__ float get(int i) const { return v[i]; }
-    __device__ __forceinline__ void set(const float (&x)[4]) { v = f32x4{x[0], x[1], x[2], x[3]}; }
-};
-template <>
-struct Vec<uint16_t, 8> {
-    u32x4 v;
+struct alignas(V * sizeof(T)) Vec {
+    using Word = std::conditional_t<sizeof(T) == 4 || V == 1, T, unsigned>;
+    static constexpr int kEach = sizeof(Word) / sizeof(T);
+    Word v[V / kEach];
     __device__ __forceinline__ float get(int i) const
     {
-        return __uint_as_float(i & 1 ? v[i >> 1] & 0xFFFF0000u : v[i >> 1] << 16);
+        if constexpr (sizeof(T) == 4)
+            return v[i];
+        else
+            return __uint_as_float(i % kEach ? v[i / kEach] & 0xFFFF0000u
+                                             : unsigned(v[i / kEach]) << 16);
     }
-    __device__ __forceinline__ void set(const float (&x)[8])
+    __device__ __forceinline__ void set(const float (&x)[V])
     {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            v[i] = __builtin_bit_cast(
-                unsigned, __builtin_convertvector(f32x2{x[2 * i], x[2 * i + 1]}, bf16x2));
-    }
-};
-template <>
-struct Vec<float, 1> {
-    float v;
-    __device__ __forceinline__ float get(int) const { return v; }
-    __device__ __forceinline__ void set(const float (&x)[1]) { v = x[0]; }
-};
-template <>
-struct Vec<uint16_t, 1> {
-    uint16_t v;
-    __device__ __forceinline__ float get(int) const { return __uint_as_float(unsigned(v) << 16); }
-    __device__ __forceinline__ void set(const float (&x)[1])
-    {
-        v = __builtin_bit_cast(uint16_t, static_cast<__bf16>(x[0]));
+        for (int i = 0; i < V / kEach; ++i)
+            if constexpr (sizeof(T) == 4)
+                v[i] = x[i];
+            else if constexpr (kEach == 2)
+                v[i] = __builtin_bit_cast(
+                    unsigned, __builtin_convertvector(f32x2{x[2 * i], x[2 * i + 1]}, bf16x2));
+            else
+                v[i] = __builtin_bit_cast(uint16_t, static_cast<__bf16>(x[i]));
     }
 };
 
@@ -99,71 +89,106 @@ __global__ __launch_bounds__(kThreads) void rope_axes_kernel(RopeArgs p)
     __shared__ float2 table[kTable];
     const int64_t token0 = int64_t(blockIdx.x) * p.per_block;
     const int n = int(min<int64_t>(p.per_block, p.tokens - token0));
-    for (int i = threadIdx.x; i < n * p.pairs; i += kThreads) {
-        const int t = i / p.pairs, pair = i - t * p.pairs;
-        const int64_t token = token0 + t;
-        const int64_t b = token / p.S;
-        const int s = int(token - b * p.S);
-        const int a = p.axis ? min(int(p.axis[pair]), p.axes - 1) : 0;
-        // In turns, in 64 bits: a far position's angle keeps its place within the
-        // turn to 2^-53 of itself.
-        const double turns = double(p.pos[b * p.pos_batch + int64_t(s) * p.axes + a]) *
-                             p.freqs[pair] * 0.15915494309189535;
-        float sn, cs;
-        sincospif(2.0f * float(turns - rint(turns)), &sn, &cs);
-        table[i] = float2{cs, p.inverse ? -sn : sn};
-    }
-    __syncthreads();
-    for (unsigned i = threadIdx.x; i < n * p.items.d; i += kThreads) {
+    // Uniform: the only 64-bit division.
+    const int64_t b0 = token0 / p.S;
+    const unsigned s0 = unsigned(token0 - b0 * p.S);
+    struct Place {
+        int64_t b;
+        int s;
+    };
+    const auto place = [&](unsigned t) {
+        const unsigned at = s0 + t;
+        const unsigned on = p.S >= p.per_block ? unsigned(at >= unsigned(p.S))
+                                               : p.sequence.quotient(at);
+        return Place{b0 + on, int(at - on * unsigned(p.S))};
+    };
+    // Where an item's two vectors lie.
+    struct Item {
+        T *dst;
+        const float2 *cs;
+        X x0, x1;
+        int d0, d1;  // d1 < 0: none
+        bool turn;
+    };
+    const auto fetch = [&](unsigned i, Item &it) {
         const unsigned t = p.per_block == 1 ? 0u : p.items.quotient(i);
         const unsigned item = i - t * p.items.d;
         int h = int(p.chunks.quotient(item));
         const int c = int(item - h * p.chunks.d);
-        const int64_t token = token0 + t;
-        const int64_t b = token / p.S;
-        const int s = int(token - b * p.S);
-        if (p.counts && s >= p.counts[b])
-            continue;
+        const Place at = place(t);
+        if (p.counts && at.s >= p.counts[at.b])
+            return false;
         const int which = h >= p.heads_q;
         h -= which ? p.heads_q : 0;
-        const T *src = static_cast<const T *>(p.in[which]) + b * p.is[which].b +
-                       h * p.is[which].h + s * p.is[which].s;
-        T *dst = static_cast<T *>(p.out[which]) + b * p.os[which].b + h * p.os[which].h +
-                 s * p.os[which].s;
-        if (c >= p.turned) {
-            const int d = 2 * p.pairs + (c - p.turned) * 2 * V;
-            *reinterpret_cast<X *>(dst + d) = *reinterpret_cast<const X *>(src + d);
-            if (d + V < p.D)
-                *reinterpret_cast<X *>(dst + d + V) = *reinterpret_cast<const X *>(src + d + V);
-            continue;
+        const T *src = static_cast<const T *>(p.in[which]) + at.b * p.is[which].b +
+                       h * p.is[which].h + at.s * p.is[which].s;
+        it.dst = static_cast<T *>(p.out[which]) + at.b * p.os[which].b + h * p.os[which].h +
+                 at.s * p.os[which].s;
+        it.turn = c < p.turned;
+        if (it.turn) {
+            it.d0 = NEIGHBOURS ? 2 * V * c : V * c;
+            it.d1 = NEIGHBOURS ? it.d0 + V : it.d0 + p.pairs;
+        } else {
+            it.d0 = 2 * p.pairs + (c - p.turned) * 2 * V;
+            it.d1 = it.d0 + V < p.D ? it.d0 + V : -1;
         }
-        const int d0 = NEIGHBOURS ? 2 * V * c : V * c, d1 = NEIGHBOURS ? d0 + V : d0 + p.pairs;
-        const X x0 = *reinterpret_cast<const X *>(src + d0);
-        const X x1 = *reinterpret_cast<const X *>(src + d1);
-        const float2 *cs = table + t * p.pairs + c * V;
+        it.cs = table + t * p.pairs + c * V;
+        it.x0 = *reinterpret_cast<const X *>(src + it.d0);
+        if (it.d1 >= 0)
+            it.x1 = *reinterpret_cast<const X *>(src + it.d1);
+        return true;
+    };
+    const auto turn = [&](Item &it) {
         float y0[V], y1[V];
         if constexpr (NEIGHBOURS && V > 1) {
 #pragma unroll
             for (int j = 0; j < V; j += 2) {
-                const float2 u = cs[j / 2], w = cs[V / 2 + j / 2];
-                y0[j] = x0.get(j) * u.x - x0.get(j + 1) * u.y;
-                y0[j + 1] = x0.get(j + 1) * u.x + x0.get(j) * u.y;
-                y1[j] = x1.get(j) * w.x - x1.get(j + 1) * w.y;
-                y1[j + 1] = x1.get(j + 1) * w.x + x1.get(j) * w.y;
+                const float2 u = it.cs[j / 2], w = it.cs[V / 2 + j / 2];
+                y0[j] = it.x0.get(j) * u.x - it.x0.get(j + 1) * u.y;
+                y0[j + 1] = it.x0.get(j + 1) * u.x + it.x0.get(j) * u.y;
+                y1[j] = it.x1.get(j) * w.x - it.x1.get(j + 1) * w.y;
+                y1[j + 1] = it.x1.get(j + 1) * w.x + it.x1.get(j) * w.y;
             }
         } else {
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float2 u = cs[j];
-                y0[j] = x0.get(j) * u.x - x1.get(j) * u.y;
-                y1[j] = x1.get(j) * u.x + x0.get(j) * u.y;
+                const float2 u = it.cs[j];
+                y0[j] = it.x0.get(j) * u.x - it.x1.get(j) * u.y;
+                y1[j] = it.x1.get(j) * u.x + it.x0.get(j) * u.y;
             }
         }
-        X z;
-        z.set(y0);
-        *reinterpret_cast<X *>(dst + d0) = z;
-        z.set(y1);
-        *reinterpret_cast<X *>(dst + d1) = z;
+        it.x0.set(y0);
+        it.x1.set(y1);
+    };
+    const unsigned items = n * p.items.d;
+    for (unsigned first = 0; first < items; first += kThreads) {
+        const unsigned i = first + threadIdx.x;
+        Item it;
+        const bool live = i < items && fetch(i, it);
+        if (first == 0) {
+            // The angles while the first rows are on their way.
+            for (unsigned j = threadIdx.x; j < unsigned(n * p.pairs); j += kThreads) {
+                const unsigned t = p.pairs_by.quotient(j), pair = j - t * p.pairs;
+                const Place at = place(t);
+                const int a = p.axis ? min(int(p.axis[pair]), p.axes - 1) : 0;
+                // In turns, in 64 bits: a far position's angle keeps its place within the
+                // turn to 2^-53 of itself.
+                const double turns =
+                    double(p.pos[at.b * p.pos_batch + int64_t(at.s) * p.axes + a]) *
+                    p.freqs[pair] * 0.15915494309189535;
+                float sn, cs;
+                sincospif(2.0f * float(turns - rint(turns)), &sn, &cs);
+                table[j] = float2{cs, p.inverse ? -sn : sn};
+            }
+            __syncthreads();
+        }
+        if (!live)
+            continue;
+        if (it.turn)
+            turn(it);
+        *reinterpret_cast<X *>(it.dst + it.d0) = it.x0;
+        if (it.d1 >= 0)
+            *reinterpret_cast<X *>(it.dst + it.d1) = it.x1;
     }
 }
 
@@ -177,8 +202,13 @@ bool run_rope(const RopeAxes &a, RopeArgs &p, bool copies, hipStream_t st)
     // At most 1024 chunks of a head and 2^12 heads: every quotient is exact.
     p.chunks = Divisor(unsigned(chunks));
     p.items = Divisor(unsigned(chunks * heads));
-    // About two items a thread, and no more angles than the table holds.
-    p.per_block = std::max(1, std::min(2 * kThreads / (chunks * heads), kTable / a.pairs));
+    // A chunk a thread, or two that share their angles' table where the GPU is full anyway
+    // (12 + 2 bf16 heads of 64: 30003 tokens 18.4 us, with one each 19.3; 8 tokens of 16 + 4
+    // heads of 128 3.8 and 3.0), and no more angles than the table holds.
+    const int each = p.tokens * chunks * heads > 2048 * kThreads ? 2 : 1;
+    p.per_block = std::max(1, std::min(each * kThreads / (chunks * heads), kTable / a.pairs));
+    p.pairs_by = Divisor(unsigned(a.pairs));
+    p.sequence = Divisor(unsigned(std::min(a.S, 2 * kThreads)));
     const int64_t blocks = (p.tokens + p.per_block - 1) / p.per_block;
     if (blocks > UINT32_MAX / kThreads)
         return fail("rope_axes_dev: too many tokens for one launch");
@@ -217,22 +247,32 @@ bool launch_rope_axes(const RopeAxes &a, hipStream_t st)
     p.D = a.D;
     p.heads_q = a.H_q;
     p.inverse = a.inverse;
-    const int V = a.type == kMx4F32 ? 4 : 8;
-    // 16-byte vectors where every piece starts and ends on one.
-    bool vec = a.pairs % V == 0 && a.D % V == 0;
+    // The widest vectors, up to 16 bytes, on which every piece starts and ends.
+    const int bytes = a.type == kMx4F32 ? 4 : 2;
+    uint64_t bits = uint64_t(a.pairs) | a.D;
     bool copies = false;  // rows that are not turned in place have a rest to copy
     for (int i = 0; i < 2; ++i) {
         if ((i ? a.H_k : a.H_q) == 0)
             continue;
         for (int64_t s : {p.is[i].b, p.is[i].h, p.is[i].s, p.os[i].b, p.os[i].h, p.os[i].s})
-            vec = vec && s % V == 0;
-        vec = vec && aligned(p.in[i], 16) && aligned(p.out[i], 16);
+            bits |= uint64_t(s);
+        bits |= (reinterpret_cast<uintptr_t>(p.in[i]) | reinterpret_cast<uintptr_t>(p.out[i])) /
+                bytes;
         copies = copies || p.in[i] != p.out[i];
     }
+    const int V = int(std::min<uint64_t>(bits & -bits, 16 / bytes));
     if (a.type == kMx4F32)
-        return vec ? run_rope<float, 4>(a, p, copies, st) : run_rope<float, 1>(a, p, copies, st);
-    return vec ? run_rope<uint16_t, 8>(a, p, copies, st)
-               : run_rope<uint16_t, 1>(a, p, copies, st);
+        switch (V) {
+        case 4: return run_rope<float, 4>(a, p, copies, st);
+        case 2: return run_rope<float, 2>(a, p, copies, st);
+        default: return run_rope<float, 1>(a, p, copies, st);
+        }
+    switch (V) {
+    case 8: return run_rope<uint16_t, 8>(a, p, copies, st);
+    case 4: return run_rope<uint16_t, 4>(a, p, copies, st);
+    case 2: return run_rope<uint16_t, 2>(a, p, copies, st);
+    default: return run_rope<uint16_t, 1>(a, p, copies, st);
+    }
 }
 
 }  // namespace anima_hip
