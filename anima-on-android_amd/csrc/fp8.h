@@ -24,6 +24,9 @@ using flash_tile::f32x4;
 using flash_tile::u32x4;
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
+// 16 bytes at any element: the hardware takes vector accesses that are not aligned.
+typedef f32x4 any_f32x4 __attribute__((aligned(4)));
+typedef u32x4 any_u32x4 __attribute__((aligned(2)));
 
 constexpr int kGroup = 128;     // elements per scale
 constexpr int kNanScale = 255;  // scale byte of a group that held an infinity or a NaN
@@ -92,13 +95,12 @@ __device__ __forceinline__ void pack_group(const float (&x)[8], uint8_t *row_cod
         row_scales[g + piece] = piece == 0 ? uint8_t(s) : uint8_t(0);
 }
 
-// Elements k0 .. k0+7 of a row of K; zero past its end.  `vec`: 16-byte loads
-// of a whole piece.
-__device__ __forceinline__ void load8(const float *row, int k0, int K, bool vec, float (&x)[8])
+// Elements k0 .. k0+7 of a row of K; zero past its end.
+__device__ __forceinline__ void load8(const float *row, int k0, int K, float (&x)[8])
 {
-    if (vec && k0 + 8 <= K) {
-        const f32x4 a = *reinterpret_cast<const f32x4 *>(row + k0);
-        const f32x4 b = *reinterpret_cast<const f32x4 *>(row + k0 + 4);
+    if (k0 + 8 <= K) {
+        const f32x4 a = *reinterpret_cast<const any_f32x4 *>(row + k0);
+        const f32x4 b = *reinterpret_cast<const any_f32x4 *>(row + k0 + 4);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             x[i] = a[i];
@@ -111,10 +113,10 @@ __device__ __forceinline__ void load8(const float *row, int k0, int K, bool vec,
         x[i] = k0 + i < K ? row[k0 + i] : 0.0f;
 }
 
-__device__ __forceinline__ void load8(const uint16_t *row, int k0, int K, bool vec, float (&x)[8])
+__device__ __forceinline__ void load8(const uint16_t *row, int k0, int K, float (&x)[8])
 {
-    if (vec && k0 + 8 <= K) {
-        const u32x4 a = *reinterpret_cast<const u32x4 *>(row + k0);
+    if (k0 + 8 <= K) {
+        const u32x4 a = *reinterpret_cast<const any_u32x4 *>(row + k0);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             x[2 * i] = __uint_as_float(a[i] << 16);
@@ -128,11 +130,11 @@ __device__ __forceinline__ void load8(const uint16_t *row, int k0, int K, bool v
 }
 
 // The same elements stored, rounded to the row's type.
-__device__ __forceinline__ void store8(float *row, int k0, int K, bool vec, const float (&x)[8])
+__device__ __forceinline__ void store8(float *row, int k0, int K, const float (&x)[8])
 {
-    if (vec && k0 + 8 <= K) {
-        *reinterpret_cast<f32x4 *>(row + k0) = f32x4{x[0], x[1], x[2], x[3]};
-        *reinterpret_cast<f32x4 *>(row + k0 + 4) = f32x4{x[4], x[5], x[6], x[7]};
+    if (k0 + 8 <= K) {
+        *reinterpret_cast<any_f32x4 *>(row + k0) = f32x4{x[0], x[1], x[2], x[3]};
+        *reinterpret_cast<any_f32x4 *>(row + k0 + 4) = f32x4{x[4], x[5], x[6], x[7]};
         return;
     }
 #pragma unroll
@@ -146,14 +148,14 @@ __device__ __forceinline__ unsigned bf16_pair(float lo, float hi)
     return __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{lo, hi}, bf16x2));
 }
 
-__device__ __forceinline__ void store8(uint16_t *row, int k0, int K, bool vec, const float (&x)[8])
+__device__ __forceinline__ void store8(uint16_t *row, int k0, int K, const float (&x)[8])
 {
     u32x4 w;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
         w[i] = bf16_pair(x[2 * i], x[2 * i + 1]);
-    if (vec && k0 + 8 <= K) {
-        *reinterpret_cast<u32x4 *>(row + k0) = w;
+    if (k0 + 8 <= K) {
+        *reinterpret_cast<any_u32x4 *>(row + k0) = w;
         return;
     }
 #pragma unroll

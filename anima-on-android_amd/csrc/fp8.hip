@@ -12,7 +12,7 @@ using namespace fp8;
 template <typename T>
 __global__ __launch_bounds__(256) void fp8_pack_kernel(const T *x, int64_t ldx, uint8_t *codes,
                                                        uint8_t *scales, unsigned groups,
-                                                       unsigned total, int K, bool vec)
+                                                       unsigned total, int K)
 {
     const unsigned gi = blockIdx.x * 16u + (threadIdx.x >> 4);
     if (gi >= total)
@@ -21,7 +21,7 @@ __global__ __launch_bounds__(256) void fp8_pack_kernel(const T *x, int64_t ldx, 
     const unsigned row = gi / groups;
     const int g = int(gi - row * groups);
     float v[8];
-    load8(x + int64_t(row) * ldx, g * kGroup + 8 * piece, K, vec, v);
+    load8(x + int64_t(row) * ldx, g * kGroup + 8 * piece, K, v);
     pack_group(v, codes + int64_t(row) * groups * kGroup,
                scales + int64_t(row) * fp8_scale_bytes(K), g, int(groups), piece);
 }
@@ -29,8 +29,7 @@ __global__ __launch_bounds__(256) void fp8_pack_kernel(const T *x, int64_t ldx, 
 template <typename T>
 __global__ __launch_bounds__(256) void fp8_unpack_kernel(const uint8_t *codes,
                                                          const uint8_t *scales, T *x, int64_t ldx,
-                                                         unsigned groups, unsigned total, int K,
-                                                         bool vec)
+                                                         unsigned groups, unsigned total, int K)
 {
     const unsigned gi = blockIdx.x * 16u + (threadIdx.x >> 4);
     if (gi >= total)
@@ -53,7 +52,7 @@ __global__ __launch_bounds__(256) void fp8_unpack_kernel(const uint8_t *codes,
         v[4 * i + 2] = hi[0] * s;
         v[4 * i + 3] = hi[1] * s;
     }
-    store8(x + int64_t(row) * ldx, g * kGroup + 8 * piece, K, vec, v);
+    store8(x + int64_t(row) * ldx, g * kGroup + 8 * piece, K, v);
 }
 
 // ------------------------------------------------------------------ norm
@@ -66,7 +65,6 @@ struct NormArgs {
     int64_t ldx, ldr, lds, ldy, rows;
     int K;
     float eps;
-    bool vec;  // 16-byte accesses of whole pieces
 };
 
 // Sum of v over the wave, in all lanes.
@@ -94,10 +92,10 @@ __device__ __forceinline__ double inv_sqrt(double m)
 template <typename T>
 __device__ __forceinline__ void load_sum(const NormArgs &p, int64_t row, int k0, float (&h)[8])
 {
-    load8(static_cast<const T *>(p.x) + row * p.ldx, k0, p.K, p.vec, h);
+    load8(static_cast<const T *>(p.x) + row * p.ldx, k0, p.K, h);
     if (p.r) {
         float r[8];
-        load8(static_cast<const T *>(p.r) + row * p.ldr, k0, p.K, p.vec, r);
+        load8(static_cast<const T *>(p.r) + row * p.ldr, k0, p.K, r);
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             h[i] += r[i];
@@ -107,7 +105,7 @@ __device__ __forceinline__ void load_sum(const NormArgs &p, int64_t row, int k0,
 __device__ __forceinline__ void load_weight(const NormArgs &p, int k0, float (&w)[8])
 {
     if (p.w) {
-        load8(p.w, k0, p.K, p.vec, w);
+        load8(p.w, k0, p.K, w);
         return;
     }
 #pragma unroll
@@ -122,14 +120,14 @@ __device__ __forceinline__ void store_normed(const NormArgs &p, int64_t row, int
 {
     const int k0 = 8 * piece;
     if (p.sum)
-        store8(static_cast<T *>(p.sum) + row * p.lds, k0, p.K, p.vec, h);
+        store8(static_cast<T *>(p.sum) + row * p.lds, k0, p.K, h);
     float w[8], y[8];
     load_weight(p, k0, w);
 #pragma unroll
     for (int i = 0; i < 8; ++i)
         y[i] = k0 + i < p.K ? float(double(h[i]) * inv) * w[i] : 0.0f;
     if (p.y)
-        store8(static_cast<T *>(p.y) + row * p.ldy, k0, p.K, p.vec, y);
+        store8(static_cast<T *>(p.y) + row * p.ldy, k0, p.K, y);
     if (p.codes)
         pack_group(y, p.codes + row * groups * kGroup, p.scales + row * fp8_scale_bytes(p.K),
                    piece >> 4, groups, piece & 15);
@@ -209,13 +207,6 @@ __global__ __launch_bounds__(1024) void add_rmsnorm_long_kernel(NormArgs p)
     }
 }
 
-// Pieces of eight elements can move as 16-byte accesses: base, and every
-// stride in elements.
-bool wide(const void *p, int64_t ld, Mx4Type t)
-{
-    return flash_tile::aligned(p, 16) && ld % (t == kMx4F32 ? 4 : 8) == 0;
-}
-
 // Groups of a call, 16 threads each, in one launch of at most 2^32 threads.
 bool group_count(const char *who, int64_t rows, int64_t groups, unsigned &total)
 {
@@ -281,14 +272,12 @@ bool launch_fp8_pack(const void *x, int64_t ldx, Mx4Type type, uint8_t *codes, u
     if (total == 0)
         return true;
     const dim3 grid((total + 15) / 16), block(256);
-    const bool vec = wide(x, ldx, type);
     if (type == kMx4F32)
         hipLaunchKernelGGL(fp8_pack_kernel<float>, grid, block, 0, st,
-                           static_cast<const float *>(x), ldx, codes, scales, groups, total, K, vec);
+                           static_cast<const float *>(x), ldx, codes, scales, groups, total, K);
     else
         hipLaunchKernelGGL(fp8_pack_kernel<uint16_t>, grid, block, 0, st,
-                           static_cast<const uint16_t *>(x), ldx, codes, scales, groups, total, K,
-                           vec);
+                           static_cast<const uint16_t *>(x), ldx, codes, scales, groups, total, K);
     return hip_ok(hipGetLastError(), "fp8_pack_kernel launch");
 }
 
@@ -302,13 +291,12 @@ bool launch_fp8_unpack(const uint8_t *codes, const uint8_t *scales, void *x, int
     if (total == 0)
         return true;
     const dim3 grid((total + 15) / 16), block(256);
-    const bool vec = wide(x, ldx, type);
     if (type == kMx4F32)
         hipLaunchKernelGGL(fp8_unpack_kernel<float>, grid, block, 0, st, codes, scales,
-                           static_cast<float *>(x), ldx, groups, total, K, vec);
+                           static_cast<float *>(x), ldx, groups, total, K);
     else
         hipLaunchKernelGGL(fp8_unpack_kernel<uint16_t>, grid, block, 0, st, codes, scales,
-                           static_cast<uint16_t *>(x), ldx, groups, total, K, vec);
+                           static_cast<uint16_t *>(x), ldx, groups, total, K);
     return hip_ok(hipGetLastError(), "fp8_unpack_kernel launch");
 }
 
@@ -331,9 +319,6 @@ bool launch_add_rmsnorm_fp8(const AddRmsNorm &a, hipStream_t st)
     p.rows = a.rows;
     p.K = a.K;
     p.eps = a.eps;
-    p.vec = wide(a.x, a.ldx, a.type) && (!a.residual || wide(a.residual, a.ldr, a.type)) &&
-            (!a.sum || wide(a.sum, a.ldsum, a.type)) && (!a.y || wide(a.y, a.ldy, a.type)) &&
-            (!a.w || flash_tile::aligned(a.w, 16));
     return a.type == kMx4F32 ? launch_norm<float>(p, st) : launch_norm<uint16_t>(p, st);
 }
 
