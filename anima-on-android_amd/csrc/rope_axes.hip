@@ -11,12 +11,10 @@
 // either member of its pairs, and computes their angles' cosines and sines once for all
 // heads into LDS while the chunks are on their way.  2 x 4096 tokens of 32 f32 heads of
 // 128: 40 us, 6.7 TB/s (much of it from the last-level cache); 30003 tokens of 14 bf16 heads
-// of 64: 18.4 us, 5.8 TB/s.  Rows that no vector fits go by single elements, a third to a
-// half of that.
+// of 64: 18.4 us, 5.8 TB/s.
 #include "flash_tile.h"
 
 #include <algorithm>
-#include <type_traits>
 
 namespace anima_hip {
 namespace {
@@ -54,39 +52,72 @@ struct RopeArgs {
     bool inverse;
 };
 
+// V elements, in words of 32 bits.
 template <typename T, int V>
-struct alignas(V * sizeof(T)) Vec {
-    using Word = std::conditional_t<sizeof(T) == 4 || V == 1, T, unsigned>;
-    static constexpr int kEach = sizeof(Word) / sizeof(T);
-    Word v[V / kEach];
+struct Vec {
+    static constexpr int kEach = 4 / sizeof(T);
+    typedef unsigned Words __attribute__((ext_vector_type(V / kEach)));
+    typedef Words Anywhere __attribute__((aligned(sizeof(T))));  // as the hardware takes them
+    Words v;
+    // All of them, or with TAIL the first n.
+    template <bool TAIL>
+    __device__ __forceinline__ void load(const T *p, int n)
+    {
+        if (!TAIL || n >= V) {
+            v = *reinterpret_cast<const Anywhere *>(p);
+            return;
+        }
+        v = Words{};
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i < n) {
+                if constexpr (sizeof(T) == 4)
+                    v[i] = __float_as_uint(p[i]);
+                else
+                    v[i / 2] |= unsigned(p[i]) << (i % 2 * 16);
+            }
+    }
+    template <bool TAIL>
+    __device__ __forceinline__ void store(T *p, int n) const
+    {
+        if (!TAIL || n >= V) {
+            *reinterpret_cast<Anywhere *>(p) = v;
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i < n) {
+                if constexpr (sizeof(T) == 4)
+                    p[i] = __uint_as_float(v[i]);
+                else
+                    p[i] = uint16_t(v[i / 2] >> (i % 2 * 16));
+            }
+    }
     __device__ __forceinline__ float get(int i) const
     {
-        if constexpr (sizeof(T) == 4)
-            return v[i];
-        else
-            return __uint_as_float(i % kEach ? v[i / kEach] & 0xFFFF0000u
-                                             : unsigned(v[i / kEach]) << 16);
+        return __uint_as_float(sizeof(T) == 4 ? v[i]
+                               : i % 2        ? v[i / kEach] & 0xFFFF0000u
+                                              : v[i / kEach] << 16);
     }
     __device__ __forceinline__ void set(const float (&x)[V])
     {
 #pragma unroll
         for (int i = 0; i < V / kEach; ++i)
             if constexpr (sizeof(T) == 4)
-                v[i] = x[i];
-            else if constexpr (kEach == 2)
+                v[i] = __float_as_uint(x[i]);
+            else
                 v[i] = __builtin_bit_cast(
                     unsigned, __builtin_convertvector(f32x2{x[2 * i], x[2 * i + 1]}, bf16x2));
-            else
-                v[i] = __builtin_bit_cast(uint16_t, static_cast<__bf16>(x[i]));
     }
 };
 
-// A chunk is two vectors of V elements: V pairs of a head, or 2 V copied elements.
-template <typename T, int V, bool NEIGHBOURS>
+// A chunk is two vectors of V elements: V pairs of a head, or 2 V copied elements; the last
+// of either may hold fewer (TAIL).
+template <typename T, int V, bool NEIGHBOURS, bool TAIL>
 __global__ __launch_bounds__(kThreads) void rope_axes_kernel(RopeArgs p)
 {
     using X = Vec<T, V>;
-    __shared__ float2 table[kTable];
+    __shared__ float2 table[kTable + V];  // a head's last chunk reads past its angles
     const int64_t token0 = int64_t(blockIdx.x) * p.per_block;
     const int n = int(min<int64_t>(p.per_block, p.tokens - token0));
     // Uniform: the only 64-bit division.
@@ -107,7 +138,7 @@ __global__ __launch_bounds__(kThreads) void rope_axes_kernel(RopeArgs p)
         T *dst;
         const float2 *cs;
         X x0, x1;
-        int d0, d1;  // d1 < 0: none
+        int d0, d1, n0, n1;  // places, elements
         bool turn;
     };
     const auto fetch = [&](unsigned i, Item &it) {
@@ -128,19 +159,23 @@ __global__ __launch_bounds__(kThreads) void rope_axes_kernel(RopeArgs p)
         if (it.turn) {
             it.d0 = NEIGHBOURS ? 2 * V * c : V * c;
             it.d1 = NEIGHBOURS ? it.d0 + V : it.d0 + p.pairs;
+            it.n0 = NEIGHBOURS ? 2 * p.pairs - it.d0 : p.pairs - it.d0;
+            it.n1 = NEIGHBOURS ? it.n0 - V : it.n0;
         } else {
             it.d0 = 2 * p.pairs + (c - p.turned) * 2 * V;
-            it.d1 = it.d0 + V < p.D ? it.d0 + V : -1;
+            it.d1 = it.d0 + V;
+            it.n0 = p.D - it.d0;
+            it.n1 = it.n0 - V;
         }
         it.cs = table + t * p.pairs + c * V;
-        it.x0 = *reinterpret_cast<const X *>(src + it.d0);
-        if (it.d1 >= 0)
-            it.x1 = *reinterpret_cast<const X *>(src + it.d1);
+        it.x0.template load<TAIL>(src + it.d0, it.n0);
+        if (it.n1 > 0)
+            it.x1.template load<TAIL>(src + it.d1, it.n1);
         return true;
     };
     const auto turn = [&](Item &it) {
         float y0[V], y1[V];
-        if constexpr (NEIGHBOURS && V > 1) {
+        if constexpr (NEIGHBOURS) {
 #pragma unroll
             for (int j = 0; j < V; j += 2) {
                 const float2 u = it.cs[j / 2], w = it.cs[V / 2 + j / 2];
@@ -186,17 +221,17 @@ __global__ __launch_bounds__(kThreads) void rope_axes_kernel(RopeArgs p)
             continue;
         if (it.turn)
             turn(it);
-        *reinterpret_cast<X *>(it.dst + it.d0) = it.x0;
-        if (it.d1 >= 0)
-            *reinterpret_cast<X *>(it.dst + it.d1) = it.x1;
+        it.x0.template store<TAIL>(it.dst + it.d0, it.n0);
+        if (it.n1 > 0)
+            it.x1.template store<TAIL>(it.dst + it.d1, it.n1);
     }
 }
 
-template <typename T, int V>
+template <typename T, int V, bool TAIL>
 bool run_rope(const RopeAxes &a, RopeArgs &p, bool copies, hipStream_t st)
 {
     const int heads = a.H_q + a.H_k;
-    p.turned = a.pairs / V;
+    p.turned = (a.pairs + V - 1) / V;
     const int rest = copies ? (a.D - 2 * a.pairs + 2 * V - 1) / (2 * V) : 0;
     const int chunks = p.turned + rest;
     // At most 1024 chunks of a head and 2^12 heads: every quotient is exact.
@@ -214,9 +249,9 @@ bool run_rope(const RopeAxes &a, RopeArgs &p, bool copies, hipStream_t st)
         return fail("rope_axes_dev: too many tokens for one launch");
     const dim3 grid(static_cast<unsigned>(blocks));
     if (a.interleaved)
-        hipLaunchKernelGGL((rope_axes_kernel<T, V, true>), grid, dim3(kThreads), 0, st, p);
+        hipLaunchKernelGGL((rope_axes_kernel<T, V, true, TAIL>), grid, dim3(kThreads), 0, st, p);
     else
-        hipLaunchKernelGGL((rope_axes_kernel<T, V, false>), grid, dim3(kThreads), 0, st, p);
+        hipLaunchKernelGGL((rope_axes_kernel<T, V, false, TAIL>), grid, dim3(kThreads), 0, st, p);
     return hip_ok(hipGetLastError(), "rope_axes_kernel launch");
 }
 
@@ -247,32 +282,19 @@ bool launch_rope_axes(const RopeAxes &a, hipStream_t st)
     p.D = a.D;
     p.heads_q = a.H_q;
     p.inverse = a.inverse;
-    // The widest vectors, up to 16 bytes, on which every piece starts and ends.
-    const int bytes = a.type == kMx4F32 ? 4 : 2;
-    uint64_t bits = uint64_t(a.pairs) | a.D;
-    bool copies = false;  // rows that are not turned in place have a rest to copy
-    for (int i = 0; i < 2; ++i) {
-        if ((i ? a.H_k : a.H_q) == 0)
-            continue;
-        for (int64_t s : {p.is[i].b, p.is[i].h, p.is[i].s, p.os[i].b, p.os[i].h, p.os[i].s})
-            bits |= uint64_t(s);
-        bits |= (reinterpret_cast<uintptr_t>(p.in[i]) | reinterpret_cast<uintptr_t>(p.out[i])) /
-                bytes;
-        copies = copies || p.in[i] != p.out[i];
-    }
-    const int V = int(std::min<uint64_t>(bits & -bits, 16 / bytes));
+    // A row that is not turned in place has a rest to copy.
+    const bool copies = (a.H_q > 0 && a.q != a.q_out) || (a.H_k > 0 && a.k != a.k_out);
+    // 16 bytes a vector, wherever rows begin.  Heads that these do not divide end in a shorter
+    // chunk, element by element: bf16 then moves 8 bytes (12 heads of 78, 10001 tokens: 18.5
+    // us, by 16 bytes 21.9, by 4 21.3, by single elements 24.3).
+    const int split = a.pairs | a.D;
     if (a.type == kMx4F32)
-        switch (V) {
-        case 4: return run_rope<float, 4>(a, p, copies, st);
-        case 2: return run_rope<float, 2>(a, p, copies, st);
-        default: return run_rope<float, 1>(a, p, copies, st);
-        }
-    switch (V) {
-    case 8: return run_rope<uint16_t, 8>(a, p, copies, st);
-    case 4: return run_rope<uint16_t, 4>(a, p, copies, st);
-    case 2: return run_rope<uint16_t, 2>(a, p, copies, st);
-    default: return run_rope<uint16_t, 1>(a, p, copies, st);
-    }
+        return split % 4 == 0 ? run_rope<float, 4, false>(a, p, copies, st)
+                              : run_rope<float, 4, true>(a, p, copies, st);
+    if (split % 8 == 0)
+        return run_rope<uint16_t, 8, false>(a, p, copies, st);
+    return split % 4 == 0 ? run_rope<uint16_t, 4, false>(a, p, copies, st)
+                          : run_rope<uint16_t, 4, true>(a, p, copies, st);
 }
 
 }  // namespace anima_hip
