@@ -24,9 +24,10 @@ using flash_tile::f32x4;
 using flash_tile::u32x4;
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
-// 16 bytes at any element: the hardware takes vector accesses that are not aligned.
+// Vectors at any element: the hardware takes vector accesses that are not aligned.
 typedef f32x4 any_f32x4 __attribute__((aligned(4)));
 typedef u32x4 any_u32x4 __attribute__((aligned(2)));
+typedef u32x2 any_u32x2 __attribute__((aligned(2)));
 
 constexpr int kGroup = 128;     // elements per scale
 constexpr int kNanScale = 255;  // scale byte of a group that held an infinity or a NaN

@@ -72,10 +72,10 @@ __device__ __forceinline__ i32x8 whole(const u32x4 &x, const u32x4 &y)
 }
 
 // Four consecutive columns of C from nn on.
-__device__ __forceinline__ void store4(float *row, int nn, int N, bool wide, f32x4 v)
+__device__ __forceinline__ void store4(float *row, int nn, int N, f32x4 v)
 {
-    if (wide && nn + 4 <= N) {
-        *reinterpret_cast<f32x4 *>(row + nn) = v;
+    if (nn + 4 <= N) {
+        *reinterpret_cast<any_f32x4 *>(row + nn) = v;
         return;
     }
 #pragma unroll
@@ -84,11 +84,11 @@ __device__ __forceinline__ void store4(float *row, int nn, int N, bool wide, f32
             row[nn + r] = v[r];
 }
 
-__device__ __forceinline__ void store4(uint16_t *row, int nn, int N, bool wide, f32x4 v)
+__device__ __forceinline__ void store4(uint16_t *row, int nn, int N, f32x4 v)
 {
     const u32x2 b = {bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3])};
-    if (wide && nn + 4 <= N) {
-        *reinterpret_cast<u32x2 *>(row + nn) = b;
+    if (nn + 4 <= N) {
+        *reinterpret_cast<any_u32x2 *>(row + nn) = b;
         return;
     }
 #pragma unroll
@@ -183,10 +183,8 @@ __global__ __launch_bounds__(WAVES * 64) void fp8_few_kernel(LinArgs p)
             acc += red[w * 64 + lane];
     }
     // Lane (n, g): columns 4g .. 4g+3 of row n.
-    const bool wide = (reinterpret_cast<uintptr_t>(p.c) & (4 * sizeof(T) - 1)) == 0 &&
-                      p.ldc % 4 == 0;
     if (m0 + n < p.M)
-        store4(static_cast<T *>(p.c) + int64_t(m0 + n) * p.ldc, row0 + 4 * g, p.N, wide, acc);
+        store4(static_cast<T *>(p.c) + int64_t(m0 + n) * p.ldc, row0 + 4 * g, p.N, acc);
 }
 
 // --------------------------------------------------------- staged tiles
@@ -469,7 +467,6 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void fp8_staged_kernel(LinArgs p)
         n0 += wn * NB * 32;
         if (p.part) {
             float *plane = p.part + int64_t(plane_of) * p.M * p.N;
-            const bool wide = p.N % 4 == 0;
 #pragma unroll
             for (int i = 0; i < MB; ++i) {
                 const int m = m0 + i * 32 + col;
@@ -479,7 +476,7 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void fp8_staged_kernel(LinArgs p)
                 for (int j = 0; j < NB; ++j)
 #pragma unroll
                     for (int r = 0; r < 16; r += 4)
-                        store4(plane + int64_t(m) * p.N, n0 + 32 * j + acc_row(r, half), p.N, wide,
+                        store4(plane + int64_t(m) * p.N, n0 + 32 * j + acc_row(r, half), p.N,
                                f32x4{acc[i][j][r], acc[i][j][r + 1], acc[i][j][r + 2],
                                      acc[i][j][r + 3]});
             }
@@ -488,9 +485,11 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void fp8_staged_kernel(LinArgs p)
         // Through LDS, so that rows go out in runs of 32 JB columns; pieces of 16 bytes are
         // placed as in the stages.
         constexpr int JB = G::JB, ROW = G::OUT_ROW;
+        // Rows that begin anywhere share cache lines, which must stay for the next store.
+        const bool aligned = (reinterpret_cast<uintptr_t>(p.c) & 15) == 0 &&
+                             p.ldc % (16 / int(sizeof(T))) == 0;
         constexpr int RUN = ROW / 16, E = 16 / int(sizeof(T));  // pieces of a row, their elements
         uint8_t *so = smem + G::OUT + wave % (WM * WN) * (32 * ROW);
-        const bool wide = (reinterpret_cast<uintptr_t>(p.c) & 15) == 0 && p.ldc % E == 0;
 #pragma unroll
         for (int i = 0; i < MB; ++i)
 #pragma unroll
@@ -501,9 +500,14 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void fp8_staged_kernel(LinArgs p)
                     for (int q = 0; q < 16; q += 4) {
                         const f32x16 &v = acc[i][jb + j];
                         const int at = (32 * j + acc_row(q, half)) * int(sizeof(T));
-                        store4(reinterpret_cast<T *>(so + col * ROW +
-                                                     ((at / 16) ^ swizzle<ROW>(col)) * 16 + at % 16),
-                               0, 4, true, f32x4{v[q], v[q + 1], v[q + 2], v[q + 3]});
+                        uint8_t *dst = so + col * ROW +
+                                       ((at / 16) ^ swizzle<ROW>(col)) * 16 + at % 16;
+                        if constexpr (sizeof(T) == 4)
+                            *reinterpret_cast<f32x4 *>(dst) =
+                                f32x4{v[q], v[q + 1], v[q + 2], v[q + 3]};
+                        else
+                            *reinterpret_cast<u32x2 *>(dst) =
+                                u32x2{bf16_pair(v[q], v[q + 1]), bf16_pair(v[q + 2], v[q + 3])};
                     }
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                 __builtin_amdgcn_wave_barrier();
@@ -516,9 +520,12 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void fp8_staged_kernel(LinArgs p)
                     if (m >= p.M)
                         continue;
                     T *dst = static_cast<T *>(p.c) + int64_t(m) * p.ldc + nn;
-                    if (wide && nn + E <= p.N)
-                        __builtin_nontemporal_store(v, reinterpret_cast<u32x4 *>(dst));
-                    else
+                    if (nn + E <= p.N) {
+                        if (aligned)
+                            __builtin_nontemporal_store(v, reinterpret_cast<u32x4 *>(dst));
+                        else
+                            *reinterpret_cast<any_u32x4 *>(dst) = v;
+                    } else
 #pragma unroll
                         for (int e = 0; e < E; ++e)
                             if (nn + e < p.N) {
