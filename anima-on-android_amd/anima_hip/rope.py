@@ -31,13 +31,17 @@ def _rotation(angles: np.ndarray) -> np.ndarray:
     return np.stack([c, -s, s, c], axis=-1)
 
 
-def generate_rope_freqs(H: int, W: int, T: int = 1, head_dim: int = 128) -> np.ndarray:
-    """Rotation table [T*H*W, head_dim/2, 2, 2] float32 for a T x H x W token grid."""
+def _split(head_dim):
+    """(temporal channels, channels of either spatial axis, the spatial axes' base)."""
     if head_dim % 2:
         raise ValueError("head_dim must be even")
     dim_h = head_dim // 6 * 2
-    dim_t = head_dim - 2 * dim_h
-    spatial_base = 10000.0 * 4.0 ** (dim_h / (dim_h - 2))
+    return head_dim - 2 * dim_h, dim_h, 10000.0 * 4.0 ** (dim_h / (dim_h - 2))
+
+
+def generate_rope_freqs(H: int, W: int, T: int = 1, head_dim: int = 128) -> np.ndarray:
+    """Rotation table [T*H*W, head_dim/2, 2, 2] float32 for a T x H x W token grid."""
+    dim_t, dim_h, spatial_base = _split(head_dim)
     blocks = [
         (_rotation(np.outer(np.arange(T, dtype=np.float32), _axis_freqs(10000.0, dim_t))), 0),
         (_rotation(np.outer(np.arange(H, dtype=np.float32), _axis_freqs(spatial_base, dim_h))), 1),
