@@ -88,18 +88,43 @@ __device__ __forceinline__ double inv_sqrt(double m)
     return r;
 }
 
-// h = x + r of a piece, zero past K.
-template <typename T>
-__device__ __forceinline__ void load_sum(const NormArgs &p, int64_t row, int k0, float (&h)[8])
+// y cut off after f32's 24 bits, the last of them set where anything was lost: rounding this
+// to fewer bits is rounding y, also next to a tie.
+__device__ __forceinline__ float to_odd(double y)
 {
-    load8(static_cast<const T *>(p.x) + row * p.ldx, k0, p.K, h);
+    const u32x2 b = __builtin_bit_cast(u32x2, y);
+    // Bit 29 where any below it is set.
+    const unsigned lost = (b[0] & 0x1FFFFFFFu) + 0x1FFFFFFFu;
+    return float(__builtin_bit_cast(double, u32x2{(b[0] & 0xE0000000u) | (lost & 0x20000000u), b[1]}));
+}
+
+// h = x + r of eight elements in 64 bits, where it is exact but for values 2^29 apart in f32
+// and 2^45 in bf16, and its f32 rounding; zero past K.
+template <typename T>
+__device__ __forceinline__ void load_sum(const NormArgs &p, int64_t row, int k0, double (&h)[8],
+                                         float (&s)[8])
+{
+    load8(static_cast<const T *>(p.x) + row * p.ldx, k0, p.K, s);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        h[i] = double(s[i]);
     if (p.r) {
         float r[8];
         load8(static_cast<const T *>(p.r) + row * p.ldr, k0, p.K, r);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            h[i] += r[i];
+        for (int i = 0; i < 8; ++i) {
+            s[i] += r[i];
+            h[i] += double(r[i]);
+        }
     }
+}
+
+template <typename T>
+__device__ __forceinline__ void store_sum(const NormArgs &p, int64_t row, int k0,
+                                          const float (&s)[8])
+{
+    if (p.sum)
+        store8(static_cast<T *>(p.sum) + row * p.lds, k0, p.K, s);
 }
 
 __device__ __forceinline__ void load_weight(const NormArgs &p, int k0, float (&w)[8])
@@ -113,23 +138,24 @@ __device__ __forceinline__ void load_weight(const NormArgs &p, int k0, float (&w
         w[i] = 1.0f;
 }
 
-// A piece of the results.  The 16 lanes of a group come here together.
+// A piece of the normed row.  The 16 lanes of a group come here together.
 template <typename T>
 __device__ __forceinline__ void store_normed(const NormArgs &p, int64_t row, int piece,
-                                             const float (&h)[8], double inv, int groups)
+                                             const double (&h)[8], double inv, int groups)
 {
     const int k0 = 8 * piece;
-    if (p.sum)
-        store8(static_cast<T *>(p.sum) + row * p.lds, k0, p.K, h);
-    float w[8], y[8];
+    float v[8], w[8], odd[8];
     load_weight(p, k0, w);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        y[i] = k0 + i < p.K ? float(double(h[i]) * inv) * w[i] : 0.0f;
+    for (int i = 0; i < 8; ++i) {
+        const double y = h[i] * inv * double(w[i]);  // past K zero, or NaN like the row
+        odd[i] = to_odd(y);
+        v[i] = sizeof(T) == 4 ? float(y) : odd[i];
+    }
     if (p.y)
-        store8(static_cast<T *>(p.y) + row * p.ldy, k0, p.K, y);
+        store8(static_cast<T *>(p.y) + row * p.ldy, k0, p.K, v);
     if (p.codes)
-        pack_group(y, p.codes + row * groups * kGroup, p.scales + row * fp8_scale_bytes(p.K),
+        pack_group(odd, p.codes + row * groups * kGroup, p.scales + row * fp8_scale_bytes(p.K),
                    piece >> 4, groups, piece & 15);
 }
 
@@ -146,14 +172,17 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void add_rmsnorm_ker
     if (row >= p.rows)
         return;  // whole waves: one wave per row where a workgroup has several
     const int groups = int(fp8_groups(p.K));
-    float h[PIECES][8];
+    double h[PIECES][8];
     double ss = 0.0;
 #pragma unroll
     for (int j = 0; j < PIECES; ++j) {
-        load_sum<T>(p, row, 8 * (j * THREADS + tid), h[j]);
+        const int k0 = 8 * (j * THREADS + tid);
+        float s[8];
+        load_sum<T>(p, row, k0, h[j], s);
+        store_sum<T>(p, row, k0, s);
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            ss = fma(double(h[j][i]), double(h[j][i]), ss);
+            ss = fma(h[j][i], h[j][i], ss);
     }
     ss = wave_sum(ss);
     if constexpr (WAVES > 1) {
@@ -185,11 +214,12 @@ __global__ __launch_bounds__(1024) void add_rmsnorm_long_kernel(NormArgs p)
     const int pieces = groups * 16;
     double ss = 0.0;
     for (int piece = tid; piece < pieces; piece += 1024) {
-        float h[8];
-        load_sum<T>(p, row, 8 * piece, h);
+        double h[8];
+        float s[8];
+        load_sum<T>(p, row, 8 * piece, h, s);
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            ss = fma(double(h[i]), double(h[i]), ss);
+            ss = fma(h[i], h[i], ss);
     }
     ss = wave_sum(ss);
     if ((tid & 63) == 0)
@@ -201,8 +231,10 @@ __global__ __launch_bounds__(1024) void add_rmsnorm_long_kernel(NormArgs p)
         ss += part[w];
     const double inv = inv_sqrt(ss / p.K + double(p.eps));
     for (int piece = tid; piece < pieces; piece += 1024) {
-        float h[8];
-        load_sum<T>(p, row, 8 * piece, h);
+        double h[8];
+        float s[8];
+        load_sum<T>(p, row, 8 * piece, h, s);
+        store_sum<T>(p, row, 8 * piece, s);
         store_normed<T>(p, row, piece, h, inv, groups);
     }
 }
@@ -226,33 +258,33 @@ bool norm_grid(int64_t blocks, int threads, dim3 &grid)
     return true;
 }
 
-template <typename T, int THREADS>
-bool run_norm(const NormArgs &p, int pieces, hipStream_t st)
+template <typename T, int THREADS, int PIECES>
+bool run_norm(const NormArgs &p, hipStream_t st)
 {
     constexpr int PER = THREADS < 256 ? 256 / THREADS : 1;  // rows of a workgroup
     const dim3 block(THREADS < 256 ? 256 : THREADS);
     dim3 grid;
     if (!norm_grid((p.rows + PER - 1) / PER, block.x, grid))
         return false;
-    if (pieces <= 1)
-        hipLaunchKernelGGL((add_rmsnorm_kernel<T, THREADS, 1>), grid, block, 0, st, p);
-    else if (pieces <= 2)
-        hipLaunchKernelGGL((add_rmsnorm_kernel<T, THREADS, 2>), grid, block, 0, st, p);
-    else
-        hipLaunchKernelGGL((add_rmsnorm_kernel<T, THREADS, 4>), grid, block, 0, st, p);
+    hipLaunchKernelGGL((add_rmsnorm_kernel<T, THREADS, PIECES>), grid, block, 0, st, p);
     return hip_ok(hipGetLastError(), "add_rmsnorm_kernel launch");
 }
 
 template <typename T>
 bool launch_norm(const NormArgs &p, hipStream_t st)
 {
-    const auto pieces = [&](int threads) { return (p.K + 8 * threads - 1) / (8 * threads); };
-    if (pieces(64) <= 1)
-        return run_norm<T, 64>(p, pieces(64), st);
-    if (pieces(256) <= 4)
-        return run_norm<T, 256>(p, pieces(256), st);
-    if (pieces(1024) <= 4)
-        return run_norm<T, 1024>(p, pieces(1024), st);
+    if (p.K <= 512)
+        return run_norm<T, 64, 1>(p, st);
+    if (p.K <= 2048)
+        return run_norm<T, 256, 1>(p, st);
+    if (p.K <= 4096)
+        return run_norm<T, 256, 2>(p, st);
+    if (p.K <= 8192)
+        return run_norm<T, 256, 4>(p, st);
+    if (p.K <= 16384)
+        return run_norm<T, 1024, 2>(p, st);
+    if (p.K <= 32768)
+        return run_norm<T, 1024, 4>(p, st);
     dim3 grid;
     if (!norm_grid(p.rows, 1024, grid))
         return false;
