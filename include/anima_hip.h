@@ -682,10 +682,10 @@ bool anima_hip_fp8_unpack_dev(const uint8_t *codes, const uint8_t *scales, void 
  *   h = x + residual,  sum = h,  y = h / sqrt(mean(h^2) + eps) * w,
  * and y as FP8 rows.  x, residual, sum and y are of `dtype`, rows ldx, ldr,
  * ldsum and ldy elements apart; w is f32 [K].  residual, w (NULL: 1), sum, y, and
- * codes with scales may each be NULL; one output at least is given.  h is
- * taken in f32 (sum is its rounding, and the norm is of h itself), the sum of
- * squares and its root in 64 bits, so that no h is too large or too small for
- * them; each output is rounded once.  An infinity in a row makes its own element
+ * codes with scales may each be NULL; one output at least is given.  h and y are
+ * taken in 64 bits, so that no h is too large or too small for the sum of
+ * squares, and each output is rounded once (a bf16 sum through f32): the 8-bit
+ * rows are those of the 64-bit y. An infinity in a row makes its own element
  * NaN and the others 0.  sum and y may be x or residual themselves (at the same
  * stride), not each other. */
 bool anima_hip_add_rmsnorm_fp8_dev(const void *x, int64_t ldx, const void *residual, int64_t ldr,

@@ -107,6 +107,21 @@ def test_pack_past_4_gib(dtype):
 
 
 @pytest.mark.parametrize("dtype", gpu.TYPES)
+@pytest.mark.parametrize("rows,K", [(900, 500), (300, 2047), (150, 4000), (80, 8192), (40, 16000),
+                                    (20, 32768), (9, 70001)])
+def test_norm_rows_are_those_of_the_64_bit_result(rows, K, dtype):
+    """Every code and scale, by each of the norm's kernels: y is off by some 2^-50 of itself before
+    its only rounding."""
+    (x, xv), (r, rv), w = gpu.norm_inputs(rows, K, dtype, K)
+    out = gpu.norm_dev(x, r, w, 1e-6, dtype)
+    _, y = ref.norm(xv, rv, w.astype(np.float64), float(np.float32(1e-6)))
+    for got, want in zip(out["c"], ref.pack(y)):
+        np.testing.assert_array_equal(got, want)
+    err = np.abs(ref.untyped(out["y"], dtype) - y)
+    assert (err <= ref.HALF[dtype] * np.abs(y) * (1 + 2.0 ** -20) + 1e-44).all()
+
+
+@pytest.mark.parametrize("dtype", gpu.TYPES)
 @pytest.mark.parametrize("B,S,H,D,P", [(2, 5000, (8, 8), 64, 32), (9000, 3, (4, 1), 64, 24),
                                        (1, 70000, (1, 0), 78, 39), (40000, 1, (3, 1), 40, 17)])
 @pytest.mark.parametrize("interleaved", [False, True])
