@@ -107,8 +107,8 @@ def test_pack_past_4_gib(dtype):
 
 
 @pytest.mark.parametrize("dtype", gpu.TYPES)
-@pytest.mark.parametrize("rows,K", [(900, 500), (300, 2047), (150, 4000), (80, 8192), (40, 16000),
-                                    (20, 32768), (9, 70001)])
+@pytest.mark.parametrize("rows,K", [(900, 500), (300, 2047), (150, 4000), (80, 8192), (300, 4000),
+                                    (270, 8192), (40, 16000), (20, 32768), (9, 70001)])
 def test_norm_rows_are_those_of_the_64_bit_result(rows, K, dtype):
     """Every code and scale, by each of the norm's kernels: y is off by some 2^-50 of itself before
     its only rounding."""
