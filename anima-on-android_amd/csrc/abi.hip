@@ -1805,6 +1805,13 @@ bool anima_hip_add_rmsnorm_fp8_dev(const void *x, int64_t ldx, const void *resid
             return fail(who + ": w must be aligned to its type");
         if (sum && sum == y)
             return fail(who + ": sum and y must be different arrays");
+        // In place, a row's results must not land on rows that are still to be read.
+        const auto replaces = [&](const void *out, int64_t ldo) {
+            return rows <= 1 || !out ||
+                   ((out != x || ldo == ldx) && (out != residual || ldo == ldr));
+        };
+        if (!replaces(sum, ldsum) || !replaces(y, ldy))
+            return fail(who + ": an output in place must have its input's stride");
         if (codes && !check_mx4("add_rmsnorm_fp8_dev", codes, scales))
             return false;
     }
@@ -1914,6 +1921,14 @@ bool anima_hip_rope_axes_dev(const void *q, const int64_t *q_strides, void *q_ou
         if ((H_q > 0 && !rows_apart(a.qos, B, H_q, S, D)) ||
             (H_k > 0 && !rows_apart(a.kos, B, H_k, S, D)))
             return fail(who + ": rows of an output overlap");
+        const auto moved = [](const Strides &i, const Strides &o, int B, int H, int S) {
+            return (B > 1 && i.b != o.b) || (H > 1 && i.h != o.h) || (S > 1 && i.s != o.s);
+        };
+        if ((H_q > 0 && q_out == q && moved(a.qs, a.qos, B, H_q, S)) ||
+            (H_k > 0 && k_out == k && moved(a.ks, a.kos, B, H_k, S)))
+            return fail(who + ": an output in place must have its input's strides");
+        if (H_q > 0 && H_k > 0 && (q_out == k_out || q_out == k || k_out == q))
+            return fail(who + ": q, k and their outputs must not overlap");
     }
     a.q = q;
     a.q_out = q_out;

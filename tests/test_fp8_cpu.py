@@ -121,3 +121,25 @@ def test_reference_packing_is_nearest():
         top = mag[:, 128 * g:128 * g + 128].max(-1)
         assert (top <= 448).all() and (top > 224).all()
     assert (codes[:, 300:] == 0).all() and (scales[:, 3:] == 0).all()
+
+
+@pytest.mark.parametrize("change", [dict(sum=P, ldsum=65), dict(sum=2 * P, ldsum=80), dict(y=P, ldy=96),
+                                    dict(y=2 * P, ldy=65)])
+def test_norm_in_place_at_another_stride_is_refused(change):
+    """Rows would land on rows that are still to be read."""
+    a = {**NORM, **dict(r=2 * P, sum=3 * P, y=4 * P), **change}
+    refused(_lib.load().anima_hip_add_rmsnorm_fp8_dev(
+        a["x"], a["ldx"], a["r"], a["ldr"], a["w"], ct.c_float(a["eps"]), a["dtype"], a["sum"],
+        a["ldsum"], a["y"], a["ldy"], a["codes"], a["scales"], a["rows"], a["K"], None), "in place")
+
+
+@pytest.mark.parametrize("change,word", [
+    (dict(qo=P, qos=(1280, 64, 256)), "in place"), (dict(ko=2 * P, ks=(640, 64, 128)), "in place"),
+    (dict(qo=3 * P, ko=3 * P), "overlap"), (dict(qo=2 * P), "overlap"), (dict(ko=P), "overlap")])
+def test_rope_overlaps_are_refused(change, word):
+    a = {**ROPE, **dict(k=2 * P, qo=3 * P, ko=4 * P), **change}
+    refused(_lib.load().anima_hip_rope_axes_dev(
+        a["q"], _lib.strides(a["qs"]), a["qo"], _lib.strides(a["qos"]), a["H_q"], a["k"],
+        _lib.strides(a["ks"]), a["ko"], _lib.strides(a["kos"]), a["H_k"], a["pos"], 15,
+        a["counts"], a["freqs"], a["axis"], a["axes"], a["pairs"], a["B"], a["S"], a["D"],
+        a["dtype"], False, False, None), word)
