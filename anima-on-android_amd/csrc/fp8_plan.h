@@ -54,8 +54,8 @@ constexpr TileShape kF32Shapes[] = {
 struct CallCost {
     double launch, sum_launch, sum_rate, few_launch, few_turn, few_weights, few_rows;
 };
-constexpr CallCost kBf16Cost = {2.195, 1.921, 1.886e6, 2.270, 0.709, 0.193, 0.271};
-constexpr CallCost kF32Cost = {2.741, 1.753, 1.907e6, 2.291, 0.666, 0.207, 0.283};
+constexpr CallCost kBf16Cost = {2.195, 1.921, 1.886e6, 2.357, 0.809, 0.453, 0.265};
+constexpr CallCost kF32Cost = {2.741, 1.753, 1.907e6, 2.300, 0.819, 0.466, 0.294};
 
 struct LinPlan {
     bool staged = false;
@@ -90,8 +90,9 @@ inline LinPlan few_plan(int M, int N, int groups)
 inline double few_us(const LinPlan &pl, int M, int N, int groups, const CallCost &c)
 {
     const int turns = (groups + pl.waves - 1) / pl.waves;
-    return c.few_launch + turns * c.few_turn +
-           strips(M, N) * groups * (c.few_weights + c.few_rows * std::min(M, 16) / 16) / 1000;
+    // Latency, or the loads' rate.
+    const double per_group = c.few_weights + c.few_rows * std::min(M, 16) / 16;
+    return c.few_launch + std::max(turns * c.few_turn, strips(M, N) * groups * per_group / 1000);
 }
 
 inline double staged_us(const LinPlan &pl, const TileShape &t, int M, int N, const CallCost &c)

@@ -44,6 +44,7 @@ def test_gpu_cases_reach_their_shapes(plans):
 @pytest.mark.parametrize("dtype,M,N,K,want", [
     (BF16, 1, 2048, 2048, "few 8"),        # 4.1
     (BF16, 1, 2048, 8192, "tile 9 8"),     # 8.7, few 9.9
+    (BF16, 1, 8192, 2048, "few 4"),        # 6.2, tiles 6.8
     (BF16, 4608, 8192, 2048, "tile 1 1"),  # 73.6, 256 x 256 tiles 80
     (F32, 8, 6144, 2048, "few 8"),         # 6.9
 ])
