@@ -130,12 +130,24 @@ __device__ __forceinline__ void load8(const uint16_t *row, int k0, int K, float 
         x[i] = k0 + i < K ? __uint_as_float(unsigned(row[k0 + i]) << 16) : 0.0f;
 }
 
+// A vector stored past the caches (STREAM), or into them.
+template <bool STREAM, typename V, typename T>
+__device__ __forceinline__ void store_vector(T *p, const V &v)
+{
+    typedef V Anywhere __attribute__((aligned(sizeof(T))));
+    if constexpr (STREAM)
+        __builtin_nontemporal_store(v, reinterpret_cast<Anywhere *>(p));
+    else
+        *reinterpret_cast<Anywhere *>(p) = v;
+}
+
 // The same elements stored, rounded to the row's type.
+template <bool STREAM>
 __device__ __forceinline__ void store8(float *row, int k0, int K, const float (&x)[8])
 {
     if (k0 + 8 <= K) {
-        *reinterpret_cast<any_f32x4 *>(row + k0) = f32x4{x[0], x[1], x[2], x[3]};
-        *reinterpret_cast<any_f32x4 *>(row + k0 + 4) = f32x4{x[4], x[5], x[6], x[7]};
+        store_vector<STREAM>(row + k0, f32x4{x[0], x[1], x[2], x[3]});
+        store_vector<STREAM>(row + k0 + 4, f32x4{x[4], x[5], x[6], x[7]});
         return;
     }
 #pragma unroll
@@ -149,6 +161,7 @@ __device__ __forceinline__ unsigned bf16_pair(float lo, float hi)
     return __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{lo, hi}, bf16x2));
 }
 
+template <bool STREAM>
 __device__ __forceinline__ void store8(uint16_t *row, int k0, int K, const float (&x)[8])
 {
     u32x4 w;
@@ -156,7 +169,7 @@ __device__ __forceinline__ void store8(uint16_t *row, int k0, int K, const float
     for (int i = 0; i < 4; ++i)
         w[i] = bf16_pair(x[2 * i], x[2 * i + 1]);
     if (k0 + 8 <= K) {
-        *reinterpret_cast<any_u32x4 *>(row + k0) = w;
+        store_vector<STREAM>(row + k0, w);
         return;
     }
 #pragma unroll

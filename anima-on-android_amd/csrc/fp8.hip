@@ -11,7 +11,9 @@ using namespace fp8;
 
 // Packing and unpacking: 16 lanes a group, eight elements each.  Bound by HBM: 20011 x 1000 f32
 // packs in 16.4 us and unpacks in 18.5, 6.1 and 5.4 TB/s with part of it from the last-level
-// cache, 24.6 and 18.0 from memory; two or four groups a thread take 16.8 to 19.2.
+// cache, 24.6 and 18.0 from memory; two or four groups a thread take 16.8 to 19.2.  bf16
+// values are stored past the caches (16384 x 2048 from cold memory 20.5 us, so 16.2; f32
+// gains nothing, 20.9 and 21.8 at 8192 x 2048).
 template <typename T>
 __global__ __launch_bounds__(256) void fp8_pack_kernel(const T *x, int64_t ldx, uint8_t *codes,
                                                        uint8_t *scales, unsigned groups,
@@ -55,7 +57,7 @@ __global__ __launch_bounds__(256) void fp8_unpack_kernel(const uint8_t *codes,
         v[4 * i + 2] = hi[0] * s;
         v[4 * i + 3] = hi[1] * s;
     }
-    store8(x + int64_t(row) * ldx, g * kGroup + 8 * piece, K, v);
+    store8<sizeof(T) == 2>(x + int64_t(row) * ldx, g * kGroup + 8 * piece, K, v);
 }
 
 // ------------------------------------------------------------------ norm
@@ -126,8 +128,11 @@ template <typename T>
 __device__ __forceinline__ void store_sum(const NormArgs &p, int64_t row, int k0,
                                           const float (&s)[8])
 {
+    // Past the caches: the sum is read a sub-layer later, the 8-bit rows next (8192 x 2048 bf16
+    // between other calls 29.0 us, so 23.4; 2001 x 2047 f32 from cold memory 20.7 and 14.7; sums of
+    // 33 MB read back at once 4 to 8 % more).
     if (p.sum)
-        store8(static_cast<T *>(p.sum) + row * p.lds, k0, p.K, s);
+        store8<true>(static_cast<T *>(p.sum) + row * p.lds, k0, p.K, s);
 }
 
 __device__ __forceinline__ void load_weight(const NormArgs &p, int k0, float (&w)[8])
@@ -156,7 +161,7 @@ __device__ __forceinline__ void store_normed(const NormArgs &p, int64_t row, int
         v[i] = sizeof(T) == 4 ? float(y) : odd[i];
     }
     if (p.y)
-        store8(static_cast<T *>(p.y) + row * p.ldy, k0, p.K, v);
+        store8<true>(static_cast<T *>(p.y) + row * p.ldy, k0, p.K, v);
     if (p.codes)
         pack_group(odd, p.codes + row * groups * kGroup, p.scales + row * fp8_scale_bytes(p.K),
                    piece >> 4, groups, piece & 15);
