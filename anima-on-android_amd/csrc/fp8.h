@@ -72,9 +72,22 @@ __device__ __forceinline__ unsigned row16_max(unsigned v)
     return v;
 }
 
+// The eight elements of a group that one of 16 lanes has: two runs of four, kSecond apart.
+// Rows in bf16: one 16-byte access; in f32: 64, so that each of a lane's two accesses
+// follows its neighbour's.
+template <typename T>
+constexpr int kSecond = sizeof(T) == 4 ? 64 : 4;
+// Where the first run of piece `piece` of a row begins, 16 pieces a group.
+template <typename T>
+__device__ __forceinline__ int run_of(int piece)
+{
+    return sizeof(T) == 4 ? (piece >> 4) * kGroup + (piece & 15) * 4 : 8 * piece;
+}
+
 // One group over the 16 lanes of a DPP row, eight elements each, group g of `groups`
 // of its row.  All 16 lanes come here together.  Groups with an infinity or a NaN
 // have zero codes, so that packing is a function of the values alone.
+template <typename T>
 __device__ __forceinline__ void pack_group(const float (&x)[8], uint8_t *row_codes,
                                            uint8_t *row_scales, int g, int groups, int piece)
 {
@@ -90,32 +103,42 @@ __device__ __forceinline__ void pack_group(const float (&x)[8], uint8_t *row_cod
         c[0] = encode4(x[0], x[1], x[2], x[3], u);
         c[1] = encode4(x[4], x[5], x[6], x[7], u);
     }
-    *reinterpret_cast<u32x2 *>(row_codes + int64_t(g) * kGroup + 8 * piece) = c;
+    uint8_t *to = row_codes + int64_t(g) * kGroup + run_of<T>(piece);
+    if constexpr (kSecond<T> == 4) {
+        *reinterpret_cast<u32x2 *>(to) = c;
+    } else {
+        *reinterpret_cast<unsigned *>(to) = c[0];
+        *reinterpret_cast<unsigned *>(to + kSecond<T>) = c[1];
+    }
     // The last group's lanes write the zeros past it too.
     if (piece == 0 || (g == groups - 1 && piece < 4 - (g & 3)))
         row_scales[g + piece] = piece == 0 ? uint8_t(s) : uint8_t(0);
 }
 
-// Elements k0 .. k0+7 of a row of K; zero past its end.
+// Elements of a row of K from k0 and from k0 + SECOND on, four each; zero past its end.
+template <int SECOND>
 __device__ __forceinline__ void load8(const float *row, int k0, int K, float (&x)[8])
 {
-    if (k0 + 8 <= K) {
-        const f32x4 a = *reinterpret_cast<const any_f32x4 *>(row + k0);
-        const f32x4 b = *reinterpret_cast<const any_f32x4 *>(row + k0 + 4);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[i] = a[i];
-            x[4 + i] = b[i];
+    for (int h = 0; h < 2; ++h) {
+        const int k = k0 + h * SECOND;
+        if (k + 4 <= K) {
+            const f32x4 a = *reinterpret_cast<const any_f32x4 *>(row + k);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                x[4 * h + i] = a[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                x[4 * h + i] = k + i < K ? row[k + i] : 0.0f;
         }
-        return;
     }
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        x[i] = k0 + i < K ? row[k0 + i] : 0.0f;
 }
 
+template <int SECOND>
 __device__ __forceinline__ void load8(const uint16_t *row, int k0, int K, float (&x)[8])
 {
+    static_assert(SECOND == 4);
     if (k0 + 8 <= K) {
         const u32x4 a = *reinterpret_cast<const any_u32x4 *>(row + k0);
 #pragma unroll
@@ -142,18 +165,22 @@ __device__ __forceinline__ void store_vector(T *p, const V &v)
 }
 
 // The same elements stored, rounded to the row's type.
-template <bool STREAM>
+template <int SECOND, bool STREAM>
 __device__ __forceinline__ void store8(float *row, int k0, int K, const float (&x)[8])
 {
-    if (k0 + 8 <= K) {
-        store_vector<STREAM>(row + k0, f32x4{x[0], x[1], x[2], x[3]});
-        store_vector<STREAM>(row + k0 + 4, f32x4{x[4], x[5], x[6], x[7]});
-        return;
-    }
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (k0 + i < K)
-            row[k0 + i] = x[i];
+    for (int h = 0; h < 2; ++h) {
+        const int k = k0 + h * SECOND;
+        if (k + 4 <= K) {
+            store_vector<STREAM>(row + k,
+                                 f32x4{x[4 * h], x[4 * h + 1], x[4 * h + 2], x[4 * h + 3]});
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (k + i < K)
+                    row[k + i] = x[4 * h + i];
+        }
+    }
 }
 
 __device__ __forceinline__ unsigned bf16_pair(float lo, float hi)
@@ -161,9 +188,10 @@ __device__ __forceinline__ unsigned bf16_pair(float lo, float hi)
     return __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{lo, hi}, bf16x2));
 }
 
-template <bool STREAM>
+template <int SECOND, bool STREAM>
 __device__ __forceinline__ void store8(uint16_t *row, int k0, int K, const float (&x)[8])
 {
+    static_assert(SECOND == 4);
     u32x4 w;
 #pragma unroll
     for (int i = 0; i < 4; ++i)

@@ -9,11 +9,12 @@ namespace {
 
 using namespace fp8;
 
-// Packing and unpacking: 16 lanes a group, eight elements each.  Bound by HBM: 20011 x 1000 f32
-// packs in 16.4 us and unpacks in 18.5, 6.1 and 5.4 TB/s with part of it from the last-level
-// cache, 24.6 and 18.0 from memory; two or four groups a thread take 16.8 to 19.2.  bf16
-// values are stored past the caches (16384 x 2048 from cold memory 20.5 us, so 16.2; f32
-// gains nothing, 20.9 and 21.8 at 8192 x 2048).
+// Packing and unpacking: 16 lanes a group, eight elements each.  Bound by HBM: from cold
+// memory 20011 x 1000 f32 packs in 19.5 us and unpacks in 22.9, 8192 x 2048 in 16.8 and 13.3,
+// 5.1, 4.4, 5.0 and 6.3 TB/s; eight elements in a row a lane unpack those in 23.3 and 20.6.
+// Two or four groups a thread are no faster.
+// STREAM: values are stored past the caches, where rows are whole cache lines (8192 x 2048 f32
+// 17.4 us, so 13.3; 20011 x 1000 22.9 and 23.6, 9000 x 1003 11.2 and 13.2).
 template <typename T>
 __global__ __launch_bounds__(256) void fp8_pack_kernel(const T *x, int64_t ldx, uint8_t *codes,
                                                        uint8_t *scales, unsigned groups,
@@ -26,12 +27,12 @@ __global__ __launch_bounds__(256) void fp8_pack_kernel(const T *x, int64_t ldx, 
     const unsigned row = gi / groups;
     const int g = int(gi - row * groups);
     float v[8];
-    load8(x + int64_t(row) * ldx, g * kGroup + 8 * piece, K, v);
-    pack_group(v, codes + int64_t(row) * groups * kGroup,
+    load8<kSecond<T>>(x + int64_t(row) * ldx, g * kGroup + run_of<T>(piece), K, v);
+    pack_group<T>(v, codes + int64_t(row) * groups * kGroup,
                scales + int64_t(row) * fp8_scale_bytes(K), g, int(groups), piece);
 }
 
-template <typename T>
+template <typename T, bool STREAM>
 __global__ __launch_bounds__(256) void fp8_unpack_kernel(const uint8_t *codes,
                                                          const uint8_t *scales, T *x, int64_t ldx,
                                                          unsigned groups, unsigned total, int K)
@@ -43,7 +44,13 @@ __global__ __launch_bounds__(256) void fp8_unpack_kernel(const uint8_t *codes,
     const unsigned row = gi / groups;
     const int g = int(gi - row * groups);
     const int byte = scales[int64_t(row) * fp8_scale_bytes(K) + g];
-    const u32x2 c = *reinterpret_cast<const u32x2 *>(codes + int64_t(gi) * kGroup + 8 * piece);
+    const uint8_t *from = codes + int64_t(gi) * kGroup + run_of<T>(piece);
+    u32x2 c;
+    if constexpr (kSecond<T> == 4)
+        c = *reinterpret_cast<const u32x2 *>(from);
+    else
+        c = u32x2{*reinterpret_cast<const unsigned *>(from),
+                  *reinterpret_cast<const unsigned *>(from + kSecond<T>)};
     // 2^(byte - 127), subnormal for byte 0, NaN for 255.
     const float s = byte == 0 ? __uint_as_float(0x400000u)
                     : byte == kNanScale ? __uint_as_float(0x7FC00000u) : scale_of(byte);
@@ -57,7 +64,7 @@ __global__ __launch_bounds__(256) void fp8_unpack_kernel(const uint8_t *codes,
         v[4 * i + 2] = hi[0] * s;
         v[4 * i + 3] = hi[1] * s;
     }
-    store8<sizeof(T) == 2>(x + int64_t(row) * ldx, g * kGroup + 8 * piece, K, v);
+    store8<kSecond<T>, STREAM>(x + int64_t(row) * ldx, g * kGroup + run_of<T>(piece), K, v);
 }
 
 // ------------------------------------------------------------------ norm
@@ -109,13 +116,13 @@ template <typename T>
 __device__ __forceinline__ void load_sum(const NormArgs &p, int64_t row, int k0, double (&h)[8],
                                          float (&s)[8])
 {
-    load8(static_cast<const T *>(p.x) + row * p.ldx, k0, p.K, s);
+    load8<kSecond<T>>(static_cast<const T *>(p.x) + row * p.ldx, k0, p.K, s);
 #pragma unroll
     for (int i = 0; i < 8; ++i)
         h[i] = double(s[i]);
     if (p.r) {
         float r[8];
-        load8(static_cast<const T *>(p.r) + row * p.ldr, k0, p.K, r);
+        load8<kSecond<T>>(static_cast<const T *>(p.r) + row * p.ldr, k0, p.K, r);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             s[i] += r[i];
@@ -132,13 +139,14 @@ __device__ __forceinline__ void store_sum(const NormArgs &p, int64_t row, int k0
     // between other calls 29.0 us, so 23.4; 2001 x 2047 f32 from cold memory 20.7 and 14.7; sums of
     // 33 MB read back at once 4 to 8 % more).
     if (p.sum)
-        store8<true>(static_cast<T *>(p.sum) + row * p.lds, k0, p.K, s);
+        store8<kSecond<T>, true>(static_cast<T *>(p.sum) + row * p.lds, k0, p.K, s);
 }
 
+template <typename T>
 __device__ __forceinline__ void load_weight(const NormArgs &p, int k0, float (&w)[8])
 {
     if (p.w) {
-        load8(p.w, k0, p.K, w);
+        load8<kSecond<T>>(p.w, k0, p.K, w);
         return;
     }
 #pragma unroll
@@ -151,9 +159,9 @@ template <typename T>
 __device__ __forceinline__ void store_normed(const NormArgs &p, int64_t row, int piece,
                                              const double (&h)[8], double inv, int groups)
 {
-    const int k0 = 8 * piece;
+    const int k0 = run_of<T>(piece);
     float v[8], w[8], odd[8];
-    load_weight(p, k0, w);
+    load_weight<T>(p, k0, w);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const double y = h[i] * inv * double(w[i]);  // past K zero, or NaN like the row
@@ -161,18 +169,19 @@ __device__ __forceinline__ void store_normed(const NormArgs &p, int64_t row, int
         v[i] = sizeof(T) == 4 ? float(y) : odd[i];
     }
     if (p.y)
-        store8<true>(static_cast<T *>(p.y) + row * p.ldy, k0, p.K, v);
+        store8<kSecond<T>, true>(static_cast<T *>(p.y) + row * p.ldy, k0, p.K, v);
     if (p.codes)
-        pack_group(odd, p.codes + row * groups * kGroup, p.scales + row * fp8_scale_bytes(p.K),
+        pack_group<T>(odd, p.codes + row * groups * kGroup, p.scales + row * fp8_scale_bytes(p.K),
                    piece >> 4, groups, piece & 15);
 }
 
 // A row's threads (64, 256 or 1024) hold it in registers, PIECES times eight
 // elements each, so x and r are read once.  Bound by HBM, and in bf16 nearly by the 64-bit
-// conversions: 8192 x 2048 with residual takes 23.7 us in bf16, 5.0 TB/s (21.3 in f32
-// arithmetic, whose rows differ from the 64-bit result's in one of 10^7 codes), 34.5 in f32,
-// 6.3 TB/s, part of it from the last-level cache.  The weights loaded before the sum over the
-// row are 2 us slower: registers, and with them waves.
+// conversions: 8192 x 2048 with residual from cold memory takes 27.0 us in bf16, 4.4 TB/s,
+// and 39.7 in f32, 5.5 (a lane's eight elements in a row 41.8).  f32 arithmetic, whose rows
+// differ from the 64-bit result's in one of 10^7 codes, takes 2 us less of 24 where all is in
+// the last-level cache; the weights loaded before the sum over the row 2 us more: registers,
+// and with them waves.
 template <typename T, int THREADS, int PIECES>
 __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void add_rmsnorm_kernel(NormArgs p)
 {
@@ -188,7 +197,7 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void add_rmsnorm_ker
     double ss = 0.0;
 #pragma unroll
     for (int j = 0; j < PIECES; ++j) {
-        const int k0 = 8 * (j * THREADS + tid);
+        const int k0 = run_of<T>(j * THREADS + tid);
         float s[8];
         load_sum<T>(p, row, k0, h[j], s);
         store_sum<T>(p, row, k0, s);
@@ -228,7 +237,7 @@ __global__ __launch_bounds__(1024) void add_rmsnorm_long_kernel(NormArgs p)
     for (int piece = tid; piece < pieces; piece += 1024) {
         double h[8];
         float s[8];
-        load_sum<T>(p, row, 8 * piece, h, s);
+        load_sum<T>(p, row, run_of<T>(piece), h, s);
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             ss = fma(h[i], h[i], ss);
@@ -245,8 +254,8 @@ __global__ __launch_bounds__(1024) void add_rmsnorm_long_kernel(NormArgs p)
     for (int piece = tid; piece < pieces; piece += 1024) {
         double h[8];
         float s[8];
-        load_sum<T>(p, row, 8 * piece, h, s);
-        store_sum<T>(p, row, 8 * piece, s);
+        load_sum<T>(p, row, run_of<T>(piece), h, s);
+        store_sum<T>(p, row, run_of<T>(piece), s);
         store_normed<T>(p, row, piece, h, inv, groups);
     }
 }
@@ -340,12 +349,16 @@ bool launch_fp8_unpack(const uint8_t *codes, const uint8_t *scales, void *x, int
     if (total == 0)
         return true;
     const dim3 grid((total + 15) / 16), block(256);
+    const bool stream = flash_tile::aligned(x, 128) && ldx % (type == kMx4F32 ? 32 : 64) == 0;
+    const auto launch = [&](auto kernel, auto *out) {
+        hipLaunchKernelGGL(kernel, grid, block, 0, st, codes, scales, out, ldx, groups, total, K);
+    };
     if (type == kMx4F32)
-        hipLaunchKernelGGL(fp8_unpack_kernel<float>, grid, block, 0, st, codes, scales,
-                           static_cast<float *>(x), ldx, groups, total, K);
+        launch(stream ? fp8_unpack_kernel<float, true> : fp8_unpack_kernel<float, false>,
+               static_cast<float *>(x));
     else
-        hipLaunchKernelGGL(fp8_unpack_kernel<uint16_t>, grid, block, 0, st, codes, scales,
-                           static_cast<uint16_t *>(x), ldx, groups, total, K);
+        launch(stream ? fp8_unpack_kernel<uint16_t, true> : fp8_unpack_kernel<uint16_t, false>,
+               static_cast<uint16_t *>(x));
     return hip_ok(hipGetLastError(), "fp8_unpack_kernel launch");
 }
 
