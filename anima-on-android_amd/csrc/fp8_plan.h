@@ -97,17 +97,17 @@ inline double few_us(const LinPlan &pl, int M, int N, int groups, const CallCost
 
 inline double staged_us(const LinPlan &pl, const TileShape &t, int M, int N, const CallCost &c)
 {
-    const double load = double(pl.tiles_m) * pl.tiles_n * pl.splits / 256;  // tiles a CU
+    const int64_t items = int64_t(pl.tiles_m) * pl.tiles_n * pl.splits;  // over 256 CUs
     double us = c.launch;
     if (t.room == 1) {
-        const double slower = std::max(0.0, 2 * std::min(1.0, load) - 1);
+        const double slower = std::max(0.0, std::min(1.0, items / 128.0 - 1));
         const double group = t.us_alone + (t.us_full - t.us_alone) * slower;
-        us += std::ceil(load) * (pl.per_split * group + t.us_tile);
+        us += double((items + 255) / 256) * (pl.per_split * group + t.us_tile);
     } else {
-        const double pairs = std::floor(load / 2), rest = load - 2 * pairs;
-        us += pairs * (pl.per_split * t.us_full + t.us_tile);
+        const int64_t pairs = items / 512, rest = items % 512;
+        us += double(pairs) * (pl.per_split * t.us_full + t.us_tile);
         if (rest > 0)
-            us += pl.per_split * (rest <= 1 ? t.us_alone : t.us_full) + t.us_tile;
+            us += pl.per_split * (rest <= 256 ? t.us_alone : t.us_full) + t.us_tile;
     }
     if (pl.splits > 1)
         us += c.sum_launch + double(pl.splits) * M * N * 4 / c.sum_rate;
@@ -125,11 +125,17 @@ inline LinPlan lin_plan(int M, int N, int groups, bool f32)
     const CallCost &cost = f32 ? kF32Cost : kBf16Cost;
     double best_us = launch_fits(strips(M, N), best.waves * 64)
                          ? few_us(best, M, N, groups, cost) : HUGE_VAL;
-    for (int shape = 0; shape < int(std::size(kBf16Shapes)); ++shape) {
+    for (int shape = int(std::size(kBf16Shapes)) - 1; shape >= 0; --shape) {
         const TileShape &t = f32 ? kF32Shapes[shape] : kBf16Shapes[shape];
         if (groups % t.groups)
             continue;
         for (const int splits : {1, 2, 3, 4, 6, 8, 12, kMaxSplits}) {
+            // One round of tiles at least, or the sum's launch: most shapes are too slow already.
+            const double least = cost.launch + t.us_tile +
+                                 (splits == 1 ? groups * std::min(t.us_alone, t.us_full)
+                                              : cost.sum_launch);
+            if (least >= best_us)
+                continue;
             LinPlan pl;
             pl.shape = shape;
             set_grid(pl, t, M, N, groups, splits);
