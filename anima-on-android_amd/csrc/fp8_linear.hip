@@ -234,6 +234,7 @@ struct Staged {
     static constexpr int ROOM = LDS <= 81920 && THREADS <= 256 ? 2 : 1;
     static_assert(STEPS % KS == 0 && LDS <= 163840, "160 KiB of LDS");
     static_assert(OUT + OUT_BY <= SCALES, "the epilogue's rows fit the stages");
+    static_assert((OUT_ROW & (OUT_ROW - 1)) == 0, "and their pieces are placed by xor");
     static_assert(S >= 2 && (S - 2) * OPS < 64, "counted by vmcnt");
 };
 
