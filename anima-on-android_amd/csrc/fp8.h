@@ -86,10 +86,11 @@ __device__ __forceinline__ int run_of(int piece)
 
 // One group over the 16 lanes of a DPP row, eight elements each, group g of `groups`
 // of its row.  All 16 lanes come here together.  Groups with an infinity or a NaN
-// have zero codes, so that packing is a function of the values alone.
-template <typename T>
-__device__ __forceinline__ void pack_group(const float (&x)[8], uint8_t *row_codes,
-                                           uint8_t *row_scales, int g, int groups, int piece)
+// have zero codes, so that packing is a function of the values alone.  small(x) is called
+// in groups of the smallest scale, the only one with a tie below f32's normal numbers.
+template <typename T, typename Small>
+__device__ __forceinline__ void pack_group(float (&x)[8], uint8_t *row_codes, uint8_t *row_scales,
+                                           int g, int groups, int piece, Small &&small)
 {
     unsigned top = 0;
 #pragma unroll
@@ -97,6 +98,8 @@ __device__ __forceinline__ void pack_group(const float (&x)[8], uint8_t *row_cod
         top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
     top = row16_max(top);
     const int s = scale_byte(top);
+    if (s == kMinScale)
+        small(x);
     u32x2 c = {0u, 0u};
     if (s != kNanScale) {
         const float u = unscale_of(s);
