@@ -1877,11 +1877,48 @@ bool anima_hip_linear_fp8_dev(const uint8_t *a_codes, const uint8_t *a_scales,
 }
 
 namespace {
-// No two rows of an output [B, H, S, D] share an element along one axis.
+// No two rows of an output [B, H, S, D] share an element.  Rows i apart along one axis, j along
+// another and k along the third begin i a + j b + k c elements apart (strides a, b, c; their signs
+// do not matter, as i, j and k have either).
 bool rows_apart(const Strides &s, int B, int H, int S, int D)
 {
-    const auto ok = [&](int n, int64_t stride) { return n <= 1 || stride >= D || stride <= -D; };
-    return ok(B, s.b) && ok(H, s.h) && ok(S, s.s);
+    typedef __int128 Wide;  // of any stride's multiples
+    struct Axis {
+        int n;
+        Wide by;
+    } axes[3] = {{B, s.b}, {H, s.h}, {S, s.s}};
+    for (Axis &x : axes) {
+        x.by = x.n <= 1 ? 0 : x.by < 0 ? -x.by : x.by;
+        if (x.n > 1 && x.by < D)
+            return false;
+    }
+    // Each axis steps over all that the shorter strides reach: every order of axes with or
+    // without gaps.
+    std::sort(axes, axes + 3, [](const Axis &x, const Axis &y) { return x.by < y.by; });
+    Wide reach = D;
+    bool nested = true;
+    for (const Axis &x : axes) {
+        nested = nested && (x.n <= 1 || x.by >= reach);
+        reach += (x.n - 1) * x.by;
+    }
+    if (nested)
+        return true;
+    // Interleaved axes: all steps of the two shorter ones, against the third's multiple next to
+    // them on either side.
+    std::sort(axes, axes + 3, [](const Axis &x, const Axis &y) { return x.n < y.n; });
+    for (Wide i = 0; i < axes[0].n; ++i)
+        for (Wide j = i == 0 ? 0 : 1 - axes[1].n; j < axes[1].n; ++j) {
+            const Wide at = i * axes[0].by + j * axes[1].by, by = axes[2].by;
+            Wide k = at / by;
+            k -= at < k * by ? 1 : 0;  // k by <= at < (k + 1) by
+            for (Wide on = k; on <= k + 1; ++on) {
+                const Wide off = at - on * by;
+                if ((i != 0 || j != 0 || on != 0) && on < axes[2].n && -on < axes[2].n &&
+                    off < D && -off < D)
+                    return false;
+            }
+        }
+    return true;
 }
 }  // namespace
 

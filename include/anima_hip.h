@@ -727,7 +727,8 @@ bool anima_hip_linear_fp8_dev(const uint8_t *a_codes, const uint8_t *a_scales,
  * [B] on the device, tokens of each sequence, or NULL for S; rows of tokens from
  * counts[b] on are not written.  Angles are taken in 64 bits, the turn in f32, and
  * outputs rounded once.  An output may be its own input (same strides); other
- * overlaps are not allowed.  D at most 1024, heads at most 2048 each. */
+ * overlaps are not allowed, and strides by which an output's own rows share
+ * elements are refused.  D at most 1024, heads at most 2048 each. */
 bool anima_hip_rope_axes_dev(const void *q, const int64_t *q_strides, void *q_out,
                              const int64_t *qo_strides, int H_q, const void *k,
                              const int64_t *k_strides, void *k_out, const int64_t *ko_strides,
