@@ -50,6 +50,8 @@ def rotate(q, k, positions, freqs, pair_axis=None, interleaved=False, inverse=Fa
     axis = None
     if pair_axis is not None:
         axis = np.asarray(pair_axis)
+        if axis.dtype.kind not in "iub" and axis.size:
+            raise ValueError(f"pair_axis must be whole numbers, got {axis.dtype}")
         if axis.shape != freqs.shape or (axis.size and (axis.min() < 0 or axis.max() >= axes)):
             raise ValueError(f"pair_axis must be {len(freqs)} axes below {axes}")
         axis = np.ascontiguousarray(axis, dtype=np.uint8)
