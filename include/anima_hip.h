@@ -574,9 +574,9 @@ bool anima_hip_dit_euler_dev(anima_hip_dit *dit, float *latent, const float *sig
  * scales 4-byte aligned.  dtype of values and activations:
  * ANIMA_HIP_DTYPE_F32 or ANIMA_HIP_DTYPE_BF16.  Nothing is allocated; all
  * entries are asynchronous on `stream` and may be captured into a HIP graph.
- * Rows and lengths of up to 2^30; a call that would take more than 2^32 threads
- * (from 2^34 values on) is refused.  Calls that overlap in time need scratch of
- * their own. */
+ * Rows and lengths of up to 2^30; a call that would take 2^32 threads (packing,
+ * unpacking and appending: from 2^29 - 63 groups of 32 or parts of one on) is
+ * refused.  Calls that overlap in time need scratch of their own. */
 
 /* x [rows][ldx] (K elements of each row) to MX4 rows.  With a the largest
  * magnitude of a group and 2^E <= a < 2^(E+1), its scale byte is E - 2 + 127,
@@ -661,8 +661,11 @@ bool anima_hip_kv4_attention_dev(const void *q, int dtype, const int64_t *q_stri
  * follow one another without gaps.  Codes are 16-byte aligned, scales 4-byte
  * aligned.  dtype of values: ANIMA_HIP_DTYPE_F32 or ANIMA_HIP_DTYPE_BF16.
  * Nothing is allocated; all entries are asynchronous on `stream` and may be
- * captured into a HIP graph.  A call that would take more than 2^32 threads
- * (from 2^35 values on) is refused. */
+ * captured into a HIP graph.  A call that would take 2^32 threads is refused:
+ * packing and unpacking take 16 for each group of 128 or part of one (2^28 - 16
+ * groups at most, 2^35 values of whole groups and fewer of narrow rows), the norm
+ * 64 for a row of up to 512 elements (67108860 rows at most), 256 for one of up to
+ * 8192 (16777215 rows) and 1024 for longer ones (4194303 rows). */
 
 /* x [rows][ldx] (K elements of each row) to FP8 rows.  The scale is the smallest
  * power of two by which the group's largest magnitude a is at most 448: with
