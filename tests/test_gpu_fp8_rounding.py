@@ -1,4 +1,5 @@
-"""Where the 8-bit operators round, on the GPU against 64-bit numpy."""
+"""Where the 8-bit operators round, on the GPU against 64-bit numpy: the norm's results below f32's
+normal numbers, and products whose large terms cancel."""
 import numpy as np
 import pytest
 
@@ -40,3 +41,19 @@ def test_norm_results_below_f32s_normal_numbers(rows, K, dtype):
     unit = 2.0 ** (-149 if dtype == ref.F32 else -133)
     np.testing.assert_array_equal(ref.untyped(out["y"], dtype)[:, :256],
                                   np.rint(y[:, :256] / unit) * unit)
+
+
+@pytest.mark.parametrize("dtype", gpu.TYPES)
+@pytest.mark.parametrize("M,N,K", [(3, 20, 1024), (40, 200, 4096), (300, 260, 2048),
+                                   (600, 512, 1024)])
+def test_products_whose_large_terms_cancel(M, N, K, dtype):
+    """Two elements of each row 2^13 times the others, their products equal but for the sign, and in
+    different eights: C in f32 keeps the sum of the small ones to f32's steps of the large ones; C in
+    bf16 may lose 7 * 2^-13 of the largest product of each eight, no more."""
+    rng = np.random.default_rng(M)
+    a, w = rng.standard_normal((M, K)), rng.standard_normal((N, K))
+    big = 2.0 ** 13
+    a[:, 5], a[:, K - 3] = big, big
+    w[:, 5], w[:, K - 3] = 1.5, -1.5
+    a, w = (ref.pack(np.float32(x).astype(np.float64)) for x in (a, w))
+    gpu.check_linear(gpu.linear_dev(a, w, K, dtype), a, w, K, dtype)
