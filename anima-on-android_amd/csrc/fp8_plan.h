@@ -22,7 +22,10 @@ struct TileShape {
     int room;    // workgroups that a CU holds
     // Time in us of one group of K while at most half of the CUs work and when all do (a
     // CU's two workgroups together where there is room for two), and of a tile's start and
-    // end.
+    // end.  Fitted to whole calls to rank the shapes, not times that a part of the kernel
+    // takes: nothing here counts bytes, and the 32 x 64 tiles of two groups come out faster
+    // when all CUs work.  Where memory bounds a call it is predicted too fast
+    // (bf16 1 x 16384 x 8192 12.0 us, measured 31.9).
     double us_alone, us_full, us_tile;
 };
 constexpr TileShape kBf16Shapes[] = {
@@ -115,8 +118,10 @@ inline double staged_us(const LinPlan &pl, const TileShape &t, int M, int N, con
 }
 
 // The plan whose predicted time is least.  The constants are fitted to 560 measured sizes
-// of 1 to 8192 rows; on them the choice is 2 % behind the best plan's time on average and
-// 8 % in one of twenty, on 92 fresh ones 2 to 4 % on average.
+// of 1 to 8192 rows; on them the measured time of the choice is 2 % behind that of the best
+// of the plans on average and 8 % in one of twenty, on 92 fresh ones 2 to 4 % on average.
+// That is about the choice alone: the predicted times are further off (TileShape), also
+// between sizes (bf16 256 x 2048 x 2048 predicted 5.8 us, 64 rows 6.5; measured 7.1 and 6.2).
 inline LinPlan lin_plan(int M, int N, int groups, bool f32)
 {
     LinPlan best = few_plan(M, N, groups);

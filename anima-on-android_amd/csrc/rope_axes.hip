@@ -9,11 +9,13 @@
 // Bound by HBM: every value is read and written once, against six operations a
 // pair.  A workgroup takes the tokens that give each thread one chunk, up to 16 bytes of
 // either member of its pairs, and computes their angles' cosines and sines once for all
-// heads into LDS while the chunks are on their way.  2 x 4096 tokens of 32 f32 heads of
-// 128: 40 us, 6.7 TB/s (much of it from the last-level cache); 30003 tokens of 14 bf16 heads
-// of 64: 18.4 us, 5.8 TB/s.  Stores stay in the caches for the attention, which reads the rows
-// next: 8192 tokens of 16 bf16 heads of 128 written and read back take 11.4 us, past the
-// caches 14.1, though alone and from cold memory the store would gain a tenth.
+// heads into LDS while the chunks are on their way.  From cold memory (calls in a captured
+// graph over arrays in turn) 2 x 4096 tokens of 32 f32 heads of 128 take 49.2 us, 5.5 TB/s, and
+// 30003 tokens of 14 bf16 heads of 64 25.7 us, 4.2 TB/s; over the same arrays again, which the
+// last-level cache then holds in part or whole, 40.6 and 18.5 us.  Stores stay in the caches for
+// the attention, which reads the rows next: 8192 tokens of 16 bf16 heads of 128 written and read
+// back take 11.4 us, past the caches 14.1, though alone and from cold memory the store would gain
+// a tenth.
 #include "flash_tile.h"
 
 #include <algorithm>
@@ -115,8 +117,8 @@ struct Vec {
 
 // A chunk is two vectors of V elements: V pairs of a head, or 2 V copied elements; the last
 // of either may hold fewer (TAIL).  Whole chunks' vectors are half a turned row apart, also
-// where pairs are neighbours, so that lanes' accesses follow one another (14 heads of 64:
-// 19.5 us, so 18.9).
+// where pairs are neighbours, so that lanes' accesses follow one another (30003
+// tokens of 14 heads of 64, arrays in the last-level cache: 19.5 us, so 18.9).
 template <typename T, int V, bool NEIGHBOURS, bool TAIL>
 __global__ __launch_bounds__(kThreads) void rope_axes_kernel(RopeArgs p)
 {
@@ -253,8 +255,9 @@ bool run_rope(const RopeAxes &a, RopeArgs &p, bool copies, hipStream_t st)
     p.chunks = Divisor(unsigned(chunks));
     p.items = Divisor(unsigned(chunks * heads));
     // A chunk a thread, or two that share their angles' table where the GPU is full anyway
-    // (12 + 2 bf16 heads of 64: 30003 tokens 18.4 us, with one each 19.3; 8 tokens of 16 + 4
-    // heads of 128 3.8 and 3.0), and no more angles than the table holds.
+    // (30003 tokens of 12 + 2 bf16 heads of 64 18.5 us from the last-level cache, where the
+    // products before leave them, with one each 19.5, though from cold memory 25.7 and 24.8; 8
+    // tokens of 16 + 4 heads of 128 3.7 and 2.9), and no more angles than the table holds.
     const int each = p.tokens * chunks * heads > 2048 * kThreads ? 2 : 1;
     p.per_block = std::max(1, std::min(each * kThreads / (chunks * heads), kTable / a.pairs));
     p.pairs_by = Divisor(unsigned(a.pairs));
@@ -300,8 +303,9 @@ bool launch_rope_axes(const RopeAxes &a, hipStream_t st)
     // A row that is not turned in place has a rest to copy.
     const bool copies = (a.H_q > 0 && a.q != a.q_out) || (a.H_k > 0 && a.k != a.k_out);
     // 16 bytes a vector, wherever rows begin.  Heads that these do not divide end in a shorter
-    // chunk, element by element: bf16 then moves 8 bytes (12 heads of 78, 10001 tokens: 18.5
-    // us, by 16 bytes 21.9, by 4 21.3, by single elements 24.3).
+    // chunk, element by element: bf16 then moves 8 bytes (12 heads of 78, 10001 tokens from the
+    // last-level cache: 18.5 us, by 16 bytes 21.9, by 4 21.3, by single elements 24.3; from cold
+    // memory 25.1).
     const int split = a.pairs | a.D;
     if (a.type == kMx4F32)
         return split % 4 == 0 ? run_rope<float, 4, false>(a, p, copies, st)
