@@ -1903,8 +1903,11 @@ bool rows_apart(const Strides &s, int B, int H, int S, int D)
     }
     if (nested)
         return true;
-    // Interleaved axes: all steps of the two shorter ones, against the third's multiple next to
-    // them on either side.
+    // Interleaved axes, and more elements than memory holds apart.
+    if (Wide(B) * H * S * D > Wide(1) << 38)
+        return false;
+    // All steps of the two shorter axes (2^26 at most, with the third as long), against the
+    // third's multiple next to them on either side.
     std::sort(axes, axes + 3, [](const Axis &x, const Axis &y) { return x.n < y.n; });
     for (Wide i = 0; i < axes[0].n; ++i)
         for (Wide j = i == 0 ? 0 : 1 - axes[1].n; j < axes[1].n; ++j) {

@@ -54,6 +54,12 @@ def test_rows_apart(which, B, H, S, strides):
     assert taken(B, H, S, 64, strides, which)
 
 
+def test_interleaved_axes_past_any_memory():
+    """Refused at once: nothing goes through 2^31 steps on the host."""
+    assert not taken(2 ** 30, 2, 2 ** 30, 64, (2 ** 40, 2 ** 36 + 64, 128))
+    assert taken(2, 2, 2 ** 20, 64, (2 ** 40, 2 ** 26 + 64, 128))
+
+
 def test_against_every_row():
     rng = np.random.default_rng(0)
     seen = [0, 0]
